@@ -373,6 +373,124 @@ MSDA_API int flash_bevpool_sca_backward(const DLTensor *out_grad, const DLTensor
                                         int num_heads, int num_points, int grid_x, int grid_y, int grid_z,
                                         int value_stride_n, float epsilon, void *stream);
 
+/*
+ * The layer around the attention: a linear product with bias, activation and
+ * residual in its epilogue, layer norm, and 8-bit activation checkpoints, each
+ * with its backward pass. No counterpart in the reference, which leaves them
+ * to its host framework.
+ *
+ * Conventions: plain device pointers on the current device; rows may be apart
+ * (a row stride in elements, 0 for one row read for all), the elements of a row
+ * are adjacent, and what is called contiguous has no gaps; storage float32 or
+ * bfloat16, sums and statistics float32. Work is enqueued on `stream` without
+ * synchronising. Optional pointers may be NULL. Results do not depend on
+ * scheduling: repeated calls give the same bits.
+ */
+
+typedef enum {
+  MSDA_ACTIVATION_NONE = 0,
+  MSDA_ACTIVATION_RELU = 1,
+  MSDA_ACTIVATION_GELU = 2, /* z * Phi(z) */
+  MSDA_ACTIVATION_SILU = 3, /* z * sigmoid(z) */
+} msda_activation_t;
+
+/*
+ * 8-bit activation checkpoint of a [rows, cols] tensor: each row in blocks of
+ * 32 columns (the last may be short), a block as integers q = rint(x / 2^e),
+ * ties to even, and the byte e + 127, e the smallest integer >= -126 with
+ * max|x| <= 127 * 2^e (at the end of float32's range, 64 * 2^122 is held as
+ * 63 * 2^122). codes [rows, cols] and exponents [rows,
+ * ceil(cols / 32)] are contiguous. A block with an infinity or a NaN has the
+ * byte 255 and comes back as NaNs. Unpacking gives q * 2^e, exact in either
+ * storage type, into a contiguous tensor.
+ */
+MSDA_API int msda_checkpoint_pack(msda_dtype_t dtype, const void *input, int64_t rows, int64_t cols,
+                                  int64_t input_stride, int8_t *codes, uint8_t *exponents, void *stream);
+MSDA_API int msda_checkpoint_unpack(msda_dtype_t dtype, const int8_t *codes, const uint8_t *exponents, int64_t rows,
+                                    int64_t cols, void *output, void *stream);
+
+/*
+ * y = act(x W^T + b) + r, and its gradients for a gradient g of y:
+ * dz = g * act'(x W^T + b), dx = dz W, dW = dz^T x, db = sum of dz over rows
+ * (r's gradient is g itself).
+ *
+ *   input x        [rows, in_features]            weight W [out_features, in_features]
+ *   bias b         [out_features] or NULL         residual r [rows, out_features] or NULL
+ *   output y       [rows, out_features]           grad_output g [rows, out_features]
+ *   slope          act'(z), [rows, out_features] contiguous: float16 beside
+ *                  bfloat16 storage, float32 beside float32. The forward writes
+ *                  it where it is not NULL. The backward reads it, or, where it
+ *                  is NULL and the activation needs it, computes z again from
+ *                  input (or codes), weight and bias.
+ *   codes, exponents  backward only: an 8-bit checkpoint of x that takes the
+ *                  place of input; the gradients are those at the x it holds.
+ *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional
+ *
+ * workspace: 256-byte aligned, of at least as many bytes as the *_workspace
+ * call gives for the same structure (it reads sizes, strides and the
+ * alignment of pointers, and may be called before workspace is set). Calls
+ * that share a workspace must be ordered on the GPU.
+ *
+ * The matrix products run on the tensor cores: bfloat16 as it stands, float32
+ * as three bfloat16 parts of each operand, which keeps 24 bits of every
+ * product. Sizes up to 2^31 - 1.
+ */
+typedef struct {
+  int32_t dtype;      /* msda_dtype_t */
+  int32_t activation; /* msda_activation_t */
+  int64_t rows, in_features, out_features;
+  int64_t input_stride, weight_stride, residual_stride, output_stride, grad_output_stride;
+  const void *input, *weight, *bias, *residual;
+  void *output, *slope;
+  const void *grad_output;
+  const int8_t *codes;
+  const uint8_t *exponents;
+  void *grad_input, *grad_weight, *grad_bias;
+  void *workspace;
+  size_t workspace_bytes;
+} msda_linear_t;
+
+MSDA_API int msda_linear_act_forward_workspace(const msda_linear_t *args, size_t *bytes);
+MSDA_API int msda_linear_act_forward(const msda_linear_t *args, void *stream);
+MSDA_API int msda_linear_act_backward_workspace(const msda_linear_t *args, size_t *bytes);
+MSDA_API int msda_linear_act_backward(const msda_linear_t *args, void *stream);
+
+/*
+ * Layer norm over the last dimension: h = (x - mean) * rstd with rstd =
+ * 1 / sqrt(var + eps) (var: the mean square of x - mean), y = h w + b;
+ * dx = rstd (g w - mean(g w) - h mean(g w h)), dw and db the sums over rows of
+ * g h and g.
+ *
+ *   input [rows, cols]; weight, bias [cols] or NULL, of weight_dtype (dtype or
+ *   float32); output, grad_input contiguous; mean, rstd [rows] float32, written
+ *   by the forward where not NULL and read by the backward;
+ *   codes, exponents: the forward writes an 8-bit checkpoint of input there
+ *   where they are not NULL; a backward that gets them takes input and its
+ *   statistics from them instead of from input, mean and rstd;
+ *   grad_input, grad_weight, grad_bias overwritten, each optional;
+ *   workspace: needed with grad_weight or grad_bias, 256-byte aligned, of
+ *   msda_layer_norm_backward_workspace bytes.
+ */
+typedef struct {
+  int32_t dtype, weight_dtype; /* msda_dtype_t */
+  int64_t rows, cols;
+  int64_t input_stride, grad_output_stride;
+  float eps;
+  const void *input, *weight, *bias;
+  void *output;
+  float *mean, *rstd;
+  int8_t *codes;
+  uint8_t *exponents;
+  const void *grad_output;
+  void *grad_input, *grad_weight, *grad_bias;
+  void *workspace;
+  size_t workspace_bytes;
+} msda_layer_norm_t;
+
+MSDA_API int msda_layer_norm_forward(const msda_layer_norm_t *args, void *stream);
+MSDA_API int msda_layer_norm_backward_workspace(const msda_layer_norm_t *args, size_t *bytes);
+MSDA_API int msda_layer_norm_backward(const msda_layer_norm_t *args, void *stream);
+
 /* Message of the last failed call on this thread ("" after a success). The
  * reference raised it as a TVM-FFI exception (csrc/ffi/tensor_utils.hpp:13-34). */
 MSDA_API const char *msda_last_error(void);

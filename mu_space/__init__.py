@@ -20,6 +20,9 @@ _SUBMODULES = (
     "ops.sca_scatter",
     "ops.deformable_aggregation",
     "ops.flash_sca",
+    "ops.linear_act",
+    "ops.layer_norm",
+    "ops.checkpoint8",
     "runtime",
     "runtime.kernel_dispatch",
     "runtime.native",

@@ -1,0 +1,268 @@
+// Device code shared by the fused linear kernels: activations, the split of a
+// float32 into three bfloat16, and the epilogue of eight neighbouring outputs.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "linear_act.h"
+
+namespace lin {
+
+using bf16 = __nv_bfloat16;
+
+// ---- activations: value and slope --------------------------------------------------
+
+// Phi(z), the normal distribution function, and its density phi(z). erfc is
+// Hastings' rational approximation (Abramowitz and Stegun 7.1.26, |error| <=
+// 1.5e-7) in t = 1 / (1 + p x); its factor exp(-x^2) with x = |z| / sqrt 2 is
+// the density's too, so the slope costs three more instructions. The bfloat16
+// kernels use it (an error of 2^-23 beside outputs of 8 bits); float32 takes
+// erff. erff's 25 to 30 instructions made the epilogue, not the memory, the
+// bound of a 256 -> 512 layer.
+__device__ __forceinline__ void normal_fast(float z, float& cdf, float& pdf) {
+  const float x = fabsf(z) * 0.70710678118654752f;
+  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+  const float e = __expf(-x * x);
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float tail = 0.5f * p * t * e;  // Phi(-|z|)
+  cdf = z < 0.f ? tail : 1.f - tail;
+  pdf = 0.39894228040143268f * e;
+}
+
+__device__ __forceinline__ void normal_exact(float z, float& cdf, float& pdf) {
+  cdf = 0.5f * erfcf(-z * 0.70710678118654752f);
+  pdf = 0.39894228040143268f * expf(-0.5f * z * z);
+}
+
+__device__ __forceinline__ float sigmoid_of(float z, bool fast) {
+  return fast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
+}
+
+// act(z) in `y`, act'(z) in `s`. relu's slope at 0 is 0; a NaN stays a NaN.
+template <bool kFast>
+__device__ __forceinline__ void activate(Act act, float z, float& y, float& s) {
+  if (act == Act::kGelu) {
+    float cdf, pdf;
+    if (kFast)
+      normal_fast(z, cdf, pdf);
+    else
+      normal_exact(z, cdf, pdf);
+    y = z * cdf;
+    s = fmaf(z, pdf, cdf);
+  } else if (act == Act::kSilu) {
+    const float g = sigmoid_of(z, kFast);
+    y = z * g;
+    s = g * fmaf(z, 1.f - g, 1.f);
+  } else if (act == Act::kRelu) {
+    y = z <= 0.f ? 0.f : z;
+    s = z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  } else {
+    y = z;
+    s = 1.f;
+  }
+}
+
+// ---- float32 as three bfloat16 --------------------------------------------------------
+
+// x = hi + mid + lo to 2^-24 of x or better: each part is the bfloat16 nearest
+// to what is left. A finite x above bfloat16's largest value is cut, not
+// rounded, to it; a non-finite x is all in hi.
+__device__ __forceinline__ void split3(float x, bf16& hi, bf16& mid, bf16& lo) {
+  hi = __float2bfloat16_rn(x);
+  const uint32_t bits = __float_as_uint(x);
+  const bool finite = (bits & 0x7f800000u) != 0x7f800000u;
+  if (finite && (__bfloat16_as_ushort(hi) & 0x7f80u) == 0x7f80u)
+    hi = __ushort_as_bfloat16(static_cast<unsigned short>(bits >> 16));
+  const float r1 = finite ? x - __bfloat162float(hi) : 0.f;
+  mid = __float2bfloat16_rn(r1);
+  lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
+}
+
+// 1: an infinity, 2: a NaN, 0: finite
+__device__ __forceinline__ uint32_t flag_of(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? 0u : (b == 0x7f800000u ? 1u : 2u);
+}
+
+// ---- eight neighbouring values ----------------------------------------------------------
+
+__device__ __forceinline__ uint32_t pack2(bf16 a, bf16 b) {
+  return static_cast<uint32_t>(__bfloat16_as_ushort(a)) | (static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16);
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ bf16 from_float<bf16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) {
+  return __float2half_rn(v);
+}
+
+__device__ __forceinline__ void load8(const bf16* p, float v[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void load8(const float* p, float v[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+  v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float v[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void store8(bf16* p, const float v[8]) {
+  *reinterpret_cast<uint4*>(p) =
+      make_uint4(pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+__device__ __forceinline__ void store8(float* p, const float v[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__half* p, const float v[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Loads / stores of up to eight elements: one vector access where the caller
+// knows that address and length allow it.
+template <typename T>
+__device__ __forceinline__ void load_some(const T* p, int count, bool vec, float v[8]) {
+  if (vec) {
+    load8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store_some(T* p, int count, bool vec, const float v[8]) {
+  if (vec) {
+    store8(p, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j < count) p[j] = from_float<T>(v[j]);
+  }
+}
+
+// Splits eight values into the three planes at p, p + plane, p + 2 plane.
+__device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, bool vec, const float v[8]) {
+  bf16 part[3][8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) split3(v[j], part[0][j], part[1][j], part[2][j]);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    if (vec) {
+      *reinterpret_cast<uint4*>(p + i * plane) =
+          make_uint4(pack2(part[i][0], part[i][1]), pack2(part[i][2], part[i][3]), pack2(part[i][4], part[i][5]),
+                     pack2(part[i][6], part[i][7]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < count) p[i * plane + j] = part[i][j];
+    }
+  }
+}
+
+// Marks the row and the columns of the non-finite ones among eight values.
+__device__ __forceinline__ void mark_flags(const float v[8], int count, uint32_t* row_flag, uint32_t* col_flags) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t f = j < count ? flag_of(v[j]) : 0u;
+    if (f) atomicOr(col_flags + j, f);
+    any |= f;
+  }
+  if (any) atomicOr(row_flag, any);
+}
+
+// ---- the epilogue -----------------------------------------------------------------------
+
+template <typename T>
+struct SlopeOf {
+  using type = __half;  // of bfloat16 outputs: 11 bits on [-0.2, 1.2]
+};
+template <>
+struct SlopeOf<float> {
+  using type = float;
+};
+
+// Epilogue of columns [n, n + 8) of row m; `b` holds their bias. `vec`: all
+// rows start on 16-byte boundaries and the eight columns exist.
+template <typename T>
+__device__ __forceinline__ void epilogue8(const Epilogue& e, float v[8], const float b[8], int64_t m, int64_t n,
+                                          int64_t cols, bool vec) {
+  constexpr bool kFast = sizeof(T) == 2;
+  const int count = vec ? 8 : static_cast<int>(cols - n < 8 ? cols - n : 8);
+  if (e.mode == Epilogue::kStore) {
+    store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, v);
+    return;
+  }
+  float x[8], s[8];
+  if (e.extra) load_some(static_cast<const T*>(e.extra) + m * e.extra_ld + n, count, vec, x);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) activate<kFast>(e.act, v[j] + b[j], v[j], s[j]);
+  if (e.mode == Epilogue::kFwd) {
+    if (e.slope) store_some(static_cast<typename SlopeOf<T>::type*>(e.slope) + m * cols + n, count, vec, s);
+    if (e.extra) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += x[j];
+    }
+    store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = x[j] * s[j];
+    if (e.out_plane) {
+      store_planes(static_cast<bf16*>(e.out) + m * e.out_ld + n, e.out_plane, count, vec, v);
+      mark_flags(v, count, e.out_row_flags + m, e.out_col_flags + n);
+    } else {
+      store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, v);
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias8(const Epilogue& e, int64_t n, int64_t cols, float b[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    b[j] = e.bias && n + j < cols ? to_float(static_cast<const T*>(e.bias)[n + j]) : 0.f;
+}
+
+}  // namespace lin

@@ -1,0 +1,178 @@
+// Operand layouts of the fused linear kernels: what the tensor maps cannot
+// read as it stands (rows off 16-byte boundaries, float32, 8-bit checkpoints,
+// gradients still to be multiplied by the activation's slope) is laid out once
+// here. All of these kernels read and write each element once and are bound by
+// memory; a thread takes eight neighbouring columns of a row.
+#include <algorithm>
+
+#include "checkpoint8.cuh"
+#include "linear_device.cuh"
+
+namespace lin {
+namespace {
+
+constexpr int kThreads = 256;
+
+inline int blocks_for(int64_t groups) {
+  return static_cast<int>(std::min<int64_t>((groups + kThreads - 1) / kThreads, 148 * 16));
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+__device__ __forceinline__ void put(bf16* dst, int64_t plane, int count, bool vec, const float v[8], uint32_t* row_flag,
+                                    uint32_t* col_flags) {
+  if (sizeof(T) == 4) {
+    store_planes(dst, plane, count, vec, v);
+    mark_flags(v, count, row_flag, col_flags);
+  } else {
+    store_some(dst, count, vec, v);
+  }
+}
+
+// dst = src, or src * slope. A row of dst is padded to a multiple of eight
+// elements, so its vectors always fit; what they hold beyond `cols` is zero.
+template <typename T, bool kScale>
+__global__ void __launch_bounds__(kThreads)
+    operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec,
+                   const typename SlopeOf<T>::type* __restrict__ slope, bool slope_vec, bf16* __restrict__ dst,
+                   int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, uint32_t* row_flags,
+                   uint32_t* col_flags) {
+  const int64_t per_row = (cols + 7) / 8, total = rows * per_row;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);
+    float v[8];
+    load_some(src + r * src_ld + c, count, src_vec && count == 8, v);
+    if (kScale) {
+      float s[8];
+      load_some(slope + r * cols + c, count, slope_vec && count == 8, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= s[j];
+    }
+    put<T>(dst + r * dst_ld + c, plane, 8, true, v, row_flags + r, col_flags + c);
+  }
+}
+
+template <typename T, bool kScale>
+cudaError_t launch_operand(const void* src, int64_t src_ld, const void* slope, Operand& dst, uint32_t* row_flags,
+                           uint32_t* col_flags, cudaStream_t stream) {
+  using S = typename SlopeOf<T>::type;
+  const int64_t groups = dst.rows * ((dst.cols + 7) / 8);
+  if (groups == 0) return cudaSuccess;
+  const bool src_vec = aligned16(src) && (src_ld * sizeof(T)) % 16 == 0;
+  const bool slope_vec = aligned16(slope) && (dst.cols * sizeof(S)) % 16 == 0;
+  operand_kernel<T, kScale><<<blocks_for(groups), kThreads, 0, stream>>>(
+      static_cast<const T*>(src), src_ld, src_vec, static_cast<const S*>(slope), slope_vec, const_cast<bf16*>(dst.p),
+      dst.ld, dst.plane, dst.rows, dst.cols, row_flags, col_flags);
+  dst.row_flags = row_flags;
+  dst.col_flags = col_flags;
+  return cudaGetLastError();
+}
+
+__global__ void __launch_bounds__(kThreads)
+    unpack_kernel(const int8_t* __restrict__ codes, bool vec, const uint8_t* __restrict__ exps, bf16* __restrict__ dst,
+                  int64_t dst_ld, int64_t rows, int64_t cols) {
+  const int64_t per_row = (cols + 7) / 8, total = rows * per_row;
+  const int64_t blocks = ckpt::blocks_of(cols);
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);
+    float v[8];
+    ckpt::load_codes8(codes + r * cols + c, count, vec, exps[r * blocks + c / ckpt::kBlock], v);
+    store8(dst + r * dst_ld + c, v);  // exact: 7 bits and a power of two
+  }
+}
+
+// ---- column sums -------------------------------------------------------------------
+
+// A block takes 64 columns (a lane two of them, a warp a row at a time) and a
+// range of rows; the ranges' sums go to `parts` and are added in order by the
+// second kernel, so the result does not depend on scheduling.
+constexpr int kSumCols = 64, kSumWarps = 8;
+
+__global__ void __launch_bounds__(32 * kSumWarps)
+    column_parts_kernel(const bf16* __restrict__ src, int64_t ld, int64_t plane, int planes, int64_t rows,
+                        int64_t cols, int64_t rows_per_part, float* __restrict__ parts) {
+  __shared__ float buf[kSumWarps][kSumCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 2;
+  const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
+  float s0 = 0.f, s1 = 0.f;
+  if (c < cols) {
+    for (int q = 0; q < planes; ++q) {
+      const bf16* p = src + q * plane + c;
+#pragma unroll 8
+      for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+        const uint32_t u = *reinterpret_cast<const uint32_t*>(p + r * ld);  // ld is even: a pair never splits
+        s0 += __uint_as_float(u << 16);
+        s1 += __uint_as_float(u & 0xffff0000u);
+      }
+    }
+  }
+  buf[warp][lane * 2] = s0;
+  buf[warp][lane * 2 + 1] = s1;
+  __syncthreads();
+  if (threadIdx.x < kSumCols) {
+    const int64_t col = blockIdx.x * static_cast<int64_t>(kSumCols) + threadIdx.x;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSumWarps; ++w) s += buf[w][threadIdx.x];
+    if (col < cols) parts[blockIdx.y * cols + col] = s;
+  }
+}
+
+template <typename T>
+__global__ void add_parts_kernel(const float* __restrict__ parts, int count, int64_t cols, T* __restrict__ sums) {
+  const int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.f;
+  for (int i = 0; i < count; ++i) s += parts[i * cols + c];
+  sums[c] = from_float<T>(s);
+}
+
+}  // namespace
+
+cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, Operand& dst, uint32_t* row_flags,
+                         uint32_t* col_flags, cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_operand<float, false>(src, src_ld, nullptr, dst, row_flags, col_flags, stream)
+                              : launch_operand<bf16, false>(src, src_ld, nullptr, dst, nullptr, nullptr, stream);
+}
+
+cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, Operand& dst,
+                          uint32_t* row_flags, uint32_t* col_flags, cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_operand<float, true>(g, g_ld, slope, dst, row_flags, col_flags, stream)
+                              : launch_operand<bf16, true>(g, g_ld, slope, dst, nullptr, nullptr, stream);
+}
+
+cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, Operand& dst, cudaStream_t stream) {
+  const int64_t groups = dst.rows * ((dst.cols + 7) / 8);
+  if (groups == 0) return cudaSuccess;
+  const bool vec = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && dst.cols % 8 == 0;
+  unpack_kernel<<<blocks_for(groups), kThreads, 0, stream>>>(codes, vec, exps, const_cast<bf16*>(dst.p), dst.ld,
+                                                            dst.rows, dst.cols);
+  return cudaGetLastError();
+}
+
+int column_parts(int64_t rows) { return static_cast<int>(std::min<int64_t>((rows + 127) / 128, 64)); }
+
+cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream) {
+  const int count = column_parts(src.rows);
+  if (src.cols == 0) return cudaSuccess;
+  if (count > 0) {
+    const int64_t per = (src.rows + count - 1) / count;
+    const dim3 grid(static_cast<unsigned>((src.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
+    column_parts_kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.plane, src.planes, src.rows, src.cols,
+                                                            per, parts);
+  }
+  const unsigned blocks = static_cast<unsigned>((src.cols + 127) / 128);
+  if (out_dtype == DType::kF32)
+    add_parts_kernel<<<blocks, 128, 0, stream>>>(parts, count, src.cols, static_cast<float*>(sums));
+  else
+    add_parts_kernel<<<blocks, 128, 0, stream>>>(parts, count, src.cols, static_cast<bf16*>(sums));
+  return cudaGetLastError();
+}
+
+}  // namespace lin

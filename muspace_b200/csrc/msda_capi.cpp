@@ -14,26 +14,25 @@
 #include <string>
 
 #include "../../include/muspace_msda.h"
+#include "capi_common.h"
 #include "deform_agg.h"
 #include "flash_sca.h"
 #include "msda_kernels.h"
 
-namespace {
+namespace capi {
 
 thread_local std::string g_last_error;
 
-struct Failure {
-  int status;
-};
+}  // namespace capi
 
-[[noreturn]] void fail(int status, const std::string& msg) {
-  g_last_error = msg;
-  throw Failure{status};
-}
+namespace {
 
-void require(bool ok, const std::string& msg) {
-  if (!ok) fail(MSDA_STATUS_INVALID_ARGUMENT, msg);
-}
+using capi::check_launch;
+using capi::DeviceGuard;
+using capi::fail;
+using capi::g_last_error;
+using capi::guarded;
+using capi::require;
 
 std::string dtype_name(DLDataType t) {
   if (t.code == kDLFloat && t.bits == 32) return "float32";
@@ -97,24 +96,6 @@ msda::Dims to_kernel_dims(const msda_dims_t& d) {
                     msda::points_magic(static_cast<int>(d.levels), static_cast<int>(d.points))};
 }
 
-void check_launch(cudaError_t err, const char* what) {
-  if (err != cudaSuccess)
-    fail(MSDA_STATUS_CUDA_ERROR, std::string(what) + ": " + cudaGetErrorName(err) + ": " + cudaGetErrorString(err));
-}
-
-// Makes `device` current for the launch and restores the caller's device.
-struct DeviceGuard {
-  int previous = -1;
-  explicit DeviceGuard(int device) {
-    if (cudaGetDevice(&previous) != cudaSuccess) previous = -1;
-    if (previous != device) check_launch(cudaSetDevice(device), "cudaSetDevice");
-  }
-  ~DeviceGuard() {
-    int now = -1;
-    if (previous >= 0 && cudaGetDevice(&now) == cudaSuccess && now != previous) cudaSetDevice(previous);
-  }
-};
-
 // Shape checks shared by both directions; fills dims from the views the way
 // the reference does (ms_deform_attn_musa.mu:521-522).
 msda_dims_t dims_from_views(const DLTensor* value, const DLTensor* spatial, const DLTensor* start,
@@ -147,20 +128,6 @@ msda::DType storage_dtype(const DLTensor* value) {
   if (same_dtype(value->dtype, kDLFloat, 32)) return msda::DType::kF32;
   if (same_dtype(value->dtype, kDLBfloat, 16)) return msda::DType::kBF16;
   fail(MSDA_STATUS_INVALID_ARGUMENT, "value must be float32 or bfloat16, got " + dtype_name(value->dtype));
-}
-
-template <typename F>
-int guarded(F&& body) {
-  try {
-    body();
-    g_last_error.clear();
-    return MSDA_STATUS_OK;
-  } catch (const Failure& f) {
-    return f.status;
-  } catch (...) {
-    g_last_error = "internal error";
-    return MSDA_STATUS_CUDA_ERROR;
-  }
 }
 
 }  // namespace

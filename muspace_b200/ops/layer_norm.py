@@ -1,0 +1,119 @@
+"""Layer norm over the last dimension, forward and backward.
+
+``y = (x - mean) / sqrt(var + eps) * weight + bias``. The forward reads a row
+once, the backward reads row and gradient once and sums the weight's and the
+bias' gradients on the way, in an order that does not depend on scheduling.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..runtime.native import LayerNormArgs, NativeModule
+from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, report, rows_of
+from .checkpoint8 import BLOCK
+
+OPERATOR_NAME = "layer_norm"
+
+
+def _ptr(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None else tensor.data_ptr()
+
+
+def _forward(module: NativeModule, x, weight, bias, eps: float, keep: str | None):
+    """``(output, statistics, codes, exponents)``; ``keep``: "statistics", "int8" or None."""
+    rows, stride = rows_of(x)
+    count, width = rows.shape
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    statistics = codes = exponents = None
+    mean = rstd = None
+    if keep == "statistics":
+        statistics = torch.empty((2, count), dtype=torch.float32, device=x.device)
+        mean = statistics.data_ptr()
+        rstd = mean + 4 * count
+    elif keep == "int8":
+        codes = torch.empty((count, width), dtype=torch.int8, device=x.device)
+        exponents = torch.empty((count, -(-width // BLOCK)), dtype=torch.uint8, device=x.device)
+    kind = weight if weight is not None else bias
+    args = LayerNormArgs(DTYPE_CODES[x.dtype], DTYPE_CODES[x.dtype if kind is None else kind.dtype], count, width,
+                         stride, 0, eps, rows.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), mean, rstd,
+                         _ptr(codes), _ptr(exponents))
+    module.plain_call("msda_layer_norm_forward")(x.device, args)
+    return out, statistics, codes, exponents
+
+
+class _LayerNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps, checkpoint):
+        module = native_module()
+        out, statistics, codes, exponents = _forward(module, x, weight, bias, eps, checkpoint or "statistics")
+        ctx.save_for_backward(x if checkpoint is None else None, weight, statistics, codes, exponents)
+        ctx.eps = eps
+        ctx.kind = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, statistics, codes, exponents = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        g, g_stride = rows_of(grad)
+        count, width = g.shape
+        dx = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if need_x else None
+        dw, db = (torch.empty(width, dtype=ctx.kind, device=grad.device) if need else None for need in (need_w, need_b))
+        stride, mean, rstd = 0, None, None
+        if x is not None:
+            x, stride = rows_of(x)
+            mean = statistics.data_ptr()
+            rstd = mean + 4 * count
+        args = LayerNormArgs(DTYPE_CODES[grad.dtype], DTYPE_CODES[ctx.kind], count, width, stride, g_stride, ctx.eps,
+                             _ptr(x), _ptr(weight), None, None, mean, rstd, _ptr(codes), _ptr(exponents),
+                             g.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db))
+        native_module().plain_call("msda_layer_norm_backward")(grad.device, args)
+        return dx, dw, db, None, None
+
+
+def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
+               eps: float = 1e-5, *, checkpoint: str | None = None, backend: str = "auto") -> torch.Tensor:
+    """``(input - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (differentiable).
+
+    input ``(..., n)`` in bfloat16, float32, or float16, which runs as float32;
+    weight and bias ``(n,)`` or None, both of input's dtype or both float32.
+    ``checkpoint="int8"`` keeps ``input`` for the backward pass in 8 bits (see
+    ``checkpoint_pack``) and no statistics: the gradients are those at the input
+    that the checkpoint holds.
+    """
+    check_tensor(input, "input")
+    check_checkpoint(checkpoint)
+    if input.dim() == 0:
+        raise ValueError("input must have at least one dimension")
+    given = {name: t for name, t in (("weight", weight), ("bias", bias)) if t is not None}
+    for name, tensor in given.items():
+        if not isinstance(tensor, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor")
+        if tensor.dtype not in (input.dtype, torch.float32):
+            raise TypeError(f"{name} must have the dtype of input ({input.dtype}) or float32")
+        if tuple(tensor.shape) != (input.size(-1),):
+            raise ValueError(f"{name} must have shape ({input.size(-1)},), got {tuple(tensor.shape)}")
+    if len({t.dtype for t in given.values()}) > 1:
+        raise TypeError("weight and bias must have one dtype")
+    module, decision = decide(OPERATOR_NAME, backend, input, given)
+    dtype = input.dtype
+    if dtype == torch.float16:
+        input, weight, bias = (t if t is None else t.float() for t in (input, weight, bias))
+    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
+    tensors = (input, weight, bias)
+    try:
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+            output = _LayerNormFunction.apply(*tensors, float(eps), checkpoint)
+        else:
+            output = _forward(module, *tensors, float(eps), None)[0]
+    except RuntimeError as exc:
+        report(OPERATOR_NAME, backend, decision, "error", str(exc), True)
+        raise
+    report(OPERATOR_NAME, backend, decision, "cuda", decision.reason, True)
+    return output if dtype != torch.float16 else output.to(dtype)
+
+
+__all__ = ["layer_norm"]

@@ -137,6 +137,50 @@ _SIGNATURES: dict[str, tuple[str, ...]] = {
 }
 
 
+class LinearArgs(ctypes.Structure):
+    """``msda_linear_t`` of include/muspace_msda.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("dtype", "activation")]
+        + [(name, ctypes.c_int64) for name in
+           ("rows", "in_features", "out_features", "input_stride", "weight_stride", "residual_stride",
+            "output_stride", "grad_output_stride")]
+        + [(name, ctypes.c_void_p) for name in
+           ("input", "weight", "bias", "residual", "output", "slope", "grad_output", "codes", "exponents",
+            "grad_input", "grad_weight", "grad_bias", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+    )
+
+
+class LayerNormArgs(ctypes.Structure):
+    """``msda_layer_norm_t`` of include/muspace_msda.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("dtype", "weight_dtype")]
+        + [(name, ctypes.c_int64) for name in ("rows", "cols", "input_stride", "grad_output_stride")]
+        + [("eps", ctypes.c_float)]
+        + [(name, ctypes.c_void_p) for name in
+           ("input", "weight", "bias", "output", "mean", "rstd", "codes", "exponents", "grad_output", "grad_input",
+            "grad_weight", "grad_bias", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+    )
+
+
+# the plain-pointer entry points of the layer operators: argument types before the stream
+_PLAIN_SIGNATURES: dict[str, tuple] = {
+    "msda_linear_act_forward": (ctypes.POINTER(LinearArgs),),
+    "msda_linear_act_backward": (ctypes.POINTER(LinearArgs),),
+    "msda_layer_norm_forward": (ctypes.POINTER(LayerNormArgs),),
+    "msda_layer_norm_backward": (ctypes.POINTER(LayerNormArgs),),
+    "msda_checkpoint_pack": (ctypes.c_int, ctypes.c_void_p) + (ctypes.c_int64,) * 3 + (ctypes.c_void_p,) * 2,
+    "msda_checkpoint_unpack": (ctypes.c_int,) + (ctypes.c_void_p,) * 2 + (ctypes.c_int64,) * 2 + (ctypes.c_void_p,),
+}
+
+
+_WORKSPACE_CALLS = {"msda_linear_act_forward_workspace", "msda_linear_act_backward_workspace",
+                    "msda_layer_norm_backward_workspace"}
+
+
 class NativeModule:
     """The loaded library; ``get_function`` mirrors tvm_ffi's Module API."""
 
@@ -148,6 +192,7 @@ class NativeModule:
         lib.msda_version.restype = ctypes.c_char_p
         lib.msda_version.argtypes = []
         self._cache: dict[str, Callable[..., None]] = {}
+        self._plain: dict[str, Callable[..., None]] = {}
 
     def last_error(self) -> str:
         return self.lib.msda_last_error().decode()
@@ -169,6 +214,45 @@ class NativeModule:
             fn = self._tensor_call(name, symbol, signature)
         self._cache[name] = fn
         return fn
+
+    def plain_call(self, name: str) -> Callable[..., None]:
+        """A plain-pointer entry point as a function ``(device, *args)``: it runs on
+        that CUDA device's current stream. A structure whose entry point has a
+        ``*_workspace`` call gets its workspace here, from torch's allocator."""
+        fn = self._plain.get(name)
+        if fn is not None:
+            return fn
+        symbol = getattr(self.lib, name)
+        symbol.restype = ctypes.c_int
+        symbol.argtypes = list(_PLAIN_SIGNATURES[name]) + [ctypes.c_void_p]
+        query = getattr(self.lib, name + "_workspace", None) if name + "_workspace" in _WORKSPACE_CALLS else None
+        if query is not None:
+            query.restype = ctypes.c_int
+            query.argtypes = [_PLAIN_SIGNATURES[name][0], ctypes.POINTER(ctypes.c_size_t)]
+
+        def enqueue(device: torch.device, *args: Any) -> None:
+            if query is not None:
+                size = ctypes.c_size_t()
+                if query(args[0], size) != 0:
+                    raise RuntimeError(f"{name}: {self.last_error()}")
+                if size.value:
+                    # freed after the call as far as torch is concerned: the next owner is on the same stream
+                    workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
+                    args[0].workspace = workspace.data_ptr()
+                    args[0].workspace_bytes = size.value
+            if symbol(*args, torch.cuda.current_stream(device).cuda_stream) != 0:
+                raise RuntimeError(f"{name}: {self.last_error()}")
+
+        def call(device: torch.device, *args: Any) -> None:
+            if device.index == torch.cuda.current_device():
+                enqueue(device, *args)
+            else:
+                with torch.cuda.device(device):
+                    enqueue(device, *args)
+
+        call.__name__ = name
+        self._plain[name] = call
+        return call
 
     def _tensor_call(self, name: str, symbol, signature: tuple[str, ...]) -> Callable[..., None]:
         def call(*args: Any) -> None:
