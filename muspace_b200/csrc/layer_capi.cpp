@@ -196,6 +196,13 @@ int msda_linear_act_backward(const msda_linear_t* args, void* stream) {
   });
 }
 
+int msda_linear_wait_timeouts(unsigned int* count) {
+  return guarded([&] {
+    require(count != nullptr, "count is null");
+    check_launch(lin::wait_timeouts(count), "msda_linear_wait_timeouts");
+  });
+}
+
 int msda_layer_norm_forward(const msda_layer_norm_t* args, void* stream) {
   return guarded([&] {
     check_launch(lnorm::forward(norm_args(args, false), static_cast<cudaStream_t>(stream)),
