@@ -39,8 +39,7 @@ constexpr int kStagingBytes = 32 * 32 * 4;  // a warp's 32 x 32 floats
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
-constexpr int kWaitPolls = 1 << 21;
-constexpr uint32_t kPollNs = 2000;
+constexpr long long kWaitClocks = 4000000000ll;  // about two seconds
 
 template <int BN, int CG>
 struct Shape {
@@ -84,9 +83,9 @@ __device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
-      : "r"(bar), "r"(parity), "r"(kPollNs)
+      : "r"(bar), "r"(parity)
       : "memory");
   return done != 0;
 }
@@ -97,8 +96,10 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& dead) {
   if (try_wait(bar, parity)) return;
   if (dead) return;
-  for (int i = 0; i < kWaitPolls; ++i)
+  const long long start = clock64();
+  do {
     if (try_wait(bar, parity)) return;
+  } while (clock64() - start < kWaitClocks);
   dead = true;
   atomicAdd(&g_wait_timeouts, 1u);
 }
@@ -290,52 +291,85 @@ __device__ __noinline__ float repaired(const Product& pr, uint32_t flags, int64_
   return s;
 }
 
-__device__ __forceinline__ void repair8(const Product& pr, float v[8], int64_t m, int64_t n) {
-  const uint32_t* fa = pr.a_mn ? pr.a.col_flags : pr.a.row_flags;
-  const uint32_t* fb = pr.b_mn ? pr.b.col_flags : pr.b.row_flags;
-  const uint32_t row = fa ? fa[m] : 0u;
+// Flags of rows / columns of the output; null where none can be set.
+__device__ __forceinline__ const uint32_t* flags_m(const Product& pr) {
+  return pr.a_mn ? pr.a.col_flags : pr.a.row_flags;
+}
+__device__ __forceinline__ const uint32_t* flags_n(const Product& pr) {
+  return pr.b_mn ? pr.b.col_flags : pr.b.row_flags;
+}
+
+__device__ __noinline__ void repair8(const Product& pr, uint32_t row, float4& lo, float4& hi, int64_t m, int64_t n) {
+  float* v[8] = {&lo.x, &lo.y, &lo.z, &lo.w, &hi.x, &hi.y, &hi.z, &hi.w};
+  const uint32_t* fb = flags_n(pr);
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     if (n + j >= pr.n) break;
     const uint32_t f = row | (fb ? fb[n + j] : 0u);
-    if (f) v[j] = repaired(pr, f, m, n + j);
+    if (f) *v[j] = repaired(pr, f, m, n + j);
   }
 }
 
 // ---- the kernel ------------------------------------------------------------------------
 
-// 32 rows x 32 columns of a warp, a row per lane, through shared memory and out:
-// a lane takes eight columns of four rows. Writing and reading, the 16-byte
-// units of a row are exchanged by its number, so no two lanes of a quarter warp
-// meet in a bank.
-template <typename T, bool kRepair>
-__device__ __forceinline__ void put32(const Job& j, const Epilogue& e, float* stage, const float v[32], int64_t m0,
-                                      int64_t n0) {
+// A warp's 32 rows x 32 columns go through shared memory: a lane writes a row,
+// and reads eight columns of every eighth row. Both ways the 16-byte units of a
+// row are exchanged by its number, so no two lanes of a quarter warp meet in a
+// bank.
+__device__ __forceinline__ void stage_row(float* stage, const float v[32]) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int q = 0; q < 8; ++q)
     *reinterpret_cast<float4*>(stage + lane * 32 + (q ^ (lane & 7)) * 4) =
         make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  __syncwarp();
+}
+
+// What was staged, through the epilogue. The residual of the next rows is
+// loaded ahead.
+template <typename T, bool kRepair>
+__device__ __forceinline__ void drain(const Job& j, const Epilogue& e, const float* stage, int64_t m0, int64_t n0) {
+  const int lane = threadIdx.x & 31, sub = lane >> 2, q = (lane & 3) * 2;
   const int64_t n = n0 + (lane & 3) * 8;
   if (n < j.pr.n) {
-    float b[8];
-    load_bias8<T>(e, n, j.pr.n, b);
     const bool vec = j.vec && n + 8 <= j.pr.n;
-#pragma unroll
+    float b[8], x[8] = {};
+    uint32_t col = 0;
+    load_bias8<T>(e, n, j.pr.n, b);
+    if (kRepair && flags_n(j.pr)) {
+      for (int c = 0; c < 8 && n + c < j.pr.n; ++c) col |= flags_n(j.pr)[n + c];
+    }
+    const T* extra = static_cast<const T*>(e.extra);
+    const bool ahead = vec && extra;
+    if (ahead && m0 + sub < j.pr.m) load8(extra + (m0 + sub) * e.extra_ld + n, x);
+#pragma unroll 1
     for (int i = 0; i < 4; ++i) {
-      const int row = i * 8 + (lane >> 2), q = (lane & 3) * 2;
+      const int row = i * 8 + sub;
       const int64_t m = m0 + row;
-      const float4 lo = *reinterpret_cast<const float4*>(stage + row * 32 + (q ^ (row & 7)) * 4);
-      const float4 hi = *reinterpret_cast<const float4*>(stage + row * 32 + ((q + 1) ^ (row & 7)) * 4);
-      float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-      if (m < j.pr.m) {
-        if (kRepair) repair8(j.pr, w, m, n);
-        epilogue8<T>(e, w, b, m, n, j.pr.n, vec);
+      if (m >= j.pr.m) break;
+      float4 lo = *reinterpret_cast<const float4*>(stage + row * 32 + (q ^ sub) * 4);
+      float4 hi = *reinterpret_cast<const float4*>(stage + row * 32 + ((q + 1) ^ sub) * 4);
+      if (kRepair) {
+        const uint32_t f = flags_m(j.pr) ? flags_m(j.pr)[m] : 0u;
+        if (f | col) repair8(j.pr, f, lo, hi, m, n);
+      }
+      if (vec) {
+        float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, y[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) y[c] = x[c];
+        if (ahead && i < 3 && m + 8 < j.pr.m) load8(extra + (m + 8) * e.extra_ld + n, x);
+        finish8<T>(e, w, y, b, m, n, j.pr.n, 8, true);
+      } else {
+        finish_some<T>(e, lo, hi, m, n, j.pr.n);
       }
     }
   }
-  __syncwarp();
+}
+
+// The same as a call: where the sums of the whole tile are held in registers,
+// the loop over its parts is unrolled.
+template <typename T, bool kRepair>
+__device__ __noinline__ void drain_apart(const Job& j, const Epilogue& e, const float* stage, int64_t m0, int64_t n0) {
+  drain<T, kRepair>(j, e, stage, m0, n0);
 }
 
 template <int BN, int CG, typename T, bool kF32>
@@ -503,17 +537,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (buf == 0) acc_phase ^= 1;
         }
 #pragma unroll
-        for (int p = 0; p < kParts; ++p)
-          if (n + p * 32 < job.pr.n) {
-            if (job.splits > 1)
-              put32<float, false>(job, e, stage, acc[p], m, n + p * 32);
-            else
-              put32<T, true>(job, e, stage, acc[p], m, n + p * 32);
-          }
+        for (int p = 0; p < kParts; ++p) {
+          stage_row(stage, acc[p]);
+          __syncwarp();
+          if (job.splits > 1)
+            drain_apart<float, false>(job, e, stage, m, n + p * 32);
+          else
+            drain_apart<T, true>(job, e, stage, m, n + p * 32);
+          __syncwarp();
+        }
       } else {
         wait(acc_full(buf), acc_phase, dead);
         fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int p = 0; p < kParts; ++p) {
           const uint32_t at = tmem + lanes + buf * BN + half * (BN / 2) + p * 32;
           uint32_t r[2][16];
@@ -529,7 +565,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
             if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
           }
-          if (n + p * 32 < job.pr.n) put32<T, false>(job, e, stage, v, m, n + p * 32);
+          stage_row(stage, v);
+          __syncwarp();
+          drain<T, false>(job, e, stage, m, n + p * 32);
+          __syncwarp();
         }
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
@@ -561,9 +600,22 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += w[j];
     }
-    load_bias8<T>(pr.epi, n, pr.n, b);
-    if (kF32 && pr.k > 0) repair8(pr, v, m, n);
-    epilogue8<T>(pr.epi, v, b, m, n, pr.n, job.vec && count == 8);
+    float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
+    if (kF32 && pr.k > 0) {
+      const uint32_t row = flags_m(pr) ? flags_m(pr)[m] : 0u;
+      uint32_t any = row;
+      if (flags_n(pr))
+        for (int j = 0; j < count; ++j) any |= flags_n(pr)[n + j];
+      if (any) repair8(pr, row, lo, hi, m, n);
+    }
+    if (job.vec && count == 8) {
+      float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, x[8] = {};
+      load_bias8<T>(pr.epi, n, pr.n, b);
+      if (pr.epi.extra) load8(static_cast<const T*>(pr.epi.extra) + m * pr.epi.extra_ld + n, x);
+      finish8<T>(pr.epi, w, x, b, m, n, pr.n, 8, true);
+    } else {
+      finish_some<T>(pr.epi, lo, hi, m, n, pr.n);
+    }
   }
 }
 
