@@ -47,12 +47,11 @@ Operand fresh(DType dtype, int64_t rows, int64_t cols, int planes, Arena& arena)
   return o;
 }
 
-// Zeroed flag words for a float32 operand's rows and columns.
-cudaError_t fresh_flags(const Operand& o, Arena& arena, uint32_t** rows, uint32_t** cols, cudaStream_t stream) {
-  const size_t bytes = static_cast<size_t>(o.rows + padded(o.cols)) * sizeof(uint32_t);
-  *rows = static_cast<uint32_t*>(arena.take(bytes));
-  *cols = arena.measuring ? nullptr : *rows + o.rows;
-  return arena.measuring || bytes == 0 ? cudaSuccess : cudaMemsetAsync(*rows, 0, bytes, stream);
+// Zeroed flags for a float32 operand.
+cudaError_t add_flags(Operand& o, Arena& arena, cudaStream_t stream) {
+  const size_t bytes = Flags::bytes(o.rows, o.cols);
+  o.flags = static_cast<Flags*>(arena.take(bytes));
+  return arena.measuring ? cudaSuccess : cudaMemsetAsync(o.flags, 0, bytes, stream);
 }
 
 bool direct(DType dtype, const void* p, int64_t cols, int64_t ld) {
@@ -68,9 +67,8 @@ cudaError_t operand_of(DType dtype, const void* p, int64_t rows, int64_t cols, i
     return cudaSuccess;
   }
   *out = fresh(dtype, rows, cols, dtype == DType::kF32 ? 3 : 1, arena);
-  uint32_t *rf = nullptr, *cf = nullptr;
-  if (dtype == DType::kF32) LIN_TRY(fresh_flags(*out, arena, &rf, &cf, stream));
-  return arena.measuring ? cudaSuccess : copy_operand(dtype, p, ld, *out, rf, cf, stream);
+  if (dtype == DType::kF32) LIN_TRY(add_flags(*out, arena, stream));
+  return arena.measuring ? cudaSuccess : copy_operand(dtype, p, ld, *out, stream);
 }
 
 int multiprocessors() {
@@ -88,8 +86,7 @@ int plane_pairs(const Operand& a, const Operand& b) {
 
 cudaError_t run_product(Product& pr, Arena& arena, cudaStream_t stream) {
   const Plan plan = plan_product(pr.m, pr.n, pr.k, plane_pairs(pr.a, pr.b), pr.a_mn || pr.b_mn, multiprocessors());
-  const size_t bytes = partial_bytes(plan, pr.m, pr.n);
-  if (bytes) pr.partial = static_cast<float*>(arena.take(bytes));
+  if (finished_apart(pr, plan)) pr.partial = static_cast<float*>(arena.take(partial_bytes(plan, pr.m, pr.n)));
   return arena.measuring ? cudaSuccess : launch_product(pr, plan, stream);
 }
 
@@ -128,8 +125,7 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
     LIN_TRY(operand_of(a.dtype, a.g, a.rows, a.out, a.g_stride, arena, &dz, stream));
   } else {
     dz = fresh(a.dtype, a.rows, a.out, f32 ? 3 : 1, arena);
-    uint32_t *rf = nullptr, *cf = nullptr;
-    if (f32) LIN_TRY(fresh_flags(dz, arena, &rf, &cf, stream));
+    if (f32) LIN_TRY(add_flags(dz, arena, stream));
     if (recompute) {
       Product pr;
       pr.a = x, pr.b = w;
@@ -142,13 +138,10 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
       pr.epi.out = const_cast<__nv_bfloat16*>(dz.p);
       pr.epi.out_ld = dz.ld;
       pr.epi.out_plane = f32 ? dz.plane : 0;
-      pr.epi.out_row_flags = rf;
-      pr.epi.out_col_flags = cf;
+      pr.epi.out_flags = dz.flags;
       if (a.rows && a.out) LIN_TRY(run_product(pr, arena, stream));
-      dz.row_flags = rf;
-      dz.col_flags = cf;
     } else if (!arena.measuring) {
-      LIN_TRY(scale_operand(a.dtype, a.g, a.g_stride, a.slope, dz, rf, cf, stream));
+      LIN_TRY(scale_operand(a.dtype, a.g, a.g_stride, a.slope, dz, stream));
     }
   }
   if (a.dx && a.rows && a.in) {

@@ -58,9 +58,17 @@ struct Operand {
   const __nv_bfloat16* p = nullptr;
   int64_t rows = 0, cols = 0, ld = 0, plane = 0;  // ld, plane: elements
   int planes = 1;
-  // float32 only: bit 0 = the row / column holds an infinity, bit 1 = a NaN
-  const uint32_t* row_flags = nullptr;
-  const uint32_t* col_flags = nullptr;
+  // float32 only, may be null: what is not finite in it
+  struct Flags* flags = nullptr;
+};
+
+// Bit 0: an infinity, bit 1: a NaN; of the whole matrix, then (behind this
+// header) of its rows and its columns.
+struct Flags {
+  uint32_t any, unused[3];
+  __host__ __device__ uint32_t* rows() { return reinterpret_cast<uint32_t*>(this + 1); }
+  __host__ __device__ uint32_t* cols(int64_t rows_count) { return rows() + rows_count; }
+  static size_t bytes(int64_t rows, int64_t cols) { return sizeof(Flags) + static_cast<size_t>(rows + cols) * 4; }
 };
 
 // What happens to the product's elements on their way out.
@@ -80,8 +88,7 @@ struct Epilogue {
   void* slope = nullptr;  // kFwd, [m, n] contiguous
   // kDz, float32: out is three bfloat16 planes, out_plane elements apart, with flags
   int64_t out_plane = 0;
-  uint32_t* out_row_flags = nullptr;
-  uint32_t* out_col_flags = nullptr;
+  Flags* out_flags = nullptr;
 };
 
 // ---- the product (linear_gemm.cu) --------------------------------------------------
@@ -94,7 +101,7 @@ struct Product {
   int64_t m = 0, n = 0, k = 0;
   DType dtype = DType::kBF16;  // of bias, extra, out
   Epilogue epi;
-  float* partial = nullptr;  // plan.splits > 1: [splits, m, n]
+  float* partial = nullptr;  // where finished apart: [splits, m, partial_ld(n)]
 };
 
 struct Plan {
@@ -105,8 +112,13 @@ struct Plan {
 };
 
 Plan plan_product(int64_t m, int64_t n, int64_t k, int pairs_of_planes, bool any_mn, int sms);
+// Whether the product leaves float32 sums that a second kernel adds up and
+// finishes: ranges of k, and outputs that TMA cannot address (rows off 16-byte
+// boundaries).
+bool finished_apart(const Product& pr, const Plan& p);
+__host__ __device__ inline int64_t partial_ld(int64_t n) { return (n + 3) / 4 * 4; }
 inline size_t partial_bytes(const Plan& p, int64_t m, int64_t n) {
-  return p.splits > 1 ? static_cast<size_t>(p.splits) * m * n * sizeof(float) : 0;
+  return static_cast<size_t>(p.splits) * m * partial_ld(n) * sizeof(float);
 }
 cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t stream);
 cudaError_t wait_timeouts(unsigned int* count);
@@ -114,12 +126,11 @@ cudaError_t wait_timeouts(unsigned int* count);
 // ---- operand layouts and column sums (linear_prep.cu) ------------------------------
 
 // dst planes (1 or 3) of src [rows, cols]; elements of dst beyond cols are not written.
-cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, Operand& dst, uint32_t* row_flags,
-                         uint32_t* col_flags, cudaStream_t stream);
+cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, const Operand& dst, cudaStream_t stream);
 // dst = g * slope
-cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, Operand& dst,
-                          uint32_t* row_flags, uint32_t* col_flags, cudaStream_t stream);
-cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, Operand& dst, cudaStream_t stream);
+cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
+                          cudaStream_t stream);
+cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream);
 // sums[c] = sum over rows of src (its planes added up); parts: [column_parts(rows), cols] floats
 int column_parts(int64_t rows);
 cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream);

@@ -5,9 +5,14 @@
 // a producer thread copies tiles of A and B into a ring of shared-memory stages
 // (TMA, 128-byte swizzle), one thread issues tcgen05.mma on them into one of
 // two accumulators in tensor memory, and eight warps carry the other
-// accumulator through the epilogue meanwhile: tensor memory -> registers ->
-// shared memory, turned so that neighbouring lanes hold neighbouring columns ->
-// bias, activation, residual -> global memory.
+// accumulator through the epilogue meanwhile. A lane holds a row there, 16
+// columns at a time: tensor memory -> registers, bias, activation, residual ->
+// shared memory -> global memory by TMA, which also brings the residual. So
+// global memory sees whole rows of 128 bytes, and the code has no addresses or
+// bounds. (First form: turned through shared memory in float32 and stored by
+// the lanes, 8 columns each; eight times the instructions, and with its loops
+// unrolled two thirds of the time went into fetching them. Value projection,
+// 184950 x 256 x 256: 360 us unrolled, 74 rolled.)
 //
 // Either operand may be stored along k or across it: the forward reads both
 // along k, dx = dz W reads W across it, dW = dz^T x both. Nothing is transposed
@@ -35,8 +40,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kProducer = kEpiWarps, kIssuer = kEpiWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageA = kTileM * kBlockK * 2;
-constexpr int kStagingBytes = 32 * 32 * 4;  // a warp's 32 x 32 floats
-constexpr int kRingBytes = 192 * 1024;
+constexpr int kBoxBytes = 32 * 128;  // a box of the epilogue: 32 rows of 128 bytes
+constexpr int kStagingBytes = 2 * kBoxBytes;  // of a warp
+constexpr int kRingBytes = 160 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
 constexpr long long kWaitClocks = 4000000000ll;  // about two seconds
@@ -47,7 +53,7 @@ struct Shape {
   static constexpr int kStageB = kRowsB * kBlockK * 2;
   static constexpr int kStage = kStageA + kStageB;
   static constexpr int kStages = kRingBytes / kStage;
-  static constexpr int kBarriers = 2 * kStages + 4;
+  static constexpr int kBarriers = 2 * kStages + 4 + 2 * kEpiWarps;
   // stages, the warps' staging, barriers, the tensor-memory address; and room to start on 1024 bytes
   static constexpr int kSmem = kStages * kStage + kEpiWarps * kStagingBytes + kBarriers * 8 + 16 + 1024;
   static constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;
@@ -57,11 +63,12 @@ struct Shape {
 // What a launch needs beside the tensor maps.
 struct Job {
   Product pr;
-  int64_t tiles_m, tiles_n;
+  uint32_t tiles_m, tiles_n;
   int splits, kblocks, kblocks_per_split, pairs;
   int box_a, box_b;  // rows of the boxes along k
   int device;
-  bool vec;          // rows of bias, extra, out and slope start on 16-byte boundaries
+  bool apart;        // the epilogue leaves sums in pr.partial
+  bool vec;          // finishing: rows of extra, out and slope start on 16-byte boundaries
 };
 
 __device__ unsigned int g_wait_timeouts;
@@ -205,6 +212,17 @@ __device__ __forceinline__ void tmem_wait(uint32_t r[16]) {
                : "memory");
 }
 
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const float v[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::"f"(v[0]),
+      "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "r"(addr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 template <int CG>
 __device__ __forceinline__ void block_or_pair_sync() {
   if (CG == 1) {
@@ -239,20 +257,21 @@ __device__ __forceinline__ uint32_t instruction(int m, int n, bool a_across, boo
 // ---- work ------------------------------------------------------------------------------
 
 struct Item {
-  int64_t m, n;  // first row and column
+  int m, n;  // first row and column
   int split, kb0, kb1;
 };
 
 template <int BN, int CG>
-__device__ __forceinline__ Item item_of(const Job& j, int64_t i) {
-  const int64_t tiles = j.tiles_m * j.tiles_n;
+__device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
+  const uint32_t tiles = j.tiles_m * j.tiles_n;
   Item t;
   t.split = static_cast<int>(i / tiles);
-  const int64_t at = i - t.split * tiles, per_group = kGroupM * j.tiles_n;
-  const int64_t group = at / per_group, first = group * kGroupM;
-  const int64_t rows = min(static_cast<int64_t>(kGroupM), j.tiles_m - first), local = at - group * per_group;
-  t.m = (first + local % rows) * (kTileM * CG);
-  t.n = local / rows * BN;
+  const uint32_t at = i - t.split * tiles, per_group = kGroupM * j.tiles_n;
+  const uint32_t group = at / per_group, first = group * kGroupM;
+  const uint32_t rows = min(static_cast<uint32_t>(kGroupM), j.tiles_m - first), local = at - group * per_group;
+  const uint32_t col = local / rows;
+  t.m = static_cast<int>((first + local - col * rows) * (kTileM * CG));
+  t.n = static_cast<int>(col * BN);
   t.kb0 = t.split * j.kblocks_per_split;
   t.kb1 = min(j.kblocks, t.kb0 + j.kblocks_per_split);
   return t;
@@ -291,97 +310,171 @@ __device__ __noinline__ float repaired(const Product& pr, uint32_t flags, int64_
   return s;
 }
 
-// Flags of rows / columns of the output; null where none can be set.
-__device__ __forceinline__ const uint32_t* flags_m(const Product& pr) {
-  return pr.a_mn ? pr.a.col_flags : pr.a.row_flags;
+// Flags of output rows / columns: of A's rows or columns, of B's; null where none can be set.
+__device__ __forceinline__ const uint32_t* flags_of(const Operand& o, bool across) {
+  return o.flags == nullptr ? nullptr : across ? o.flags->cols(o.rows) : o.flags->rows();
 }
-__device__ __forceinline__ const uint32_t* flags_n(const Product& pr) {
-  return pr.b_mn ? pr.b.col_flags : pr.b.row_flags;
+__device__ __forceinline__ bool some_flag(const Product& pr) {
+  return (pr.a.flags && pr.a.flags->any) || (pr.b.flags && pr.b.flags->any);
 }
 
-__device__ __noinline__ void repair8(const Product& pr, uint32_t row, float4& lo, float4& hi, int64_t m, int64_t n) {
-  float* v[8] = {&lo.x, &lo.y, &lo.z, &lo.w, &hi.x, &hi.y, &hi.z, &hi.w};
-  const uint32_t* fb = flags_n(pr);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (n + j >= pr.n) break;
+// Outputs [n, n + N) of row m.
+template <int N>
+__device__ __noinline__ void repair(const Product& pr, float* v, int64_t m, int64_t n) {
+  const uint32_t *fa = flags_of(pr.a, pr.a_mn), *fb = flags_of(pr.b, pr.b_mn);
+  if (m >= pr.m) return;
+  const uint32_t row = fa ? fa[m] : 0u;
+  for (int j = 0; j < N && n + j < pr.n; ++j) {
     const uint32_t f = row | (fb ? fb[n + j] : 0u);
-    if (f) *v[j] = repaired(pr, f, m, n + j);
+    if (f) v[j] = repaired(pr, f, m, n + j);
   }
+}
+
+// ---- the epilogue ------------------------------------------------------------------------
+
+// A warp's box in shared memory: 32 rows of 128 or 64 bytes, whose 16-byte units
+// are exchanged by the row's number as TMA's swizzle has it; eight neighbouring
+// rows' units at one place then lie in different banks.
+template <int kRowBytes>
+__device__ __forceinline__ uint32_t unit_at(uint32_t box, int row, int unit) {
+  return kRowBytes == 128 ? box + row * 128 + ((unit ^ (row & 7)) << 4)
+                          : box + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+}
+
+__device__ __forceinline__ void put_unit(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ void get_unit(uint32_t addr, uint32_t v[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+               : "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 values of a row into the box from column `col` on.
+template <int kRowBytes>
+__device__ __forceinline__ void put16(uint32_t box, int row, int col, const float v[16], bf16) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 8 + u), pack2(v[8 * u], v[8 * u + 1]), pack2(v[8 * u + 2], v[8 * u + 3]),
+             pack2(v[8 * u + 4], v[8 * u + 5]), pack2(v[8 * u + 6], v[8 * u + 7]));
+}
+template <int kRowBytes>
+__device__ __forceinline__ void put16(uint32_t box, int row, int col, const float v[16], __half) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 8 + u), pack_half2(v[8 * u], v[8 * u + 1]),
+             pack_half2(v[8 * u + 2], v[8 * u + 3]), pack_half2(v[8 * u + 4], v[8 * u + 5]),
+             pack_half2(v[8 * u + 6], v[8 * u + 7]));
+}
+template <int kRowBytes>
+__device__ __forceinline__ void put16(uint32_t box, int row, int col, const float v[16], float) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 4 + u), __float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]),
+             __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3]));
+}
+
+template <int kRowBytes>
+__device__ __forceinline__ void get16(uint32_t box, int row, int col, float v[16], bf16) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint32_t w[4];
+    get_unit(unit_at<kRowBytes>(box, row, col / 8 + u), w);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      v[8 * u + 2 * x] = __uint_as_float(w[x] << 16);
+      v[8 * u + 2 * x + 1] = __uint_as_float(w[x] & 0xffff0000u);
+    }
+  }
+}
+template <int kRowBytes>
+__device__ __forceinline__ void get16(uint32_t box, int row, int col, float v[16], float) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    uint32_t w[4];
+    get_unit(unit_at<kRowBytes>(box, row, col / 4 + u), w);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) v[4 * u + x] = __uint_as_float(w[x]);
+  }
+}
+
+// Bias of columns [n, n + 16): the same for all lanes.
+template <typename T>
+__device__ __forceinline__ void add_bias16(const void* bias, int n, int cols, float v[16]) {
+  const T* p = static_cast<const T*>(bias) + n;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && n + 16 <= cols) {
+    float b[16];
+    load8(p, b);
+    load8(p + 8, b + 8);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) v[j] += b[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (n + j < cols) v[j] += to_float(p[j]);
+  }
+}
+
+// Marks what is not finite among 16 outputs of row m.
+__device__ __forceinline__ void mark16(Flags* flags, const Product& pr, const float v[16], int64_t m, int64_t n) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) any |= flag_of(v[j]);
+  if (any == 0 || m >= pr.m) return;
+  any = 0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const uint32_t f = n + j < pr.n ? flag_of(v[j]) : 0u;
+    if (f) atomicOr(flags->cols(pr.m) + n + j, f);
+    any |= f;
+  }
+  if (any) {
+    atomicOr(flags->rows() + m, any);
+    atomicOr(&flags->any, any);
+  }
+}
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bytes,
+                                         uint32_t bar) {
+  expect_bytes(bar, bytes);
+  copy_box<1>(dst, map, x, y, 0, bar);
+}
+
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
+               "r"(y), "r"(z), "r"(src)
+               : "memory");
+}
+
+__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+
+// At most N groups of stores still read their boxes.
+template <int N>
+__device__ __forceinline__ void stores_read() {
+  asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
 
 // ---- the kernel ------------------------------------------------------------------------
 
-// A warp's 32 rows x 32 columns go through shared memory: a lane writes a row,
-// and reads eight columns of every eighth row. Both ways the 16-byte units of a
-// row are exchanged by its number, so no two lanes of a quarter warp meet in a
-// bank.
-__device__ __forceinline__ void stage_row(float* stage, const float v[32]) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    *reinterpret_cast<float4*>(stage + lane * 32 + (q ^ (lane & 7)) * 4) =
-        make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-}
-
-// What was staged, through the epilogue. The residual of the next rows is
-// loaded ahead.
-template <typename T, bool kRepair>
-__device__ __forceinline__ void drain(const Job& j, const Epilogue& e, const float* stage, int64_t m0, int64_t n0) {
-  const int lane = threadIdx.x & 31, sub = lane >> 2, q = (lane & 3) * 2;
-  const int64_t n = n0 + (lane & 3) * 8;
-  if (n < j.pr.n) {
-    const bool vec = j.vec && n + 8 <= j.pr.n;
-    float b[8], x[8] = {};
-    uint32_t col = 0;
-    load_bias8<T>(e, n, j.pr.n, b);
-    if (kRepair && flags_n(j.pr)) {
-      for (int c = 0; c < 8 && n + c < j.pr.n; ++c) col |= flags_n(j.pr)[n + c];
-    }
-    const T* extra = static_cast<const T*>(e.extra);
-    const bool ahead = vec && extra;
-    if (ahead && m0 + sub < j.pr.m) load8(extra + (m0 + sub) * e.extra_ld + n, x);
-#pragma unroll 1
-    for (int i = 0; i < 4; ++i) {
-      const int row = i * 8 + sub;
-      const int64_t m = m0 + row;
-      if (m >= j.pr.m) break;
-      float4 lo = *reinterpret_cast<const float4*>(stage + row * 32 + (q ^ sub) * 4);
-      float4 hi = *reinterpret_cast<const float4*>(stage + row * 32 + ((q + 1) ^ sub) * 4);
-      if (kRepair) {
-        const uint32_t f = flags_m(j.pr) ? flags_m(j.pr)[m] : 0u;
-        if (f | col) repair8(j.pr, f, lo, hi, m, n);
-      }
-      if (vec) {
-        float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, y[8];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) y[c] = x[c];
-        if (ahead && i < 3 && m + 8 < j.pr.m) load8(extra + (m + 8) * e.extra_ld + n, x);
-        finish8<T>(e, w, y, b, m, n, j.pr.n, 8, true);
-      } else {
-        finish_some<T>(e, lo, hi, m, n, j.pr.n);
-      }
-    }
-  }
-}
-
-// The same as a call: where the sums of the whole tile are held in registers,
-// the loop over its parts is unrolled.
-template <typename T, bool kRepair>
-__device__ __noinline__ void drain_apart(const Job& j, const Epilogue& e, const float* stage, int64_t m0, int64_t n0) {
-  drain<T, kRepair>(j, e, stage, m0, n0);
-}
+struct Maps {
+  CUtensorMap a, b, out, extra, slope;
+};
 
 template <int BN, int CG, typename T, bool kF32>
 __global__ void __launch_bounds__(kThreads, 1)
-    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ Job job) {
+    product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Job job) {
   using S = Shape<BN, CG>;
   extern __shared__ uint8_t raw[];
-  uint8_t* base = raw + ((1024 - (smem_addr(raw) & 1023)) & 1023);
-  const uint32_t ring = smem_addr(base);
-  float* staging = reinterpret_cast<float*>(base + S::kStages * S::kStage);
-  const uint32_t bars = ring + S::kStages * S::kStage + kEpiWarps * kStagingBytes;
+  const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
+  const uint32_t boxes_base = ring + S::kStages * S::kStage;
+  const uint32_t bars = boxes_base + kEpiWarps * kStagingBytes;
   const uint32_t tmem_slot = bars + S::kBarriers * 8;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
@@ -401,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       barrier_init(acc_full(b), 1);
       barrier_init(acc_empty(b), kEpiWarps * CG);
     }
+    for (int x = 0; x < 2 * kEpiWarps; ++x) barrier_init(bars + 8 * (2 * S::kStages + 4 + x), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssuer) tmem_alloc<CG>(tmem_slot, S::kColumns);
@@ -410,26 +504,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
 
-  const int64_t items = job.tiles_m * job.tiles_n * job.splits;
-  const int64_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
+  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
   const int chunk = kF32 ? kPromote : job.kblocks;
   bool dead = false;
 
   if (warp == kProducer && lane == 0) {
     int s = 0;
     uint32_t phase = 0;
-    for (int64_t i = first; i < items; i += step) {
+    const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
+    for (uint32_t i = first; i < items; i += step) {
       const Item t = item_of<BN, CG>(job, i);
       // boxes that hold rows of the tile; what a skipped box leaves in its place reaches no row or column that is kept
-      const auto boxes = [](int64_t have, int most) {
-        return static_cast<int>(have <= 0 ? 0 : have >= most * 64ll ? most : (have + 63) / 64);
+      const auto boxes = [](int have, int most) { return have <= 0 ? 0 : min(most, (have - 1) / 64 + 1); };
+      const auto bytes_of = [&](int ma, int nb) {
+        return (job.pr.a_mn ? boxes(rows_m - ma, kTileM / 64) * 8192 : job.box_a * 128) +
+               (job.pr.b_mn ? boxes(rows_n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128);
       };
-      const auto bytes_of = [&](int64_t ma, int64_t nb) {
-        return (job.pr.a_mn ? boxes(job.pr.m - ma, kTileM / 64) * 8192 : job.box_a * 128) +
-               (job.pr.b_mn ? boxes(job.pr.n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128);
-      };
-      const int64_t ma = t.m + rank * kTileM, nb = t.n + rank * S::kRowsB;
-      const int boxes_a = boxes(job.pr.m - ma, kTileM / 64), boxes_b = boxes(job.pr.n - nb, S::kRowsB / 64);
+      const int ma = t.m + rank * kTileM, nb = t.n + rank * S::kRowsB;
+      const int boxes_a = boxes(rows_m - ma, kTileM / 64), boxes_b = boxes(rows_n - nb, S::kRowsB / 64);
       uint32_t bytes = bytes_of(t.m, t.n);
       if (CG == 2) bytes += bytes_of(t.m + kTileM, t.n + S::kRowsB);
       for (int c = t.kb0; c < t.kb1; c += chunk) {
@@ -444,16 +537,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t a = ring + s * S::kStage, b = a + kStageA;
             const int k = kb * kBlockK;
             if (job.pr.a_mn) {
-              for (int x = 0; x < boxes_a; ++x)
-                copy_box<CG>(a + x * 8192, &map_a, static_cast<int>(ma) + x * 64, k, pa, bar);
+              for (int x = 0; x < boxes_a; ++x) copy_box<CG>(a + x * 8192, &maps.a, ma + x * 64, k, pa, bar);
             } else {
-              copy_box<CG>(a, &map_a, k, static_cast<int>(ma), pa, bar);
+              copy_box<CG>(a, &maps.a, k, ma, pa, bar);
             }
             if (job.pr.b_mn) {
-              for (int x = 0; x < boxes_b; ++x)
-                copy_box<CG>(b + x * 8192, &map_b, static_cast<int>(nb) + x * 64, k, pb, bar);
+              for (int x = 0; x < boxes_b; ++x) copy_box<CG>(b + x * 8192, &maps.b, nb + x * 64, k, pb, bar);
             } else {
-              copy_box<CG>(b, &map_b, k, static_cast<int>(nb), pb, bar);
+              copy_box<CG>(b, &maps.b, k, nb, pb, bar);
             }
             if (++s == S::kStages) s = 0, phase ^= 1;
           }
@@ -471,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t step_a = k_step(job.pr.a_mn) >> 4, step_b = k_step(job.pr.b_mn) >> 4;
     int s = 0, buf = 0;
     uint32_t phase = 0, acc_phase = 0;
-    for (int64_t i = first; i < items; i += step) {
+    for (uint32_t i = first; i < items; i += step) {
       const Item t = item_of<BN, CG>(job, i);
       for (int c = t.kb0; c < t.kb1; c += chunk) {
         const int steps = (min(c + chunk, t.kb1) - c) * job.pairs;
@@ -498,82 +589,182 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < kEpiWarps) {
-    Epilogue e = job.pr.epi;
+    constexpr int kHalf = BN / 2;  // columns of a warp
+    constexpr int kBoxCols = 128 / sizeof(T) < kHalf ? 128 / sizeof(T) : kHalf;
+    constexpr int kRowBytes = kBoxCols * sizeof(T);
+    constexpr int kParts = kHalf / kBoxCols;
     const int quad = warp & 3, half = warp >> 2;
-    float* stage = staging + warp * (kStagingBytes / 4);
+    const uint32_t boxes = boxes_base + warp * kStagingBytes;
+    const uint32_t arrived = bars + 8 * (2 * S::kStages + 4 + 2 * warp);  // the residual's boxes
+    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
+    const Epilogue& e = job.pr.epi;
+    const int mode = job.apart ? Epilogue::kStore : e.mode;
+    const bool extra = mode != Epilogue::kStore && e.extra != nullptr;
+    const bool slope = mode == Epilogue::kFwd && e.slope != nullptr;
+    const bool planes = sizeof(T) == 4 && mode == Epilogue::kDz;
+    const bool one_box = slope || planes;  // the second box holds the second output
+    const bool repairs = kF32 && !job.apart && some_flag(job.pr);
+    const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
+    const auto col_of = [&](const Item& t, int p) { return t.n + half * kHalf + p * kBoxCols; };
     int buf = 0;
-    uint32_t acc_phase = 0;
-    constexpr int kParts = BN / 64;  // of 32 columns
-    for (int64_t i = first; i < items; i += step) {
-      const Item t = item_of<BN, CG>(job, i);
-      if (job.splits > 1) {
-        e = Epilogue();
-        e.out = job.pr.partial + t.split * job.pr.m * job.pr.n;
-        e.out_ld = job.pr.n;
-      }
-      const int64_t m = t.m + rank * kTileM + quad * 32, n = t.n + half * (BN / 2);
-      const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+    uint32_t acc_phase = 0, box = 0, extra_phase = 0;
+    Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
+    if (extra && !one_box && first < items && lane == 0) 
+      load_box(boxes, &maps.extra, col_of(t, 0), row_of(t), 32 * kRowBytes, arrived);
+    for (uint32_t i = first; i < items; i += step) {
+      const Item next = i + step < items ? item_of<BN, CG>(job, i + step) : Item{};
+      const int m = row_of(t);
       if (kF32) {
-        float acc[kParts][32] = {};
+        float acc[kHalf / 16][16] = {};
+        int last = 0;
         for (int c = t.kb0; c < t.kb1; c += chunk) {
           wait(acc_full(buf), acc_phase, dead);
           fence_after();
+          const bool more = c + chunk < t.kb1;
+          last = buf;
 #pragma unroll
-          for (int p = 0; p < kParts; ++p) {
-            const uint32_t at = tmem + lanes + buf * BN + half * (BN / 2) + p * 32;
+          for (int q = 0; q < kHalf / 16; ++q) {
+            const uint32_t at = tmem + lanes + buf * BN + half * kHalf + q * 16;
+            uint32_t r[16];
+            tmem_load16(at, r);
+            tmem_wait(r);
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t r[16];
-              tmem_load16(at + q * 16, r);
-              tmem_wait(r);
-#pragma unroll
-              for (int x = 0; x < 16; ++x) acc[p][q * 16 + x] += __uint_as_float(r[x]);
-            }
+            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
+            if (!more) tmem_store16(at, acc[q]);
           }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
-          buf ^= 1;
-          if (buf == 0) acc_phase ^= 1;
-        }
-#pragma unroll
-        for (int p = 0; p < kParts; ++p) {
-          stage_row(stage, acc[p]);
-          __syncwarp();
-          if (job.splits > 1)
-            drain_apart<float, false>(job, e, stage, m, n + p * 32);
-          else
-            drain_apart<T, true>(job, e, stage, m, n + p * 32);
-          __syncwarp();
-        }
-      } else {
-        wait(acc_full(buf), acc_phase, dead);
-        fence_after();
-#pragma unroll 1
-        for (int p = 0; p < kParts; ++p) {
-          const uint32_t at = tmem + lanes + buf * BN + half * (BN / 2) + p * 32;
-          uint32_t r[2][16];
-          tmem_load16(at, r[0]);
-          tmem_load16(at + 16, r[1]);
-          tmem_wait(r[0]);
-          tmem_wait(r[1]);
-          float v[32];
-#pragma unroll
-          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(r[x / 16][x % 16]);
-          if (p + 1 == kParts) {
+          if (more) {
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
           }
-          stage_row(stage, v);
-          __syncwarp();
-          drain<T, false>(job, e, stage, m, n + p * 32);
-          __syncwarp();
+          buf ^= 1;
+          if (buf == 0) acc_phase ^= 1;
         }
-        buf ^= 1;
-        if (buf == 0) acc_phase ^= 1;
+        tmem_stored();
+        buf = last;
+        if (buf == 1) acc_phase ^= 1;
+      } else {
+        wait(acc_full(buf), acc_phase, dead);
+        fence_after();
       }
+      const uint32_t acc_at = tmem + lanes + buf * BN + half * kHalf;
+#pragma unroll 1
+      for (int p = 0; p < kParts; ++p) {
+        const int n = col_of(t, p);
+        const uint32_t here = one_box ? boxes : boxes + (box & 1) * kBoxBytes;
+        if (lane == 0) {
+          if (one_box || extra)
+            stores_read<0>();
+          else
+            stores_read<1>();
+          if (extra) {
+            if (one_box) {
+              load_box(boxes, &maps.extra, n, m, 32 * kRowBytes, arrived);
+            } else {
+              const uint32_t other = (box + 1) & 1;
+              const bool same = p + 1 < kParts;
+              if (same || i + step < items)
+                load_box(boxes + other * kBoxBytes, &maps.extra, same ? col_of(t, p + 1) : col_of(next, 0),
+                         same ? m : row_of(next), 32 * kRowBytes, arrived + 8 * other);
+            }
+          }
+        }
+        __syncwarp();
+        if (extra) {
+          const uint32_t which = one_box ? 0 : box & 1;
+          wait(arrived + 8 * which, (extra_phase >> which) & 1, dead);
+          extra_phase ^= 1u << which;
+        }
+        uint32_t held[8];
+#pragma unroll 1
+        for (int c = 0; c < kBoxCols; c += 16) {
+          uint32_t r[16];
+          tmem_load16(acc_at + p * kBoxCols + c, r);
+          float x[16], v[16], s[16];
+          if (extra) get16<kRowBytes>(here, lane, c, x, T());
+          tmem_wait(r);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+          if (repairs) {
+            float w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = v[j];
+            repair<16>(job.pr, w, m + lane, n + c);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = w[j];
+          }
+          if (mode != Epilogue::kStore) {
+            if (e.bias) add_bias16<T>(e.bias, n + c, rows_n, v);
+            activate<sizeof(T) == 2, 16>(e.act, v, s);
+            if (mode == Epilogue::kFwd) {
+              if (extra) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] += x[j];
+              }
+              if (slope) put16<kRowBytes>(boxes + kBoxBytes, lane, c, s, typename SlopeOf<T>::type());
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
+            }
+          }
+          if (sizeof(T) == 4 && planes) {
+            // hi and mid into the second box; lo into the first, once all lanes have read the gradient there
+            uint32_t part[3][8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              bf16 a[3], b[3];
+              split3(v[2 * j], a[0], a[1], a[2]);
+              split3(v[2 * j + 1], b[0], b[1], b[2]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+              for (int u = 0; u < 2; ++u)
+                put_unit(unit_at<64>(boxes + kBoxBytes + k * 2048, lane, c / 8 + u), part[k][4 * u], part[k][4 * u + 1],
+                         part[k][4 * u + 2], part[k][4 * u + 3]);
+            if (c > 0) {
+              __syncwarp();
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                put_unit(unit_at<64>(here, lane, u), held[4 * u], held[4 * u + 1], held[4 * u + 2], held[4 * u + 3]);
+                put_unit(unit_at<64>(here, lane, 2 + u), part[2][4 * u], part[2][4 * u + 1], part[2][4 * u + 2],
+                         part[2][4 * u + 3]);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) held[j] = part[2][j];
+            mark16(e.out_flags, job.pr, v, m + lane, n + c);
+          }
+          if (!planes) put16<kRowBytes>(here, lane, c, v, T());
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
+          if (m < rows_m && n < rows_n) {
+            if (sizeof(T) == 4 && planes) {
+              store_box(&maps.out, n, m, 0, boxes + kBoxBytes);
+              store_box(&maps.out, n, m, 1, boxes + kBoxBytes + 2048);
+              store_box(&maps.out, n, m, 2, boxes);
+            } else {
+              store_box(&maps.out, n, m, job.apart ? t.split : 0, here);
+            }
+            if (slope) store_box(&maps.slope, n, m, 0, boxes + kBoxBytes);
+          }
+          stores_commit();
+        }
+        ++box;
+      }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
+      buf ^= 1;
+      if (buf == 0) acc_phase ^= 1;
+      t = next;
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   fence_before();
@@ -588,33 +779,35 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, bool kF32>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job job) {
   const Product& pr = job.pr;
-  const int64_t per_row = (pr.n + 7) / 8, total = pr.m * per_row;
-  const bool part_vec = pr.n % 4 == 0;
+  const int64_t per_row = (pr.n + 7) / 8, total = pr.m * per_row, ld = partial_ld(pr.n);
+  const bool repairs = kF32 && pr.k > 0 && some_flag(pr);
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t m = i / per_row, n = (i - m * per_row) * 8;
-    const int count = static_cast<int>(pr.n - n < 8 ? pr.n - n : 8);
-    float v[8] = {}, b[8];
+    const bool whole8 = n + 8 <= pr.n;
+    float v[8] = {};
     for (int s = 0; s < job.splits; ++s) {
+      const float* p = pr.partial + (s * pr.m + m) * ld + n;
       float w[8];
-      load_some(pr.partial + (s * pr.m + m) * pr.n + n, count, part_vec && count == 8, w);
+      load_some(p, static_cast<int>(pr.n - n), whole8, w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += w[j];
     }
-    float4 lo = make_float4(v[0], v[1], v[2], v[3]), hi = make_float4(v[4], v[5], v[6], v[7]);
-    if (kF32 && pr.k > 0) {
-      const uint32_t row = flags_m(pr) ? flags_m(pr)[m] : 0u;
-      uint32_t any = row;
-      if (flags_n(pr))
-        for (int j = 0; j < count; ++j) any |= flags_n(pr)[n + j];
-      if (any) repair8(pr, row, lo, hi, m, n);
+    if (repairs) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = v[j];
+      repair<8>(pr, w, m, n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = w[j];
     }
-    if (job.vec && count == 8) {
-      float w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, x[8] = {};
-      load_bias8<T>(pr.epi, n, pr.n, b);
+    if (job.vec && whole8) {
+      float x[8] = {}, b[8] = {};
+      if (pr.epi.bias) load_some(static_cast<const T*>(pr.epi.bias) + n, 8, false, b);
       if (pr.epi.extra) load8(static_cast<const T*>(pr.epi.extra) + m * pr.epi.extra_ld + n, x);
-      finish8<T>(pr.epi, w, x, b, m, n, pr.n, 8, true);
+      finish8<T>(pr.epi, v, x, b, m, n, pr.m, pr.n, 8, true);
     } else {
-      finish_some<T>(pr.epi, lo, hi, m, n, pr.n);
+      finish_some<T>(pr.epi, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), m, n, pr.m,
+                     pr.n);
     }
   }
 }
@@ -637,36 +830,67 @@ EncodeTiledFn encoder() {
   return fn;
 }
 
-// Boxes of 64 columns (128 bytes, swizzled) and `rows` rows of one plane;
-// columns start at multiples of 64, and what lies outside reads as zero.
-bool make_map(CUtensorMap* map, const Operand& o, int rows) {
+// Boxes of `box_cols` columns and `box_rows` rows of one plane, swizzled over
+// the box's rows of 128 or 64 bytes; what lies outside the matrix reads as zero
+// and is not written.
+bool make_map(CUtensorMap* map, CUtensorMapDataType type, const void* p, int64_t cols, int64_t rows, int64_t planes,
+              int64_t ld_bytes, int64_t plane_bytes, int box_cols, int box_rows, int row_bytes) {
   const EncodeTiledFn encode = encoder();
   if (!encode) return false;
-  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(o.cols), static_cast<cuuint64_t>(o.rows),
-                              static_cast<cuuint64_t>(o.planes)};
-  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(o.ld) * 2,
-                                 static_cast<cuuint64_t>(o.planes > 1 ? o.plane : o.ld) * 2};
-  const cuuint32_t box[3] = {kBlockK, static_cast<cuuint32_t>(rows), 1};
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_bytes),
+                                 static_cast<cuuint64_t>(planes > 1 ? plane_bytes : ld_bytes)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   const cuuint32_t unit[3] = {1, 1, 1};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(o.p), dims, strides, box, unit,
-                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode(map, type, 3, const_cast<void*>(p), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool operand_map(CUtensorMap* map, const Operand& o, int rows) {
+  return make_map(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, o.p, o.cols, o.rows, o.planes, o.ld * 2, o.plane * 2, kBlockK,
+                  rows, 128);
+}
+
+// The maps of the epilogue's outputs and of the residual or gradient.
+bool epilogue_maps(Maps& maps, const Product& pr, const Plan& plan, bool apart) {
+  const Epilogue& e = pr.epi;
+  const auto f32 = CU_TENSOR_MAP_DATA_TYPE_FLOAT32, b16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  if (apart)
+    return make_map(&maps.out, f32, pr.partial, pr.n, pr.m, plan.splits, partial_ld(pr.n) * 4,
+                    pr.m * partial_ld(pr.n) * 4, 32, 32, 128);
+  const bool wide = pr.dtype == DType::kF32;
+  const int64_t size = wide ? 4 : 2;
+  const int row_bytes = std::min<int>(128, plan.bn / 2 * static_cast<int>(size));
+  const int cols = row_bytes / static_cast<int>(size);
+  bool ok = true;
+  if (e.mode == Epilogue::kDz && wide)
+    ok = make_map(&maps.out, b16, e.out, pr.n, pr.m, 3, e.out_ld * 2, e.out_plane * 2, 32, 32, 64);
+  else
+    ok = make_map(&maps.out, wide ? f32 : b16, e.out, pr.n, pr.m, 1, e.out_ld * size, 0, cols, 32, row_bytes);
+  if (ok && e.mode != Epilogue::kStore && e.extra)
+    ok = make_map(&maps.extra, wide ? f32 : b16, e.extra, pr.n, pr.m, 1, e.extra_ld * size, 0, cols, 32, row_bytes);
+  if (ok && e.mode == Epilogue::kFwd && e.slope)
+    ok = make_map(&maps.slope, wide ? f32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, e.slope, pr.n, pr.m, 1, pr.n * size, 0,
+                  cols, 32, row_bytes);
+  return ok;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Whether eight columns at a multiple of eight are one aligned vector everywhere.
+// Whether rows of extra, out and slope are what TMA and vectors of eight columns can address.
 bool vectors_fit(const Product& pr) {
   const Epilogue& e = pr.epi;
   const int64_t size = pr.dtype == DType::kF32 ? 4 : 2;
   bool ok = aligned16(e.out) && (e.out_ld * (e.out_plane ? 2 : size)) % 16 == 0 && (e.out_plane * 2) % 16 == 0;
-  if (e.extra) ok = ok && aligned16(e.extra) && (e.extra_ld * size) % 16 == 0;
+  if (e.extra) ok = ok && aligned16(e.extra) && (e.extra_ld * size) % 16 == 0 && e.extra_ld >= pr.n;
   if (e.slope) ok = ok && aligned16(e.slope) && (pr.n * size) % 16 == 0;
   return ok;
 }
 
 template <int BN, int CG, typename T, bool kF32>
-cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const Job& job, int sms, cudaStream_t stream) {
+cudaError_t launch(const Maps& maps, const Job& job, int sms, cudaStream_t stream) {
   using S = Shape<BN, CG>;
   const auto kernel = product_kernel<BN, CG, T, kF32>;
   static std::atomic<uint64_t> ready{0};  // devices (of the first 64) that know the kernel's shared memory
@@ -676,7 +900,7 @@ cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const Job& job, i
     if (err != cudaSuccess) return err;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int64_t items = job.tiles_m * job.tiles_n * job.splits;
+  const int64_t items = static_cast<int64_t>(job.tiles_m) * job.tiles_n * job.splits;
   const int blocks = static_cast<int>(std::min<int64_t>(items, sms / CG)) * CG;
   cudaLaunchConfig_t config{};
   config.gridDim = dim3(blocks);
@@ -689,19 +913,18 @@ cudaError_t launch(const CUtensorMap& a, const CUtensorMap& b, const Job& job, i
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   config.attrs = attr;
   config.numAttrs = CG > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&config, kernel, a, b, job);
+  return cudaLaunchKernelEx(&config, kernel, maps, job);
 }
 
 template <typename T, bool kF32>
-cudaError_t launch_tile(const Plan& plan, const CUtensorMap& a, const CUtensorMap& b, const Job& job, int sms,
-                        cudaStream_t stream) {
+cudaError_t launch_tile(const Plan& plan, const Maps& maps, const Job& job, int sms, cudaStream_t stream) {
   if constexpr (!kF32) {
     if (plan.bn == 256)
-      return plan.pair == 2 ? launch<256, 2, T, kF32>(a, b, job, sms, stream)
-                            : launch<256, 1, T, kF32>(a, b, job, sms, stream);
+      return plan.pair == 2 ? launch<256, 2, T, kF32>(maps, job, sms, stream)
+                            : launch<256, 1, T, kF32>(maps, job, sms, stream);
   }
-  return plan.bn == 128 ? launch<128, 1, T, kF32>(a, b, job, sms, stream)
-                        : launch<64, 1, T, kF32>(a, b, job, sms, stream);
+  return plan.bn == 128 ? launch<128, 1, T, kF32>(maps, job, sms, stream)
+                        : launch<64, 1, T, kF32>(maps, job, sms, stream);
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -741,6 +964,8 @@ Plan plan_product(int64_t m, int64_t n, int64_t k, int pairs, bool any_mn, int s
   return best;
 }
 
+bool finished_apart(const Product& pr, const Plan& plan) { return plan.splits > 1 || !vectors_fit(pr); }
+
 cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t stream) {
   if (pr.m == 0 || pr.n == 0) return cudaSuccess;
   Job job{};
@@ -749,33 +974,34 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
   job.splits = plan.splits;
   const bool f32 = pr.dtype == DType::kF32;
   if (pr.k > 0) {
-    int device = 0, sms = 148;
-    cudaError_t err = cudaGetDevice(&device);
+    int sms = 148;
+    cudaError_t err = cudaGetDevice(&job.device);
     // binds the device's context to this thread (autograd's threads may have none yet): the encoder needs one
-    if (err == cudaSuccess) err = cudaSetDevice(device);
-    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (err == cudaSuccess) err = cudaSetDevice(job.device);
+    if (err == cudaSuccess) err = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, job.device);
     if (err != cudaSuccess) return err;
-    job.device = device;
-    if (plan.splits > 1) job.vec = pr.n % 4 == 0;  // of the partial sums
-    job.tiles_m = ceil_div(pr.m, kTileM * plan.pair);
-    job.tiles_n = ceil_div(pr.n, plan.bn);
+    const int64_t tiles_m = ceil_div(pr.m, kTileM * plan.pair), tiles_n = ceil_div(pr.n, plan.bn);
+    if (tiles_m * tiles_n * plan.splits >= 1ll << 31) return cudaErrorInvalidValue;
+    job.tiles_m = static_cast<uint32_t>(tiles_m);
+    job.tiles_n = static_cast<uint32_t>(tiles_n);
     job.kblocks = static_cast<int>(ceil_div(pr.k, kBlockK));
     job.kblocks_per_split = plan.kblocks;
     job.pairs = pr.a.planes == 3 ? (pr.b.planes == 3 ? 6 : 3) : (pr.b.planes == 3 ? 3 : 1);
+    job.apart = finished_apart(pr, plan);
     const int64_t rows_b = plan.bn / plan.pair;
     job.box_a = pr.a_mn ? 64 : static_cast<int>(std::min<int64_t>(kTileM, ceil_div(pr.m, 8) * 8));
     job.box_b = pr.b_mn ? 64 : static_cast<int>(std::min<int64_t>(rows_b, ceil_div(pr.n, 8) * 8));
-    CUtensorMap a, b;
-    if (!make_map(&a, pr.a, job.box_a) || !make_map(&b, pr.b, job.box_b)) return cudaErrorInvalidValue;
-    if (f32) {
-      err = launch_tile<float, true>(plan, a, b, job, sms, stream);
-    } else if (plan.splits > 1) {
-      err = launch_tile<float, false>(plan, a, b, job, sms, stream);
-    } else {
-      err = launch_tile<bf16, false>(plan, a, b, job, sms, stream);
-    }
-    if (err != cudaSuccess || plan.splits == 1) return err;
-    job.vec = vectors_fit(pr);
+    Maps maps{};
+    if (!operand_map(&maps.a, pr.a, job.box_a) || !operand_map(&maps.b, pr.b, job.box_b) ||
+        !epilogue_maps(maps, pr, plan, job.apart))
+      return cudaErrorInvalidValue;
+    if (f32)
+      err = launch_tile<float, true>(plan, maps, job, sms, stream);
+    else if (job.apart)
+      err = launch_tile<float, false>(plan, maps, job, sms, stream);
+    else
+      err = launch_tile<bf16, false>(plan, maps, job, sms, stream);
+    if (err != cudaSuccess || !job.apart) return err;
   } else {
     job.splits = 0;  // an empty sum
   }

@@ -20,11 +20,11 @@ inline int blocks_for(int64_t groups) {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T>
-__device__ __forceinline__ void put(bf16* dst, int64_t plane, int count, bool vec, const float v[8], uint32_t* row_flag,
-                                    uint32_t* col_flags) {
+__device__ __forceinline__ void put(bf16* dst, int64_t plane, int count, bool vec, const float v[8], Flags* flags,
+                                    int64_t rows, int64_t r, int64_t c) {
   if (sizeof(T) == 4) {
     store_planes(dst, plane, count, vec, v);
-    mark_flags(v, count, row_flag, col_flags);
+    mark_flags(v, count, flags, rows, r, c);
   } else {
     store_some(dst, count, vec, v);
   }
@@ -36,8 +36,7 @@ template <typename T, bool kScale>
 __global__ void __launch_bounds__(kThreads)
     operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec,
                    const typename SlopeOf<T>::type* __restrict__ slope, bool slope_vec, bf16* __restrict__ dst,
-                   int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, uint32_t* row_flags,
-                   uint32_t* col_flags) {
+                   int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, Flags* flags) {
   const int64_t per_row = (cols + 7) / 8, total = rows * per_row;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -51,13 +50,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= s[j];
     }
-    put<T>(dst + r * dst_ld + c, plane, 8, true, v, row_flags + r, col_flags + c);
+    put<T>(dst + r * dst_ld + c, plane, 8, true, v, flags, rows, r, c);
   }
 }
 
 template <typename T, bool kScale>
-cudaError_t launch_operand(const void* src, int64_t src_ld, const void* slope, Operand& dst, uint32_t* row_flags,
-                           uint32_t* col_flags, cudaStream_t stream) {
+cudaError_t launch_operand(const void* src, int64_t src_ld, const void* slope, const Operand& dst, cudaStream_t stream) {
   using S = typename SlopeOf<T>::type;
   const int64_t groups = dst.rows * ((dst.cols + 7) / 8);
   if (groups == 0) return cudaSuccess;
@@ -65,9 +63,7 @@ cudaError_t launch_operand(const void* src, int64_t src_ld, const void* slope, O
   const bool slope_vec = aligned16(slope) && (dst.cols * sizeof(S)) % 16 == 0;
   operand_kernel<T, kScale><<<blocks_for(groups), kThreads, 0, stream>>>(
       static_cast<const T*>(src), src_ld, src_vec, static_cast<const S*>(slope), slope_vec, const_cast<bf16*>(dst.p),
-      dst.ld, dst.plane, dst.rows, dst.cols, row_flags, col_flags);
-  dst.row_flags = row_flags;
-  dst.col_flags = col_flags;
+      dst.ld, dst.plane, dst.rows, dst.cols, dst.flags);
   return cudaGetLastError();
 }
 
@@ -135,19 +131,18 @@ __global__ void add_parts_kernel(const float* __restrict__ parts, int count, int
 
 }  // namespace
 
-cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, Operand& dst, uint32_t* row_flags,
-                         uint32_t* col_flags, cudaStream_t stream) {
-  return dtype == DType::kF32 ? launch_operand<float, false>(src, src_ld, nullptr, dst, row_flags, col_flags, stream)
-                              : launch_operand<bf16, false>(src, src_ld, nullptr, dst, nullptr, nullptr, stream);
+cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, const Operand& dst, cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_operand<float, false>(src, src_ld, nullptr, dst, stream)
+                              : launch_operand<bf16, false>(src, src_ld, nullptr, dst, stream);
 }
 
-cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, Operand& dst,
-                          uint32_t* row_flags, uint32_t* col_flags, cudaStream_t stream) {
-  return dtype == DType::kF32 ? launch_operand<float, true>(g, g_ld, slope, dst, row_flags, col_flags, stream)
-                              : launch_operand<bf16, true>(g, g_ld, slope, dst, nullptr, nullptr, stream);
+cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
+                          cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_operand<float, true>(g, g_ld, slope, dst, stream)
+                              : launch_operand<bf16, true>(g, g_ld, slope, dst, stream);
 }
 
-cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, Operand& dst, cudaStream_t stream) {
+cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream) {
   const int64_t groups = dst.rows * ((dst.cols + 7) / 8);
   if (groups == 0) return cudaSuccess;
   const bool vec = (reinterpret_cast<uintptr_t>(codes) & 7) == 0 && dst.cols % 8 == 0;
