@@ -14,64 +14,101 @@ using bf16 = __nv_bfloat16;
 
 // ---- activations: value and slope --------------------------------------------------
 
-// Phi(z), the normal distribution function, and its density phi(z). erfc is
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float reciprocal_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
+
+// Two float32 in one register pair: one instruction for both.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Phi(z), the normal distribution function, and exp(-z^2 / 2), for two z. erfc is
 // Hastings' rational approximation (Abramowitz and Stegun 7.1.26, |error| <=
 // 1.5e-7) in t = 1 / (1 + p x); its factor exp(-x^2) with x = |z| / sqrt 2 is
-// the density's too, so the slope costs three more instructions. The bfloat16
+// the density's too, so the slope costs two more instructions. The bfloat16
 // kernels use it (an error of 2^-23 beside outputs of 8 bits); float32 takes
-// erff. erff's 25 to 30 instructions made the epilogue, not the memory, the
-// bound of a 256 -> 512 layer.
-__device__ __forceinline__ void normal_fast(float z, float& cdf, float& pdf) {
-  const float x = fabsf(z) * 0.70710678118654752f;
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  const float e = __expf(-x * x);
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float tail = 0.5f * p * t * e;  // Phi(-|z|)
-  cdf = z < 0.f ? tail : 1.f - tail;
-  pdf = 0.39894228040143268f * e;
+// erfcf. It is bound by its reciprocal and exponential (16 of them a clock
+// on an SM, 2 a value): 20 million values take 9 us.
+__device__ __forceinline__ void normal2(float2 z, float2& cdf, float2& bell) {
+  const float2 t = make_float2(reciprocal_fast(fmaf(fabsf(z.x), 0.3275911f * 0.70710678118654752f, 1.f)),
+                               reciprocal_fast(fmaf(fabsf(z.y), 0.3275911f * 0.70710678118654752f, 1.f)));
+  const float2 w = mul2(mul2(z, z), both(-0.5f * kLog2e));
+  bell = make_float2(exp2_fast(w.x), exp2_fast(w.y));
+  float2 p = fma2(both(0.5f * 1.061405429f), t, both(0.5f * -1.453152027f));
+  p = fma2(p, t, both(0.5f * 1.421413741f));
+  p = fma2(p, t, both(0.5f * -0.284496736f));
+  p = fma2(p, t, both(0.5f * 0.254829592f));
+  const float2 tail = mul2(mul2(p, t), bell);  // Phi(-|z|)
+  cdf = make_float2(z.x < 0.f ? tail.x : 1.f - tail.x, z.y < 0.f ? tail.y : 1.f - tail.y);
 }
 
-__device__ __forceinline__ void normal_exact(float z, float& cdf, float& pdf) {
-  cdf = 0.5f * erfcf(-z * 0.70710678118654752f);
-  pdf = 0.39894228040143268f * expf(-0.5f * z * z);
-}
-
-__device__ __forceinline__ float sigmoid_of(float z, bool fast) {
-  return fast ? __fdividef(1.f, 1.f + __expf(-z)) : 1.f / (1.f + expf(-z));
-}
-
-// act(z) in place of z, act'(z) in `s`, of N values: one branch for all of
-// them. relu's slope at 0 is 0; a NaN stays a NaN.
-template <bool kFast, int N>
+// act(z) in place of z (kY) and act'(z) in `s` (kS), of N values: one branch for
+// all of them. relu's slope at 0 is 0; a NaN stays a NaN. kFast: for bfloat16
+// results.
+template <bool kFast, bool kY, bool kS, int N>
 __device__ __forceinline__ void activate(Act act, float* z, float* s) {
   if (act == Act::kGelu) {
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      float cdf, pdf;
-      if (kFast)
-        normal_fast(z[j], cdf, pdf);
-      else
-        normal_exact(z[j], cdf, pdf);
-      s[j] = fmaf(z[j], pdf, cdf);
-      z[j] *= cdf;
+    for (int j = 0; j < N; j += 2) {
+      const float2 x = make_float2(z[j], z[j + 1]);
+      float2 cdf, bell;
+      if (kFast) {
+        normal2(x, cdf, bell);
+      } else {
+        cdf = make_float2(0.5f * erfcf(-x.x * 0.70710678118654752f), 0.5f * erfcf(-x.y * 0.70710678118654752f));
+        if (kS) bell = make_float2(expf(-0.5f * x.x * x.x), expf(-0.5f * x.y * x.y));
+      }
+      if (kS) {
+        const float2 d = fma2(mul2(x, both(kInvSqrt2Pi)), bell, cdf);
+        s[j] = d.x, s[j + 1] = d.y;
+      }
+      if (kY) {
+        const float2 y = mul2(x, cdf);
+        z[j] = y.x, z[j + 1] = y.y;
+      }
     }
   } else if (act == Act::kSilu) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float g = sigmoid_of(z[j], kFast);
-      s[j] = g * fmaf(z[j], 1.f - g, 1.f);
-      z[j] *= g;
+      const float g = kFast ? reciprocal_fast(1.f + exp2_fast(-kLog2e * z[j])) : 1.f / (1.f + expf(-z[j]));
+      if (kS) s[j] = g * fmaf(z[j], 1.f - g, 1.f);
+      if (kY) z[j] *= g;
     }
   } else if (act == Act::kRelu) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      s[j] = z[j] > 0.f ? 1.f : (z[j] <= 0.f ? 0.f : z[j]);
-      z[j] = z[j] <= 0.f ? 0.f : z[j];
+      if (kS) s[j] = z[j] > 0.f ? 1.f : (z[j] <= 0.f ? 0.f : z[j]);
+      if (kY) z[j] = z[j] <= 0.f ? 0.f : z[j];
     }
-  } else {
+  } else if (kS) {
 #pragma unroll
     for (int j = 0; j < N; ++j) s[j] = 1.f;
   }
@@ -246,7 +283,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], const flo
     float s[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] += b[j];
-    activate<sizeof(T) == 2, 8>(e.act, v, s);
+    activate<sizeof(T) == 2, true, true, 8>(e.act, v, s);
     if (e.mode == Epilogue::kFwd) {
       if (e.slope) store_some(static_cast<typename SlopeOf<T>::type*>(e.slope) + m * cols + n, count, vec, s);
       if (e.extra) {

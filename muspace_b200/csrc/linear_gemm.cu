@@ -1,10 +1,10 @@
 // The product D[m, n] = sum_k A(m, k) B(n, k) of the fused linear operator on
 // the fifth-generation tensor cores, with the operator's epilogues.
 //
-// One persistent block per SM (or a pair of them on two SMs) of ten warps:
+// One persistent block per SM (or a pair of them on two SMs) of 18 warps:
 // a producer thread copies tiles of A and B into a ring of shared-memory stages
 // (TMA, 128-byte swizzle), one thread issues tcgen05.mma on them into one of
-// two accumulators in tensor memory, and eight warps carry the other
+// two accumulators in tensor memory, and sixteen warps carry the other
 // accumulator through the epilogue meanwhile. A lane holds a row there, 16
 // columns at a time: tensor memory -> registers, bias, activation, residual ->
 // shared memory -> global memory by TMA, which also brings the residual. So
@@ -36,12 +36,11 @@ namespace {
 
 constexpr int kTileM = 128;       // rows of a block's tile
 constexpr int kBlockK = 64;       // k of a stage: 128 bytes, one swizzle row
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarps = 16;     // eight issued half the time: gelu, 40000 x 256 x 512, 52 us
 constexpr int kProducer = kEpiWarps, kIssuer = kEpiWarps + 1;
 constexpr int kThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageA = kTileM * kBlockK * 2;
 constexpr int kBoxBytes = 32 * 128;  // a box of the epilogue: 32 rows of 128 bytes
-constexpr int kStagingBytes = 2 * kBoxBytes;  // of a warp
 constexpr int kRingBytes = 160 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
@@ -53,10 +52,13 @@ struct Shape {
   static constexpr int kStageB = kRowsB * kBlockK * 2;
   static constexpr int kStage = kStageA + kStageB;
   static constexpr int kStages = kRingBytes / kStage;
-  static constexpr int kBarriers = 2 * kStages + 4 + 2 * kEpiWarps;
+  static constexpr int kBarriers = 2 * kStages + 4 + kEpiWarps;
   // stages, the warps' staging, barriers, the tensor-memory address; and room to start on 1024 bytes
-  static constexpr int kSmem = kStages * kStage + kEpiWarps * kStagingBytes + kBarriers * 8 + 16 + 1024;
-  static constexpr uint32_t kColumns = 2 * BN < 32 ? 32 : 2 * BN;
+  static constexpr int kSmem = kStages * kStage + kEpiWarps * kBoxBytes + kBarriers * 8 + 16 + 1024;
+  static constexpr uint32_t kColumns = 2 * BN;
+  // a warp of the epilogue takes 32 rows and this many columns
+  static constexpr int kCols = BN / 4 < 32 ? 32 : BN / 4;
+  static constexpr int kWarps = 4 * (BN / kCols);
   static_assert(kSmem <= 232448, "more shared memory than a block may have");
 };
 
@@ -218,6 +220,22 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const float v[16]) {
       "%15};" ::"f"(v[0]),
       "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
       "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "r"(addr)
+      : "memory");
+}
+
+// Eight columns, stored; and loaded and waited for.
+__device__ __forceinline__ void tmem_store8(uint32_t addr, const uint32_t r[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr)
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_load8(uint32_t addr, uint32_t r[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr)
       : "memory");
 }
 
@@ -405,6 +423,32 @@ __device__ __forceinline__ void get16(uint32_t box, int row, int col, float v[16
   }
 }
 
+// 16 slopes put aside in the tensor memory that their sums came from, and taken back into the box.
+__device__ __forceinline__ void put_aside(uint32_t at, const float s[16], __half) {
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = pack_half2(s[2 * j], s[2 * j + 1]);
+  tmem_store8(at, w);
+}
+__device__ __forceinline__ void put_aside(uint32_t at, const float s[16], float) { tmem_store16(at, s); }
+template <int kRowBytes>
+__device__ __forceinline__ void take_back(uint32_t box, int row, int col, uint32_t at, __half) {
+  uint32_t w[8];
+  tmem_load8(at, w);
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 8 + u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+}
+template <int kRowBytes>
+__device__ __forceinline__ void take_back(uint32_t box, int row, int col, uint32_t at, float) {
+  uint32_t w[16];
+  tmem_load16(at, w);
+  tmem_wait(w);
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 4 + u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+}
+
 // Bias of columns [n, n + 16): the same for all lanes.
 template <typename T>
 __device__ __forceinline__ void add_bias16(const void* bias, int n, int cols, float v[16]) {
@@ -474,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t raw[];
   const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t boxes_base = ring + S::kStages * S::kStage;
-  const uint32_t bars = boxes_base + kEpiWarps * kStagingBytes;
+  const uint32_t bars = boxes_base + kEpiWarps * kBoxBytes;
   const uint32_t tmem_slot = bars + S::kBarriers * 8;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
@@ -492,9 +536,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       barrier_init(acc_full(b), 1);
-      barrier_init(acc_empty(b), kEpiWarps * CG);
+      barrier_init(acc_empty(b), S::kWarps * CG);
     }
-    for (int x = 0; x < 2 * kEpiWarps; ++x) barrier_init(bars + 8 * (2 * S::kStages + 4 + x), 1);
+    for (int x = 0; x < kEpiWarps; ++x) barrier_init(bars + 8 * (2 * S::kStages + 4 + x), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssuer) tmem_alloc<CG>(tmem_slot, S::kColumns);
@@ -588,14 +632,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (buf == 0) acc_phase ^= 1;
       }
     }
-  } else if (warp < kEpiWarps) {
-    constexpr int kHalf = BN / 2;  // columns of a warp
-    constexpr int kBoxCols = 128 / sizeof(T) < kHalf ? 128 / sizeof(T) : kHalf;
+  } else if (warp < S::kWarps) {
+    constexpr int kBoxCols = 128 / sizeof(T) < S::kCols ? 128 / sizeof(T) : S::kCols;
     constexpr int kRowBytes = kBoxCols * sizeof(T);
-    constexpr int kParts = kHalf / kBoxCols;
-    const int quad = warp & 3, half = warp >> 2;
-    const uint32_t boxes = boxes_base + warp * kStagingBytes;
-    const uint32_t arrived = bars + 8 * (2 * S::kStages + 4 + 2 * warp);  // the residual's boxes
+    constexpr bool kFast = sizeof(T) == 2;
+    constexpr int kParts = S::kCols / kBoxCols;  // more than one only for partial sums
+    const int quad = warp & 3, group = warp >> 2;
+    const uint32_t box = boxes_base + warp * kBoxBytes;
+    const uint32_t arrived = bars + 8 * (2 * S::kStages + 4 + warp);  // the residual's box
     const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
     const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
     const Epilogue& e = job.pr.epi;
@@ -603,86 +647,72 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool extra = mode != Epilogue::kStore && e.extra != nullptr;
     const bool slope = mode == Epilogue::kFwd && e.slope != nullptr;
     const bool planes = sizeof(T) == 4 && mode == Epilogue::kDz;
-    const bool one_box = slope || planes;  // the second box holds the second output
     const bool repairs = kF32 && !job.apart && some_flag(job.pr);
     const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
-    const auto col_of = [&](const Item& t, int p) { return t.n + half * kHalf + p * kBoxCols; };
+    const auto col_of = [&](const Item& t) { return t.n + group * S::kCols; };
+    // a box on its way out; the next may be written when `read`
+    const auto send = [&](const CUtensorMap* map, int n, int m, int z, uint32_t src) {
+      if (m < rows_m && n < rows_n) store_box(map, n, m, z, src);
+    };
+    const auto box_written = [&] {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    };
+    const auto box_read = [&] {
+      if (lane == 0) stores_read<0>();
+      __syncwarp();
+    };
     int buf = 0;
-    uint32_t acc_phase = 0, box = 0, extra_phase = 0;
+    uint32_t acc_phase = 0, extra_phase = 0;
     Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
-    if (extra && !one_box && first < items && lane == 0) 
-      load_box(boxes, &maps.extra, col_of(t, 0), row_of(t), 32 * kRowBytes, arrived);
+    if (extra && first < items && lane == 0) load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
     for (uint32_t i = first; i < items; i += step) {
-      const Item next = i + step < items ? item_of<BN, CG>(job, i + step) : Item{};
-      const int m = row_of(t);
+      const int m = row_of(t), n0 = col_of(t);
+      uint32_t acc_at = tmem + lanes + buf * BN + group * S::kCols;
       if (kF32) {
-        float acc[kHalf / 16][16] = {};
-        int last = 0;
+        float acc[S::kCols / 16][16] = {};
         for (int c = t.kb0; c < t.kb1; c += chunk) {
           wait(acc_full(buf), acc_phase, dead);
           fence_after();
           const bool more = c + chunk < t.kb1;
-          last = buf;
+          acc_at = tmem + lanes + buf * BN + group * S::kCols;
 #pragma unroll
-          for (int q = 0; q < kHalf / 16; ++q) {
-            const uint32_t at = tmem + lanes + buf * BN + half * kHalf + q * 16;
+          for (int q = 0; q < S::kCols / 16; ++q) {
             uint32_t r[16];
-            tmem_load16(at, r);
+            tmem_load16(acc_at + q * 16, r);
             tmem_wait(r);
 #pragma unroll
             for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
-            if (!more) tmem_store16(at, acc[q]);
+            if (!more) tmem_store16(acc_at + q * 16, acc[q]);
           }
           if (more) {
             fence_before();
             __syncwarp();
             if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
+            buf ^= 1;
+            if (buf == 0) acc_phase ^= 1;
           }
-          buf ^= 1;
-          if (buf == 0) acc_phase ^= 1;
         }
         tmem_stored();
-        buf = last;
-        if (buf == 1) acc_phase ^= 1;
       } else {
         wait(acc_full(buf), acc_phase, dead);
         fence_after();
       }
-      const uint32_t acc_at = tmem + lanes + buf * BN + half * kHalf;
+      if (extra) {
+        wait(arrived, extra_phase, dead);
+        extra_phase ^= 1;
+      }
 #pragma unroll 1
       for (int p = 0; p < kParts; ++p) {
-        const int n = col_of(t, p);
-        const uint32_t here = one_box ? boxes : boxes + (box & 1) * kBoxBytes;
-        if (lane == 0) {
-          if (one_box || extra)
-            stores_read<0>();
-          else
-            stores_read<1>();
-          if (extra) {
-            if (one_box) {
-              load_box(boxes, &maps.extra, n, m, 32 * kRowBytes, arrived);
-            } else {
-              const uint32_t other = (box + 1) & 1;
-              const bool same = p + 1 < kParts;
-              if (same || i + step < items)
-                load_box(boxes + other * kBoxBytes, &maps.extra, same ? col_of(t, p + 1) : col_of(next, 0),
-                         same ? m : row_of(next), 32 * kRowBytes, arrived + 8 * other);
-            }
-          }
-        }
-        __syncwarp();
-        if (extra) {
-          const uint32_t which = one_box ? 0 : box & 1;
-          wait(arrived + 8 * which, (extra_phase >> which) & 1, dead);
-          extra_phase ^= 1u << which;
-        }
-        uint32_t held[8];
+        const int n = n0 + p * kBoxCols;
+        if (!extra) box_read();
 #pragma unroll 1
         for (int c = 0; c < kBoxCols; c += 16) {
+          const uint32_t at = acc_at + p * kBoxCols + c;
           uint32_t r[16];
-          tmem_load16(acc_at + p * kBoxCols + c, r);
+          tmem_load16(at, r);
           float x[16], v[16], s[16];
-          if (extra) get16<kRowBytes>(here, lane, c, x, T());
+          if (extra) get16<kRowBytes>(box, lane, c, x, T());
           tmem_wait(r);
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
@@ -696,73 +726,101 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (mode != Epilogue::kStore) {
             if (e.bias) add_bias16<T>(e.bias, n + c, rows_n, v);
-            activate<sizeof(T) == 2, 16>(e.act, v, s);
-            if (mode == Epilogue::kFwd) {
+            if (mode == Epilogue::kDz) {
+              activate<kFast, false, true, 16>(e.act, v, s);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
+              if (planes) {
+                tmem_store16(at, v);
+                mark16(e.out_flags, job.pr, v, m + lane, n + c);
+                continue;
+              }
+            } else {
+              if (slope) {
+                activate<kFast, true, true, 16>(e.act, v, s);
+                put_aside(at, s, typename SlopeOf<T>::type());
+              } else {
+                activate<kFast, true, false, 16>(e.act, v, s);
+              }
               if (extra) {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) v[j] += x[j];
               }
-              if (slope) put16<kRowBytes>(boxes + kBoxBytes, lane, c, s, typename SlopeOf<T>::type());
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
             }
           }
-          if (sizeof(T) == 4 && planes) {
-            // hi and mid into the second box; lo into the first, once all lanes have read the gradient there
-            uint32_t part[3][8];
+          put16<kRowBytes>(box, lane, c, v, T());
+        }
+        if (sizeof(T) == 4 && planes) {
+          // dz waits in tensor memory: hi and mid take the gradient's place, then lo theirs
+          tmem_stored();
+          __syncwarp();
+#pragma unroll 1
+          for (int pass = 0; pass < 2; ++pass) {
+            if (pass) box_read();
+#pragma unroll 1
+            for (int c = 0; c < kBoxCols; c += 16) {
+              uint32_t r[16], part[3][8];
+              tmem_load16(acc_at + c, r);
+              tmem_wait(r);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              bf16 a[3], b[3];
-              split3(v[2 * j], a[0], a[1], a[2]);
-              split3(v[2 * j + 1], b[0], b[1], b[2]);
+              for (int j = 0; j < 8; ++j) {
+                bf16 a[3], b[3];
+                split3(__uint_as_float(r[2 * j]), a[0], a[1], a[2]);
+                split3(__uint_as_float(r[2 * j + 1]), b[0], b[1], b[2]);
 #pragma unroll
-              for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 2; ++k)
-#pragma unroll
-              for (int u = 0; u < 2; ++u)
-                put_unit(unit_at<64>(boxes + kBoxBytes + k * 2048, lane, c / 8 + u), part[k][4 * u], part[k][4 * u + 1],
-                         part[k][4 * u + 2], part[k][4 * u + 3]);
-            if (c > 0) {
-              __syncwarp();
+                for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
+              }
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
-                put_unit(unit_at<64>(here, lane, u), held[4 * u], held[4 * u + 1], held[4 * u + 2], held[4 * u + 3]);
-                put_unit(unit_at<64>(here, lane, 2 + u), part[2][4 * u], part[2][4 * u + 1], part[2][4 * u + 2],
-                         part[2][4 * u + 3]);
+                const int k = 4 * u;
+                if (pass) {
+                  put_unit(unit_at<64>(box, lane, c / 8 + u), part[2][k], part[2][k + 1], part[2][k + 2], part[2][k + 3]);
+                } else {
+                  put_unit(unit_at<64>(box, lane, c / 8 + u), part[0][k], part[0][k + 1], part[0][k + 2], part[0][k + 3]);
+                  put_unit(unit_at<64>(box + 2048, lane, c / 8 + u), part[1][k], part[1][k + 1], part[1][k + 2],
+                           part[1][k + 3]);
+                }
               }
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) held[j] = part[2][j];
-            mark16(e.out_flags, job.pr, v, m + lane, n + c);
-          }
-          if (!planes) put16<kRowBytes>(here, lane, c, v, T());
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-          if (m < rows_m && n < rows_n) {
-            if (sizeof(T) == 4 && planes) {
-              store_box(&maps.out, n, m, 0, boxes + kBoxBytes);
-              store_box(&maps.out, n, m, 1, boxes + kBoxBytes + 2048);
-              store_box(&maps.out, n, m, 2, boxes);
-            } else {
-              store_box(&maps.out, n, m, job.apart ? t.split : 0, here);
+            box_written();
+            if (lane == 0) {
+              send(&maps.out, n, m, 2 * pass, box);
+              if (!pass) send(&maps.out, n, m, 1, box + 2048);
+              stores_commit();
             }
-            if (slope) store_box(&maps.slope, n, m, 0, boxes + kBoxBytes);
           }
-          stores_commit();
+        } else {
+          box_written();
+          if (lane == 0) {
+            send(&maps.out, n, m, job.apart ? t.split : 0, box);
+            stores_commit();
+          }
+          if (slope) {
+            // the slopes wait in tensor memory for the box
+            tmem_stored();
+            box_read();
+#pragma unroll 1
+            for (int c = 0; c < kBoxCols; c += 16) take_back<kRowBytes>(box, lane, c, acc_at + c, typename SlopeOf<T>::type());
+            box_written();
+            if (lane == 0) {
+              send(&maps.slope, n, m, 0, box);
+              stores_commit();
+            }
+          }
         }
-        ++box;
       }
       fence_before();
       __syncwarp();
       if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
       buf ^= 1;
       if (buf == 0) acc_phase ^= 1;
-      t = next;
+      if (i + step < items) {
+        t = item_of<BN, CG>(job, i + step);
+        if (extra && lane == 0) {
+          stores_read<0>();
+          load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
+        }
+      }
     }
     if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
@@ -862,7 +920,7 @@ bool epilogue_maps(Maps& maps, const Product& pr, const Plan& plan, bool apart) 
                     pr.m * partial_ld(pr.n) * 4, 32, 32, 128);
   const bool wide = pr.dtype == DType::kF32;
   const int64_t size = wide ? 4 : 2;
-  const int row_bytes = std::min<int>(128, plan.bn / 2 * static_cast<int>(size));
+  const int row_bytes = std::min<int>(128, std::max(32, plan.bn / 4) * static_cast<int>(size));
   const int cols = row_bytes / static_cast<int>(size);
   bool ok = true;
   if (e.mode == Epilogue::kDz && wide)
