@@ -58,17 +58,22 @@ __device__ __forceinline__ void store_codes8(int8_t* p, int count, bool vec, uin
   }
 }
 
+// Eight codes of one block as numbers.
+__device__ __forceinline__ void values_of(uint2 u, uint32_t e, float v[8]) {
+  const float s = scale_of(e);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t w = j < 4 ? u.x : u.y;
+    v[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * (j & 3)))) * s;
+  }
+}
+
 // Up to eight codes of one block as numbers.
 __device__ __forceinline__ void load_codes8(const int8_t* p, int count, bool vec, uint32_t e, float v[8]) {
-  const float s = scale_of(e);
   if (vec) {
-    const uint2 u = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t w = j < 4 ? u.x : u.y;
-      v[j] = static_cast<float>(static_cast<int8_t>(w >> (8 * (j & 3)))) * s;
-    }
+    values_of(*reinterpret_cast<const uint2*>(p), e, v);
   } else {
+    const float s = scale_of(e);
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j < count ? static_cast<float>(p[j]) * s : 0.f;
   }

@@ -55,122 +55,156 @@ __device__ __forceinline__ Sums row_sums(Sums s, Sums* buf, int& turn) {
   return t;
 }
 
-// The columns of a thread: eight neighbours at a time where vectors fit, else
-// one at a time, neighbours in neighbouring threads.
-template <int G>
-__device__ __forceinline__ int64_t column(bool vec, int lane, int i, int j) {
-  return vec ? (static_cast<int64_t>(i) * G + lane) * 8 + j : (static_cast<int64_t>(i) * 8 + j) * G + lane;
+// The columns of a thread, eight to a chunk: neighbours where vectors fit
+// (kVec), else one at a time, neighbours in neighbouring threads.
+template <int G, bool kVec>
+__device__ __forceinline__ int column(int lane, int i, int j) {
+  return kVec ? (i * G + lane) * 8 + j : (i * 8 + j) * G + lane;
 }
 
-template <int G, int NV, typename T>
-__device__ __forceinline__ void load_row(const T* row, int64_t cols, bool vec, int lane, float v[NV * 8]) {
+// Eight values as they lie in memory: they stay so in registers until they are
+// used, so that more rows are on their way.
+template <typename T, bool kVec>
+struct Chunk {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (vec) {
-      const int64_t c = column<G>(true, lane, i, 0);
-      if (c < cols) {
-        lin::load8(row + c, v + i * 8);
-      } else {
+    for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) u[k] = make_uint4(0, 0, 0, 0);
+  }
+  template <int G>
+  __device__ __forceinline__ void load(const T* row, int cols, int lane, int i) {
+    const int c = column<G, true>(lane, i, 0);
+    if (c < cols) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i * 8 + j] = 0.f;
-      }
+      for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) u[k] = __ldg(reinterpret_cast<const uint4*>(row + c) + k);
     } else {
+      zero();
+    }
+  }
+  __device__ __forceinline__ void get(float v[8]) const { lin::load8(reinterpret_cast<const T*>(u), v); }
+};
+template <typename T>
+struct Chunk<T, false> {
+  float v[8];
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = column<G>(false, lane, i, j);
-        v[i * 8 + j] = c < cols ? to_float(row[c]) : 0.f;
-      }
+    for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  }
+  template <int G>
+  __device__ __forceinline__ void load(const T* row, int cols, int lane, int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<G, false>(lane, i, j);
+      v[j] = c < cols ? to_float(row[c]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float w[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = v[j];
+  }
+};
+
+// The same of an 8-bit checkpoint.
+template <bool kVec>
+struct Codes {
+  uint2 u;
+  uint32_t e;
+  template <int G>
+  __device__ __forceinline__ void load(const int8_t* row, const uint8_t* exps, int cols, int lane, int i) {
+    const int c = column<G, true>(lane, i, 0);
+    u = make_uint2(0, 0);
+    e = 1;
+    if (c < cols) {
+      u = __ldg(reinterpret_cast<const uint2*>(row + c));
+      e = __ldg(exps + c / ckpt::kBlock);
+    }
+  }
+  __device__ __forceinline__ void get(float v[8]) const { ckpt::values_of(u, e, v); }
+};
+template <>
+struct Codes<false> {
+  float v[8];
+  template <int G>
+  __device__ __forceinline__ void load(const int8_t* row, const uint8_t* exps, int cols, int lane, int i) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<G, false>(lane, i, j);
+      v[j] = c < cols ? row[c] * ckpt::scale_of(exps[c / ckpt::kBlock]) : 0.f;
+    }
+  }
+  __device__ __forceinline__ void get(float w[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = v[j];
+  }
+};
+
+template <int G, bool kVec, typename T>
+__device__ __forceinline__ void store_chunk(T* row, int cols, int lane, int i, const float v[8]) {
+  if (kVec) {
+    const int c = column<G, true>(lane, i, 0);
+    if (c < cols) lin::store8(row + c, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<G, false>(lane, i, j);
+      if (c < cols) row[c] = from_float<T>(v[j]);
     }
   }
 }
 
-template <int G, int NV, typename T>
-__device__ __forceinline__ void store_row(T* row, int64_t cols, bool vec, int lane, const float v[NV * 8]) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (vec) {
-      const int64_t c = column<G>(true, lane, i, 0);
-      if (c < cols) lin::store8(row + c, v + i * 8);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = column<G>(false, lane, i, j);
-        if (c < cols) row[c] = from_float<T>(v[i * 8 + j]);
-      }
-    }
-  }
-}
-
-// A row of an 8-bit checkpoint. A block of 32 columns is four threads' vectors,
+// A chunk into the checkpoint. A block of 32 columns is four threads' chunks,
 // or one column of a warp's threads.
-template <int G, int NV>
-__device__ __forceinline__ void load_codes(const int8_t* row, const uint8_t* exps, int64_t cols, bool vec, int lane,
-                                           float v[NV * 8]) {
+template <int G, bool kVec>
+__device__ __forceinline__ void store_codes(int8_t* row, uint8_t* exps, int cols, int lane, int i, const float v[8]) {
+  if (kVec) {
+    const int c = column<G, true>(lane, i, 0);
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (vec) {
-      const int64_t c = column<G>(true, lane, i, 0);
-      if (c < cols) {
-        ckpt::load_codes8(row + c, 8, true, exps[c / ckpt::kBlock], v + i * 8);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i * 8 + j] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = column<G>(false, lane, i, j);
-        v[i * 8 + j] = c < cols ? row[c] * ckpt::scale_of(exps[c / ckpt::kBlock]) : 0.f;
-      }
+    for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const uint32_t e = ckpt::exponent_of(top);
+    if (c < cols) {
+      ckpt::store_codes8(row + c, 8, true, e, v);
+      if ((lane & 3) == 0) exps[c / ckpt::kBlock] = static_cast<uint8_t>(e);
     }
-  }
-}
-
-template <int G, int NV>
-__device__ __forceinline__ void store_codes(int8_t* row, uint8_t* exps, int64_t cols, bool vec, int lane,
-                                            const float v[NV * 8]) {
+  } else {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (vec) {
-      const int64_t c = column<G>(true, lane, i, 0);
-      uint32_t top = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i * 8 + j]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    for (int j = 0; j < 8; ++j) {
+      const int c = column<G, false>(lane, i, j);
+      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[j]) & 0x7fffffffu);
       const uint32_t e = ckpt::exponent_of(top);
       if (c < cols) {
-        ckpt::store_codes8(row + c, 8, true, e, v + i * 8);
-        if ((lane & 3) == 0) exps[c / ckpt::kBlock] = static_cast<uint8_t>(e);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int64_t c = column<G>(false, lane, i, j);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(v[i * 8 + j]) & 0x7fffffffu);
-        const uint32_t e = ckpt::exponent_of(top);
-        if (c < cols) {
-          row[c] = static_cast<int8_t>(ckpt::code_of(v[i * 8 + j], e, ckpt::inverse_scale(e)));
-          if ((lane & 31) == 0) exps[c / ckpt::kBlock] = static_cast<uint8_t>(e);
-        }
+        row[c] = static_cast<int8_t>(ckpt::code_of(v[j], e, ckpt::inverse_scale(e)));
+        if ((lane & 31) == 0) exps[c / ckpt::kBlock] = static_cast<uint8_t>(e);
       }
     }
   }
 }
 
-template <int G, int NV>
-__device__ __forceinline__ void statistics(const float v[NV * 8], int64_t cols, bool vec, int lane, float eps,
-                                           Sums* buf, int& turn, float& mean, float& rstd) {
+template <int G, int NV, bool kVec, typename C>
+__device__ __forceinline__ void statistics(const C x[NV], int cols, int lane, float eps, Sums* buf, int& turn,
+                                           float& mean, float& rstd) {
   Sums s = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < NV * 8; ++i) s.a += v[i];
+  for (int i = 0; i < NV; ++i) {
+    float v[8];
+    x[i].get(v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s.a += v[j];
+  }
   const float n = static_cast<float>(cols);
   mean = row_sums<G>(s, buf, turn).a / n;
   s.a = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV * 8; ++i) {
-    const float d = column<G>(vec, lane, i / 8, i % 8) < cols ? v[i] - mean : 0.f;
-    s.a = fmaf(d, d, s.a);
+  for (int i = 0; i < NV; ++i) {
+    float v[8];
+    x[i].get(v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float d = column<G, kVec>(lane, i, kVec ? 0 : j) < cols ? v[j] - mean : 0.f;
+      s.a = fmaf(d, d, s.a);
+    }
   }
   rstd = rsqrtf(row_sums<G>(s, buf, turn).a / n + eps);
 }
@@ -183,89 +217,153 @@ struct Shape {
   static constexpr int kBuf = G == 32 ? 1 : 2 * (G / 32);
 };
 
-template <int G, int NV, typename T, typename W>
-__global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args a, bool vec) {
+template <int G, int NV, bool kVec, bool kCodes, typename T, typename W>
+__global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args a) {
   __shared__ Sums buf[Shape<G>::kBuf];
   int turn = 0;
-  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
+  const int lane = threadIdx.x % G, cols = static_cast<int>(a.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * Shape<G>::kRows, blocks = ckpt::blocks_of(a.cols);
   const T* x = static_cast<const T*>(a.x);
-  const W *w = static_cast<const W*>(a.w), *b = static_cast<const W*>(a.b);
-  const int64_t blocks = ckpt::blocks_of(a.cols);
-  for (int64_t r = blockIdx.x * static_cast<int64_t>(Shape<G>::kRows) + slot; r < a.rows;
-       r += static_cast<int64_t>(gridDim.x) * Shape<G>::kRows) {
-    float v[NV * 8], p[NV * 8];
-    load_row<G, NV>(x + r * a.x_stride, a.cols, vec, lane, v);
-    if (a.codes) store_codes<G, NV>(a.codes + r * a.cols, a.exps + r * blocks, a.cols, vec, lane, v);
+  int64_t r = blockIdx.x * static_cast<int64_t>(Shape<G>::kRows) + threadIdx.x / G;
+  Chunk<T, kVec> next[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (r < a.rows) next[i].template load<G>(x + r * a.x_stride, cols, lane, i);
+  for (; r < a.rows; r += step) {
+    Chunk<T, kVec> here[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) here[i] = next[i];
+    if (r + step < a.rows) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) next[i].template load<G>(x + (r + step) * a.x_stride, cols, lane, i);
+    }
     float mean, rstd;
-    statistics<G, NV>(v, a.cols, vec, lane, a.eps, buf, turn, mean, rstd);
+    statistics<G, NV, kVec>(here, cols, lane, a.eps, buf, turn, mean, rstd);
     if (a.mean && lane == 0) {
       a.mean[r] = mean;
       a.rstd[r] = rstd;
     }
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) v[i] = (v[i] - mean) * rstd;
-    if (w) {
-      load_row<G, NV>(w, a.cols, vec, lane, p);
+    for (int i = 0; i < NV; ++i) {
+      float v[8], p[8];
+      here[i].get(v);
+      if (kCodes) store_codes<G, kVec>(a.codes + r * a.cols, a.exps + r * blocks, cols, lane, i, v);
 #pragma unroll
-      for (int i = 0; i < NV * 8; ++i) v[i] *= p[i];
-    }
-    if (b) {
-      load_row<G, NV>(b, a.cols, vec, lane, p);
+      for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd;
+      if (a.w) {
+        Chunk<W, kVec> w;
+        w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
+        w.get(p);
 #pragma unroll
-      for (int i = 0; i < NV * 8; ++i) v[i] += p[i];
+        for (int j = 0; j < 8; ++j) v[j] *= p[j];
+      }
+      if (a.b) {
+        Chunk<W, kVec> b;
+        b.template load<G>(static_cast<const W*>(a.b), cols, lane, i);
+        b.get(p);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += p[j];
+      }
+      store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, v);
     }
-    store_row<G, NV>(static_cast<T*>(a.y) + r * a.cols, a.cols, vec, lane, v);
   }
 }
 
-template <int G, int NV, typename T, typename W>
-__global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args a, bool vec) {
+// The input of the backward pass: x, or what a checkpoint holds of it.
+template <int G, int NV, bool kVec, bool kCodes, typename T>
+struct Input {
+  Chunk<T, kVec> x[NV];
+  float mean, rstd;
+  __device__ __forceinline__ void load(const Args& a, int64_t r, int cols, int lane) {
+    mean = a.mean[r];
+    rstd = a.rstd[r];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      x[i].template load<G>(static_cast<const T*>(a.x) + r * a.x_stride, cols, lane, i);
+  }
+  __device__ __forceinline__ void prepare(const Args&, int, int, Sums*, int&) {}
+};
+template <int G, int NV, bool kVec, typename T>
+struct Input<G, NV, kVec, true, T> {
+  Codes<kVec> x[NV];
+  float mean, rstd;
+  __device__ __forceinline__ void load(const Args& a, int64_t r, int cols, int lane) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      x[i].template load<G>(a.codes_in + r * a.cols, a.exps_in + r * ckpt::blocks_of(a.cols), cols, lane, i);
+  }
+  __device__ __forceinline__ void prepare(const Args& a, int cols, int lane, Sums* buf, int& turn) {
+    statistics<G, NV, kVec>(x, cols, lane, a.eps, buf, turn, mean, rstd);
+  }
+};
+
+template <int G, int NV, bool kVec, bool kCodes, typename T, typename W>
+__global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args a) {
   constexpr int kRows = Shape<G>::kRows;
   __shared__ Sums buf[Shape<G>::kBuf];
   __shared__ float fold[kRows > 1 ? kRows * 32 * 8 : 1];
   int turn = 0;
-  const int lane = threadIdx.x % G, slot = threadIdx.x / G;
-  const W* w = static_cast<const W*>(a.w);
+  const int lane = threadIdx.x % G, slot = threadIdx.x / G, cols = static_cast<int>(a.cols);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
+  const T* gradient = static_cast<const T*>(a.g);
   const float n = static_cast<float>(a.cols);
-  const int64_t blocks = ckpt::blocks_of(a.cols);
   float dw[NV * 8] = {}, db[NV * 8] = {};
-  for (int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + slot; r < a.rows;
-       r += static_cast<int64_t>(gridDim.x) * kRows) {
-    float h[NV * 8], g[NV * 8];
-    float mean, rstd;
-    load_row<G, NV>(static_cast<const T*>(a.g) + r * a.g_stride, a.cols, vec, lane, g);
-    if (a.codes_in) {
-      load_codes<G, NV>(a.codes_in + r * a.cols, a.exps_in + r * blocks, a.cols, vec, lane, h);
-      statistics<G, NV>(h, a.cols, vec, lane, a.eps, buf, turn, mean, rstd);
-    } else {
-      load_row<G, NV>(static_cast<const T*>(a.x) + r * a.x_stride, a.cols, vec, lane, h);
-      mean = a.mean[r];
-      rstd = a.rstd[r];
-    }
+  Input<G, NV, kVec, kCodes, T> next, here;
+  Chunk<T, kVec> next_g[NV], g[NV];
+  int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + slot;
+  const auto load = [&](int64_t row) {
+    next.load(a, row, cols, lane);
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) {
-      h[i] = (h[i] - mean) * rstd;  // beyond the row g is 0, so h counts for nothing
-      dw[i] = fmaf(g[i], h[i], dw[i]);
-      db[i] += g[i];
-    }
-    if (!a.dx) continue;
-    if (w) {
-      float p[NV * 8];
-      load_row<G, NV>(w, a.cols, vec, lane, p);
+    for (int i = 0; i < NV; ++i) next_g[i].template load<G>(gradient + row * a.g_stride, cols, lane, i);
+  };
+  if (r < a.rows) load(r);
+  for (; r < a.rows; r += step) {
+    here = next;
 #pragma unroll
-      for (int i = 0; i < NV * 8; ++i) g[i] *= p[i];
-    }
+    for (int i = 0; i < NV; ++i) g[i] = next_g[i];
+    if (r + step < a.rows) load(r + step);
+    here.prepare(a, cols, lane, buf, turn);
     Sums s = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) {
-      s.a += g[i];
-      s.b = fmaf(g[i], h[i], s.b);
+    for (int i = 0; i < NV; ++i) {
+      float h[8], d[8], p[8];
+      here.x[i].get(h);
+      g[i].get(d);
+      if (a.w) {
+        Chunk<W, kVec> w;
+        w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
+        w.get(p);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = (h[j] - here.mean) * here.rstd;  // beyond the row the gradient is 0, and counts for nothing
+        dw[i * 8 + j] = fmaf(d[j], x, dw[i * 8 + j]);
+        db[i * 8 + j] += d[j];
+        const float gw = a.w ? d[j] * p[j] : d[j];
+        s.a += gw;
+        s.b = fmaf(gw, x, s.b);
+      }
     }
+    if (!a.dx) continue;
     s = row_sums<G>(s, buf, turn);
     const float c1 = s.a / n, c2 = s.b / n;
 #pragma unroll
-    for (int i = 0; i < NV * 8; ++i) g[i] = rstd * (g[i] - c1 - h[i] * c2);
-    store_row<G, NV>(static_cast<T*>(a.dx) + r * a.cols, a.cols, vec, lane, g);
+    for (int i = 0; i < NV; ++i) {
+      float h[8], d[8], p[8];
+      here.x[i].get(h);
+      g[i].get(d);
+      if (a.w) {
+        Chunk<W, kVec> w;
+        w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
+        w.get(p);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float x = (h[j] - here.mean) * here.rstd;
+        d[j] = here.rstd * ((a.w ? d[j] * p[j] : d[j]) - c1 - x * c2);
+      }
+      store_chunk<G, kVec>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, d);
+    }
   }
   if (!a.dw && !a.db) return;
   float* part = a.parts + blockIdx.x * 2 * a.cols;
@@ -282,16 +380,16 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
         for (int j = 0; j < 8; ++j) fold[(slot * 8 + j) * 32 + lane] = v[j];
         __syncthreads();
         // thread (slot, lane) adds up column j = slot of lane's eight
-        float s = 0.f;
+        float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) s += fold[(k * 8 + slot) * 32 + lane];
-        const int64_t c = column<G>(vec, lane, i, slot);
-        if (c < a.cols) part[which * a.cols + c] = s;
+        for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + slot) * 32 + lane];
+        const int c = column<G, kVec>(lane, i, slot);
+        if (c < cols) part[which * a.cols + c] = sum;
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int64_t c = column<G>(vec, lane, i, j);
-          if (c < a.cols) part[which * a.cols + c] = v[j];
+          const int c = column<G, kVec>(lane, i, j);
+          if (c < cols) part[which * a.cols + c] = v[j];
         }
       }
     }
@@ -440,39 +538,84 @@ bool vectors_fit(const Args& a, bool backward) {
   return ok;
 }
 
-constexpr int64_t kMaxRegisters = 16384;
+// Threads a row and chunks a thread. A backward pass also sums 16 floats a chunk, so it takes fewer.
+struct Form {
+  int threads, chunks;
+};
+Form forward_form(int64_t rows, int64_t cols) {
+  if (cols <= 1024) return {32, cols <= 256 ? 1 : cols <= 512 ? 2 : 4};
+  if (rows < 296 && cols <= 4096) return {512, 1};  // few rows: short ones in time, not many in flight
+  return cols <= 4096 ? Form{128, 4} : cols <= 8192 ? Form{256, 4} : cols <= 16384 ? Form{512, 4} : Form{kLong, 0};
+}
+Form backward_form(int64_t cols) {
+  if (cols <= 512) return {32, cols <= 256 ? 1 : 2};
+  return cols <= 2048 ? Form{128, 2} : cols <= 4096 ? Form{256, 2} : cols <= 8192 ? Form{512, 2} : Form{kLong, 0};
+}
 
-// Threads a row: as few as hold it in 16 values each.
-int threads_for(int64_t cols) { return cols <= 512 ? 32 : cols <= 2048 ? 128 : cols <= 8192 ? 512 : 1024; }
+int blocks_of_rows(int64_t rows, const Form& f, int per_sm) {
+  const int64_t groups = f.threads == 32 ? (rows + 7) / 8 : rows;
+  return static_cast<int>(std::min<int64_t>(groups, 148ll * per_sm));
+}
 
-template <typename T, typename W, int G, int NV>
-cudaError_t launch(const Args& a, bool backward, int grid, bool vec, cudaStream_t stream) {
-  if (backward)
-    backward_kernel<G, NV, T, W><<<grid, Shape<G>::kThreads, 0, stream>>>(a, vec);
-  else
-    forward_kernel<G, NV, T, W><<<grid, Shape<G>::kThreads, 0, stream>>>(a, vec);
+template <typename T, typename W, int G, int NV, bool kVec, bool kCodes>
+cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
+  const int per_sm = std::max(1, 2048 / Shape<G>::kThreads / 2);
+  const int grid = blocks_of_rows(a.rows, Form{G, NV}, per_sm);
+  forward_kernel<G, NV, kVec, kCodes, T, W><<<grid, Shape<G>::kThreads, 0, stream>>>(a);
   return cudaGetLastError();
+}
+
+template <typename T, typename W, bool kVec, bool kCodes>
+cudaError_t dispatch_forward(const Args& a, cudaStream_t stream) {
+  const Form f = forward_form(a.rows, a.cols);
+  if (f.threads == 32)
+    return !kVec || f.chunks == 4 ? launch_forward<T, W, 32, 4, kVec, kCodes>(a, stream)
+           : f.chunks == 2        ? launch_forward<T, W, 32, kVec ? 2 : 4, kVec, kCodes>(a, stream)
+                                  : launch_forward<T, W, 32, kVec ? 1 : 4, kVec, kCodes>(a, stream);
+  if (f.threads == 512)
+    return f.chunks == 1 ? launch_forward<T, W, 512, 1, kVec, kCodes>(a, stream)
+                         : launch_forward<T, W, 512, 4, kVec, kCodes>(a, stream);
+  return f.threads == 128 && kVec ? launch_forward<T, W, kVec ? 128 : 256, 4, kVec, kCodes>(a, stream)
+                                  : launch_forward<T, W, 256, 4, kVec, kCodes>(a, stream);
+}
+
+template <typename T, typename W, int G, int NV, bool kVec, bool kCodes>
+cudaError_t launch_backward(const Args& a, cudaStream_t stream) {
+  backward_kernel<G, NV, kVec, kCodes, T, W>
+      <<<backward_parts(a.rows, a.cols), Shape<G>::kThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T, typename W, bool kVec, bool kCodes>
+cudaError_t dispatch_backward(const Args& a, cudaStream_t stream) {
+  const Form f = backward_form(a.cols);
+  if (f.threads == 32)
+    return f.chunks == 1 && kVec ? launch_backward<T, W, 32, kVec ? 1 : 2, kVec, kCodes>(a, stream)
+                                 : launch_backward<T, W, 32, 2, kVec, kCodes>(a, stream);
+  if (f.threads == 512) return launch_backward<T, W, 512, 2, kVec, kCodes>(a, stream);
+  return f.threads == 128 ? launch_backward<T, W, 128, 2, kVec, kCodes>(a, stream)
+                          : launch_backward<T, W, 256, 2, kVec, kCodes>(a, stream);
 }
 
 template <typename T, typename W>
 cudaError_t dispatch(const Args& a, bool backward, cudaStream_t stream) {
-  const int grid =
-      backward ? backward_parts(a.rows, a.cols)
-               : static_cast<int>(std::min<int64_t>(a.cols <= 512 ? (a.rows + 7) / 8 : a.rows, 148 * 64));
   const bool vec = vectors_fit<T, W>(a, backward);
-  if (a.cols > kMaxRegisters) {
-    if (backward)
-      backward_long_kernel<T, W><<<grid, kLong, 0, stream>>>(a);
-    else
-      forward_long_kernel<T, W><<<grid, kLong, 0, stream>>>(a);
+  if (backward) {
+    if (backward_form(a.cols).threads == kLong) {
+      backward_long_kernel<T, W><<<backward_parts(a.rows, a.cols), kLong, 0, stream>>>(a);
+      return cudaGetLastError();
+    }
+    if (a.codes_in)
+      return vec ? dispatch_backward<T, W, true, true>(a, stream) : dispatch_backward<T, W, false, true>(a, stream);
+    return vec ? dispatch_backward<T, W, true, false>(a, stream) : dispatch_backward<T, W, false, false>(a, stream);
+  }
+  if (forward_form(a.rows, a.cols).threads == kLong) {
+    forward_long_kernel<T, W><<<blocks_of_rows(a.rows, Form{kLong, 0}, 2), kLong, 0, stream>>>(a);
     return cudaGetLastError();
   }
-  const int g = threads_for(a.cols);
-  const bool one = a.cols <= 8ll * g;
-  if (g == 32) return one ? launch<T, W, 32, 1>(a, backward, grid, vec, stream) : launch<T, W, 32, 2>(a, backward, grid, vec, stream);
-  if (g == 128) return one ? launch<T, W, 128, 1>(a, backward, grid, vec, stream) : launch<T, W, 128, 2>(a, backward, grid, vec, stream);
-  if (g == 512) return one ? launch<T, W, 512, 1>(a, backward, grid, vec, stream) : launch<T, W, 512, 2>(a, backward, grid, vec, stream);
-  return launch<T, W, 1024, 2>(a, backward, grid, vec, stream);
+  if (a.codes)
+    return vec ? dispatch_forward<T, W, true, true>(a, stream) : dispatch_forward<T, W, false, true>(a, stream);
+  return vec ? dispatch_forward<T, W, true, false>(a, stream) : dispatch_forward<T, W, false, false>(a, stream);
 }
 
 cudaError_t dispatch_types(const Args& a, bool backward, cudaStream_t stream) {
@@ -484,9 +627,8 @@ cudaError_t dispatch_types(const Args& a, bool backward, cudaStream_t stream) {
 }  // namespace
 
 int backward_parts(int64_t rows, int64_t cols) {
-  const int64_t groups = cols <= 512 ? (rows + 7) / 8 : rows;
-  const int per_sm = cols <= 512 ? 4 : cols <= 2048 ? 4 : 1;
-  return static_cast<int>(std::min<int64_t>(groups, 148 * per_sm));
+  const Form f = backward_form(cols);
+  return blocks_of_rows(rows, f, f.threads == 32 ? 3 : f.threads == 128 ? 4 : f.threads == 256 ? 2 : 1);
 }
 
 cudaError_t forward(const Args& a, cudaStream_t stream) {

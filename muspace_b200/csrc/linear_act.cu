@@ -163,7 +163,7 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   }
   if (a.db && a.out) {
     float* parts =
-        static_cast<float*>(arena.take(static_cast<size_t>(column_parts(a.rows)) * a.out * sizeof(float)));
+        static_cast<float*>(arena.take(static_cast<size_t>(column_parts(a.rows, a.out)) * a.out * sizeof(float)));
     if (!arena.measuring) LIN_TRY(column_sums(a.dtype, dz, parts, a.db, stream));
   }
   return cudaSuccess;

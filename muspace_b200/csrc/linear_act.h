@@ -131,8 +131,8 @@ cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, const Ope
 cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
                           cudaStream_t stream);
 cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream);
-// sums[c] = sum over rows of src (its planes added up); parts: [column_parts(rows), cols] floats
-int column_parts(int64_t rows);
+// sums[c] = sum over rows of src (its planes added up); parts: [column_parts(rows, cols), cols] floats
+int column_parts(int64_t rows, int64_t cols);
 cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream);
 
 }  // namespace lin

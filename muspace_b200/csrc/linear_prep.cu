@@ -84,49 +84,61 @@ __global__ void __launch_bounds__(kThreads)
 
 // ---- column sums -------------------------------------------------------------------
 
-// A block takes 64 columns (a lane two of them, a warp a row at a time) and a
+// A block takes 256 columns (a lane eight of them, a warp a row at a time) and a
 // range of rows; the ranges' sums go to `parts` and are added in order by the
-// second kernel, so the result does not depend on scheduling.
-constexpr int kSumCols = 64, kSumWarps = 8;
+// second kernel, so the result does not depend on scheduling. 40000 x 512:
+// two columns a lane and at most 64 ranges left too few loads on their way
+// (25 us, 1.6 TB/s).
+constexpr int kSumCols = 256, kSumWarps = 8;
 
 __global__ void __launch_bounds__(32 * kSumWarps)
     column_parts_kernel(const bf16* __restrict__ src, int64_t ld, int64_t plane, int planes, int64_t rows,
                         int64_t cols, int64_t rows_per_part, float* __restrict__ parts) {
   __shared__ float buf[kSumWarps][kSumCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 2;
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
   const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
-  float s0 = 0.f, s1 = 0.f;
-  if (c < cols) {
-    for (int q = 0; q < planes; ++q) {
+  const int count = static_cast<int>(min(static_cast<int64_t>(8), cols - c));
+  float s[8] = {};
+  if (count > 0) {
+    for (int q = planes - 1; q >= 0; --q) {
       const bf16* p = src + q * plane + c;
-#pragma unroll 8
+#pragma unroll 4
       for (int64_t r = begin + warp; r < end; r += kSumWarps) {
-        const uint32_t u = *reinterpret_cast<const uint32_t*>(p + r * ld);  // ld is even: a pair never splits
-        s0 += __uint_as_float(u << 16);
-        s1 += __uint_as_float(u & 0xffff0000u);
+        float v[8];
+        load8(p + r * ld, v);  // rows are padded to eight: what lies beyond is not kept
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] += v[j];
       }
     }
   }
-  buf[warp][lane * 2] = s0;
-  buf[warp][lane * 2 + 1] = s1;
-  __syncthreads();
-  if (threadIdx.x < kSumCols) {
-    const int64_t col = blockIdx.x * static_cast<int64_t>(kSumCols) + threadIdx.x;
-    float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kSumWarps; ++w) s += buf[w][threadIdx.x];
-    if (col < cols) parts[blockIdx.y * cols + col] = s;
-  }
+  for (int j = 0; j < 8; ++j) buf[warp][lane + 32 * j] = s[j];
+  __syncthreads();
+  const int j = threadIdx.x >> 5;  // column j of the lane's eight
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSumWarps; ++w) sum += buf[w][lane + 32 * j];
+  if (j < count) parts[blockIdx.y * cols + c + j] = sum;
 }
 
 template <typename T>
-__global__ void add_parts_kernel(const float* __restrict__ parts, int count, int64_t cols, T* __restrict__ sums) {
-  const int64_t c = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  if (c >= cols) return;
+__global__ void __launch_bounds__(1024)
+    add_parts_kernel(const float* __restrict__ parts, int count, int64_t cols, T* __restrict__ sums) {
+  __shared__ float buf[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * 32ll + lane;
   float s = 0.f;
-  for (int i = 0; i < count; ++i) s += parts[i * cols + c];
-  sums[c] = from_float<T>(s);
+  if (c < cols)
+    for (int i = warp; i < count; i += 32) s += parts[i * cols + c];
+  buf[warp][lane] = s;
+  __syncthreads();
+  if (warp == 0 && c < cols) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += buf[i][lane];
+    sums[c] = from_float<T>(s);
+  }
 }
 
 }  // namespace
@@ -151,22 +163,26 @@ cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Opera
   return cudaGetLastError();
 }
 
-int column_parts(int64_t rows) { return static_cast<int>(std::min<int64_t>((rows + 127) / 128, 64)); }
+int column_parts(int64_t rows, int64_t cols) {
+  const int64_t across = (cols + kSumCols - 1) / kSumCols;
+  return static_cast<int>(std::min<int64_t>((rows + 31) / 32, std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(across, 1))));
+}
 
 cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream) {
-  const int count = column_parts(src.rows);
+  const int count = column_parts(src.rows, src.cols);
   if (src.cols == 0) return cudaSuccess;
-  if (count > 0) {
+  if (src.rows > 0) {
     const int64_t per = (src.rows + count - 1) / count;
     const dim3 grid(static_cast<unsigned>((src.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
     column_parts_kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.plane, src.planes, src.rows, src.cols,
                                                             per, parts);
   }
-  const unsigned blocks = static_cast<unsigned>((src.cols + 127) / 128);
+  const unsigned blocks = static_cast<unsigned>((src.cols + 31) / 32);
+  const int filled = src.rows > 0 ? count : 0;
   if (out_dtype == DType::kF32)
-    add_parts_kernel<<<blocks, 128, 0, stream>>>(parts, count, src.cols, static_cast<float*>(sums));
+    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, filled, src.cols, static_cast<float*>(sums));
   else
-    add_parts_kernel<<<blocks, 128, 0, stream>>>(parts, count, src.cols, static_cast<bf16*>(sums));
+    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, filled, src.cols, static_cast<bf16*>(sums));
   return cudaGetLastError();
 }
 

@@ -54,16 +54,25 @@ def report(operator: str, backend: str, decision: DispatchDecision, selected: st
     record_dispatch_report(_report_of(operator, backend, selected, decision.device, reason, native_available))
 
 
-def decide(operator: str, backend: str, tensor: torch.Tensor, others: dict[str, torch.Tensor | None]):
-    """``(native module, decision)`` of a call, or RuntimeError with its report."""
+# the decisions for CUDA tensors with the native library at hand, which depend on nothing else
+_CUDA_DECISIONS: dict[tuple[str, str], DispatchDecision] = {}
+
+
+def decide(operator: str, backend: str, tensor: torch.Tensor, *others: torch.Tensor | None):
+    """``(native module, decision)`` of a call whose tensors share a device, or RuntimeError with its report."""
     module = native_module()
-    decision = _explain_dispatch(tensor, backend=backend, native_available=module is not None, operator=operator)
+    usual = module is not None and tensor.is_cuda
+    decision = _CUDA_DECISIONS.get((operator, backend)) if usual else None
+    if decision is None:
+        decision = _explain_dispatch(tensor, backend=backend, native_available=module is not None, operator=operator)
+        if usual:
+            _CUDA_DECISIONS[operator, backend] = decision
     reason = decision.reason if decision.backend == "error" else None
     if reason is None:
         device = tensor.device
-        for name, other in others.items():
+        for other in others:
             if other is not None and other.device != device:
-                reason = f"{name} is on {other.device}, input is on {device}"
+                reason = f"a tensor is on {other.device}, input is on {device}"
                 break
     if reason is not None:
         report(operator, backend, decision, "error", reason, module is not None)
@@ -77,6 +86,12 @@ def rows_of(tensor: torch.Tensor) -> tuple[torch.Tensor, int]:
     if tensor.dim() != 2:
         tensor = tensor.reshape(-1, tensor.size(-1)) if tensor.numel() else tensor.new_empty(
             (tensor.shape[:-1].numel(), tensor.size(-1)))
-    if tensor.stride(1) != 1 and tensor.size(1) > 1:
+    stride, inner = tensor.stride()
+    if inner != 1 and tensor.size(1) > 1:
         tensor = tensor.contiguous()
-    return tensor, tensor.stride(0)
+        stride = tensor.stride(0)
+    return tensor, stride
+
+
+def pointer(tensor: torch.Tensor | None) -> int | None:
+    return None if tensor is None else tensor.data_ptr()

@@ -49,7 +49,7 @@ def checkpoint_pack(input: torch.Tensor, *, backend: str = "auto") -> Checkpoint
     check_tensor(input, "input")
     if input.dim() == 0:
         raise ValueError("input must have at least one dimension")
-    module, decision = decide("checkpoint_pack", backend, input, {})
+    module, decision = decide("checkpoint_pack", backend, input)
     source = input.detach()
     rows, stride = rows_of(source.float() if source.dtype == torch.float16 else source)
     codes, exponents = pack_rows(module, rows, stride)
@@ -70,7 +70,7 @@ def checkpoint_unpack(checkpoint: Checkpoint8, dtype: torch.dtype | None = None,
         raise TypeError("dtype must be float16, bfloat16 or float32")
     if codes.dim() == 0 or tuple(exponents.shape) != (*codes.shape[:-1], -(-codes.size(-1) // BLOCK)):
         raise ValueError("exponents must have the leading shape of codes and one byte for each block of 32")
-    module, decision = decide("checkpoint_unpack", backend, codes, {"exponents": exponents})
+    module, decision = decide("checkpoint_unpack", backend, codes, exponents)
     codes, exponents = codes.contiguous(), exponents.contiguous()
     out = torch.empty(codes.shape, dtype=torch.float32 if dtype == torch.float16 else dtype, device=codes.device)
     width = codes.size(-1)

@@ -11,21 +11,17 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ..runtime.native import LayerNormArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, report, rows_of
+from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, pointer, report, rows_of
 from .checkpoint8 import BLOCK
 
 OPERATOR_NAME = "layer_norm"
-
-
-def _ptr(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None else tensor.data_ptr()
 
 
 def _forward(module: NativeModule, x, weight, bias, eps: float, keep: str | None):
     """``(output, statistics, codes, exponents)``; ``keep``: "statistics", "int8" or None."""
     rows, stride = rows_of(x)
     count, width = rows.shape
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(x.shape)
     statistics = codes = exponents = None
     mean = rstd = None
     if keep == "statistics":
@@ -37,8 +33,8 @@ def _forward(module: NativeModule, x, weight, bias, eps: float, keep: str | None
         exponents = torch.empty((count, -(-width // BLOCK)), dtype=torch.uint8, device=x.device)
     kind = weight if weight is not None else bias
     args = LayerNormArgs(DTYPE_CODES[x.dtype], DTYPE_CODES[x.dtype if kind is None else kind.dtype], count, width,
-                         stride, 0, eps, rows.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), mean, rstd,
-                         _ptr(codes), _ptr(exponents))
+                         stride, 0, eps, rows.data_ptr(), pointer(weight), pointer(bias), out.data_ptr(), mean, rstd,
+                         pointer(codes), pointer(exponents))
     module.plain_call("msda_layer_norm_forward")(x.device, args)
     return out, statistics, codes, exponents
 
@@ -60,7 +56,7 @@ class _LayerNormFunction(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         g, g_stride = rows_of(grad)
         count, width = g.shape
-        dx = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if need_x else None
+        dx = grad.new_empty(grad.shape) if need_x else None
         dw, db = (torch.empty(width, dtype=ctx.kind, device=grad.device) if need else None for need in (need_w, need_b))
         stride, mean, rstd = 0, None, None
         if x is not None:
@@ -68,8 +64,8 @@ class _LayerNormFunction(torch.autograd.Function):
             mean = statistics.data_ptr()
             rstd = mean + 4 * count
         args = LayerNormArgs(DTYPE_CODES[grad.dtype], DTYPE_CODES[ctx.kind], count, width, stride, g_stride, ctx.eps,
-                             _ptr(x), _ptr(weight), None, None, mean, rstd, _ptr(codes), _ptr(exponents),
-                             g.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db))
+                             pointer(x), pointer(weight), None, None, mean, rstd, pointer(codes), pointer(exponents),
+                             g.data_ptr(), pointer(dx), pointer(dw), pointer(db))
         native_module().plain_call("msda_layer_norm_backward")(grad.device, args)
         return dx, dw, db, None, None
 
@@ -88,17 +84,18 @@ def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     check_checkpoint(checkpoint)
     if input.dim() == 0:
         raise ValueError("input must have at least one dimension")
-    given = {name: t for name, t in (("weight", weight), ("bias", bias)) if t is not None}
-    for name, tensor in given.items():
+    for name, tensor in (("weight", weight), ("bias", bias)):
+        if tensor is None:
+            continue
         if not isinstance(tensor, torch.Tensor):
             raise TypeError(f"{name} must be a tensor")
         if tensor.dtype not in (input.dtype, torch.float32):
             raise TypeError(f"{name} must have the dtype of input ({input.dtype}) or float32")
-        if tuple(tensor.shape) != (input.size(-1),):
+        if tensor.shape != input.shape[-1:]:
             raise ValueError(f"{name} must have shape ({input.size(-1)},), got {tuple(tensor.shape)}")
-    if len({t.dtype for t in given.values()}) > 1:
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one dtype")
-    module, decision = decide(OPERATOR_NAME, backend, input, given)
+    module, decision = decide(OPERATOR_NAME, backend, input, weight, bias)
     dtype = input.dtype
     if dtype == torch.float16:
         input, weight, bias = (t if t is None else t.float() for t in (input, weight, bias))

@@ -16,7 +16,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ..runtime.native import LinearArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, report, rows_of
+from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, pointer, report, rows_of
 from .checkpoint8 import pack_rows
 
 OPERATOR_NAME = "linear_act"
@@ -31,16 +31,11 @@ def _keeps_slope(activation: str, in_features: int, checkpoint: str | None) -> b
     return activation != "none" and checkpoint is None and in_features > _RECOMPUTE_UP_TO
 
 
-def _ptr(tensor: torch.Tensor | None) -> int | None:
-    return None if tensor is None else tensor.data_ptr()
-
-
 def _forward(module: NativeModule, x, weight, bias, residual, activation: str, keep_slope: bool):
     """``(output, slope)``; every tensor float32 or bfloat16."""
     rows, x_stride = rows_of(x)
     weight, w_stride = rows_of(weight)
-    shape = (*x.shape[:-1], weight.size(0))
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty((*x.shape[:-1], weight.size(0)))
     slope = None
     if keep_slope:
         slope = torch.empty(rows.size(0), weight.size(0), device=x.device,
@@ -51,8 +46,8 @@ def _forward(module: NativeModule, x, weight, bias, residual, activation: str, k
     if bias is not None:
         bias = bias.contiguous()
     args = LinearArgs(DTYPE_CODES[x.dtype], ACTIVATIONS[activation], rows.size(0), weight.size(1), weight.size(0),
-                      x_stride, w_stride, r_stride, weight.size(0), 0, rows.data_ptr(), weight.data_ptr(), _ptr(bias),
-                      _ptr(residual), out.data_ptr(), _ptr(slope))
+                      x_stride, w_stride, r_stride, weight.size(0), 0, rows.data_ptr(), weight.data_ptr(), pointer(bias),
+                      pointer(residual), out.data_ptr(), pointer(slope))
     module.plain_call("msda_linear_act_forward")(x.device, args)
     return out, slope
 
@@ -86,13 +81,12 @@ class _LinearActFunction(torch.autograd.Function):
         dx = dw = db = None
         if need_x or need_w or need_b:
             g, g_stride = rows_of(grad)
-            new = lambda shape: torch.empty(shape, dtype=grad.dtype, device=grad.device)  # noqa: E731
             if need_x:
-                dx = new(x_shape)
+                dx = grad.new_empty(x_shape)
             if need_w:
-                dw = new(w_shape)
+                dw = grad.new_empty(w_shape)
             if need_b:
-                db = new(w_shape[:1])
+                db = grad.new_empty(w_shape[:1])
             x_stride = w_stride = 0
             if x is not None:
                 x, x_stride = rows_of(x)
@@ -101,8 +95,9 @@ class _LinearActFunction(torch.autograd.Function):
             if bias is not None:
                 bias = bias.contiguous()
             args = LinearArgs(DTYPE_CODES[grad.dtype], ACTIVATIONS[ctx.activation], g.size(0), w_shape[1], w_shape[0],
-                              x_stride, w_stride, 0, 0, g_stride, _ptr(x), _ptr(weight), _ptr(bias), None, None,
-                              _ptr(slope), g.data_ptr(), _ptr(codes), _ptr(exponents), _ptr(dx), _ptr(dw), _ptr(db))
+                              x_stride, w_stride, 0, 0, g_stride, pointer(x), pointer(weight), pointer(bias), None,
+                              None, pointer(slope), g.data_ptr(), pointer(codes), pointer(exponents), pointer(dx),
+                              pointer(dw), pointer(db))
             native_module().plain_call("msda_linear_act_backward")(grad.device, args)
         return dx, dw, db, grad if need_r else None, None, None
 
@@ -135,7 +130,7 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
     out_features, in_features = weight.shape
     if input.size(-1) != in_features:
         raise ValueError(f"input has {input.size(-1)} features, weight takes {in_features}")
-    if bias is not None and tuple(bias.shape) != (out_features,):
+    if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"bias must have shape ({out_features},), got {tuple(bias.shape)}")
     if residual is not None:
         shape = (*input.shape[:-1], out_features)
@@ -144,7 +139,7 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
                 residual = residual.expand(shape)
             except RuntimeError as exc:
                 raise ValueError(f"residual {tuple(residual.shape)} cannot be broadcast to {tuple(shape)}") from exc
-    module, decision = decide(OPERATOR_NAME, backend, input, {"weight": weight, "bias": bias, "residual": residual})
+    module, decision = decide(OPERATOR_NAME, backend, input, weight, bias, residual)
     dtype = input.dtype
     if dtype == torch.float16:
         input, weight, bias, residual = (t if t is None else t.float() for t in (input, weight, bias, residual))

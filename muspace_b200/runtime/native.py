@@ -120,6 +120,11 @@ def _stream_of(tensors) -> int:
     return 0
 
 
+# the current stream as a number; torch.cuda.current_stream builds an object for it (2 us)
+_raw_stream: Callable[[int], int] = getattr(
+    torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 # argument kinds of the DLPack entry points: "t" tensor, "i" int, "f" float (the stream is appended)
 _SIGNATURES: dict[str, tuple[str, ...]] = {
     "ms_deform_attn_forward": ("t",) * 6 + ("i",),
@@ -240,7 +245,7 @@ class NativeModule:
                     workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
                     args[0].workspace = workspace.data_ptr()
                     args[0].workspace_bytes = size.value
-            if symbol(*args, torch.cuda.current_stream(device).cuda_stream) != 0:
+            if symbol(*args, _raw_stream(device.index)) != 0:
                 raise RuntimeError(f"{name}: {self.last_error()}")
 
         def call(device: torch.device, *args: Any) -> None:
