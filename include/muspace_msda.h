@@ -455,11 +455,6 @@ MSDA_API int msda_linear_act_forward(const msda_linear_t *args, void *stream);
 MSDA_API int msda_linear_act_backward_workspace(const msda_linear_t *args, size_t *bytes);
 MSDA_API int msda_linear_act_backward(const msda_linear_t *args, void *stream);
 
-/* Waits inside the linear kernels that gave up on the current device since the
- * library loaded. 0 is expected; anything else means that results since then
- * may be wrong. Synchronises with the device. */
-MSDA_API int msda_linear_wait_timeouts(unsigned int *count);
-
 /*
  * Layer norm over the last dimension: h = (x - mean) * rstd with rstd =
  * 1 / sqrt(var + eps) (var: the mean square of x - mean), y = h w + b;
@@ -495,6 +490,11 @@ typedef struct {
 MSDA_API int msda_layer_norm_forward(const msda_layer_norm_t *args, void *stream);
 MSDA_API int msda_layer_norm_backward_workspace(const msda_layer_norm_t *args, size_t *bytes);
 MSDA_API int msda_layer_norm_backward(const msda_layer_norm_t *args, void *stream);
+
+/* Waits inside the linear and layer-norm kernels that gave up on the current
+ * device since the library loaded. 0 is expected; anything else means that
+ * results since then may be wrong. Synchronises with the device. */
+MSDA_API int msda_layer_wait_timeouts(unsigned int *count);
 
 /* Message of the last failed call on this thread ("" after a success). The
  * reference raised it as a TVM-FFI exception (csrc/ffi/tensor_utils.hpp:13-34). */

@@ -196,10 +196,13 @@ int msda_linear_act_backward(const msda_linear_t* args, void* stream) {
   });
 }
 
-int msda_linear_wait_timeouts(unsigned int* count) {
+int msda_layer_wait_timeouts(unsigned int* count) {
   return guarded([&] {
     require(count != nullptr, "count is null");
-    check_launch(lin::wait_timeouts(count), "msda_linear_wait_timeouts");
+    unsigned int linear = 0, norm = 0;
+    check_launch(lin::wait_timeouts(&linear), "msda_layer_wait_timeouts");
+    check_launch(lnorm::wait_timeouts(&norm), "msda_layer_wait_timeouts");
+    *count = linear + norm;
   });
 }
 

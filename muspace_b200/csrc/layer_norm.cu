@@ -14,6 +14,7 @@
 // are read again for each pass, from L2 where they fit.
 #include <algorithm>
 
+#include "async_device.cuh"
 #include "checkpoint8.cuh"
 #include "layer_norm.h"
 #include "linear_device.cuh"
@@ -21,8 +22,12 @@
 namespace lnorm {
 namespace {
 
+using lin::add2;
 using lin::bf16;
+using lin::both;
+using lin::fma2;
 using lin::from_float;
+using lin::mul2;
 using lin::to_float;
 
 struct Sums {
@@ -37,21 +42,30 @@ __device__ __forceinline__ Sums warp_sums(Sums s) {
   }
   return s;
 }
+__device__ __forceinline__ float warp_sums(float s) {
+#pragma unroll
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+__device__ __forceinline__ Sums operator+(Sums s, Sums t) { return Sums{s.a + t.a, s.b + t.b}; }
 
 // Sums over the G threads of a row. With more than a warp, `buf` alternates
 // between two halves, so one barrier per sum is enough.
-template <int G>
-__device__ __forceinline__ Sums row_sums(Sums s, Sums* buf, int& turn) {
+template <int G, bool kNamed = false, typename S>
+__device__ __forceinline__ S row_sums(S s, Sums* buf, int& turn) {
   s = warp_sums(s);
   if (G == 32) return s;
   constexpr int kWarps = G / 32;
-  Sums* half = buf + turn * kWarps;
+  S* half = reinterpret_cast<S*>(buf + turn * kWarps);
   turn ^= 1;
-  if ((threadIdx.x & 31) == 0) half[threadIdx.x >> 5] = s;
-  __syncthreads();
-  Sums t = {0.f, 0.f};
+  if ((threadIdx.x & 31) == 0) half[(threadIdx.x % G) >> 5] = s;
+  if (kNamed)  // one of several groups of G threads in the block
+    asm volatile("bar.sync %0, %1;" ::"r"(static_cast<int>(threadIdx.x / G) + 1), "n"(G) : "memory");
+  else
+    __syncthreads();
+  S t = half[0];
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) t.a += half[w].a, t.b += half[w].b;
+  for (int w = 1; w < kWarps; ++w) t = t + half[w];
   return t;
 }
 
@@ -81,7 +95,7 @@ struct Chunk {
       zero();
     }
   }
-  __device__ __forceinline__ void get(float v[8]) const { lin::load8(reinterpret_cast<const T*>(u), v); }
+  __device__ __forceinline__ void get(float2 v[4]) const { lin::load8(reinterpret_cast<const T*>(u), &v[0].x); }
 };
 template <typename T>
 struct Chunk<T, false> {
@@ -98,9 +112,9 @@ struct Chunk<T, false> {
       v[j] = c < cols ? to_float(row[c]) : 0.f;
     }
   }
-  __device__ __forceinline__ void get(float w[8]) const {
+  __device__ __forceinline__ void get(float2 w[4]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = v[j];
+    for (int j = 0; j < 4; ++j) w[j] = make_float2(v[2 * j], v[2 * j + 1]);
   }
 };
 
@@ -119,7 +133,7 @@ struct Codes {
       e = __ldg(exps + c / ckpt::kBlock);
     }
   }
-  __device__ __forceinline__ void get(float v[8]) const { ckpt::values_of(u, e, v); }
+  __device__ __forceinline__ void get(float2 v[4]) const { ckpt::values_of(u, e, &v[0].x); }
 };
 template <>
 struct Codes<false> {
@@ -132,9 +146,9 @@ struct Codes<false> {
       v[j] = c < cols ? row[c] * ckpt::scale_of(exps[c / ckpt::kBlock]) : 0.f;
     }
   }
-  __device__ __forceinline__ void get(float w[8]) const {
+  __device__ __forceinline__ void get(float2 w[4]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = v[j];
+    for (int j = 0; j < 4; ++j) w[j] = make_float2(v[2 * j], v[2 * j + 1]);
   }
 };
 
@@ -185,28 +199,31 @@ __device__ __forceinline__ void store_codes(int8_t* row, uint8_t* exps, int cols
 template <int G, int NV, bool kVec, typename C>
 __device__ __forceinline__ void statistics(const C x[NV], int cols, int lane, float eps, Sums* buf, int& turn,
                                            float& mean, float& rstd) {
-  Sums s = {0.f, 0.f};
+  float2 t = both(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float v[8];
+    float2 v[4];
     x[i].get(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s.a += v[j];
+    for (int j = 0; j < 4; ++j) t = add2(t, v[j]);
   }
   const float n = static_cast<float>(cols);
-  mean = row_sums<G>(s, buf, turn).a / n;
-  s.a = 0.f;
+  mean = row_sums<G>(t.x + t.y, buf, turn) / n;
+  const float2 minus = both(-mean);
+  t = both(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    float v[8];
+    float2 v[4];
     x[i].get(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float d = column<G, kVec>(lane, i, kVec ? 0 : j) < cols ? v[j] - mean : 0.f;
-      s.a = fmaf(d, d, s.a);
+    for (int j = 0; j < 4; ++j) {
+      float2 d = add2(v[j], minus);
+      if (column<G, kVec>(lane, i, kVec ? 0 : 2 * j) >= cols) d.x = 0.f;
+      if (column<G, kVec>(lane, i, kVec ? 0 : 2 * j + 1) >= cols) d.y = 0.f;
+      t = fma2(d, d, t);
     }
   }
-  rstd = rsqrtf(row_sums<G>(s, buf, turn).a / n + eps);
+  rstd = rsqrtf(row_sums<G>(t.x + t.y, buf, turn) / n + eps);
 }
 
 // Rows per block and block size for G threads a row.
@@ -243,28 +260,29 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       a.mean[r] = mean;
       a.rstd[r] = rstd;
     }
+    const float2 scale = both(rstd), minus = both(-mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float v[8], p[8];
+      float2 v[4], p[4];
       here[i].get(v);
-      if (kCodes) store_codes<G, kVec>(a.codes + r * a.cols, a.exps + r * blocks, cols, lane, i, v);
+      if (kCodes) store_codes<G, kVec>(a.codes + r * a.cols, a.exps + r * blocks, cols, lane, i, &v[0].x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean) * rstd;
+      for (int j = 0; j < 4; ++j) v[j] = mul2(add2(v[j], minus), scale);
       if (a.w) {
         Chunk<W, kVec> w;
         w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
         w.get(p);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= p[j];
+        for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], p[j]);
       }
       if (a.b) {
         Chunk<W, kVec> b;
         b.template load<G>(static_cast<const W*>(a.b), cols, lane, i);
         b.get(p);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += p[j];
+        for (int j = 0; j < 4; ++j) v[j] = add2(v[j], p[j]);
       }
-      store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, v);
+      store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, &v[0].x);
     }
   }
 }
@@ -297,8 +315,14 @@ struct Input<G, NV, kVec, true, T> {
   }
 };
 
+// Blocks that an SM holds; as many are launched, so that all rows are under way at once.
+constexpr int backward_blocks(int threads) {
+  return threads == 32 ? 3 : threads == 128 ? 4 : threads == 256 ? 2 : 1;
+}
+
 template <int G, int NV, bool kVec, bool kCodes, typename T, typename W>
-__global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<G>::kThreads, G == 32 && (NV > 1 || !kVec) ? 2 : backward_blocks(G))
+    backward_kernel(const Args a) {
   constexpr int kRows = Shape<G>::kRows;
   __shared__ Sums buf[Shape<G>::kBuf];
   __shared__ float fold[kRows > 1 ? kRows * 32 * 8 : 1];
@@ -307,7 +331,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
   const int64_t step = static_cast<int64_t>(gridDim.x) * kRows;
   const T* gradient = static_cast<const T*>(a.g);
   const float n = static_cast<float>(a.cols);
-  float dw[NV * 8] = {}, db[NV * 8] = {};
+  float2 dw[NV][4] = {}, db[NV][4] = {};
   Input<G, NV, kVec, kCodes, T> next, here;
   Chunk<T, kVec> next_g[NV], g[NV];
   int64_t r = blockIdx.x * static_cast<int64_t>(kRows) + slot;
@@ -316,6 +340,11 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
 #pragma unroll
     for (int i = 0; i < NV; ++i) next_g[i].template load<G>(gradient + row * a.g_stride, cols, lane, i);
   };
+  const auto weight = [&](int i, float2 p[4]) {
+    Chunk<W, kVec> w;
+    w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
+    w.get(p);
+  };
   if (r < a.rows) load(r);
   for (; r < a.rows; r += step) {
     here = next;
@@ -323,46 +352,41 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
     for (int i = 0; i < NV; ++i) g[i] = next_g[i];
     if (r + step < a.rows) load(r + step);
     here.prepare(a, cols, lane, buf, turn);
-    Sums s = {0.f, 0.f};
+    const float2 scale = both(here.rstd), minus = both(-here.mean);
+    float2 sum = both(0.f), dot = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float h[8], d[8], p[8];
+      float2 h[4], d[4], p[4];
       here.x[i].get(h);
       g[i].get(d);
-      if (a.w) {
-        Chunk<W, kVec> w;
-        w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
-        w.get(p);
-      }
+      if (a.w) weight(i, p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = (h[j] - here.mean) * here.rstd;  // beyond the row the gradient is 0, and counts for nothing
-        dw[i * 8 + j] = fmaf(d[j], x, dw[i * 8 + j]);
-        db[i * 8 + j] += d[j];
-        const float gw = a.w ? d[j] * p[j] : d[j];
-        s.a += gw;
-        s.b = fmaf(gw, x, s.b);
+      for (int j = 0; j < 4; ++j) {
+        h[j] = mul2(add2(h[j], minus), scale);  // beyond the row the gradient is 0, and counts for nothing
+        dw[i][j] = fma2(d[j], h[j], dw[i][j]);
+        db[i][j] = add2(db[i][j], d[j]);
+        if (a.w) d[j] = mul2(d[j], p[j]);
+        sum = add2(sum, d[j]);
+        dot = fma2(d[j], h[j], dot);
       }
     }
     if (!a.dx) continue;
-    s = row_sums<G>(s, buf, turn);
-    const float c1 = s.a / n, c2 = s.b / n;
+    const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
+    // rstd (g w - c1 - h c2), with h = (x - mean) rstd
+    const float2 c1 = both(-here.rstd * (s.a / n)), c2 = both(-here.rstd * (s.b / n));
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      float h[8], d[8], p[8];
+      float2 h[4], d[4], p[4];
       here.x[i].get(h);
       g[i].get(d);
-      if (a.w) {
-        Chunk<W, kVec> w;
-        w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
-        w.get(p);
-      }
+      if (a.w) weight(i, p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float x = (h[j] - here.mean) * here.rstd;
-        d[j] = here.rstd * ((a.w ? d[j] * p[j] : d[j]) - c1 - x * c2);
+      for (int j = 0; j < 4; ++j) {
+        h[j] = mul2(add2(h[j], minus), scale);
+        if (a.w) d[j] = mul2(d[j], p[j]);
+        d[j] = fma2(h[j], c2, fma2(d[j], scale, c1));
       }
-      store_chunk<G, kVec>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, d);
+      store_chunk<G, kVec>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, &d[0].x);
     }
   }
   if (!a.dw && !a.db) return;
@@ -373,7 +397,10 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
     for (int i = 0; i < NV; ++i) {
       float v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = which ? db[i * 8 + j] : dw[i * 8 + j];
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = which ? db[i][j].x : dw[i][j].x;
+        v[2 * j + 1] = which ? db[i][j].y : dw[i][j].y;
+      }
       if (kRows > 1) {  // the block's rows, in order
         __syncthreads();
 #pragma unroll
@@ -396,6 +423,199 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) backward_kernel(const Args
   }
 }
 
+// The backward pass of long rows. A row's sums need a barrier in its middle, and
+// registers hold no more than the next row meanwhile (8192 columns of bfloat16:
+// 129 us for 8192 rows); so here the rows' data comes to shared memory by bulk
+// copies, several rows ahead, and is read from there twice. Two groups of 256
+// threads take rows in turn, so that one computes while the other waits at its
+// barrier (one group of 512: 113 us). A group's stage is free again when its
+// next row's barrier has been passed.
+constexpr int kRingThreads = 512, kGroup = 256;
+constexpr int kRingBytes = 192 * 1024;
+constexpr int kMaxStages = 8;
+
+template <int NV, bool kCodes, typename T, typename W>
+__global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Args a, int stages) {
+  constexpr int G = kGroup, kGroups = kRingThreads / kGroup;
+  extern __shared__ __align__(16) uint8_t ring[];  // stages of x (or codes) and g, `stages` for each group
+  __shared__ Sums bufs[kGroups][2 * (G / 32)];
+  __shared__ __align__(8) uint64_t bars[kGroups][kMaxStages];
+  int turn = 0;
+  const int lane = threadIdx.x % G, group = threadIdx.x / G, cols = static_cast<int>(a.cols);
+  const T* gradient = static_cast<const T*>(a.g);
+  const float n = static_cast<float>(a.cols);
+  const uint32_t x_bytes = cols * (kCodes ? 1 : sizeof(T)), g_bytes = cols * sizeof(T);
+  const uint32_t stage_bytes = x_bytes + g_bytes;
+  const int64_t blocks = ckpt::blocks_of(a.cols);
+  Sums* buf = bufs[group];
+  const uint8_t* mine = ring + group * stages * stage_bytes;
+  const uint32_t bar0 = async::smem_addr(bars[group]), ring0 = async::smem_addr(mine);
+  if (lane == 0) {
+    for (int s = 0; s < stages; ++s) async::barrier_init(bar0 + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+  const auto fetch = [&](int64_t r, int s) {
+    const uint32_t bar = bar0 + 8 * s, dst = ring0 + s * stage_bytes;
+    async::expect_bytes(bar, stage_bytes);
+    async::copy_bytes(dst, kCodes ? static_cast<const void*>(a.codes_in + r * a.cols)
+                                  : static_cast<const void*>(static_cast<const T*>(a.x) + r * a.x_stride),
+                      x_bytes, bar);
+    async::copy_bytes(dst + x_bytes, gradient + r * a.g_stride, g_bytes, bar);
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups, first = blockIdx.x + static_cast<int64_t>(group) * gridDim.x;
+  if (lane == 0)
+    for (int s = 0; s < stages; ++s)
+      if (first + s * step < a.rows) fetch(first + s * step, s);
+  const auto weight = [&](int i, float2 p[4]) {
+    Chunk<W, true> w;
+    w.template load<G>(static_cast<const W*>(a.w), cols, lane, i);
+    w.get(p);
+  };
+  float2 dw[NV][4] = {}, db[NV][4] = {};
+  int stage = 0, last = -1;
+  uint32_t phase = 0;
+  bool dead = false;
+  for (int64_t r = first; r < a.rows; r += step) {
+    const uint8_t* at = mine + stage * stage_bytes;
+    const T* g_row = reinterpret_cast<const T*>(at + x_bytes);
+    uint32_t exps[NV];
+    if (kCodes) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = column<G, true>(lane, i, 0);
+        exps[i] = c < cols ? __ldg(a.exps_in + r * blocks + c / ckpt::kBlock) : 1u;
+      }
+    }
+    async::wait(bar0 + 8 * stage, phase, dead);
+    const auto x_at = [&](int i, float2 v[4]) {
+      const int c = column<G, true>(lane, i, 0);
+      if (c >= cols) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = both(0.f);
+      } else if (kCodes) {
+        ckpt::values_of(*reinterpret_cast<const uint2*>(at + c), exps[i], &v[0].x);
+      } else {
+        lin::load8(reinterpret_cast<const T*>(at) + c, &v[0].x);
+      }
+    };
+    const auto g_at = [&](int i, float2 v[4]) {
+      const int c = column<G, true>(lane, i, 0);
+      if (c >= cols) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = both(0.f);
+      } else {
+        lin::load8(g_row + c, &v[0].x);
+      }
+    };
+    float mean, rstd;
+    if (kCodes) {
+      float2 t = both(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float2 v[4];
+        x_at(i, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t = add2(t, v[j]);
+      }
+      mean = row_sums<G, true>(t.x + t.y, buf, turn) / n;
+      t = both(0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float2 v[4];
+        x_at(i, v);
+        if (column<G, true>(lane, i, 0) < cols) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[j] = add2(v[j], both(-mean));
+            t = fma2(v[j], v[j], t);
+          }
+        }
+      }
+      rstd = rsqrtf(row_sums<G, true>(t.x + t.y, buf, turn) / n + a.eps);
+    } else {
+      mean = __ldg(a.mean + r);
+      rstd = __ldg(a.rstd + r);
+    }
+    const float2 scale = both(rstd), minus = both(-mean);
+    float2 sum = both(0.f), dot = both(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float2 h[4], d[4], p[4];
+      x_at(i, h);
+      g_at(i, d);
+      if (a.w) weight(i, p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        h[j] = mul2(add2(h[j], minus), scale);
+        dw[i][j] = fma2(d[j], h[j], dw[i][j]);
+        db[i][j] = add2(db[i][j], d[j]);
+        if (a.w) d[j] = mul2(d[j], p[j]);
+        sum = add2(sum, d[j]);
+        dot = fma2(d[j], h[j], dot);
+      }
+    }
+    const Sums s = row_sums<G, true>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
+    // every thread is past the row before: its stage takes the row that comes `stages` after it
+    if (lane == 0 && last >= 0) {
+      const int64_t ahead = r + (stages - 1) * step;
+      if (ahead < a.rows) fetch(ahead, last);
+    }
+    if (a.dx) {
+      const float2 c1 = both(-rstd * (s.a / n)), c2 = both(-rstd * (s.b / n));
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        float2 h[4], d[4], p[4];
+        x_at(i, h);
+        g_at(i, d);
+        if (a.w) weight(i, p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          h[j] = mul2(add2(h[j], minus), scale);
+          if (a.w) d[j] = mul2(d[j], p[j]);
+          d[j] = fma2(h[j], c2, fma2(d[j], scale, c1));
+        }
+        store_chunk<G, true>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, &d[0].x);
+      }
+    }
+    last = stage;
+    if (++stage == stages) stage = 0, phase ^= 1;
+  }
+  if (!a.dw && !a.db) return;
+  // the groups' sums, in order, over the ring
+  static_assert(kGroups == 2, "the first group adds the second's sums");
+  float4* left = reinterpret_cast<float4*>(ring);
+  __syncthreads();
+  if (group == 1) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; j += 2) {
+        left[((i * 4 + j) / 2 * 2) * G + lane] = make_float4(dw[i][j].x, dw[i][j].y, dw[i][j + 1].x, dw[i][j + 1].y);
+        left[((i * 4 + j) / 2 * 2 + 1) * G + lane] = make_float4(db[i][j].x, db[i][j].y, db[i][j + 1].x, db[i][j + 1].y);
+      }
+  }
+  __syncthreads();
+  if (group == 1) return;
+  float* part = a.parts + blockIdx.x * 2 * a.cols;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const float4 p = left[((i * 4 + j) / 2 * 2) * G + lane], q = left[((i * 4 + j) / 2 * 2 + 1) * G + lane];
+      dw[i][j] = add2(dw[i][j], make_float2(p.x, p.y));
+      dw[i][j + 1] = add2(dw[i][j + 1], make_float2(p.z, p.w));
+      db[i][j] = add2(db[i][j], make_float2(q.x, q.y));
+      db[i][j + 1] = add2(db[i][j + 1], make_float2(q.z, q.w));
+    }
+    const int c = column<G, true>(lane, i, 0);
+    if (c < cols) {
+      lin::store8(part + c, &dw[i][0].x);
+      lin::store8(part + a.cols + c, &db[i][0].x);
+    }
+  }
+}
+
 // Rows beyond the registers: a block of 1024 threads a row, the row read again
 // for each pass; dw and db are summed in `parts`, whose columns a thread owns.
 constexpr int kLong = 1024;
@@ -414,15 +634,15 @@ template <typename T>
 __device__ __forceinline__ void long_statistics(const Args& a, int64_t r, Sums* buf, int& turn, float& mean,
                                                 float& rstd) {
   const float n = static_cast<float>(a.cols);
-  Sums s = {0.f, 0.f};
-  for (int64_t c = threadIdx.x; c < a.cols; c += kLong) s.a += value_at<T>(a, r, c);
-  mean = row_sums<kLong>(s, buf, turn).a / n;
-  s.a = 0.f;
+  float s = 0.f;
+  for (int64_t c = threadIdx.x; c < a.cols; c += kLong) s += value_at<T>(a, r, c);
+  mean = row_sums<kLong>(s, buf, turn) / n;
+  s = 0.f;
   for (int64_t c = threadIdx.x; c < a.cols; c += kLong) {
     const float d = value_at<T>(a, r, c) - mean;
-    s.a = fmaf(d, d, s.a);
+    s = fmaf(d, d, s);
   }
-  rstd = rsqrtf(row_sums<kLong>(s, buf, turn).a / n + a.eps);
+  rstd = rsqrtf(row_sums<kLong>(s, buf, turn) / n + a.eps);
 }
 
 template <typename T, typename W>
@@ -597,10 +817,35 @@ cudaError_t dispatch_backward(const Args& a, cudaStream_t stream) {
                           : launch_backward<T, W, 256, 2, kVec, kCodes>(a, stream);
 }
 
+// Rows of the ring: whole 16-byte units, and at least two stages.
+template <typename T>
+int ring_stages(const Args& a) {
+  const int64_t bytes = a.cols * ((a.codes_in ? 1 : sizeof(T)) + sizeof(T));
+  if (a.cols % 16 != 0 || (a.codes_in && reinterpret_cast<uintptr_t>(a.codes_in) % 16 != 0)) return 0;
+  return static_cast<int>(std::min<int64_t>(kRingBytes / bytes / (kRingThreads / kGroup), kMaxStages));  // of a group
+}
+
+template <typename T, typename W, int NV, bool kCodes>
+cudaError_t launch_ring(const Args& a, int stages, cudaStream_t stream) {
+  const auto kernel = backward_ring_kernel<NV, kCodes, T, W>;
+  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (err != cudaSuccess) return err;
+  const size_t rows = static_cast<size_t>(stages) * (kRingThreads / kGroup) * a.cols * ((kCodes ? 1 : sizeof(T)) + sizeof(T));
+  const size_t bytes = std::max<size_t>(rows, static_cast<size_t>(NV) * 8 * 2 * kGroup * sizeof(float));  // and one group's sums
+  kernel<<<backward_parts(a.rows, a.cols), kRingThreads, bytes, stream>>>(a, stages);
+  return cudaGetLastError();
+}
+
 template <typename T, typename W>
 cudaError_t dispatch(const Args& a, bool backward, cudaStream_t stream) {
   const bool vec = vectors_fit<T, W>(a, backward);
   if (backward) {
+    const int stages = ring_stages<T>(a);
+    if (vec && a.cols > 2048 && a.cols <= 8192 && stages >= 2) {
+      if (a.codes_in)
+        return a.cols <= 4096 ? launch_ring<T, W, 2, true>(a, stages, stream) : launch_ring<T, W, 4, true>(a, stages, stream);
+      return a.cols <= 4096 ? launch_ring<T, W, 2, false>(a, stages, stream) : launch_ring<T, W, 4, false>(a, stages, stream);
+    }
     if (backward_form(a.cols).threads == kLong) {
       backward_long_kernel<T, W><<<backward_parts(a.rows, a.cols), kLong, 0, stream>>>(a);
       return cudaGetLastError();
@@ -628,8 +873,10 @@ cudaError_t dispatch_types(const Args& a, bool backward, cudaStream_t stream) {
 
 int backward_parts(int64_t rows, int64_t cols) {
   const Form f = backward_form(cols);
-  return blocks_of_rows(rows, f, f.threads == 32 ? 3 : f.threads == 128 ? 4 : f.threads == 256 ? 2 : 1);
+  return blocks_of_rows(rows, f, f.threads == 32 && f.chunks > 1 ? 2 : backward_blocks(f.threads));
 }
+
+cudaError_t wait_timeouts(unsigned int* count) { return async::read_timeouts(count); }
 
 cudaError_t forward(const Args& a, cudaStream_t stream) {
   return a.rows == 0 || a.cols == 0 ? cudaSuccess : dispatch_types(a, false, stream);

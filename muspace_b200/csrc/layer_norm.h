@@ -35,6 +35,7 @@ struct Args {
 int backward_parts(int64_t rows, int64_t cols);
 cudaError_t forward(const Args& a, cudaStream_t stream);
 cudaError_t backward(const Args& a, cudaStream_t stream);
+cudaError_t wait_timeouts(unsigned int* count);
 
 }  // namespace lnorm
 

@@ -29,10 +29,16 @@
 #include <algorithm>
 #include <atomic>
 
+#include "async_device.cuh"
 #include "linear_device.cuh"
 
 namespace lin {
 namespace {
+
+using async::barrier_init;
+using async::expect_bytes;
+using async::smem_addr;
+using async::wait;
 
 constexpr int kTileM = 128;       // rows of a block's tile
 constexpr int kBlockK = 64;       // k of a stage: 128 bytes, one swizzle row
@@ -44,7 +50,6 @@ constexpr int kBoxBytes = 32 * 128;  // a box of the epilogue: 32 rows of 128 by
 constexpr int kRingBytes = 160 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
-constexpr long long kWaitClocks = 4000000000ll;  // about two seconds
 
 template <int BN, int CG>
 struct Shape {
@@ -73,45 +78,7 @@ struct Job {
   bool vec;          // finishing: rows of extra, out and slope start on 16-byte boundaries
 };
 
-__device__ unsigned int g_wait_timeouts;
-
 // ---- PTX ---------------------------------------------------------------------------
-
-__device__ __forceinline__ uint32_t smem_addr(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void barrier_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// Waits have a limit. One that runs out is counted, and from then on the
-// thread polls each barrier once: the kernel ends, with wrong results and a
-// count that msda_linear_wait_timeouts reports.
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& dead) {
-  if (try_wait(bar, parity)) return;
-  if (dead) return;
-  const long long start = clock64();
-  do {
-    if (try_wait(bar, parity)) return;
-  } while (clock64() - start < kWaitClocks);
-  dead = true;
-  atomicAdd(&g_wait_timeouts, 1u);
-}
 
 // The address of `addr` in block `rank` of the cluster.
 __device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
@@ -596,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     // the copies that are still in flight land before the block's memory goes
+    dead = false;
     for (int x = 0; x < S::kStages; ++x) {
       wait(empty(s), phase ^ 1, dead);
       if (++s == S::kStages) s = 0, phase ^= 1;
@@ -1072,6 +1040,6 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
   return cudaGetLastError();
 }
 
-cudaError_t wait_timeouts(unsigned int* count) { return cudaMemcpyFromSymbol(count, g_wait_timeouts, sizeof(*count)); }
+cudaError_t wait_timeouts(unsigned int* count) { return async::read_timeouts(count); }
 
 }  // namespace lin
