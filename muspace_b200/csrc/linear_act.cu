@@ -85,7 +85,7 @@ int plane_pairs(const Operand& a, const Operand& b) {
 }
 
 cudaError_t run_product(Product& pr, Arena& arena, cudaStream_t stream) {
-  const Plan plan = plan_product(pr.m, pr.n, pr.k, plane_pairs(pr.a, pr.b), pr.a_mn || pr.b_mn, multiprocessors());
+  const Plan plan = plan_product(pr.dtype, pr.m, pr.n, pr.k, plane_pairs(pr.a, pr.b), multiprocessors());
   if (finished_apart(pr, plan)) pr.partial = static_cast<float*>(arena.take(partial_bytes(plan, pr.m, pr.n)));
   return arena.measuring ? cudaSuccess : launch_product(pr, plan, stream);
 }

@@ -111,7 +111,7 @@ struct Plan {
   int kblocks;   // k blocks of 64 in one range
 };
 
-Plan plan_product(int64_t m, int64_t n, int64_t k, int pairs_of_planes, bool any_mn, int sms);
+Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs_of_planes, int sms);
 // Whether the product leaves float32 sums that a second kernel adds up and
 // finishes: ranges of k, and outputs that TMA cannot address (rows off 16-byte
 // boundaries).

@@ -27,6 +27,8 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2eLow = 1.9259630e-8f;  // log2(e) - kLog2e
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 
 // Two float32 in one register pair: one instruction for both.
@@ -83,7 +85,17 @@ __device__ __forceinline__ void activate(Act act, float* z, float* s) {
   } else if (act == Act::kSilu) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const float g = kFast ? reciprocal_fast(1.f + exp2_fast(-kLog2e * z[j])) : 1.f / (1.f + expf(-z[j]));
+      float e;
+      if (kFast) {
+        e = exp2_fast(-kLog2e * z[j]);
+      } else {
+        // float32: with what the exponent lost in its rounding, to first order; below -88 the result is 0
+        const float x = fmaxf(z[j], -88.f), t = kLog2e * x;
+        const float lost = fmaf(-kLog2e, x, t) - kLog2eLow * x;
+        e = exp2_fast(-t);
+        e = fmaf(e, kLn2 * fminf(fmaxf(lost, -1.f), 1.f), e);
+      }
+      const float g = reciprocal_fast(1.f + e);
       if (kS) s[j] = g * fmaf(z[j], 1.f - g, 1.f);
       if (kY) z[j] *= g;
     }

@@ -18,12 +18,13 @@
 // along k, dx = dz W reads W across it, dW = dz^T x both. Nothing is transposed
 // in memory; the instruction and the tile's layout differ.
 //
-// float32 (three bfloat16 planes an operand): the same loop runs over the six
-// products of planes that reach 2^-24 of the result. The tensor core's float32
-// accumulator cuts where an FMA would round: 2^-25 of the result per step on
-// average, always towards zero. So the small products go first, and the sums
-// over 128 of k at a time are added up in registers: relative error 2.9e-6 with
-// 256 of k and the large products first, see planes_of.
+// float32 (three bfloat16 planes an operand): a stage holds all planes of its k,
+// and the six products of planes that reach 2^-24 of the result are issued on
+// it. The tensor core's float32 accumulator cuts where an FMA would round:
+// 2^-25 of what it holds per step on average, always towards zero. So the five
+// small products, 2^-8 of the result and below, have an accumulator of their
+// own, and the sums over 128 of k at a time are added up in registers: the
+// relative error is 1.3e-7, where one accumulator over 256 of k had 2.9e-6.
 #include <cuda.h>  // CUtensorMap and its enums only: the encoder comes from cudaGetDriverEntryPoint
 
 #include <algorithm>
@@ -51,16 +52,18 @@ constexpr int kRingBytes = 160 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
 
-template <int BN, int CG>
+template <int BN, int CG, bool kF32>
 struct Shape {
+  static constexpr int kPlanes = kF32 ? 3 : 1;
   static constexpr int kRowsB = BN / CG;  // rows of B in one block's stage
   static constexpr int kStageB = kRowsB * kBlockK * 2;
-  static constexpr int kStage = kStageA + kStageB;
+  static constexpr int kStage = kPlanes * (kStageA + kStageB);
   static constexpr int kStages = kRingBytes / kStage;
   static constexpr int kBarriers = 2 * kStages + 4 + kEpiWarps;
   // stages, the warps' staging, barriers, the tensor-memory address; and room to start on 1024 bytes
   static constexpr int kSmem = kStages * kStage + kEpiWarps * kBoxBytes + kBarriers * 8 + 16 + 1024;
-  static constexpr uint32_t kColumns = 2 * BN;
+  static constexpr int kAcc = kF32 ? 2 * BN : BN;  // columns of an accumulator: float32 has the small products' beside it
+  static constexpr uint32_t kColumns = 2 * kAcc;
   // a warp of the epilogue takes 32 rows and this many columns
   static constexpr int kCols = BN / 4 < 32 ? 32 : BN / 4;
   static constexpr int kWarps = 4 * (BN / kCols);
@@ -262,9 +265,8 @@ __device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
   return t;
 }
 
-// The planes of A and B in product `i`, the smallest products first: the
-// accumulator cuts at each step by up to 2^-24 of what it holds, and holds
-// 2^-8 of the result until the last product of planes begins.
+// The planes of A and B in product `i` of a stage; the last one is that of the
+// first planes.
 __device__ __forceinline__ void planes_of(const Job& j, int i, int& pa, int& pb) {
   if (j.pairs == 6) {
     pa = (0x010120 >> (4 * i)) & 3;
@@ -481,7 +483,7 @@ struct Maps {
 template <int BN, int CG, typename T, bool kF32>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Job job) {
-  using S = Shape<BN, CG>;
+  using S = Shape<BN, CG, kF32>;
   extern __shared__ uint8_t raw[];
   const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t boxes_base = ring + S::kStages * S::kStage;
@@ -529,37 +531,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       // boxes that hold rows of the tile; what a skipped box leaves in its place reaches no row or column that is kept
       const auto boxes = [](int have, int most) { return have <= 0 ? 0 : min(most, (have - 1) / 64 + 1); };
       const auto bytes_of = [&](int ma, int nb) {
-        return (job.pr.a_mn ? boxes(rows_m - ma, kTileM / 64) * 8192 : job.box_a * 128) +
-               (job.pr.b_mn ? boxes(rows_n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128);
+        return (job.pr.a_mn ? boxes(rows_m - ma, kTileM / 64) * 8192 : job.box_a * 128) * job.pr.a.planes +
+               (job.pr.b_mn ? boxes(rows_n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128) * job.pr.b.planes;
       };
       const int ma = t.m + rank * kTileM, nb = t.n + rank * S::kRowsB;
       const int boxes_a = boxes(rows_m - ma, kTileM / 64), boxes_b = boxes(rows_n - nb, S::kRowsB / 64);
       uint32_t bytes = bytes_of(t.m, t.n);
       if (CG == 2) bytes += bytes_of(t.m + kTileM, t.n + S::kRowsB);
-      for (int c = t.kb0; c < t.kb1; c += chunk) {
-        const int c1 = min(c + chunk, t.kb1);
-        for (int p = 0; p < job.pairs; ++p) {
-          int pa, pb;
-          planes_of(job, p, pa, pb);
-          for (int kb = c; kb < c1; ++kb) {
-            wait(empty(s), phase ^ 1, dead);
-            if (rank == 0) expect_bytes(full(s), bytes);
-            const uint32_t bar = CG == 2 ? in_block(full(s), 0) : full(s);
-            const uint32_t a = ring + s * S::kStage, b = a + kStageA;
-            const int k = kb * kBlockK;
-            if (job.pr.a_mn) {
-              for (int x = 0; x < boxes_a; ++x) copy_box<CG>(a + x * 8192, &maps.a, ma + x * 64, k, pa, bar);
-            } else {
-              copy_box<CG>(a, &maps.a, k, ma, pa, bar);
-            }
-            if (job.pr.b_mn) {
-              for (int x = 0; x < boxes_b; ++x) copy_box<CG>(b + x * 8192, &maps.b, nb + x * 64, k, pb, bar);
-            } else {
-              copy_box<CG>(b, &maps.b, k, nb, pb, bar);
-            }
-            if (++s == S::kStages) s = 0, phase ^= 1;
+      for (int kb = t.kb0; kb < t.kb1; ++kb) {
+        wait(empty(s), phase ^ 1, dead);
+        if (rank == 0) expect_bytes(full(s), bytes);
+        const uint32_t bar = CG == 2 ? in_block(full(s), 0) : full(s);
+        const uint32_t a = ring + s * S::kStage, b = a + S::kPlanes * kStageA;
+        const int k = kb * kBlockK;
+        for (int p = 0; p < job.pr.a.planes; ++p) {
+          if (job.pr.a_mn) {
+            for (int x = 0; x < boxes_a; ++x)
+              copy_box<CG>(a + p * kStageA + x * 8192, &maps.a, ma + x * 64, k, p, bar);
+          } else {
+            copy_box<CG>(a + p * kStageA, &maps.a, k, ma, p, bar);
           }
         }
+        for (int p = 0; p < job.pr.b.planes; ++p) {
+          if (job.pr.b_mn) {
+            for (int x = 0; x < boxes_b; ++x)
+              copy_box<CG>(b + p * S::kStageB + x * 8192, &maps.b, nb + x * 64, k, p, bar);
+          } else {
+            copy_box<CG>(b + p * S::kStageB, &maps.b, k, nb, p, bar);
+          }
+        }
+        if (++s == S::kStages) s = 0, phase ^= 1;
       }
     }
     // the copies that are still in flight land before the block's memory goes
@@ -577,18 +578,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (uint32_t i = first; i < items; i += step) {
       const Item t = item_of<BN, CG>(job, i);
       for (int c = t.kb0; c < t.kb1; c += chunk) {
-        const int steps = (min(c + chunk, t.kb1) - c) * job.pairs;
+        const int steps = min(c + chunk, t.kb1) - c;
         wait(acc_empty(buf), acc_phase ^ 1, dead);
         fence_after();
         for (int x = 0; x < steps; ++x) {
           wait(full(s), phase, dead);
           fence_after();
           if (lane == 0) {
-            const uint32_t a = ring + s * S::kStage;
-            const uint64_t da = tile_descriptor(a, job.pr.a_mn), db = tile_descriptor(a + kStageA, job.pr.b_mn);
+            const uint32_t a = ring + s * S::kStage, b = a + S::kPlanes * kStageA, acc = tmem + buf * S::kAcc;
+            for (int p = 0; p < (kF32 ? job.pairs : 1); ++p) {
+              int pa = 0, pb = 0;
+              if (kF32) planes_of(job, p, pa, pb);
+              const bool large = !kF32 || p + 1 == job.pairs;
+              const uint64_t da = tile_descriptor(a + pa * kStageA, job.pr.a_mn);
+              const uint64_t db = tile_descriptor(b + pb * S::kStageB, job.pr.b_mn);
 #pragma unroll
-            for (int kk = 0; kk < kBlockK / 16; ++kk)
-              mma<CG>(tmem + buf * BN, da + kk * step_a, db + kk * step_b, idesc, x > 0 || kk > 0);
+              for (int kk = 0; kk < kBlockK / 16; ++kk)
+                mma<CG>(large ? acc : acc + BN, da + kk * step_a, db + kk * step_b, idesc,
+                        x > 0 || kk > 0 || (!large && p > 0));
+            }
             commit<CG>(empty(s));
           }
           __syncwarp();
@@ -636,21 +644,23 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (extra && first < items && lane == 0) load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
     for (uint32_t i = first; i < items; i += step) {
       const int m = row_of(t), n0 = col_of(t);
-      uint32_t acc_at = tmem + lanes + buf * BN + group * S::kCols;
+      uint32_t acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
       if (kF32) {
         float acc[S::kCols / 16][16] = {};
         for (int c = t.kb0; c < t.kb1; c += chunk) {
           wait(acc_full(buf), acc_phase, dead);
           fence_after();
           const bool more = c + chunk < t.kb1;
-          acc_at = tmem + lanes + buf * BN + group * S::kCols;
+          acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
 #pragma unroll
           for (int q = 0; q < S::kCols / 16; ++q) {
-            uint32_t r[16];
+            uint32_t r[16], small[16];
             tmem_load16(acc_at + q * 16, r);
+            tmem_load16(acc_at + BN + q * 16, small);
             tmem_wait(r);
+            tmem_wait(small);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
+            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]) + __uint_as_float(small[x]);
             if (!more) tmem_store16(acc_at + q * 16, acc[q]);
           }
           if (more) {
@@ -917,7 +927,7 @@ bool vectors_fit(const Product& pr) {
 
 template <int BN, int CG, typename T, bool kF32>
 cudaError_t launch(const Maps& maps, const Job& job, int sms, cudaStream_t stream) {
-  using S = Shape<BN, CG>;
+  using S = Shape<BN, CG, kF32>;
   const auto kernel = product_kernel<BN, CG, T, kF32>;
   static std::atomic<uint64_t> ready{0};  // devices (of the first 64) that know the kernel's shared memory
   const uint64_t bit = job.device < 64 ? 1ull << job.device : 0;
@@ -944,13 +954,15 @@ cudaError_t launch(const Maps& maps, const Job& job, int sms, cudaStream_t strea
 
 template <typename T, bool kF32>
 cudaError_t launch_tile(const Plan& plan, const Maps& maps, const Job& job, int sms, cudaStream_t stream) {
-  if constexpr (!kF32) {
+  if constexpr (kF32) {
+    if (plan.bn == 128) return launch<128, 2, T, kF32>(maps, job, sms, stream);
+  } else {
     if (plan.bn == 256)
       return plan.pair == 2 ? launch<256, 2, T, kF32>(maps, job, sms, stream)
                             : launch<256, 1, T, kF32>(maps, job, sms, stream);
+    if (plan.bn == 128) return launch<128, 1, T, kF32>(maps, job, sms, stream);
   }
-  return plan.bn == 128 ? launch<128, 1, T, kF32>(maps, job, sms, stream)
-                        : launch<64, 1, T, kF32>(maps, job, sms, stream);
+  return launch<64, 1, T, kF32>(maps, job, sms, stream);
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -961,19 +973,21 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // one SM: a stage costs the longer of its products (2 clocks per column) and
 // its copies (64 bytes a clock), tiles overlap with the epilogue of the one
 // before, and partial sums cost their trip through L2 and a second launch.
-Plan plan_product(int64_t m, int64_t n, int64_t k, int pairs, bool any_mn, int sms) {
+Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs, int sms) {
+  const bool f32 = dtype == DType::kF32;
   const int kblocks = static_cast<int>(ceil_div(k, kBlockK));
   Plan best{64, 1, 1, kblocks};
   if (m == 0 || n == 0 || k == 0) return best;
   double best_time = 1e300;
   const struct {
     int bn, pair;
-  } shapes[] = {{64, 1}, {128, 1}, {256, 1}, {256, 2}};
+    bool bf16, f32;
+  } shapes[] = {{64, 1, true, true}, {128, 1, true, false}, {128, 2, false, true}, {256, 1, true, false}, {256, 2, true, false}};
   for (const auto& s : shapes) {
-    if (pairs > 1 && s.bn == 256) continue;  // float32 holds its sums in registers
+    if (!(f32 ? s.f32 : s.bf16)) continue;
     const int64_t tiles = ceil_div(m, kTileM * s.pair) * ceil_div(n, s.bn);
     const int64_t slots = sms / s.pair;
-    const double stage = std::max(2.0 * s.bn, (kStageA + s.bn * 128.0 / s.pair) / 64.0) * pairs;
+    const double stage = std::max(2.0 * s.bn * pairs, (f32 ? 3 : 1) * (kStageA + s.bn * 128.0 / s.pair) / 64.0);
     const double epilogue = 8.0 * s.bn + 600.0;
     for (int splits = 1; splits <= std::min(kblocks, 64); splits = splits < 4 ? splits + 1 : splits * 5 / 4) {
       const int per = static_cast<int>(ceil_div(kblocks, splits));
