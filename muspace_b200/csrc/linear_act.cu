@@ -92,6 +92,7 @@ cudaError_t run_product(Product& pr, Arena& arena, cudaStream_t stream) {
 
 cudaError_t forward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   if (a.rows == 0 || a.out == 0) return cudaSuccess;
+  if (few_rows(a)) return arena.measuring ? cudaSuccess : forward_few_rows(a, stream);
   Product pr;
   LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &pr.a, stream));
   LIN_TRY(operand_of(a.dtype, a.w, a.out, a.in, a.w_stride, arena, &pr.b, stream));
@@ -121,8 +122,15 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
       LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &x, stream));
     }
   }
-  if (a.act == Act::kNone) {
+  // db: the columns' sums come from whatever makes dz, over ranges of rows
+  const bool need_b = a.db != nullptr && a.out > 0;
+  const bool as_it_is = a.act == Act::kNone && direct(a.dtype, a.g, a.out, a.g_stride);
+  const int64_t parts_count = a.rows == 0 ? 0 : recompute ? (a.rows + 31) / 32 : column_parts(a.rows, a.out);
+  float* parts = nullptr;
+  if (need_b) parts = static_cast<float*>(arena.take(static_cast<size_t>(parts_count) * a.out * sizeof(float)));
+  if (as_it_is) {
     LIN_TRY(operand_of(a.dtype, a.g, a.rows, a.out, a.g_stride, arena, &dz, stream));
+    if (need_b && !arena.measuring) LIN_TRY(column_sums(dz, parts, stream));
   } else {
     dz = fresh(a.dtype, a.rows, a.out, f32 ? 3 : 1, arena);
     if (f32) LIN_TRY(add_flags(dz, arena, stream));
@@ -139,11 +147,19 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
       pr.epi.out_ld = dz.ld;
       pr.epi.out_plane = f32 ? dz.plane : 0;
       pr.epi.out_flags = dz.flags;
+      pr.epi.sums = parts;
       if (a.rows && a.out) LIN_TRY(run_product(pr, arena, stream));
     } else if (!arena.measuring) {
-      LIN_TRY(scale_operand(a.dtype, a.g, a.g_stride, a.slope, dz, stream));
+      const void* slope = a.act == Act::kNone ? nullptr : a.slope;
+      if (need_b)
+        LIN_TRY(operand_and_sums(a.dtype, a.g, a.g_stride, slope, dz, parts, stream));
+      else if (slope)
+        LIN_TRY(scale_operand(a.dtype, a.g, a.g_stride, slope, dz, stream));
+      else
+        LIN_TRY(copy_operand(a.dtype, a.g, a.g_stride, dz, stream));
     }
   }
+  if (need_b && !arena.measuring) LIN_TRY(add_parts(a.dtype, parts, parts_count, a.out, a.db, stream));
   if (a.dx && a.rows && a.in) {
     Product pr;
     pr.a = dz, pr.b = w, pr.b_mn = true;
@@ -160,11 +176,6 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
     pr.epi.out = a.dw;
     pr.epi.out_ld = a.in;
     LIN_TRY(run_product(pr, arena, stream));
-  }
-  if (a.db && a.out) {
-    float* parts =
-        static_cast<float*>(arena.take(static_cast<size_t>(column_parts(a.rows, a.out)) * a.out * sizeof(float)));
-    if (!arena.measuring) LIN_TRY(column_sums(a.dtype, dz, parts, a.db, stream));
   }
   return cudaSuccess;
 }

@@ -89,6 +89,7 @@ struct Epilogue {
   // kDz, float32: out is three bfloat16 planes, out_plane elements apart, with flags
   int64_t out_plane = 0;
   Flags* out_flags = nullptr;
+  float* sums = nullptr;  // kDz, may be null: [ceil(m / 32), n], the columns' sums over 32 rows
 };
 
 // ---- the product (linear_gemm.cu) --------------------------------------------------
@@ -130,9 +131,20 @@ cudaError_t copy_operand(DType dtype, const void* src, int64_t src_ld, const Ope
 // dst = g * slope
 cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
                           cudaStream_t stream);
+// Either of them (slope null: the copy), with the sums of dst's columns over
+// ranges of rows on the way: parts [column_parts(rows, cols), cols].
+cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
+                             float* parts, cudaStream_t stream);
 cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream);
-// sums[c] = sum over rows of src (its planes added up); parts: [column_parts(rows, cols), cols] floats
+// The sums of src's columns over ranges of rows; and of parts [count, cols], in order.
 int column_parts(int64_t rows, int64_t cols);
-cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream);
+cudaError_t column_sums(const Operand& src, float* parts, cudaStream_t stream);
+cudaError_t add_parts(DType out_dtype, const float* parts, int64_t count, int64_t cols, void* sums,
+                      cudaStream_t stream);
+
+// ---- few rows (linear_gemv.cu) -----------------------------------------------------
+
+bool few_rows(const Args& a);
+cudaError_t forward_few_rows(const Args& a, cudaStream_t stream);
 
 }  // namespace lin

@@ -111,6 +111,23 @@ __device__ __forceinline__ void activate(Act act, float* z, float* s) {
   }
 }
 
+// The sums over a warp's lanes of 16 values each: lane l gets that of value
+// l / 2. Each step halves the values a lane still carries.
+__device__ __forceinline__ float lane_sums16(const float v[16]) {
+  const int lane = threadIdx.x & 31;
+  float w[8];
+#pragma unroll
+  for (int n = 8, d = 16; n; n >>= 1, d >>= 1) {
+    const bool high = lane & d;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float lo = n == 8 ? v[j] : w[j], hi = n == 8 ? v[j + 8] : w[j + n];
+      w[j] = (high ? hi : lo) + __shfl_xor_sync(0xffffffffu, high ? lo : hi, d);
+    }
+  }
+  return w[0] + __shfl_xor_sync(0xffffffffu, w[0], 1);
+}
+
 // ---- float32 as three bfloat16 --------------------------------------------------------
 
 // x = hi + mid + lo to 2^-24 of x or better: each part is the bfloat16 nearest

@@ -418,22 +418,36 @@ __device__ __forceinline__ void take_back(uint32_t box, int row, int col, uint32
     put_unit(unit_at<kRowBytes>(box, row, col / 4 + u), w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
 }
 
-// Bias of columns [n, n + 16): the same for all lanes.
+// Bias of columns [n, n + 16), the same for all lanes: asked for before the sums
+// it is added to have come.
 template <typename T>
-__device__ __forceinline__ void add_bias16(const void* bias, int n, int cols, float v[16]) {
-  const T* p = static_cast<const T*>(bias) + n;
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && n + 16 <= cols) {
-    float b[16];
-    load8(p, b);
-    load8(p + 8, b + 8);
+struct Bias16 {
+  uint4 u[sizeof(T)];
+  __device__ __forceinline__ void load(const T* p, bool vec, int count) {
+    if (vec && count >= 16) {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) v[j] += b[j];
-  } else {
+      for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) u[k] = __ldg(reinterpret_cast<const uint4*>(p) + k);
+    } else {
+      uint4 few[sizeof(T)];  // only this copy has an address
+      copy_few(p, count, reinterpret_cast<T*>(few));
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (n + j < cols) v[j] += to_float(p[j]);
+      for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) u[k] = few[k];
+    }
   }
-}
+  static __device__ __noinline__ void copy_few(const T* p, int count, T* out) {
+    for (int j = 0; j < 16; ++j) out[j] = j < count ? p[j] : from_float<T>(0.f);
+  }
+  __device__ __forceinline__ void add(float v[16]) const {
+    float b[16];
+    load8(reinterpret_cast<const T*>(u), b);
+    load8(reinterpret_cast<const T*>(u) + 8, b + 8);
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float2 s = add2(make_float2(v[j], v[j + 1]), make_float2(b[j], b[j + 1]));
+      v[j] = s.x, v[j + 1] = s.y;
+    }
+  }
+};
 
 // Marks what is not finite among 16 outputs of row m.
 __device__ __forceinline__ void mark16(Flags* flags, const Product& pr, const float v[16], int64_t m, int64_t n) {
@@ -623,6 +637,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool extra = mode != Epilogue::kStore && e.extra != nullptr;
     const bool slope = mode == Epilogue::kFwd && e.slope != nullptr;
     const bool planes = sizeof(T) == 4 && mode == Epilogue::kDz;
+    const bool with_bias = mode != Epilogue::kStore && e.bias != nullptr;
+    const bool bias_vec = reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
     const bool repairs = kF32 && !job.apart && some_flag(job.pr);
     const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
     const auto col_of = [&](const Item& t) { return t.n + group * S::kCols; };
@@ -690,6 +706,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t r[16];
           tmem_load16(at, r);
           float x[16], v[16], s[16];
+          Bias16<T> bias;
+          if (with_bias) bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
           if (extra) get16<kRowBytes>(box, lane, c, x, T());
           tmem_wait(r);
 #pragma unroll
@@ -703,11 +721,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int j = 0; j < 16; ++j) v[j] = w[j];
           }
           if (mode != Epilogue::kStore) {
-            if (e.bias) add_bias16<T>(e.bias, n + c, rows_n, v);
+            if (with_bias) bias.add(v);
             if (mode == Epilogue::kDz) {
               activate<kFast, false, true, 16>(e.act, v, s);
 #pragma unroll
               for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
+              if (e.sums) {
+                if (m + lane >= rows_m) {  // rows of nothing: their gradient is zero, their slope may be anything
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) v[j] = 0.f;
+                }
+                const float sum = lane_sums16(v);
+                const int col = n + c + lane / 2;
+                if ((lane & 1) == 0 && m < rows_m && col < rows_n)
+                  e.sums[static_cast<int64_t>(m / 32) * rows_n + col] = sum;
+              }
               if (planes) {
                 tmem_store16(at, v);
                 mark16(e.out_flags, job.pr, v, m + lane, n + c);
@@ -811,23 +839,34 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Sums the ranges of k in order and runs the epilogue: a thread per eight columns.
-template <typename T, bool kF32>
+// Adds up the ranges of k and runs the epilogue: eight columns to kLanes lanes,
+// which take the ranges in turn. The order of the additions is fixed.
+template <typename T, bool kF32, int kLanes>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job job) {
   const Product& pr = job.pr;
   const int64_t per_row = (pr.n + 7) / 8, total = pr.m * per_row, ld = partial_ld(pr.n);
+  const int sub = threadIdx.x % kLanes;
   const bool repairs = kF32 && pr.k > 0 && some_flag(pr);
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t m = i / per_row, n = (i - m * per_row) * 8;
-    const bool whole8 = n + 8 <= pr.n;
+  for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) / kLanes; i - threadIdx.x % 32 / kLanes < total;
+       i += gridDim.x * 256ll / kLanes) {
+    const bool some = i < total;
+    const int64_t m = some ? i / per_row : 0, n = some ? (i - m * per_row) * 8 : 0;
     float v[8] = {};
-    for (int s = 0; s < job.splits; ++s) {
-      const float* p = pr.partial + (s * pr.m + m) * ld + n;
-      float w[8];
-      load_some(p, static_cast<int>(pr.n - n), whole8, w);
+    if (some) {
+      const float* p = pr.partial + m * ld + n;  // rows are padded to eight
+#pragma unroll 4
+      for (int s = sub; s < job.splits; s += kLanes) {
+        float w[8];
+        load8(p + s * pr.m * ld, w);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] += w[j];
+        for (int j = 0; j < 8; ++j) v[j] += w[j];
+      }
     }
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], d);
+    if (!some || sub != 0) continue;
     if (repairs) {
       float w[8];
 #pragma unroll
@@ -836,7 +875,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = w[j];
     }
-    if (job.vec && whole8) {
+    if (job.vec && n + 8 <= pr.n) {
       float x[8] = {}, b[8] = {};
       if (pr.epi.bias) load_some(static_cast<const T*>(pr.epi.bias) + n, 8, false, b);
       if (pr.epi.extra) load8(static_cast<const T*>(pr.epi.extra) + m * pr.epi.extra_ld + n, x);
@@ -845,6 +884,22 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job
       finish_some<T>(pr.epi, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), m, n, pr.m,
                      pr.n);
     }
+  }
+}
+
+// The columns' sums over 32 rows of what a finished epilogue left in `out`.
+template <typename T>
+__global__ void __launch_bounds__(256) sums_kernel(const __grid_constant__ Job job) {
+  const Product& pr = job.pr;
+  const int64_t total = (pr.m + 31) / 32 * pr.n;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t part = i / pr.n, n = i - part * pr.n;
+    float s = 0.f;
+    for (int64_t m = part * 32; m < min(pr.m, part * 32 + 32); ++m) {
+      const bf16* p = static_cast<const bf16*>(pr.epi.out) + m * pr.epi.out_ld + n;
+      for (int q = sizeof(T) == 4 ? 2 : 0; q >= 0; --q) s += __bfloat162float(p[q * pr.epi.out_plane]);
+    }
+    pr.epi.sums[i] = s;
   }
 }
 
@@ -1046,11 +1101,16 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
     job.splits = 0;  // an empty sum
   }
   const int64_t groups = pr.m * ((pr.n + 7) / 8);
-  const int blocks = static_cast<int>(std::min<int64_t>((groups + 255) / 256, 148 * 8));
+  const bool spread = job.splits >= 8;
+  const int blocks = static_cast<int>(std::min<int64_t>((groups * (spread ? 8 : 1) + 255) / 256, 148 * 8));
   if (f32)
-    finish_kernel<float, true><<<blocks, 256, 0, stream>>>(job);
+    (spread ? finish_kernel<float, true, 8> : finish_kernel<float, true, 1>)<<<blocks, 256, 0, stream>>>(job);
   else
-    finish_kernel<bf16, false><<<blocks, 256, 0, stream>>>(job);
+    (spread ? finish_kernel<bf16, false, 8> : finish_kernel<bf16, false, 1>)<<<blocks, 256, 0, stream>>>(job);
+  if (pr.epi.mode == Epilogue::kDz && pr.epi.sums) {
+    const int count = static_cast<int>(std::min<int64_t>(((pr.m + 31) / 32 * pr.n + 255) / 256, 148 * 8));
+    (f32 ? sums_kernel<float> : sums_kernel<bf16>)<<<count, 256, 0, stream>>>(job);
+  }
   return cudaGetLastError();
 }
 

@@ -91,46 +91,97 @@ __global__ void __launch_bounds__(kThreads)
 // (25 us, 1.6 TB/s).
 constexpr int kSumCols = 256, kSumWarps = 8;
 
+// The block's warps' sums, in order, as part blockIdx.y.
+__device__ __forceinline__ void put_sums(float (*buf)[kSumCols], const float s[8], int64_t cols, float* parts) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) buf[warp][lane + 32 * j] = s[j];
+  __syncthreads();
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8 + warp;  // column `warp` of the lane's eight
+  float sum = 0.f;
+#pragma unroll
+  for (int w = 0; w < kSumWarps; ++w) sum += buf[w][lane + 32 * warp];
+  if (c < cols) parts[blockIdx.y * cols + c] = sum;
+}
+
 __global__ void __launch_bounds__(32 * kSumWarps)
-    column_parts_kernel(const bf16* __restrict__ src, int64_t ld, int64_t plane, int planes, int64_t rows,
-                        int64_t cols, int64_t rows_per_part, float* __restrict__ parts) {
+    column_parts_kernel(const bf16* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, int64_t rows_per_part,
+                        float* __restrict__ parts) {
   __shared__ float buf[kSumWarps][kSumCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
   const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
-  const int count = static_cast<int>(min(static_cast<int64_t>(8), cols - c));
   float s[8] = {};
-  if (count > 0) {
-    for (int q = planes - 1; q >= 0; --q) {
-      const bf16* p = src + q * plane + c;
+  if (c < cols) {
 #pragma unroll 4
-      for (int64_t r = begin + warp; r < end; r += kSumWarps) {
-        float v[8];
-        load8(p + r * ld, v);  // rows are padded to eight: what lies beyond is not kept
+    for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+      float v[8];
+      load8(src + r * ld + c, v);  // rows are padded to eight: what lies beyond is not kept
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] += v[j];
-      }
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
   }
+  put_sums(buf, s, cols, parts);
+}
+
+// operand_kernel with the sums of what it writes, before it is rounded.
+template <typename T, bool kScale>
+__global__ void __launch_bounds__(32 * kSumWarps)
+    operand_sums_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec,
+                        const typename SlopeOf<T>::type* __restrict__ slope, bool slope_vec, bf16* __restrict__ dst,
+                        int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, Flags* flags,
+                        int64_t rows_per_part, float* __restrict__ parts) {
+  __shared__ float buf[kSumWarps][kSumCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
+  const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
+  const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);
+  float s[8] = {};
+  if (c < cols) {
+#pragma unroll 4
+    for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+      float v[8];
+      load_some(src + r * src_ld + c, count, src_vec && count == 8, v);
+      if (kScale) {
+        float f[8];
+        load_some(slope + r * cols + c, count, slope_vec && count == 8, f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) buf[warp][lane + 32 * j] = s[j];
-  __syncthreads();
-  const int j = threadIdx.x >> 5;  // column j of the lane's eight
-  float sum = 0.f;
+        for (int j = 0; j < 8; ++j) v[j] *= f[j];
+      }
 #pragma unroll
-  for (int w = 0; w < kSumWarps; ++w) sum += buf[w][lane + 32 * j];
-  if (j < count) parts[blockIdx.y * cols + c + j] = sum;
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+      put<T>(dst + r * dst_ld + c, plane, 8, true, v, flags, rows, r, c);
+    }
+  }
+  put_sums(buf, s, cols, parts);
+}
+
+template <typename T, bool kScale>
+cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slope, const Operand& dst, float* parts,
+                                cudaStream_t stream) {
+  using S = typename SlopeOf<T>::type;
+  const int64_t count = column_parts(dst.rows, dst.cols);
+  if (dst.rows == 0 || dst.cols == 0) return cudaSuccess;
+  const bool src_vec = aligned16(src) && (src_ld * sizeof(T)) % 16 == 0;
+  const bool slope_vec = aligned16(slope) && (dst.cols * sizeof(S)) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((dst.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
+  operand_sums_kernel<T, kScale><<<grid, 32 * kSumWarps, 0, stream>>>(
+      static_cast<const T*>(src), src_ld, src_vec, static_cast<const S*>(slope), slope_vec, const_cast<bf16*>(dst.p),
+      dst.ld, dst.plane, dst.rows, dst.cols, dst.flags, (dst.rows + count - 1) / count, parts);
+  return cudaGetLastError();
 }
 
 template <typename T>
 __global__ void __launch_bounds__(1024)
-    add_parts_kernel(const float* __restrict__ parts, int count, int64_t cols, T* __restrict__ sums) {
+    add_parts_kernel(const float* __restrict__ parts, int64_t count, int64_t cols, T* __restrict__ sums) {
   __shared__ float buf[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * 32ll + lane;
   float s = 0.f;
-  if (c < cols)
-    for (int i = warp; i < count; i += 32) s += parts[i * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t i = warp; i < count; i += 32) s += parts[i * cols + c];
+  }
   buf[warp][lane] = s;
   __syncthreads();
   if (warp == 0 && c < cols) {
@@ -168,21 +219,32 @@ int column_parts(int64_t rows, int64_t cols) {
   return static_cast<int>(std::min<int64_t>((rows + 31) / 32, std::max<int64_t>(1, 148 * 4 / std::max<int64_t>(across, 1))));
 }
 
-cudaError_t column_sums(DType out_dtype, const Operand& src, float* parts, void* sums, cudaStream_t stream) {
+cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
+                             float* parts, cudaStream_t stream) {
+  if (dtype == DType::kF32)
+    return slope ? launch_operand_sums<float, true>(g, g_ld, slope, dst, parts, stream)
+                 : launch_operand_sums<float, false>(g, g_ld, nullptr, dst, parts, stream);
+  return slope ? launch_operand_sums<bf16, true>(g, g_ld, slope, dst, parts, stream)
+               : launch_operand_sums<bf16, false>(g, g_ld, nullptr, dst, parts, stream);
+}
+
+cudaError_t column_sums(const Operand& src, float* parts, cudaStream_t stream) {
+  if (src.cols == 0 || src.rows == 0) return cudaSuccess;
   const int count = column_parts(src.rows, src.cols);
-  if (src.cols == 0) return cudaSuccess;
-  if (src.rows > 0) {
-    const int64_t per = (src.rows + count - 1) / count;
-    const dim3 grid(static_cast<unsigned>((src.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
-    column_parts_kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.plane, src.planes, src.rows, src.cols,
-                                                            per, parts);
-  }
-  const unsigned blocks = static_cast<unsigned>((src.cols + 31) / 32);
-  const int filled = src.rows > 0 ? count : 0;
+  const dim3 grid(static_cast<unsigned>((src.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
+  column_parts_kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.rows, src.cols,
+                                                          (src.rows + count - 1) / count, parts);
+  return cudaGetLastError();
+}
+
+cudaError_t add_parts(DType out_dtype, const float* parts, int64_t count, int64_t cols, void* sums,
+                      cudaStream_t stream) {
+  const unsigned blocks = static_cast<unsigned>((cols + 31) / 32);
+  if (blocks == 0) return cudaSuccess;
   if (out_dtype == DType::kF32)
-    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, filled, src.cols, static_cast<float*>(sums));
+    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, count, cols, static_cast<float*>(sums));
   else
-    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, filled, src.cols, static_cast<bf16*>(sums));
+    add_parts_kernel<<<blocks, 1024, 0, stream>>>(parts, count, cols, static_cast<bf16*>(sums));
   return cudaGetLastError();
 }
 
