@@ -3,7 +3,7 @@ share: storage types, rows of a tensor, dispatch reports."""
 
 from __future__ import annotations
 
-from functools import lru_cache
+from dataclasses import replace
 
 import torch
 
@@ -42,55 +42,56 @@ def check_checkpoint(checkpoint) -> None:
         raise ValueError(f"checkpoint must be None or 'int8', got {checkpoint!r}")
 
 
-@lru_cache(maxsize=256)
-def _report_of(operator: str, requested: str, selected: str, device: str, reason: str,
+# What a call with CUDA tensors and the native library at hand is decided and
+# reported as depends on the operator and the requested backend alone.
+_USUAL: dict[tuple[str, str], DispatchReport] = {}
+
+
+def _report_of(operator: str, backend: str, decision: DispatchDecision, selected: str, reason: str,
                native_available: bool) -> DispatchReport:
-    return DispatchReport(operator=operator, requested_backend=requested, selected_backend=selected, device=device,
-                          reason=reason, native_available=native_available)
-
-
-def report(operator: str, backend: str, decision: DispatchDecision, selected: str, reason: str,
-           native_available: bool) -> None:
-    record_dispatch_report(_report_of(operator, backend, selected, decision.device, reason, native_available))
-
-
-# the decisions for CUDA tensors with the native library at hand, which depend on nothing else
-_CUDA_DECISIONS: dict[tuple[str, str], DispatchDecision] = {}
+    return DispatchReport(operator=operator, requested_backend=backend, selected_backend=selected,
+                          device=decision.device, reason=reason, native_available=native_available)
 
 
 def decide(operator: str, backend: str, tensor: torch.Tensor, *others: torch.Tensor | None):
-    """``(native module, decision)`` of a call whose tensors share a device, or RuntimeError with its report."""
+    """``(native module, report of success)`` of a call whose tensors share a
+    device. Otherwise RuntimeError, and the report that says so."""
     module = native_module()
-    usual = module is not None and tensor.is_cuda
-    decision = _CUDA_DECISIONS.get((operator, backend)) if usual else None
-    if decision is None:
+    report = _USUAL.get((operator, backend)) if module is not None and tensor.is_cuda else None
+    decision = None
+    if report is None:
         decision = _explain_dispatch(tensor, backend=backend, native_available=module is not None, operator=operator)
-        if usual:
-            _CUDA_DECISIONS[operator, backend] = decision
-    reason = decision.reason if decision.backend == "error" else None
-    if reason is None:
-        device = tensor.device
-        for other in others:
-            if other is not None and other.device != device:
-                reason = f"a tensor is on {other.device}, input is on {device}"
-                break
-    if reason is not None:
-        report(operator, backend, decision, "error", reason, module is not None)
-        raise RuntimeError(reason)
-    return module, decision
+        if decision.backend == "error":
+            record_dispatch_report(_report_of(operator, backend, decision, "error", decision.reason,
+                                              module is not None))
+            raise RuntimeError(decision.reason)
+        report = _report_of(operator, backend, decision, "cuda", decision.reason, True)
+        _USUAL[operator, backend] = report
+    device = tensor.device
+    for other in others:
+        if other is not None and other.device != device:
+            raise failed(report, f"a tensor is on {other.device}, input is on {device}")
+    return module, report
+
+
+def failed(report: DispatchReport, reason: str) -> RuntimeError:
+    """The error of a call that would have been reported as ``report``, after reporting it."""
+    record_dispatch_report(replace(report, selected_backend="error", reason=reason))
+    return RuntimeError(reason)
 
 
 def rows_of(tensor: torch.Tensor) -> tuple[torch.Tensor, int]:
     """The tensor as rows of its last dimension, whose elements are adjacent, and
     the rows' distance: a view where the strides allow it, else a copy."""
-    if tensor.dim() != 2:
+    strides = tensor.stride()
+    if len(strides) != 2:
         tensor = tensor.reshape(-1, tensor.size(-1)) if tensor.numel() else tensor.new_empty(
             (tensor.shape[:-1].numel(), tensor.size(-1)))
-    stride, inner = tensor.stride()
-    if inner != 1 and tensor.size(1) > 1:
+        strides = tensor.stride()
+    if strides[1] != 1 and tensor.size(1) > 1:
         tensor = tensor.contiguous()
-        stride = tensor.stride(0)
-    return tensor, stride
+        strides = tensor.stride()
+    return tensor, strides[0]
 
 
 def pointer(tensor: torch.Tensor | None) -> int | None:

@@ -19,8 +19,9 @@ from typing import NamedTuple
 
 import torch
 
+from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import NativeModule
-from ._layer_common import DTYPE_CODES, STORAGE, check_tensor, decide, report, rows_of
+from ._layer_common import DTYPE_CODES, STORAGE, check_tensor, decide, rows_of
 
 BLOCK = 32
 
@@ -49,11 +50,11 @@ def checkpoint_pack(input: torch.Tensor, *, backend: str = "auto") -> Checkpoint
     check_tensor(input, "input")
     if input.dim() == 0:
         raise ValueError("input must have at least one dimension")
-    module, decision = decide("checkpoint_pack", backend, input)
+    module, report = decide("checkpoint_pack", backend, input)
     source = input.detach()
     rows, stride = rows_of(source.float() if source.dtype == torch.float16 else source)
     codes, exponents = pack_rows(module, rows, stride)
-    report("checkpoint_pack", backend, decision, "cuda", decision.reason, True)
+    record_dispatch_report(report)
     return Checkpoint8(codes.view(input.shape), exponents.view(*input.shape[:-1], exponents.size(1)), input.dtype)
 
 
@@ -70,14 +71,14 @@ def checkpoint_unpack(checkpoint: Checkpoint8, dtype: torch.dtype | None = None,
         raise TypeError("dtype must be float16, bfloat16 or float32")
     if codes.dim() == 0 or tuple(exponents.shape) != (*codes.shape[:-1], -(-codes.size(-1) // BLOCK)):
         raise ValueError("exponents must have the leading shape of codes and one byte for each block of 32")
-    module, decision = decide("checkpoint_unpack", backend, codes, exponents)
+    module, report = decide("checkpoint_unpack", backend, codes, exponents)
     codes, exponents = codes.contiguous(), exponents.contiguous()
     out = torch.empty(codes.shape, dtype=torch.float32 if dtype == torch.float16 else dtype, device=codes.device)
     width = codes.size(-1)
     module.plain_call("msda_checkpoint_unpack")(codes.device, DTYPE_CODES[out.dtype], codes.data_ptr(),
                                                 exponents.data_ptr(), codes.numel() // max(width, 1), width,
                                                 out.data_ptr())
-    report("checkpoint_unpack", backend, decision, "cuda", decision.reason, True)
+    record_dispatch_report(report)
     return out.to(dtype)
 
 

@@ -10,8 +10,9 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import LayerNormArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, pointer, report, rows_of
+from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of
 from .checkpoint8 import BLOCK
 
 OPERATOR_NAME = "layer_norm"
@@ -50,24 +51,31 @@ class _LayerNormFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        x, weight, statistics, codes, exponents = ctx.saved_tensors
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        g, g_stride = rows_of(grad)
-        count, width = g.shape
-        dx = grad.new_empty(grad.shape) if need_x else None
-        dw, db = (torch.empty(width, dtype=ctx.kind, device=grad.device) if need else None for need in (need_w, need_b))
-        stride, mean, rstd = 0, None, None
-        if x is not None:
-            x, stride = rows_of(x)
-            mean = statistics.data_ptr()
-            rstd = mean + 4 * count
-        args = LayerNormArgs(DTYPE_CODES[grad.dtype], DTYPE_CODES[ctx.kind], count, width, stride, g_stride, ctx.eps,
-                             pointer(x), pointer(weight), None, None, mean, rstd, pointer(codes), pointer(exponents),
-                             g.data_ptr(), pointer(dx), pointer(dw), pointer(db))
-        native_module().plain_call("msda_layer_norm_backward")(grad.device, args)
-        return dx, dw, db, None, None
+        # the wrapper costs 3 us; it is needed where a graph of this pass is asked for
+        return _backward_once(ctx, grad) if torch.is_grad_enabled() else _backward(ctx, grad)
+
+
+def _backward(ctx, grad):
+    x, weight, statistics, codes, exponents = ctx.saved_tensors
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    g, g_stride = rows_of(grad)
+    count, width = g.shape
+    dx = grad.new_empty(grad.shape) if need_x else None
+    dw, db = (torch.empty(width, dtype=ctx.kind, device=grad.device) if need else None for need in (need_w, need_b))
+    stride, mean, rstd = 0, None, None
+    if x is not None:
+        x, stride = rows_of(x)
+        mean = statistics.data_ptr()
+        rstd = mean + 4 * count
+    args = LayerNormArgs(DTYPE_CODES[grad.dtype], DTYPE_CODES[ctx.kind], count, width, stride, g_stride, ctx.eps,
+                         pointer(x), pointer(weight), None, None, mean, rstd, pointer(codes), pointer(exponents),
+                         g.data_ptr(), pointer(dx), pointer(dw), pointer(db))
+    native_module().plain_call("msda_layer_norm_backward")(grad.device, args)
+    return dx, dw, db, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -95,7 +103,7 @@ def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: to
             raise ValueError(f"{name} must have shape ({input.size(-1)},), got {tuple(tensor.shape)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError("weight and bias must have one dtype")
-    module, decision = decide(OPERATOR_NAME, backend, input, weight, bias)
+    module, report = decide(OPERATOR_NAME, backend, input, weight, bias)
     dtype = input.dtype
     if dtype == torch.float16:
         input, weight, bias = (t if t is None else t.float() for t in (input, weight, bias))
@@ -107,9 +115,8 @@ def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: to
         else:
             output = _forward(module, *tensors, float(eps), None)[0]
     except RuntimeError as exc:
-        report(OPERATOR_NAME, backend, decision, "error", str(exc), True)
-        raise
-    report(OPERATOR_NAME, backend, decision, "cuda", decision.reason, True)
+        raise failed(report, str(exc)) from exc
+    record_dispatch_report(report)
     return output if dtype != torch.float16 else output.to(dtype)
 
 

@@ -15,8 +15,9 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
+from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import LinearArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, native_module, pointer, report, rows_of
+from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of
 from .checkpoint8 import pack_rows
 
 OPERATOR_NAME = "linear_act"
@@ -73,33 +74,40 @@ class _LinearActFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        x, weight, bias, slope, codes, exponents = ctx.saved_tensors
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        x_shape, w_shape = ctx.sizes
-        dx = dw = db = None
-        if need_x or need_w or need_b:
-            g, g_stride = rows_of(grad)
-            if need_x:
-                dx = grad.new_empty(x_shape)
-            if need_w:
-                dw = grad.new_empty(w_shape)
-            if need_b:
-                db = grad.new_empty(w_shape[:1])
-            x_stride = w_stride = 0
-            if x is not None:
-                x, x_stride = rows_of(x)
-            if weight is not None:
-                weight, w_stride = rows_of(weight)
-            if bias is not None:
-                bias = bias.contiguous()
-            args = LinearArgs(DTYPE_CODES[grad.dtype], ACTIVATIONS[ctx.activation], g.size(0), w_shape[1], w_shape[0],
-                              x_stride, w_stride, 0, 0, g_stride, pointer(x), pointer(weight), pointer(bias), None,
-                              None, pointer(slope), g.data_ptr(), pointer(codes), pointer(exponents), pointer(dx),
-                              pointer(dw), pointer(db))
-            native_module().plain_call("msda_linear_act_backward")(grad.device, args)
-        return dx, dw, db, grad if need_r else None, None, None
+        # the wrapper costs 3 us; it is needed where a graph of this pass is asked for
+        return _backward_once(ctx, grad) if torch.is_grad_enabled() else _backward(ctx, grad)
+
+
+def _backward(ctx, grad):
+    x, weight, bias, slope, codes, exponents = ctx.saved_tensors
+    need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+    x_shape, w_shape = ctx.sizes
+    dx = dw = db = None
+    if need_x or need_w or need_b:
+        g, g_stride = rows_of(grad)
+        if need_x:
+            dx = grad.new_empty(x_shape)
+        if need_w:
+            dw = grad.new_empty(w_shape)
+        if need_b:
+            db = grad.new_empty(w_shape[:1])
+        x_stride = w_stride = 0
+        if x is not None:
+            x, x_stride = rows_of(x)
+        if weight is not None:
+            weight, w_stride = rows_of(weight)
+        if bias is not None:
+            bias = bias.contiguous()
+        args = LinearArgs(DTYPE_CODES[grad.dtype], ACTIVATIONS[ctx.activation], g.size(0), w_shape[1], w_shape[0],
+                          x_stride, w_stride, 0, 0, g_stride, pointer(x), pointer(weight), pointer(bias), None,
+                          None, pointer(slope), g.data_ptr(), pointer(codes), pointer(exponents), pointer(dx),
+                          pointer(dw), pointer(db))
+        native_module().plain_call("msda_linear_act_backward")(grad.device, args)
+    return dx, dw, db, grad if need_r else None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
@@ -139,7 +147,7 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
                 residual = residual.expand(shape)
             except RuntimeError as exc:
                 raise ValueError(f"residual {tuple(residual.shape)} cannot be broadcast to {tuple(shape)}") from exc
-    module, decision = decide(OPERATOR_NAME, backend, input, weight, bias, residual)
+    module, report = decide(OPERATOR_NAME, backend, input, weight, bias, residual)
     dtype = input.dtype
     if dtype == torch.float16:
         input, weight, bias, residual = (t if t is None else t.float() for t in (input, weight, bias, residual))
@@ -150,9 +158,8 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         else:
             output, _ = _forward(module, *tensors, activation, False)
     except RuntimeError as exc:
-        report(OPERATOR_NAME, backend, decision, "error", str(exc), True)
-        raise
-    report(OPERATOR_NAME, backend, decision, "cuda", decision.reason, True)
+        raise failed(report, str(exc)) from exc
+    record_dispatch_report(report)
     return output if dtype != torch.float16 else output.to(dtype)
 
 

@@ -235,25 +235,25 @@ class NativeModule:
             query.restype = ctypes.c_int
             query.argtypes = [_PLAIN_SIGNATURES[name][0], ctypes.POINTER(ctypes.c_size_t)]
 
-        def enqueue(device: torch.device, *args: Any) -> None:
-            if query is not None:
-                size = ctypes.c_size_t()
-                if query(args[0], size) != 0:
-                    raise RuntimeError(f"{name}: {self.last_error()}")
-                if size.value:
-                    # freed after the call as far as torch is concerned: the next owner is on the same stream
-                    workspace = torch.empty(size.value, dtype=torch.uint8, device=device)
-                    args[0].workspace = workspace.data_ptr()
-                    args[0].workspace_bytes = size.value
-            if symbol(*args, _raw_stream(device.index)) != 0:
-                raise RuntimeError(f"{name}: {self.last_error()}")
+        size = ctypes.c_size_t
+        current_device = torch.cuda.current_device
 
         def call(device: torch.device, *args: Any) -> None:
-            if device.index == torch.cuda.current_device():
-                enqueue(device, *args)
-            else:
+            index = device.index
+            if index != current_device():
                 with torch.cuda.device(device):
-                    enqueue(device, *args)
+                    return call(device, *args)
+            if query is not None:
+                needed = size()
+                if query(args[0], needed) != 0:
+                    raise RuntimeError(f"{name}: {self.last_error()}")
+                if needed.value:
+                    # freed after the call as far as torch is concerned: the next owner is on the same stream
+                    workspace = torch.empty(needed.value, dtype=torch.uint8, device=device)
+                    args[0].workspace = workspace.data_ptr()
+                    args[0].workspace_bytes = needed.value
+            if symbol(*args, _raw_stream(index)) != 0:
+                raise RuntimeError(f"{name}: {self.last_error()}")
 
         call.__name__ = name
         self._plain[name] = call

@@ -647,7 +647,7 @@ def _refused(name, args, match):
 
 def test_plain_entries_refuse_before_any_launch():
     p = 4096  # never dereferenced: every call fails its checks
-    good = dict(dtype=1, activation=2, rows=4, in_features=8, out_features=16, input_stride=8, weight_stride=8,
+    good = dict(dtype=1, activation=2, rows=64, in_features=8, out_features=16, input_stride=8, weight_stride=8,
                 output_stride=16, grad_output_stride=16, input=p, weight=p, output=p, grad_output=p)
     for change, match in ((dict(dtype=5), "dtype must be"), (dict(activation=9), "activation must be"),
                           (dict(rows=-1), "non-negative"), (dict(rows=2 ** 31), "rows exceeds"),
