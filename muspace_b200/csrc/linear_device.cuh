@@ -103,7 +103,7 @@ __device__ __forceinline__ void activate(Act act, float* z, float* s) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       if (kS) s[j] = z[j] > 0.f ? 1.f : (z[j] <= 0.f ? 0.f : z[j]);
-      if (kY) z[j] = z[j] <= 0.f ? 0.f : z[j];
+      if (kY) asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z[j]));
     }
   } else if (kS) {
 #pragma unroll

@@ -74,6 +74,7 @@ struct Shape {
 struct Job {
   Product pr;
   uint32_t tiles_m, tiles_n;
+  uint64_t by_tiles, by_group, by_last;  // divided()
   int splits, kblocks, kblocks_per_split, pairs;
   int box_a, box_b;  // rows of the boxes along k
   int device;
@@ -175,6 +176,18 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t r[16]) {
       : "memory");
 }
 
+// The same with the wait.
+__device__ __forceinline__ void tmem_take16(uint32_t addr, float v[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+      : "r"(addr)
+      : "memory");
+}
+
 // The loads so far have arrived; the registers pass through, so none is read before.
 __device__ __forceinline__ void tmem_wait(uint32_t r[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -249,16 +262,22 @@ struct Item {
   int split, kb0, kb1;
 };
 
+// x / d for 32-bit x: `magic` is floor(2^64 / d) + 1 (0 stands for d = 1). The
+// divisions were a tenth of an epilogue's time.
+__device__ __forceinline__ uint32_t divided(uint32_t x, uint64_t magic) {
+  return magic ? static_cast<uint32_t>(__umul64hi(x, magic)) : x;
+}
+
 template <int BN, int CG>
 __device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
-  const uint32_t tiles = j.tiles_m * j.tiles_n;
   Item t;
-  t.split = static_cast<int>(i / tiles);
-  const uint32_t at = i - t.split * tiles, per_group = kGroupM * j.tiles_n;
-  const uint32_t group = at / per_group, first = group * kGroupM;
-  const uint32_t rows = min(static_cast<uint32_t>(kGroupM), j.tiles_m - first), local = at - group * per_group;
-  const uint32_t col = local / rows;
-  t.m = static_cast<int>((first + local - col * rows) * (kTileM * CG));
+  t.split = static_cast<int>(divided(i, j.by_tiles));
+  const uint32_t at = i - t.split * j.tiles_m * j.tiles_n;
+  const uint32_t group = divided(at, j.by_group), first = group * kGroupM;
+  const uint32_t local = at - group * (kGroupM * j.tiles_n);
+  const uint32_t rows = j.tiles_m - first;  // of tiles in the group, if fewer than usual
+  const uint32_t col = rows >= kGroupM ? local / kGroupM : divided(local, j.by_last);
+  t.m = static_cast<int>((first + local - col * min(rows, static_cast<uint32_t>(kGroupM))) * (kTileM * CG));
   t.n = static_cast<int>(col * BN);
   t.kb0 = t.split * j.kblocks_per_split;
   t.kb1 = min(j.kblocks, t.kb0 + j.kblocks_per_split);
@@ -490,9 +509,238 @@ __device__ __forceinline__ void stores_read() {
 
 // ---- the kernel ------------------------------------------------------------------------
 
+constexpr int kFwdSlope = 3;  // beside Epilogue::Mode: kFwd that also writes the slope
+
 struct Maps {
   CUtensorMap a, b, out, extra, slope;
 };
+
+// Where a block's things are: addresses in tensor and shared memory, and its rank in a pair.
+struct Place {
+  uint32_t tmem, boxes, bars, rank;
+};
+
+// The epilogue's warps, from the first tile to the last. kKind: the mode, the
+// activation and whether there is a residual, as constants: with branches in
+// here, 16 columns took 170 instructions and more where 50 do, and issuing them
+// was the bound of short products; as one function with all kinds it spilled.
+template <int BN, int CG, typename T, bool kF32, int kKind>
+__device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Place place) {
+  using S = Shape<BN, CG, kF32>;
+  constexpr int kMode = kKind / 8;
+  constexpr Act kAct = static_cast<Act>(kKind / 2 % 4);
+  constexpr bool kExtra = kKind % 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tmem = place.tmem, rank = place.rank;
+  const auto acc_full = [&](int b) { return place.bars + 8 * (2 * S::kStages + b); };
+  const auto acc_empty = [&](int b) { return place.bars + 8 * (2 * S::kStages + 2 + b); };
+  const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
+  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int chunk = kF32 ? kPromote : job.kblocks;
+  bool dead = false;
+  constexpr int kBoxCols = 128 / sizeof(T) < S::kCols ? 128 / sizeof(T) : S::kCols;
+  constexpr int kRowBytes = kBoxCols * sizeof(T);
+  constexpr bool kFast = sizeof(T) == 2;
+  constexpr int kParts = S::kCols / kBoxCols;  // more than one only for partial sums
+  const int quad = warp & 3, group = warp >> 2;
+  const uint32_t box = place.boxes + warp * kBoxBytes;
+  const uint32_t arrived = place.bars + 8 * (2 * S::kStages + 4 + warp);  // the residual's box
+  const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+  const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
+  const Epilogue& e = job.pr.epi;
+  constexpr bool kSlope = kMode == kFwdSlope, kPlanes = sizeof(T) == 4 && kMode == Epilogue::kDz;
+  const bool extra = kSlope ? e.extra != nullptr : kExtra;
+  const bool with_bias = kMode != Epilogue::kStore && e.bias != nullptr;
+  const bool bias_vec = reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
+  const bool repairs = kF32 && !job.apart && some_flag(job.pr);
+  const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
+  const auto col_of = [&](const Item& t) { return t.n + group * S::kCols; };
+  // a box on its way out; the next may be written when `read`
+  const auto send = [&](const CUtensorMap* map, int n, int m, int z, uint32_t src) {
+    if (m < rows_m && n < rows_n) store_box(map, n, m, z, src);
+  };
+  const auto box_written = [&] {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+  };
+  const auto box_read = [&] {
+    if (lane == 0) stores_read<0>();
+    __syncwarp();
+  };
+  int buf = 0;
+  uint32_t acc_phase = 0, extra_phase = 0;
+  Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
+  if (extra && first < items && lane == 0) load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
+  for (uint32_t i = first; i < items; i += step) {
+    const int m = row_of(t), n0 = col_of(t);
+    uint32_t acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
+    if (kF32) {
+      float acc[S::kCols / 16][16] = {};
+      for (int c = t.kb0; c < t.kb1; c += chunk) {
+        wait(acc_full(buf), acc_phase, dead);
+        fence_after();
+        const bool more = c + chunk < t.kb1;
+        acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
+#pragma unroll
+        for (int q = 0; q < S::kCols / 16; ++q) {
+          uint32_t r[16], small[16];
+          tmem_load16(acc_at + q * 16, r);
+          tmem_load16(acc_at + BN + q * 16, small);
+          tmem_wait(r);
+          tmem_wait(small);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]) + __uint_as_float(small[x]);
+          if (!more) tmem_store16(acc_at + q * 16, acc[q]);
+        }
+        if (more) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
+          buf ^= 1;
+          if (buf == 0) acc_phase ^= 1;
+        }
+      }
+      tmem_stored();
+    } else {
+      wait(acc_full(buf), acc_phase, dead);
+      fence_after();
+    }
+    if (extra) {
+      wait(arrived, extra_phase, dead);
+      extra_phase ^= 1;
+    }
+#pragma unroll 1
+    for (int p = 0; p < kParts; ++p) {
+      const int n = n0 + p * kBoxCols;
+      if (!extra) box_read();
+#pragma unroll 1
+      for (int c = 0; c < kBoxCols; c += 16) {
+        const uint32_t at = acc_at + p * kBoxCols + c;
+        float x[16], v[16], s[16];
+        Bias16<T> bias;
+        if (kMode != Epilogue::kStore && with_bias)
+          bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
+        if (kExtra) get16<kRowBytes>(box, lane, c, x, T());
+        tmem_take16(at, v);
+        if (kF32 && repairs) {
+          float w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = v[j];
+          repair<16>(job.pr, w, m + lane, n + c);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = w[j];
+        }
+        if (kMode != Epilogue::kStore && with_bias) bias.add(v);
+        if (kMode == Epilogue::kDz) {
+          activate<kFast, false, true, 16>(kAct, v, s);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
+          if (e.sums) {
+            if (m + lane >= rows_m) {  // rows of nothing: their gradient is zero, their slope may be anything
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = 0.f;
+            }
+            const float sum = lane_sums16(v);
+            const int col = n + c + lane / 2;
+            if ((lane & 1) == 0 && m < rows_m && col < rows_n)
+              e.sums[static_cast<int64_t>(m / 32) * rows_n + col] = sum;
+          }
+          if (sizeof(T) == 4) {
+            tmem_store16(at, v);
+            mark16(e.out_flags, job.pr, v, m + lane, n + c);
+            continue;
+          }
+        } else if (kSlope) {
+          activate<kFast, true, true, 16>(e.act, v, s);
+          put_aside(at, s, typename SlopeOf<T>::type());
+          if (extra) {
+            get16<kRowBytes>(box, lane, c, x, T());
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += x[j];
+          }
+        } else if (kMode == Epilogue::kFwd) {
+          activate<kFast, true, false, 16>(kAct, v, s);
+          if (kExtra) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += x[j];
+          }
+        }
+        put16<kRowBytes>(box, lane, c, v, T());
+      }
+      if constexpr (kPlanes) {
+        // dz waits in tensor memory: hi and mid take the gradient's place, then lo theirs
+        tmem_stored();
+        __syncwarp();
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+          if (pass) box_read();
+#pragma unroll 1
+          for (int c = 0; c < kBoxCols; c += 16) {
+            uint32_t r[16], part[3][8];
+            tmem_load16(acc_at + c, r);
+            tmem_wait(r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              bf16 a[3], b[3];
+              split3(__uint_as_float(r[2 * j]), a[0], a[1], a[2]);
+              split3(__uint_as_float(r[2 * j + 1]), b[0], b[1], b[2]);
+#pragma unroll
+              for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int k = 4 * u;
+              if (pass) {
+                put_unit(unit_at<64>(box, lane, c / 8 + u), part[2][k], part[2][k + 1], part[2][k + 2], part[2][k + 3]);
+              } else {
+                put_unit(unit_at<64>(box, lane, c / 8 + u), part[0][k], part[0][k + 1], part[0][k + 2], part[0][k + 3]);
+                put_unit(unit_at<64>(box + 2048, lane, c / 8 + u), part[1][k], part[1][k + 1], part[1][k + 2],
+                         part[1][k + 3]);
+              }
+            }
+          }
+          box_written();
+          if (lane == 0) {
+            send(&maps.out, n, m, 2 * pass, box);
+            if (!pass) send(&maps.out, n, m, 1, box + 2048);
+            stores_commit();
+          }
+        }
+      } else {
+        box_written();
+        if (lane == 0) {
+          send(&maps.out, n, m, job.apart ? t.split : 0, box);
+          stores_commit();
+        }
+        if constexpr (kSlope) {
+          // the slopes wait in tensor memory for the box
+          tmem_stored();
+          box_read();
+#pragma unroll 1
+          for (int c = 0; c < kBoxCols; c += 16) take_back<kRowBytes>(box, lane, c, acc_at + c, typename SlopeOf<T>::type());
+          box_written();
+          if (lane == 0) {
+            send(&maps.slope, n, m, 0, box);
+            stores_commit();
+          }
+        }
+      }
+    }
+    fence_before();
+    __syncwarp();
+    if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
+    buf ^= 1;
+    if (buf == 0) acc_phase ^= 1;
+    if (i + step < items) {
+      t = item_of<BN, CG>(job, i + step);
+      if (extra && lane == 0) {
+        stores_read<0>();
+        load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
+      }
+    }
+  }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
 
 template <int BN, int CG, typename T, bool kF32>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -500,8 +748,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   using S = Shape<BN, CG, kF32>;
   extern __shared__ uint8_t raw[];
   const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
-  const uint32_t boxes_base = ring + S::kStages * S::kStage;
-  const uint32_t bars = boxes_base + kEpiWarps * kBoxBytes;
+  const uint32_t bars = ring + S::kStages * S::kStage + kEpiWarps * kBoxBytes;
   const uint32_t tmem_slot = bars + S::kBarriers * 8;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
@@ -623,212 +870,32 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < S::kWarps) {
-    constexpr int kBoxCols = 128 / sizeof(T) < S::kCols ? 128 / sizeof(T) : S::kCols;
-    constexpr int kRowBytes = kBoxCols * sizeof(T);
-    constexpr bool kFast = sizeof(T) == 2;
-    constexpr int kParts = S::kCols / kBoxCols;  // more than one only for partial sums
-    const int quad = warp & 3, group = warp >> 2;
-    const uint32_t box = boxes_base + warp * kBoxBytes;
-    const uint32_t arrived = bars + 8 * (2 * S::kStages + 4 + warp);  // the residual's box
-    const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-    const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
     const Epilogue& e = job.pr.epi;
     const int mode = job.apart ? Epilogue::kStore : e.mode;
     const bool extra = mode != Epilogue::kStore && e.extra != nullptr;
-    const bool slope = mode == Epilogue::kFwd && e.slope != nullptr;
-    const bool planes = sizeof(T) == 4 && mode == Epilogue::kDz;
-    const bool with_bias = mode != Epilogue::kStore && e.bias != nullptr;
-    const bool bias_vec = reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
-    const bool repairs = kF32 && !job.apart && some_flag(job.pr);
-    const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
-    const auto col_of = [&](const Item& t) { return t.n + group * S::kCols; };
-    // a box on its way out; the next may be written when `read`
-    const auto send = [&](const CUtensorMap* map, int n, int m, int z, uint32_t src) {
-      if (m < rows_m && n < rows_n) store_box(map, n, m, z, src);
-    };
-    const auto box_written = [&] {
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-    };
-    const auto box_read = [&] {
-      if (lane == 0) stores_read<0>();
-      __syncwarp();
-    };
-    int buf = 0;
-    uint32_t acc_phase = 0, extra_phase = 0;
-    Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
-    if (extra && first < items && lane == 0) load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
-    for (uint32_t i = first; i < items; i += step) {
-      const int m = row_of(t), n0 = col_of(t);
-      uint32_t acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
-      if (kF32) {
-        float acc[S::kCols / 16][16] = {};
-        for (int c = t.kb0; c < t.kb1; c += chunk) {
-          wait(acc_full(buf), acc_phase, dead);
-          fence_after();
-          const bool more = c + chunk < t.kb1;
-          acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
-#pragma unroll
-          for (int q = 0; q < S::kCols / 16; ++q) {
-            uint32_t r[16], small[16];
-            tmem_load16(acc_at + q * 16, r);
-            tmem_load16(acc_at + BN + q * 16, small);
-            tmem_wait(r);
-            tmem_wait(small);
-#pragma unroll
-            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]) + __uint_as_float(small[x]);
-            if (!more) tmem_store16(acc_at + q * 16, acc[q]);
-          }
-          if (more) {
-            fence_before();
-            __syncwarp();
-            if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
-            buf ^= 1;
-            if (buf == 0) acc_phase ^= 1;
-          }
-        }
-        tmem_stored();
-      } else {
-        wait(acc_full(buf), acc_phase, dead);
-        fence_after();
-      }
-      if (extra) {
-        wait(arrived, extra_phase, dead);
-        extra_phase ^= 1;
-      }
-#pragma unroll 1
-      for (int p = 0; p < kParts; ++p) {
-        const int n = n0 + p * kBoxCols;
-        if (!extra) box_read();
-#pragma unroll 1
-        for (int c = 0; c < kBoxCols; c += 16) {
-          const uint32_t at = acc_at + p * kBoxCols + c;
-          uint32_t r[16];
-          tmem_load16(at, r);
-          float x[16], v[16], s[16];
-          Bias16<T> bias;
-          if (with_bias) bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
-          if (extra) get16<kRowBytes>(box, lane, c, x, T());
-          tmem_wait(r);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-          if (repairs) {
-            float w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = v[j];
-            repair<16>(job.pr, w, m + lane, n + c);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = w[j];
-          }
-          if (mode != Epilogue::kStore) {
-            if (with_bias) bias.add(v);
-            if (mode == Epilogue::kDz) {
-              activate<kFast, false, true, 16>(e.act, v, s);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) v[j] = x[j] * s[j];
-              if (e.sums) {
-                if (m + lane >= rows_m) {  // rows of nothing: their gradient is zero, their slope may be anything
-#pragma unroll
-                  for (int j = 0; j < 16; ++j) v[j] = 0.f;
-                }
-                const float sum = lane_sums16(v);
-                const int col = n + c + lane / 2;
-                if ((lane & 1) == 0 && m < rows_m && col < rows_n)
-                  e.sums[static_cast<int64_t>(m / 32) * rows_n + col] = sum;
-              }
-              if (planes) {
-                tmem_store16(at, v);
-                mark16(e.out_flags, job.pr, v, m + lane, n + c);
-                continue;
-              }
-            } else {
-              if (slope) {
-                activate<kFast, true, true, 16>(e.act, v, s);
-                put_aside(at, s, typename SlopeOf<T>::type());
-              } else {
-                activate<kFast, true, false, 16>(e.act, v, s);
-              }
-              if (extra) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] += x[j];
-              }
-            }
-          }
-          put16<kRowBytes>(box, lane, c, v, T());
-        }
-        if (sizeof(T) == 4 && planes) {
-          // dz waits in tensor memory: hi and mid take the gradient's place, then lo theirs
-          tmem_stored();
-          __syncwarp();
-#pragma unroll 1
-          for (int pass = 0; pass < 2; ++pass) {
-            if (pass) box_read();
-#pragma unroll 1
-            for (int c = 0; c < kBoxCols; c += 16) {
-              uint32_t r[16], part[3][8];
-              tmem_load16(acc_at + c, r);
-              tmem_wait(r);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                bf16 a[3], b[3];
-                split3(__uint_as_float(r[2 * j]), a[0], a[1], a[2]);
-                split3(__uint_as_float(r[2 * j + 1]), b[0], b[1], b[2]);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
-              }
-#pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                const int k = 4 * u;
-                if (pass) {
-                  put_unit(unit_at<64>(box, lane, c / 8 + u), part[2][k], part[2][k + 1], part[2][k + 2], part[2][k + 3]);
-                } else {
-                  put_unit(unit_at<64>(box, lane, c / 8 + u), part[0][k], part[0][k + 1], part[0][k + 2], part[0][k + 3]);
-                  put_unit(unit_at<64>(box + 2048, lane, c / 8 + u), part[1][k], part[1][k + 1], part[1][k + 2],
-                           part[1][k + 3]);
-                }
-              }
-            }
-            box_written();
-            if (lane == 0) {
-              send(&maps.out, n, m, 2 * pass, box);
-              if (!pass) send(&maps.out, n, m, 1, box + 2048);
-              stores_commit();
-            }
-          }
-        } else {
-          box_written();
-          if (lane == 0) {
-            send(&maps.out, n, m, job.apart ? t.split : 0, box);
-            stores_commit();
-          }
-          if (slope) {
-            // the slopes wait in tensor memory for the box
-            tmem_stored();
-            box_read();
-#pragma unroll 1
-            for (int c = 0; c < kBoxCols; c += 16) take_back<kRowBytes>(box, lane, c, acc_at + c, typename SlopeOf<T>::type());
-            box_written();
-            if (lane == 0) {
-              send(&maps.slope, n, m, 0, box);
-              stores_commit();
-            }
-          }
-        }
-      }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
-      buf ^= 1;
-      if (buf == 0) acc_phase ^= 1;
-      if (i + step < items) {
-        t = item_of<BN, CG>(job, i + step);
-        if (extra && lane == 0) {
-          stores_read<0>();
-          load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
-        }
+    const int kind = mode == Epilogue::kFwd && e.slope ? kFwdSlope * 8
+                     : mode == Epilogue::kStore        ? Epilogue::kStore * 8
+                                                       : mode * 8 + static_cast<int>(e.act) * 2 + (extra ? 1 : 0);
+    const Place at{tmem, ring + S::kStages * S::kStage, bars, rank};
+    if constexpr (sizeof(T) == 4 && !kF32) {  // partial sums
+      epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at);
+    } else {
+      switch (kind) {
+        case Epilogue::kStore * 8: epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at); break;
+        case Epilogue::kFwd * 8: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 1: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 1>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 2: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 2>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 3: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 3>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 4: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 4>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 5: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 5>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 6: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 6>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 7: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 7>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 3: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 3>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 5: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 5>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 7: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 7>(maps, job, at); break;
+        default: epilogue<BN, CG, T, kF32, kFwdSlope * 8>(maps, job, at);
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   __syncwarp();
   fence_before();
@@ -1079,6 +1146,10 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
     if (tiles_m * tiles_n * plan.splits >= 1ll << 31) return cudaErrorInvalidValue;
     job.tiles_m = static_cast<uint32_t>(tiles_m);
     job.tiles_n = static_cast<uint32_t>(tiles_n);
+    const auto magic = [](uint64_t d) { return d <= 1 ? 0ull : ~0ull / d + 1; };
+    job.by_tiles = magic(job.tiles_m * static_cast<uint64_t>(job.tiles_n));
+    job.by_group = magic(kGroupM * static_cast<uint64_t>(job.tiles_n));
+    job.by_last = magic(job.tiles_m % kGroupM);
     job.kblocks = static_cast<int>(ceil_div(pr.k, kBlockK));
     job.kblocks_per_split = plan.kblocks;
     job.pairs = pr.a.planes == 3 ? (pr.b.planes == 3 ? 6 : 3) : (pr.b.planes == 3 ? 3 : 1);
