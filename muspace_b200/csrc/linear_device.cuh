@@ -144,14 +144,6 @@ __device__ __forceinline__ void split3(float x, bf16& hi, bf16& mid, bf16& lo) {
   lo = __float2bfloat16_rn(r1 - __bfloat162float(mid));
 }
 
-// 1: an infinity, 2: a NaN, 0: finite
-__device__ __forceinline__ uint32_t flag_of(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? 0u : (b == 0x7f800000u ? 1u : 2u);
-}
-
-// ---- eight neighbouring values ----------------------------------------------------------
-
 __device__ __forceinline__ uint32_t pack2(bf16 a, bf16 b) {
   return static_cast<uint32_t>(__bfloat16_as_ushort(a)) | (static_cast<uint32_t>(__bfloat16_as_ushort(b)) << 16);
 }
@@ -160,6 +152,54 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+
+__device__ __forceinline__ float2 unpack2(uint32_t u) {
+  return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// The largest magnitude's bits among N values; NaNs have the largest.
+template <int N>
+__device__ __forceinline__ uint32_t top_bits(const float* v) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+  return top;
+}
+
+// N values as N / 2 pairs in each plane: two at a time where none is so large
+// that bfloat16 rounds it to infinity.
+template <int N>
+__device__ __forceinline__ void split_pairs(const float* v, uint32_t top, uint32_t part[3][N / 2]) {
+  if (top < 0x7f7f8000u) {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      const float2 minus = make_float2(-1.f, -1.f);
+      float2 left = make_float2(v[2 * j], v[2 * j + 1]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        part[k][j] = pack2(left.x, left.y);
+        if (k < 2) left = fma2(unpack2(part[k][j]), minus, left);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N / 2; ++j) {
+      bf16 a[3], b[3];
+      split3(v[2 * j], a[0], a[1], a[2]);
+      split3(v[2 * j + 1], b[0], b[1], b[2]);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
+    }
+  }
+}
+
+// 1: an infinity, 2: a NaN, 0: finite
+__device__ __forceinline__ uint32_t flag_of(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? 0u : (b == 0x7f800000u ? 1u : 2u);
+}
+
+// ---- eight neighbouring values ----------------------------------------------------------
 
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(bf16 v) { return __bfloat162float(v); }
@@ -245,19 +285,17 @@ __device__ __forceinline__ void store_some(T* p, int count, bool vec, const floa
 
 // Splits eight values into the three planes at p, p + plane, p + 2 plane.
 __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, bool vec, const float v[8]) {
-  bf16 part[3][8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) split3(v[j], part[0][j], part[1][j], part[2][j]);
+  uint32_t part[3][4];
+  split_pairs<8>(v, top_bits<8>(v), part);
 #pragma unroll
   for (int i = 0; i < 3; ++i) {
     if (vec) {
-      *reinterpret_cast<uint4*>(p + i * plane) =
-          make_uint4(pack2(part[i][0], part[i][1]), pack2(part[i][2], part[i][3]), pack2(part[i][4], part[i][5]),
-                     pack2(part[i][6], part[i][7]));
+      *reinterpret_cast<uint4*>(p + i * plane) = make_uint4(part[i][0], part[i][1], part[i][2], part[i][3]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j < count) p[i * plane + j] = part[i][j];
+        if (j < count)
+          p[i * plane + j] = __ushort_as_bfloat16(static_cast<unsigned short>(part[i][j / 2] >> (16 * (j % 2))));
     }
   }
 }
@@ -265,17 +303,18 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, 
 // Marks what is not finite among `count` <= 8 values at (r, c).
 __device__ __forceinline__ void mark_flags(const float v[8], int count, Flags* flags, int64_t rows, int64_t r,
                                            int64_t c) {
+  if (top_bits<8>(v) < 0x7f800000u) return;
   uint32_t any = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) any |= j < count ? flag_of(v[j]) : 0u;
-  if (!any) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint32_t f = j < count ? flag_of(v[j]) : 0u;
     if (f) atomicOr(flags->cols(rows) + c + j, f);
+    any |= f;
   }
-  atomicOr(flags->rows() + r, any);
-  atomicOr(&flags->any, any);
+  if (any) {
+    atomicOr(flags->rows() + r, any);
+    atomicOr(&flags->any, any);
+  }
 }
 
 // ---- the epilogue -----------------------------------------------------------------------

@@ -470,16 +470,11 @@ struct Bias16 {
 };
 
 // Marks what is not finite among 16 outputs of row m.
-__device__ __forceinline__ void mark16(Flags* flags, const Product& pr, const float v[16], int64_t m, int64_t n) {
+__device__ __noinline__ void mark16(Flags* flags, int64_t rows, int64_t cols, const float* v, int64_t m, int64_t n) {
   uint32_t any = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) any |= flag_of(v[j]);
-  if (any == 0 || m >= pr.m) return;
-  any = 0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const uint32_t f = n + j < pr.n ? flag_of(v[j]) : 0u;
-    if (f) atomicOr(flags->cols(pr.m) + n + j, f);
+  for (int j = 0; j < 16 && m < rows && n + j < cols; ++j) {
+    const uint32_t f = flag_of(v[j]);
+    if (f) atomicOr(flags->cols(rows) + n + j, f);
     any |= f;
   }
   if (any) {
@@ -648,7 +643,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           }
           if (sizeof(T) == 4) {
             tmem_store16(at, v);
-            mark16(e.out_flags, job.pr, v, m + lane, n + c);
             continue;
           }
         } else if (kSlope) {
@@ -673,39 +667,40 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
         tmem_stored();
         __syncwarp();
 #pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-          if (pass) box_read();
+        for (int c = 0; c < kBoxCols; c += 16) {
+          float v[16];
+          uint32_t part[3][8];
+          tmem_take16(acc_at + c, v);
+          const uint32_t top = top_bits<16>(v);
+          if (top >= 0x7f800000u) {
+            float w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = v[j];
+            mark16(e.out_flags, job.pr.m, job.pr.n, w, m + lane, n + c);
+          }
+          split_pairs<16>(v, top, part);
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              put_unit(unit_at<64>(box + 2048 * k, lane, c / 8 + u), part[k][4 * u], part[k][4 * u + 1],
+                       part[k][4 * u + 2], part[k][4 * u + 3]);
+          tmem_store8(acc_at + c, part[2]);
+        }
+        box_written();
+        if (lane == 0) {
+          send(&maps.out, n, m, 0, box);
+          send(&maps.out, n, m, 1, box + 2048);
+          stores_commit();
+        }
+        tmem_stored();
+        box_read();
 #pragma unroll 1
-          for (int c = 0; c < kBoxCols; c += 16) {
-            uint32_t r[16], part[3][8];
-            tmem_load16(acc_at + c, r);
-            tmem_wait(r);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              bf16 a[3], b[3];
-              split3(__uint_as_float(r[2 * j]), a[0], a[1], a[2]);
-              split3(__uint_as_float(r[2 * j + 1]), b[0], b[1], b[2]);
-#pragma unroll
-              for (int k = 0; k < 3; ++k) part[k][j] = pack2(a[k], b[k]);
-            }
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int k = 4 * u;
-              if (pass) {
-                put_unit(unit_at<64>(box, lane, c / 8 + u), part[2][k], part[2][k + 1], part[2][k + 2], part[2][k + 3]);
-              } else {
-                put_unit(unit_at<64>(box, lane, c / 8 + u), part[0][k], part[0][k + 1], part[0][k + 2], part[0][k + 3]);
-                put_unit(unit_at<64>(box + 2048, lane, c / 8 + u), part[1][k], part[1][k + 1], part[1][k + 2],
-                         part[1][k + 3]);
-              }
-            }
-          }
-          box_written();
-          if (lane == 0) {
-            send(&maps.out, n, m, 2 * pass, box);
-            if (!pass) send(&maps.out, n, m, 1, box + 2048);
-            stores_commit();
-          }
+        for (int c = 0; c < kBoxCols; c += 16) take_back<64>(box, lane, c, acc_at + c, __half());
+        box_written();
+        if (lane == 0) {
+          send(&maps.out, n, m, 2, box);
+          stores_commit();
         }
       } else {
         box_written();
