@@ -213,13 +213,16 @@ __device__ __forceinline__ void statistics(const C x[NV], int cols, int lane, fl
   t = both(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
+    if (kVec && column<G, true>(lane, i, 0) >= cols) continue;
     float2 v[4];
     x[i].get(v);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float2 d = add2(v[j], minus);
-      if (column<G, kVec>(lane, i, kVec ? 0 : 2 * j) >= cols) d.x = 0.f;
-      if (column<G, kVec>(lane, i, kVec ? 0 : 2 * j + 1) >= cols) d.y = 0.f;
+      if (!kVec) {
+        if (column<G, false>(lane, i, 2 * j) >= cols) d.x = 0.f;
+        if (column<G, false>(lane, i, 2 * j + 1) >= cols) d.y = 0.f;
+      }
       t = fma2(d, d, t);
     }
   }
@@ -372,8 +375,8 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, G == 32 && (NV > 1 || !kVe
     }
     if (!a.dx) continue;
     const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
-    // rstd (g w - c1 - h c2), with h = (x - mean) rstd
-    const float2 c1 = both(-here.rstd * (s.a / n)), c2 = both(-here.rstd * (s.b / n));
+    // rstd (g w - mean(g w) - h mean(g w h)), with h = (x - mean) rstd
+    const float2 c1 = both(-here.rstd * (s.a / n)), c2 = both(-here.rstd * here.rstd * (s.b / n));  // of x - mean
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       float2 h[4], d[4], p[4];
@@ -382,9 +385,8 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, G == 32 && (NV > 1 || !kVe
       if (a.w) weight(i, p);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        h[j] = mul2(add2(h[j], minus), scale);
         if (a.w) d[j] = mul2(d[j], p[j]);
-        d[j] = fma2(h[j], c2, fma2(d[j], scale, c1));
+        d[j] = fma2(add2(h[j], minus), c2, fma2(d[j], scale, c1));
       }
       store_chunk<G, kVec>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, &d[0].x);
     }
@@ -490,29 +492,20 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
     async::wait(bar0 + 8 * stage, phase, dead);
     const auto x_at = [&](int i, float2 v[4]) {
       const int c = column<G, true>(lane, i, 0);
-      if (c >= cols) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = both(0.f);
-      } else if (kCodes) {
+      if (kCodes) {
         ckpt::values_of(*reinterpret_cast<const uint2*>(at + c), exps[i], &v[0].x);
       } else {
         lin::load8(reinterpret_cast<const T*>(at) + c, &v[0].x);
       }
     };
-    const auto g_at = [&](int i, float2 v[4]) {
-      const int c = column<G, true>(lane, i, 0);
-      if (c >= cols) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = both(0.f);
-      } else {
-        lin::load8(g_row + c, &v[0].x);
-      }
-    };
+    const auto g_at = [&](int i, float2 v[4]) { lin::load8(g_row + column<G, true>(lane, i, 0), &v[0].x); };
+    const auto beyond = [&](int i) { return column<G, true>(lane, i, 0) >= cols; };
     float mean, rstd;
     if (kCodes) {
       float2 t = both(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (beyond(i)) continue;
         float2 v[4];
         x_at(i, v);
 #pragma unroll
@@ -522,14 +515,13 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
       t = both(0.f);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (beyond(i)) continue;
         float2 v[4];
         x_at(i, v);
-        if (column<G, true>(lane, i, 0) < cols) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            v[j] = add2(v[j], both(-mean));
-            t = fma2(v[j], v[j], t);
-          }
+        for (int j = 0; j < 4; ++j) {
+          v[j] = add2(v[j], both(-mean));
+          t = fma2(v[j], v[j], t);
         }
       }
       rstd = rsqrtf(row_sums<G, true>(t.x + t.y, buf, turn) / n + a.eps);
@@ -541,6 +533,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
     float2 sum = both(0.f), dot = both(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if (beyond(i)) continue;
       float2 h[4], d[4], p[4];
       x_at(i, h);
       g_at(i, d);
@@ -562,18 +555,18 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
       if (ahead < a.rows) fetch(ahead, last);
     }
     if (a.dx) {
-      const float2 c1 = both(-rstd * (s.a / n)), c2 = both(-rstd * (s.b / n));
+      const float2 c1 = both(-rstd * (s.a / n)), c2 = both(-rstd * rstd * (s.b / n));  // of x - mean
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
+        if (beyond(i)) continue;
         float2 h[4], d[4], p[4];
         x_at(i, h);
         g_at(i, d);
         if (a.w) weight(i, p);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          h[j] = mul2(add2(h[j], minus), scale);
           if (a.w) d[j] = mul2(d[j], p[j]);
-          d[j] = fma2(h[j], c2, fma2(d[j], scale, c1));
+          d[j] = fma2(add2(h[j], minus), c2, fma2(d[j], scale, c1));
         }
         store_chunk<G, true>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, &d[0].x);
       }
@@ -779,7 +772,12 @@ int blocks_of_rows(int64_t rows, const Form& f, int per_sm) {
 
 template <typename T, typename W, int G, int NV, bool kVec, bool kCodes>
 cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
-  const int per_sm = std::max(1, 2048 / Shape<G>::kThreads / 2);
+  // as many blocks as are under way together: one more a multiprocessor would run alone at the end
+  static const int per_sm = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, forward_kernel<G, NV, kVec, kCodes, T, W>,
+                                                         Shape<G>::kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
+  }();
   const int grid = blocks_of_rows(a.rows, Form{G, NV}, per_sm);
   forward_kernel<G, NV, kVec, kCodes, T, W><<<grid, Shape<G>::kThreads, 0, stream>>>(a);
   return cudaGetLastError();
