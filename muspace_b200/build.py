@@ -70,6 +70,8 @@ def build_native(force: bool = False, verbose: bool = False, output: Path | None
         "-lineinfo",
         "-std=c++17",
         "-shared",
+        "--threads",
+        "0",
         "-Xcompiler",
         "-fPIC,-fvisibility=hidden",
         "-cudart",

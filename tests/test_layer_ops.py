@@ -339,6 +339,27 @@ def test_layer_ops_on_a_side_stream_and_in_a_graph(cuda_device):
     assert torch.equal(captured, both()) and not torch.equal(captured, expected)
 
 
+@pytest.mark.gpu
+def test_layer_ops_past_two_to_the_31_elements(cuda_device):
+    """Rows whose offsets need 64 bits equal the same rows of a small call, forward and backward."""
+    rows, width = 263000, 8200  # 2.16e9 outputs
+    x = torch.randn(rows, 32, device=cuda_device, dtype=BF16)
+    w = torch.randn(width, 32, device=cuda_device, dtype=BF16) / 4
+    y = linear_act(x, w, activation="gelu")
+    tail = slice(rows - 300, rows)
+    assert torch.equal(y[tail], linear_act(x[tail], w, activation="gelu"))
+    scale = torch.rand(width, device=cuda_device, dtype=BF16)
+    leaf = y.requires_grad_(True)
+    n = layer_norm(leaf, scale)
+    assert torch.equal(n[tail].detach(), layer_norm(leaf.detach()[tail], scale))
+    (d,) = torch.autograd.grad(n, [leaf], y.detach())
+    small = leaf.detach()[tail].clone().requires_grad_(True)
+    assert torch.equal(d[tail], torch.autograd.grad(layer_norm(small, scale), [small], small.detach())[0])
+    del n, d
+    kept = checkpoint_pack(leaf)
+    assert torch.equal(checkpoint_unpack(kept)[tail], checkpoint_unpack(checkpoint_pack(leaf.detach()[tail])))
+
+
 # ---- layer norm ---------------------------------------------------------------------------
 
 
