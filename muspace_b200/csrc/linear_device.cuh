@@ -102,7 +102,13 @@ __device__ __forceinline__ void activate(Act act, float* z, float* s) {
   } else if (act == Act::kRelu) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      if (kS) s[j] = z[j] > 0.f ? 1.f : (z[j] <= 0.f ? 0.f : z[j]);
+      // two selects, by name: as nested ?: it became a branch per value, and the lanes parted
+      // (forward with slope, 40000 x 256 x 512 bfloat16: 41 us instead of 32)
+      if (kS)
+        asm("{.reg .pred p; .reg .f32 t; setp.gt.f32 p, %1, 0f00000000; selp.f32 t, 0f3f800000, 0f00000000, p; "
+            "setp.nan.f32 p, %1, %1; selp.f32 %0, %1, t, p;}"
+            : "=f"(s[j])
+            : "f"(z[j]));
       if (kY) asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(z[j]));
     }
   } else if (kS) {

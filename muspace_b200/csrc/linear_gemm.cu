@@ -483,12 +483,6 @@ __device__ __noinline__ void mark16(Flags* flags, int64_t rows, int64_t cols, co
   }
 }
 
-__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bytes,
-                                         uint32_t bar) {
-  expect_bytes(bar, bytes);
-  copy_box<1>(dst, map, x, y, 0, bar);
-}
-
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
                "r"(y), "r"(z), "r"(src)
@@ -526,6 +520,7 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
   constexpr int kMode = kKind / 8;
   constexpr Act kAct = static_cast<Act>(kKind / 2 % 4);
   constexpr bool kExtra = kKind % 2;
+  constexpr bool kSlope = kMode == kFwdSlope;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t tmem = place.tmem, rank = place.rank;
   const auto acc_full = [&](int b) { return place.bars + 8 * (2 * S::kStages + b); };
@@ -538,13 +533,15 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
   constexpr int kRowBytes = kBoxCols * sizeof(T);
   constexpr bool kFast = sizeof(T) == 2;
   constexpr int kParts = S::kCols / kBoxCols;  // more than one only for partial sums
+  constexpr int kHalfCols = 64 / sizeof(T), kHalves = S::kCols / kHalfCols;  // with the slope: rows of 64 bytes
+  static_assert(!kSlope || kHalves <= 2, "a part to each half of the box");
   const int quad = warp & 3, group = warp >> 2;
   const uint32_t box = place.boxes + warp * kBoxBytes;
   const uint32_t arrived = place.bars + 8 * (2 * S::kStages + 4 + warp);  // the residual's box
   const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
   const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
   const Epilogue& e = job.pr.epi;
-  constexpr bool kSlope = kMode == kFwdSlope, kPlanes = sizeof(T) == 4 && kMode == Epilogue::kDz;
+  constexpr bool kPlanes = sizeof(T) == 4 && kMode == Epilogue::kDz;
   const bool extra = kSlope ? e.extra != nullptr : kExtra;
   const bool with_bias = kMode != Epilogue::kStore && e.bias != nullptr;
   const bool bias_vec = reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
@@ -563,10 +560,25 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
     if (lane == 0) stores_read<0>();
     __syncwarp();
   };
+  const auto half_read = [&] {
+    if (lane == 0) stores_read<1>();
+    __syncwarp();
+  };
+  const auto load_extra = [&](const Item& t) {
+    if constexpr (kSlope) {
+      expect_bytes(arrived, kHalves * kBoxBytes / 2);
+#pragma unroll
+      for (int p = 0; p < kHalves; ++p)
+        copy_box<1>(box + p * kBoxBytes / 2, &maps.extra, col_of(t) + p * kHalfCols, row_of(t), 0, arrived);
+    } else {
+      expect_bytes(arrived, 32 * kRowBytes);
+      copy_box<1>(box, &maps.extra, col_of(t), row_of(t), 0, arrived);
+    }
+  };
   int buf = 0;
   uint32_t acc_phase = 0, extra_phase = 0;
   Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
-  if (extra && first < items && lane == 0) load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
+  if (extra && first < items && lane == 0) load_extra(t);
   for (uint32_t i = first; i < items; i += step) {
     const int m = row_of(t), n0 = col_of(t);
     uint32_t acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
@@ -605,8 +617,65 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
       wait(arrived, extra_phase, dead);
       extra_phase ^= 1;
     }
+    if constexpr (kSlope) {
+      // Half a box for a part of y, half for a part of the slope, which waits in
+      // tensor memory meanwhile: a half is written when all stores but the last
+      // one have been read, so no part waits for the store just before it. (Whole
+      // boxes in turn: float32, 22223 x 256 x 1024, 130 us; halves 122. In bfloat16
+      // the bytes of y and the slope are the bound, 40000 x 256 x 512 37 us either way.)
 #pragma unroll 1
-    for (int p = 0; p < kParts; ++p) {
+      for (int p = 0; p < kHalves; ++p) {
+        const int n = n0 + p * kHalfCols;
+        const uint32_t half = box + p * kBoxBytes / 2;
+        if (!extra) half_read();
+#pragma unroll 1
+        for (int c = 0; c < kHalfCols; c += 16) {
+          const uint32_t at = acc_at + p * kHalfCols + c;
+          float v[16], s[16];
+          Bias16<T> bias;
+          if (with_bias) bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
+          tmem_take16(at, v);
+          if (kF32 && repairs) {
+            float w[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = v[j];
+            repair<16>(job.pr, w, m + lane, n + c);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = w[j];
+          }
+          if (with_bias) bias.add(v);
+          activate<kFast, true, true, 16>(kAct, v, s);
+          put_aside(at, s, typename SlopeOf<T>::type());
+          if (extra) {
+            get16<64>(half, lane, c, s, T());
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += s[j];
+          }
+          put16<64>(half, lane, c, v, T());
+        }
+        box_written();
+        if (lane == 0) {
+          send(&maps.out, n, m, 0, half);
+          stores_commit();
+        }
+      }
+      tmem_stored();
+#pragma unroll 1
+      for (int p = 0; p < kHalves; ++p) {
+        const uint32_t half = box + (kHalves == 1 ? 1 : p) * kBoxBytes / 2;
+        half_read();
+#pragma unroll 1
+        for (int c = 0; c < kHalfCols; c += 16)
+          take_back<64>(half, lane, c, acc_at + p * kHalfCols + c, typename SlopeOf<T>::type());
+        box_written();
+        if (lane == 0) {
+          send(&maps.slope, n0 + p * kHalfCols, m, 0, half);
+          stores_commit();
+        }
+      }
+    }
+#pragma unroll 1
+    for (int p = 0; p < (kSlope ? 0 : kParts); ++p) {
       const int n = n0 + p * kBoxCols;
       if (!extra) box_read();
 #pragma unroll 1
@@ -644,14 +713,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           if (sizeof(T) == 4) {
             tmem_store16(at, v);
             continue;
-          }
-        } else if (kSlope) {
-          activate<kFast, true, true, 16>(e.act, v, s);
-          put_aside(at, s, typename SlopeOf<T>::type());
-          if (extra) {
-            get16<kRowBytes>(box, lane, c, x, T());
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += x[j];
           }
         } else if (kMode == Epilogue::kFwd) {
           activate<kFast, true, false, 16>(kAct, v, s);
@@ -708,18 +769,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           send(&maps.out, n, m, job.apart ? t.split : 0, box);
           stores_commit();
         }
-        if constexpr (kSlope) {
-          // the slopes wait in tensor memory for the box
-          tmem_stored();
-          box_read();
-#pragma unroll 1
-          for (int c = 0; c < kBoxCols; c += 16) take_back<kRowBytes>(box, lane, c, acc_at + c, typename SlopeOf<T>::type());
-          box_written();
-          if (lane == 0) {
-            send(&maps.slope, n, m, 0, box);
-            stores_commit();
-          }
-        }
       }
     }
     fence_before();
@@ -731,7 +780,7 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
       t = item_of<BN, CG>(job, i + step);
       if (extra && lane == 0) {
         stores_read<0>();
-        load_box(box, &maps.extra, col_of(t), row_of(t), 32 * kRowBytes, arrived);
+        load_extra(t);
       }
     }
   }
@@ -798,7 +847,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (CG == 2) bytes += bytes_of(t.m + kTileM, t.n + S::kRowsB);
       // One thread issues a stage's copies while the tensor core works on another
       // (512 clocks): the layouts are constants, as counted loops over boxes and
-      // planes took longer than that (8192 x 4096 x 8192, dW: 491 us, now 419).
+      // planes took longer than that (8192 x 4096 x 8192, dW: 491 us, now 387).
       const auto stages = [&](auto a_across, auto b_across) {
         constexpr bool kA = decltype(a_across)::value, kB = decltype(b_across)::value;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
@@ -890,7 +939,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Epilogue& e = job.pr.epi;
     const int mode = job.apart ? Epilogue::kStore : e.mode;
     const bool extra = mode != Epilogue::kStore && e.extra != nullptr;
-    const int kind = mode == Epilogue::kFwd && e.slope ? kFwdSlope * 8
+    const int kind = mode == Epilogue::kFwd && e.slope ? kFwdSlope * 8 + static_cast<int>(e.act) * 2
                      : mode == Epilogue::kStore        ? Epilogue::kStore * 8
                                                        : mode * 8 + static_cast<int>(e.act) * 2 + (extra ? 1 : 0);
     const Place at{tmem, ring + S::kStages * S::kStage, bars, rank};
@@ -910,6 +959,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         case Epilogue::kDz * 8 + 3: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 3>(maps, job, at); break;
         case Epilogue::kDz * 8 + 5: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 5>(maps, job, at); break;
         case Epilogue::kDz * 8 + 7: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 7>(maps, job, at); break;
+        case kFwdSlope * 8 + 2: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 2>(maps, job, at); break;
+        case kFwdSlope * 8 + 4: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 4>(maps, job, at); break;
+        case kFwdSlope * 8 + 6: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 6>(maps, job, at); break;
         default: epilogue<BN, CG, T, kF32, kFwdSlope * 8>(maps, job, at);
       }
     }
@@ -1037,7 +1089,8 @@ bool epilogue_maps(Maps& maps, const Product& pr, const Plan& plan, bool apart) 
                     pr.m * partial_ld(pr.n) * 4, 32, 32, 128);
   const bool wide = pr.dtype == DType::kF32;
   const int64_t size = wide ? 4 : 2;
-  const int row_bytes = std::min<int>(128, std::max(32, plan.bn / 4) * static_cast<int>(size));
+  const bool slope = e.mode == Epilogue::kFwd && e.slope;
+  const int row_bytes = slope ? 64 : std::min<int>(128, std::max(32, plan.bn / 4) * static_cast<int>(size));
   const int cols = row_bytes / static_cast<int>(size);
   bool ok = true;
   if (e.mode == Epilogue::kDz && wide)
@@ -1046,7 +1099,7 @@ bool epilogue_maps(Maps& maps, const Product& pr, const Plan& plan, bool apart) 
     ok = make_map(&maps.out, wide ? f32 : b16, e.out, pr.n, pr.m, 1, e.out_ld * size, 0, cols, 32, row_bytes);
   if (ok && e.mode != Epilogue::kStore && e.extra)
     ok = make_map(&maps.extra, wide ? f32 : b16, e.extra, pr.n, pr.m, 1, e.extra_ld * size, 0, cols, 32, row_bytes);
-  if (ok && e.mode == Epilogue::kFwd && e.slope)
+  if (ok && slope)
     ok = make_map(&maps.slope, wide ? f32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, e.slope, pr.n, pr.m, 1, pr.n * size, 0,
                   cols, 32, row_bytes);
   return ok;
