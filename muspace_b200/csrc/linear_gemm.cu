@@ -53,12 +53,18 @@ constexpr int kRingBytes = 160 * 1024;
 constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
 
+// float32: the order in which a stage's planes are copied, used and given back.
+// A plane of A and of B has a slot of the ring to itself. Half the products want
+// no third plane, and the second is free again after half of them: so the copies
+// of the next stage begin, and its products do, before the stage is whole.
+__host__ __device__ constexpr int plane_of(int i) { return i == 0 ? 1 : i == 1 ? 0 : 2; }
+
 template <int BN, int CG, bool kF32>
 struct Shape {
   static constexpr int kPlanes = kF32 ? 3 : 1;
   static constexpr int kRowsB = BN / CG;  // rows of B in one block's stage
   static constexpr int kStageB = kRowsB * kBlockK * 2;
-  static constexpr int kStage = kPlanes * (kStageA + kStageB);
+  static constexpr int kStage = kStageA + kStageB;  // one plane of both
   static constexpr int kStages = kRingBytes / kStage;
   static constexpr int kBarriers = 2 * kStages + 4 + kEpiWarps;
   // stages, the warps' staging, barriers, the tensor-memory address; and room to start on 1024 bytes
@@ -76,7 +82,7 @@ struct Job {
   Product pr;
   uint32_t tiles_m, tiles_n;
   uint64_t by_tiles, by_group, by_last;  // divided()
-  int splits, kblocks, kblocks_per_split, pairs;
+  int splits, kblocks, kblocks_per_split;
   int box_a, box_b;  // rows of the boxes along k
   int device;
   bool apart;        // the epilogue leaves sums in pr.partial
@@ -283,18 +289,6 @@ __device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
   t.kb0 = t.split * j.kblocks_per_split;
   t.kb1 = min(j.kblocks, t.kb0 + j.kblocks_per_split);
   return t;
-}
-
-// The planes of A and B in product `i` of a stage; the last one is that of the
-// first planes.
-__device__ __forceinline__ void planes_of(const Job& j, int i, int& pa, int& pb) {
-  if (j.pairs == 6) {
-    pa = (0x010120 >> (4 * i)) & 3;
-    pb = (0x001102 >> (4 * i)) & 3;
-  } else {
-    pa = j.pr.a.planes == 3 ? j.pairs - 1 - i : 0;
-    pb = j.pr.b.planes == 3 ? j.pairs - 1 - i : 0;
-  }
 }
 
 // ---- float32: what planes cannot hold -----------------------------------------------
@@ -837,47 +831,44 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item t = item_of<BN, CG>(job, i);
       // boxes that hold rows of the tile; what a skipped box leaves in its place reaches no row or column that is kept
       const auto boxes = [](int have, int most) { return have <= 0 ? 0 : min(most, (have - 1) / 64 + 1); };
-      const auto bytes_of = [&](int ma, int nb) {
-        return (job.pr.a_mn ? boxes(rows_m - ma, kTileM / 64) * 8192 : job.box_a * 128) * job.pr.a.planes +
-               (job.pr.b_mn ? boxes(rows_n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128) * job.pr.b.planes;
+      const auto bytes_a = [&](int ma) { return job.pr.a_mn ? boxes(rows_m - ma, kTileM / 64) * 8192 : job.box_a * 128; };
+      const auto bytes_b = [&](int nb) {
+        return job.pr.b_mn ? boxes(rows_n - nb, S::kRowsB / 64) * 8192 : job.box_b * 128;
       };
       const int ma = t.m + rank * kTileM, nb = t.n + rank * S::kRowsB;
       const int boxes_a = boxes(rows_m - ma, kTileM / 64), boxes_b = boxes(rows_n - nb, S::kRowsB / 64);
-      uint32_t bytes = bytes_of(t.m, t.n);
-      if (CG == 2) bytes += bytes_of(t.m + kTileM, t.n + S::kRowsB);
+      const uint32_t from_a = bytes_a(t.m) + (CG == 2 ? bytes_a(t.m + kTileM) : 0);
+      const uint32_t from_b = bytes_b(t.n) + (CG == 2 ? bytes_b(t.n + S::kRowsB) : 0);
       // One thread issues a stage's copies while the tensor core works on another
       // (512 clocks): the layouts are constants, as counted loops over boxes and
       // planes took longer than that (8192 x 4096 x 8192, dW: 491 us, now 387).
       const auto stages = [&](auto a_across, auto b_across) {
         constexpr bool kA = decltype(a_across)::value, kB = decltype(b_across)::value;
         for (int kb = t.kb0; kb < t.kb1; ++kb) {
-          const uint32_t bar = full0 + 8 * s, a = ring + s * S::kStage, b = a + S::kPlanes * kStageA;
           const int k = kb * kBlockK;
-          wait(empty(s), phase ^ 1, dead);
-          if (rank == 0) expect_bytes(full(s), bytes);
 #pragma unroll
-          for (int p = 0; p < S::kPlanes; ++p) {
-            if (kF32 && p >= job.pr.a.planes) break;
+          for (int u = 0; u < S::kPlanes; ++u) {
+            const int p = kF32 ? plane_of(u) : 0;
+            const bool has_a = !kF32 || p < job.pr.a.planes, has_b = !kF32 || p < job.pr.b.planes;
+            const uint32_t bar = full0 + 8 * s, a = ring + s * S::kStage, b = a + kStageA;
+            wait(empty(s), phase ^ 1, dead);
+            if (rank == 0) expect_bytes(full(s), (has_a ? from_a : 0) + (has_b ? from_b : 0));
             if (kA) {
 #pragma unroll
               for (int x = 0; x < kTileM / 64; ++x)
-                if (x < boxes_a) copy_box<CG>(a + p * kStageA + x * 8192, &maps.a, ma + x * 64, k, p, bar);
+                if (has_a && x < boxes_a) copy_box<CG>(a + x * 8192, &maps.a, ma + x * 64, k, p, bar);
             } else {
-              copy_box<CG>(a + p * kStageA, &maps.a, k, ma, p, bar);
+              if (has_a) copy_box<CG>(a, &maps.a, k, ma, p, bar);
             }
-          }
-#pragma unroll
-          for (int p = 0; p < S::kPlanes; ++p) {
-            if (kF32 && p >= job.pr.b.planes) break;
             if (kB) {
 #pragma unroll
               for (int x = 0; x < S::kRowsB / 64; ++x)
-                if (x < boxes_b) copy_box<CG>(b + p * S::kStageB + x * 8192, &maps.b, nb + x * 64, k, p, bar);
+                if (has_b && x < boxes_b) copy_box<CG>(b + x * 8192, &maps.b, nb + x * 64, k, p, bar);
             } else {
-              copy_box<CG>(b + p * S::kStageB, &maps.b, k, nb, p, bar);
+              if (has_b) copy_box<CG>(b, &maps.b, k, nb, p, bar);
             }
+            if (++s == S::kStages) s = 0, phase ^= 1;
           }
-          if (++s == S::kStages) s = 0, phase ^= 1;
         }
       };
       if (job.pr.a_mn)
@@ -898,7 +889,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t idesc = instruction(kTileM * CG, BN, job.pr.a_mn, job.pr.b_mn);
     const uint32_t step_a = k_step(job.pr.a_mn) >> 4, step_b = k_step(job.pr.b_mn) >> 4;
     const uint64_t first_a = tile_descriptor(ring, job.pr.a_mn);
-    const uint64_t first_b = tile_descriptor(ring + S::kPlanes * kStageA, job.pr.b_mn);
+    const uint64_t first_b = tile_descriptor(ring + kStageA, job.pr.b_mn);
+    const bool more_a = job.pr.a.planes > 1, more_b = job.pr.b.planes > 1;
     int s = 0, buf = 0;
     uint32_t phase = 0, acc_phase = 0;
     for (uint32_t i = first; i < items; i += step) {
@@ -907,27 +899,47 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int steps = min(c + chunk, t.kb1) - c;
         wait(acc_empty(buf), acc_phase ^ 1, dead);
         fence_after();
-        for (int x = 0; x < steps; ++x) {
+        const uint32_t acc = tmem + buf * S::kAcc;
+        // the stage's A of slot sa times its B of slot sb
+        const auto product = [&](uint32_t to, int sa, int sb, bool add) {
+          const uint64_t da = first_a + sa * (S::kStage >> 4), db = first_b + sb * (S::kStage >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 16; ++kk) mma<CG>(to, da + kk * step_a, db + kk * step_b, idesc, add || kk > 0);
+        };
+        const auto arrived = [&] {  // the next slot, once it is full
+          const int at = s;
           wait(full(s), phase, dead);
           fence_after();
-          if (lane == 0) {
-            const uint32_t acc = tmem + buf * S::kAcc;
-            const uint64_t da0 = first_a + s * (S::kStage >> 4), db0 = first_b + s * (S::kStage >> 4);
-#pragma unroll 1
-            for (int p = 0; p < (kF32 ? job.pairs : 1); ++p) {
-              int pa = 0, pb = 0;
-              if (kF32) planes_of(job, p, pa, pb);
-              const bool large = !kF32 || p + 1 == job.pairs;
-              const uint64_t da = da0 + pa * (kStageA >> 4), db = db0 + pb * (S::kStageB >> 4);
-#pragma unroll
-              for (int kk = 0; kk < kBlockK / 16; ++kk)
-                mma<CG>(large ? acc : acc + BN, da + kk * step_a, db + kk * step_b, idesc,
-                        x > 0 || kk > 0 || (!large && p > 0));
+          if (++s == S::kStages) s = 0, phase ^= 1;
+          return at;
+        };
+        for (int x = 0; x < steps; ++x) {
+          if constexpr (kF32) {
+            bool add = x > 0;  // in the small products' accumulator
+            const int mid = arrived();
+            if (lane == 0 && more_a && more_b) product(acc + BN, mid, mid, add), add = true;
+            const int hi = arrived();
+            if (lane == 0) {
+              if (more_a) product(acc + BN, mid, hi, add), add = true;
+              if (more_b) product(acc + BN, hi, mid, add);
+              commit<CG>(empty(mid));
+              product(acc, hi, hi, x > 0);
             }
-            commit<CG>(empty(s));
+            const int lo = arrived();
+            if (lane == 0) {
+              if (more_a) product(acc + BN, lo, hi, true);
+              if (more_b) product(acc + BN, hi, lo, true);
+              commit<CG>(empty(hi));
+              commit<CG>(empty(lo));
+            }
+          } else {
+            const int at = arrived();
+            if (lane == 0) {
+              product(acc, at, at, x > 0);
+              commit<CG>(empty(at));
+            }
           }
           __syncwarp();
-          if (++s == S::kStages) s = 0, phase ^= 1;
         }
         if (lane == 0) commit<CG>(acc_full(buf));
         __syncwarp();
@@ -1222,7 +1234,6 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
     job.by_last = magic(job.tiles_m % kGroupM);
     job.kblocks = static_cast<int>(ceil_div(pr.k, kBlockK));
     job.kblocks_per_split = plan.kblocks;
-    job.pairs = pr.a.planes == 3 ? (pr.b.planes == 3 ? 6 : 3) : (pr.b.planes == 3 ? 3 : 1);
     job.apart = finished_apart(pr, plan);
     const int64_t rows_b = plan.bn / plan.pair;
     job.box_a = pr.a_mn ? 64 : static_cast<int>(std::min<int64_t>(kTileM, ceil_div(pr.m, 8) * 8));
