@@ -18,13 +18,20 @@
 // along k, dx = dz W reads W across it, dW = dz^T x both. Nothing is transposed
 // in memory; the instruction and the tile's layout differ.
 //
-// float32 (three bfloat16 planes an operand): a stage holds all planes of its k,
-// and the six products of planes that reach 2^-24 of the result are issued on
-// it. The tensor core's float32 accumulator cuts where an FMA would round:
+// float32 (three bfloat16 planes an operand): a stage is the three planes of its
+// k, and the six products of planes that reach 2^-24 of the result are issued on
+// them. The tensor core's float32 accumulator cuts where an FMA would round:
 // 2^-25 of what it holds per step on average, always towards zero. So the five
 // small products, 2^-8 of the result and below, have an accumulator of their
-// own, and the sums over 128 of k at a time are added up in registers: the
-// relative error is 1.3e-7, where one accumulator over 256 of k had 2.9e-6.
+// own, taken over 1024 of k, and the sums over 128 of k of the first product are
+// added up in registers: the relative error is 1.3e-7, where one accumulator
+// over 256 of k had 2.9e-6. A finished tile waits in the small products' columns
+// for its epilogue, so the next tile's products go on (22223 x 256 x 1024 with
+// slope: 98 us; with the two accumulators side by side and held by the epilogue
+// 107). What bounds it: a product of 128 columns takes the time of one of 256
+// (2048 x 2048 x 2048: 107 us). Tiles of 256 leave room for one accumulator only;
+// with both sums read after every 128 of k they took 105 us there, read after
+// every 1024 70, and 20 us more than now where k is 256.
 #include <cuda.h>  // CUtensorMap and its enums only: the encoder comes from cudaGetDriverEntryPoint
 
 #include <algorithm>
@@ -50,7 +57,8 @@ constexpr int kThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageA = kTileM * kBlockK * 2;
 constexpr int kBoxBytes = 32 * 128;  // a box of the epilogue: 32 rows of 128 bytes
 constexpr int kRingBytes = 160 * 1024;
-constexpr int kPromote = 2;       // k blocks between additions in registers (float32)
+constexpr int kPromote = 2;       // k blocks between additions in registers (float32): 4 would take 10 % off, at twice the error
+constexpr int kFold = 8;          // and how many of those additions to one of the small products' sums
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
 
 // float32: the order in which a stage's planes are copied, used and given back.
@@ -66,11 +74,12 @@ struct Shape {
   static constexpr int kStageB = kRowsB * kBlockK * 2;
   static constexpr int kStage = kStageA + kStageB;  // one plane of both
   static constexpr int kStages = kRingBytes / kStage;
-  static constexpr int kBarriers = 2 * kStages + 4 + kEpiWarps;
+  static constexpr int kBarriers = 2 * kStages + 4 + kEpiWarps + (kF32 ? 2 : 0);
   // stages, the warps' staging, barriers, the tensor-memory address; and room to start on 1024 bytes
   static constexpr int kSmem = kStages * kStage + kEpiWarps * kBoxBytes + kBarriers * 8 + 16 + 1024;
-  static constexpr int kAcc = kF32 ? 2 * BN : BN;  // columns of an accumulator: float32 has the small products' beside it
-  static constexpr uint32_t kColumns = 2 * kAcc;
+  // tensor memory: two accumulators; float32 has two more behind them, the small products'
+  static constexpr int kSmall = 2 * BN;
+  static constexpr uint32_t kColumns = kF32 ? 4 * BN : 2 * BN;
   // a warp of the epilogue takes 32 rows and this many columns
   static constexpr int kCols = BN / 4 < 32 ? 32 : BN / 4;
   static constexpr int kWarps = 4 * (BN / kCols);
@@ -519,6 +528,7 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
   const uint32_t tmem = place.tmem, rank = place.rank;
   const auto acc_full = [&](int b) { return place.bars + 8 * (2 * S::kStages + b); };
   const auto acc_empty = [&](int b) { return place.bars + 8 * (2 * S::kStages + 2 + b); };
+  const auto small_empty = [&](int b) { return place.bars + 8 * (2 * S::kStages + 4 + kEpiWarps + b); };
   const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
   const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
   const int chunk = kF32 ? kPromote : job.kblocks;
@@ -569,38 +579,49 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
       copy_box<1>(box, &maps.extra, col_of(t), row_of(t), 0, arrived);
     }
   };
-  int buf = 0;
+  int buf = 0, small = 0;
   uint32_t acc_phase = 0, extra_phase = 0;
   Item t = first < items ? item_of<BN, CG>(job, first) : Item{};
   if (extra && first < items && lane == 0) load_extra(t);
   for (uint32_t i = first; i < items; i += step) {
     const int m = row_of(t), n0 = col_of(t);
-    uint32_t acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
+    uint32_t acc_at = tmem + lanes + buf * BN + group * S::kCols;
     if (kF32) {
       float acc[S::kCols / 16][16] = {};
-      for (int c = t.kb0; c < t.kb1; c += chunk) {
+      for (int c = t.kb0, n = 1; c < t.kb1; c += chunk, ++n) {
         wait(acc_full(buf), acc_phase, dead);
         fence_after();
-        const bool more = c + chunk < t.kb1;
-        acc_at = tmem + lanes + buf * S::kAcc + group * S::kCols;
+        const bool last = c + chunk >= t.kb1, fold = last || n % kFold == 0;
+        const uint32_t main_at = tmem + lanes + buf * BN + group * S::kCols;
+        acc_at = tmem + lanes + S::kSmall + small * BN + group * S::kCols;
 #pragma unroll
         for (int q = 0; q < S::kCols / 16; ++q) {
-          uint32_t r[16], small[16];
-          tmem_load16(acc_at + q * 16, r);
-          tmem_load16(acc_at + BN + q * 16, small);
+          uint32_t r[16];
+          tmem_load16(main_at + q * 16, r);
           tmem_wait(r);
-          tmem_wait(small);
 #pragma unroll
-          for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]) + __uint_as_float(small[x]);
-          if (!more) tmem_store16(acc_at + q * 16, acc[q]);
+          for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
         }
-        if (more) {
-          fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
-          buf ^= 1;
-          if (buf == 0) acc_phase ^= 1;
+        if (fold) {
+#pragma unroll
+          for (int q = 0; q < S::kCols / 16; ++q) {
+            uint32_t r[16];
+            tmem_load16(acc_at + q * 16, r);
+            tmem_wait(r);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
+            if (last) tmem_store16(acc_at + q * 16, acc[q]);  // the tile waits there for its epilogue
+          }
         }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          arrive_in(in_block(acc_empty(buf), 0));
+          if (fold && !last) arrive_in(in_block(small_empty(small), 0));
+        }
+        if (fold && !last) small ^= 1;
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
       }
       tmem_stored();
     } else {
@@ -767,9 +788,14 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
     }
     fence_before();
     __syncwarp();
-    if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
-    buf ^= 1;
-    if (buf == 0) acc_phase ^= 1;
+    if (kF32) {
+      if (lane == 0) arrive_in(in_block(small_empty(small), 0));
+      small ^= 1;
+    } else {
+      if (lane == 0) arrive_in(in_block(acc_empty(buf), 0));
+      buf ^= 1;
+      if (buf == 0) acc_phase ^= 1;
+    }
     if (i + step < items) {
       t = item_of<BN, CG>(job, i + step);
       if (extra && lane == 0) {
@@ -793,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
   const auto acc_full = [&](int b) { return bars + 8 * (2 * S::kStages + b); };
   const auto acc_empty = [&](int b) { return bars + 8 * (2 * S::kStages + 2 + b); };
+  const auto small_empty = [&](int b) { return bars + 8 * (2 * S::kStages + 4 + kEpiWarps + b); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t rank = 0;
@@ -806,6 +833,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int b = 0; b < 2; ++b) {
       barrier_init(acc_full(b), 1);
       barrier_init(acc_empty(b), S::kWarps * CG);
+      if (kF32) barrier_init(small_empty(b), S::kWarps * CG);
     }
     for (int x = 0; x < kEpiWarps; ++x) barrier_init(bars + 8 * (2 * S::kStages + 4 + x), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -891,15 +919,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t first_a = tile_descriptor(ring, job.pr.a_mn);
     const uint64_t first_b = tile_descriptor(ring + kStageA, job.pr.b_mn);
     const bool more_a = job.pr.a.planes > 1, more_b = job.pr.b.planes > 1;
-    int s = 0, buf = 0;
-    uint32_t phase = 0, acc_phase = 0;
+    int s = 0, buf = 0, small_buf = 0;
+    uint32_t phase = 0, acc_phase = 0, small_phase = 0;
     for (uint32_t i = first; i < items; i += step) {
       const Item t = item_of<BN, CG>(job, i);
-      for (int c = t.kb0; c < t.kb1; c += chunk) {
+      for (int c = t.kb0, n = 1; c < t.kb1; c += chunk, ++n) {
         const int steps = min(c + chunk, t.kb1) - c;
+        const bool fresh = n % kFold == 1;  // the small products' sums begin anew
         wait(acc_empty(buf), acc_phase ^ 1, dead);
+        if (kF32 && fresh) wait(small_empty(small_buf), small_phase ^ 1, dead);
         fence_after();
-        const uint32_t acc = tmem + buf * S::kAcc;
+        const uint32_t small = tmem + S::kSmall + small_buf * BN;
+        const uint32_t acc = tmem + buf * BN;
         // the stage's A of slot sa times its B of slot sb
         const auto product = [&](uint32_t to, int sa, int sb, bool add) {
           const uint64_t da = first_a + sa * (S::kStage >> 4), db = first_b + sb * (S::kStage >> 4);
@@ -915,20 +946,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         };
         for (int x = 0; x < steps; ++x) {
           if constexpr (kF32) {
-            bool add = x > 0;  // in the small products' accumulator
+            bool add = x > 0 || !fresh;  // in the small products' accumulator
             const int mid = arrived();
-            if (lane == 0 && more_a && more_b) product(acc + BN, mid, mid, add), add = true;
+            if (lane == 0 && more_a && more_b) product(small, mid, mid, add), add = true;
             const int hi = arrived();
             if (lane == 0) {
-              if (more_a) product(acc + BN, mid, hi, add), add = true;
-              if (more_b) product(acc + BN, hi, mid, add);
+              if (more_a) product(small, mid, hi, add), add = true;
+              if (more_b) product(small, hi, mid, add);
               commit<CG>(empty(mid));
               product(acc, hi, hi, x > 0);
             }
             const int lo = arrived();
             if (lane == 0) {
-              if (more_a) product(acc + BN, lo, hi, true);
-              if (more_b) product(acc + BN, hi, lo, true);
+              if (more_a) product(small, lo, hi, true);
+              if (more_b) product(small, hi, lo, true);
               commit<CG>(empty(hi));
               commit<CG>(empty(lo));
             }
@@ -943,6 +974,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (lane == 0) commit<CG>(acc_full(buf));
         __syncwarp();
+        if (kF32 && (c + chunk >= t.kb1 || n % kFold == 0) && (small_buf ^= 1) == 0) small_phase ^= 1;
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       }
