@@ -9,9 +9,9 @@ Backward: ``dz = g * act'(z)``, ``dx = dz W``, ``dW = dz^T x``, ``db`` the sum o
 forward (in float16 beside bfloat16: 11 bits of a number in [-0.2, 1.2]), which
 holds as much between the passes as ``z`` itself would, or, with a checkpoint, from
 computing ``z`` again in the epilogue that makes ``dz``. Forward and backward,
-kept and computed again, on a B200: 40000 x 256 x 512 bfloat16 111 and 126 us,
-40000 x 2048 x 512 261 and 317; 22223 x 256 x 1024 float32 376 and 449. Kept was
-the faster one at every size from 128 input features on, in both types.
+kept and computed again, on a B200: 40000 x 256 x 512 bfloat16 108 and 125 us,
+40000 x 2048 x 512 260 and 321; 22223 x 256 x 1024 float32 359 and 418. Kept was
+the faster one at every size from 64 input features on, in both types.
 """
 
 from __future__ import annotations
