@@ -136,10 +136,64 @@ def test_linear_matches_the_formulas(cuda_device, rows, k, n, dtype):
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
 @pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
 @pytest.mark.parametrize("checkpoint", [None, "int8"])
-@pytest.mark.parametrize("k", [72, 640])  # the slope computed again / kept
+@pytest.mark.parametrize("k", [72, 640])
 def test_linear_activations_and_checkpoints(cuda_device, activation, checkpoint, k, dtype):
     check_linear(*linear_inputs(321, k, 200, dtype, cuda_device, seed=k), activation, checkpoint)
     check_linear(*linear_inputs(130, k + 3, 77, dtype, cuda_device, seed=k, residual=False), activation, checkpoint)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("rows,k,n", [(2048, 1024, 1152), (2050, 2100, 1152), (1024, 2048, 2304)])
+def test_linear_long_sums_of_whole_tiles(cuda_device, rows, k, n, dtype):
+    """So many tiles that no sum is split, over k that is and is not a multiple of 1024."""
+    check_linear(*linear_inputs(rows, k, n, dtype, cuda_device, seed=k), "silu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(300, 72, 200), (130, 67, 77)])
+def test_linear_backward_without_a_slope(cuda_device, rows, k, n, activation, dtype):
+    """The C entry computes z again where it is given no slope: the gradients are the formulas' too."""
+    x, w, b, _, g = linear_inputs(rows, k, n, dtype, cuda_device, seed=k)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    args = native.LinearArgs(0 if dtype == F32 else 1, {"relu": 1, "gelu": 2, "silu": 3}[activation], rows, k, n, k, k, 0,
+                             0, n, x.data_ptr(), w.data_ptr(), b.data_ptr(), None, None, None, g.data_ptr(), None, None,
+                             dx.data_ptr(), dw.data_ptr(), db.data_ptr())
+    native.load_native_module().plain_call("msda_linear_act_backward")(x.device, args)
+    x6, w6, g6 = x.double(), w.double(), g.double()
+    z = x6 @ w6.T + b.double()
+    size = x6.abs() @ w6.abs().T + b.double().abs()
+    dz = g6 * slope64(activation, z)
+    loose = dz.abs() * (0 if dtype == F32 else 2.0 ** -8) + g6.abs() * 2 * SUM * size
+    if activation == "relu":  # where z is within its error of 0, the slope may be either
+        loose = loose + g6.abs() * (z.abs() <= 2 * SUM * size)
+    near(dx, dz @ w6, dz.abs() @ w6.abs() + loose @ w6.abs() / SUM, dtype)
+    near(dw, dz.T @ x6, dz.abs().T @ x6.abs() + loose.T @ x6.abs() / SUM, dtype)
+    near(db, dz.sum(0), dz.abs().sum(0) + loose.sum(0) / SUM, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("activation", [0, 1, 2, 3])
+@pytest.mark.parametrize("rows,k,n", [(300, 72, 200), (300, 72, 77), (1, 72, 200)])
+def test_linear_slope_of_the_c_entry(cuda_device, rows, k, n, activation, dtype):
+    x, w, b, r, _ = linear_inputs(rows, k, n, dtype, cuda_device, seed=n)
+    y = torch.empty_like(r)
+    slope = torch.full((rows, n), float("nan"), device=cuda_device, dtype=F32 if dtype == F32 else F16)
+    args = native.LinearArgs(0 if dtype == F32 else 1, activation, rows, k, n, k, k, n, n, 0, x.data_ptr(), w.data_ptr(),
+                             b.data_ptr(), r.data_ptr(), y.data_ptr(), slope.data_ptr())
+    native.load_native_module().plain_call("msda_linear_act_forward")(x.device, args)
+    name = ["none", "relu", "gelu", "silu"][activation]
+    z = x.double() @ w.double().T + b.double()
+    size = x.double().abs() @ w.double().abs().T + b.double().abs()
+    near(y, act64(name, z) + r.double(), 2 * size + 1 + r.double().abs(), dtype)
+    expected = slope64(name, z) if activation else torch.ones_like(z)
+    terms = 2 * size + 1
+    if name == "relu":
+        terms = terms + (z.abs() <= 2 * SUM * size) / SUM
+    near(slope, expected, terms, slope.dtype, extra=0.0 if dtype == F32 else 2.0 ** -23)
 
 
 @pytest.mark.gpu
