@@ -430,8 +430,8 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, G == 32 && (NV > 1 || !kVe
 // 129 us for 8192 rows); so here the rows' data comes to shared memory by bulk
 // copies, several rows ahead, and is read from there twice. Two groups of 256
 // threads take rows in turn, so that one computes while the other waits at its
-// barrier (one group of 512: 113 us; two: 89, 403 MB in and out at 4.5 TB/s). A group's stage is free again when its next row's barrier has been
-// passed.
+// barrier (one group of 512: 113 us; two: 89, 403 MB in and out at 4.5 TB/s). A
+// group's stage is free again when its next row's barrier has been passed.
 constexpr int kRingThreads = 512, kGroup = 256;
 constexpr int kRingBytes = 192 * 1024;
 constexpr int kMaxStages = 8;

@@ -57,7 +57,9 @@ constexpr int kThreads = 32 * (kEpiWarps + 2);
 constexpr int kStageA = kTileM * kBlockK * 2;
 constexpr int kBoxBytes = 32 * 128;  // a box of the epilogue: 32 rows of 128 bytes
 constexpr int kRingBytes = 160 * 1024;
-constexpr int kPromote = 2;       // k blocks between additions in registers (float32): 4 takes 9 % off 2048^3, with twice the steps that cut
+// float32: k blocks between additions in registers (4 takes 9 % off 2048^3, with
+// twice the steps that cut)
+constexpr int kPromote = 2;
 constexpr int kFold = 8;          // and how many of those additions to one of the small products' sums
 constexpr int kGroupM = 8;        // rows of tiles walked together, for L2
 
