@@ -117,7 +117,8 @@ Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs_of_pla
 // finishes: ranges of k, and outputs that TMA cannot address (rows off 16-byte
 // boundaries).
 bool finished_apart(const Product& pr, const Plan& p);
-__host__ __device__ inline int64_t partial_ld(int64_t n) { return (n + 3) / 4 * 4; }
+// Floats from one row of the sums to the next: they are read in whole eights, the last of a row too.
+__host__ __device__ inline int64_t partial_ld(int64_t n) { return (n + 7) / 8 * 8; }
 inline size_t partial_bytes(const Plan& p, int64_t m, int64_t n) {
   return static_cast<size_t>(p.splits) * m * partial_ld(n) * sizeof(float);
 }
