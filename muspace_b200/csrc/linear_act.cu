@@ -47,26 +47,12 @@ Operand fresh(DType dtype, int64_t rows, int64_t cols, int planes, Arena& arena)
   return o;
 }
 
-// The flags of a call's float32 operands: side by side, zeroed together.
-struct Zeroed {
-  char* p = nullptr;
-  static size_t bytes(int64_t rows, int64_t cols) { return (Flags::bytes(rows, cols) + 15) & ~static_cast<size_t>(15); }
-  cudaError_t take(size_t total, Arena& arena, cudaStream_t stream) {
-    p = static_cast<char*>(arena.take(total));
-    return arena.measuring || total == 0 ? cudaSuccess : cudaMemsetAsync(p, 0, total, stream);
-  }
-  void give(Operand& o) {
-    o.flags = reinterpret_cast<Flags*>(p);
-    if (p) p += bytes(o.rows, o.cols);
-  }
-};
-
 bool direct(DType dtype, const void* p, int64_t cols, int64_t ld) {
   return dtype == DType::kBF16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld >= cols;
 }
 
 // A caller's matrix as an operand: as it stands, or laid out in the workspace.
-cudaError_t operand_of(DType dtype, const void* p, int64_t rows, int64_t cols, int64_t ld, Arena& arena, Zeroed& flags,
+cudaError_t operand_of(DType dtype, const void* p, int64_t rows, int64_t cols, int64_t ld, Arena& arena,
                        Operand* out, cudaStream_t stream) {
   if (direct(dtype, p, cols, ld)) {
     out->p = static_cast<const __nv_bfloat16*>(p);
@@ -74,7 +60,6 @@ cudaError_t operand_of(DType dtype, const void* p, int64_t rows, int64_t cols, i
     return cudaSuccess;
   }
   *out = fresh(dtype, rows, cols, dtype == DType::kF32 ? 3 : 1, arena);
-  if (dtype == DType::kF32) flags.give(*out);
   return arena.measuring ? cudaSuccess : copy_operand(dtype, p, ld, *out, stream);
 }
 
@@ -101,11 +86,8 @@ cudaError_t forward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   if (a.rows == 0 || a.out == 0) return cudaSuccess;
   if (few_rows(a)) return arena.measuring ? cudaSuccess : forward_few_rows(a, stream);
   Product pr;
-  Zeroed flags;
-  if (a.dtype == DType::kF32)
-    LIN_TRY(flags.take(Zeroed::bytes(a.rows, a.in) + Zeroed::bytes(a.out, a.in), arena, stream));
-  LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, flags, &pr.a, stream));
-  LIN_TRY(operand_of(a.dtype, a.w, a.out, a.in, a.w_stride, arena, flags, &pr.b, stream));
+  LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &pr.a, stream));
+  LIN_TRY(operand_of(a.dtype, a.w, a.out, a.in, a.w_stride, arena, &pr.b, stream));
   pr.m = a.rows, pr.n = a.out, pr.k = a.in, pr.dtype = a.dtype;
   pr.epi.mode = Epilogue::kFwd;
   pr.epi.act = a.act;
@@ -123,18 +105,13 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   const bool recompute = a.act != Act::kNone && a.slope == nullptr;
   const bool need_w = a.dx != nullptr || recompute, need_x = a.dw != nullptr || recompute;
   Operand x, w, dz;
-  Zeroed flags;
-  if (f32)
-    LIN_TRY(flags.take((need_w ? Zeroed::bytes(a.out, a.in) : 0) +
-                           (need_x && !a.codes ? Zeroed::bytes(a.rows, a.in) : 0) + Zeroed::bytes(a.rows, a.out),
-                       arena, stream));
-  if (need_w) LIN_TRY(operand_of(a.dtype, a.w, a.out, a.in, a.w_stride, arena, flags, &w, stream));
+  if (need_w) LIN_TRY(operand_of(a.dtype, a.w, a.out, a.in, a.w_stride, arena, &w, stream));
   if (need_x) {
     if (a.codes) {
       x = fresh(a.dtype, a.rows, a.in, 1, arena);  // 7 bits and a power of two: one plane holds a code exactly
       if (!arena.measuring) LIN_TRY(unpack_operand(a.codes, a.exps, x, stream));
     } else {
-      LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, flags, &x, stream));
+      LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &x, stream));
     }
   }
   // db: the columns' sums come from whatever makes dz, over ranges of rows
@@ -144,11 +121,10 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   float* parts = nullptr;
   if (need_b) parts = static_cast<float*>(arena.take(static_cast<size_t>(parts_count) * a.out * sizeof(float)));
   if (as_it_is) {
-    LIN_TRY(operand_of(a.dtype, a.g, a.rows, a.out, a.g_stride, arena, flags, &dz, stream));
+    LIN_TRY(operand_of(a.dtype, a.g, a.rows, a.out, a.g_stride, arena, &dz, stream));
     if (need_b && !arena.measuring) LIN_TRY(column_sums(dz, parts, stream));
   } else {
     dz = fresh(a.dtype, a.rows, a.out, f32 ? 3 : 1, arena);
-    if (f32) flags.give(dz);
     if (recompute) {
       Product pr;
       pr.a = x, pr.b = w;
@@ -161,7 +137,6 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
       pr.epi.out = const_cast<__nv_bfloat16*>(dz.p);
       pr.epi.out_ld = dz.ld;
       pr.epi.out_plane = f32 ? dz.plane : 0;
-      pr.epi.out_flags = dz.flags;
       pr.epi.sums = parts;
       if (a.rows && a.out) LIN_TRY(run_product(pr, arena, stream));
     } else if (!arena.measuring) {

@@ -58,17 +58,6 @@ struct Operand {
   const __nv_bfloat16* p = nullptr;
   int64_t rows = 0, cols = 0, ld = 0, plane = 0;  // ld, plane: elements
   int planes = 1;
-  // float32 only, may be null: what is not finite in it
-  struct Flags* flags = nullptr;
-};
-
-// Bit 0: an infinity, bit 1: a NaN; of the whole matrix, then (behind this
-// header) of its rows and its columns.
-struct Flags {
-  uint32_t any, unused[3];
-  __host__ __device__ uint32_t* rows() { return reinterpret_cast<uint32_t*>(this + 1); }
-  __host__ __device__ uint32_t* cols(int64_t rows_count) { return rows() + rows_count; }
-  static size_t bytes(int64_t rows, int64_t cols) { return sizeof(Flags) + static_cast<size_t>(rows + cols) * 4; }
 };
 
 // What happens to the product's elements on their way out.
@@ -86,9 +75,7 @@ struct Epilogue {
   void* out = nullptr;
   int64_t out_ld = 0;
   void* slope = nullptr;  // kFwd, [m, n] contiguous
-  // kDz, float32: out is three bfloat16 planes, out_plane elements apart, with flags
-  int64_t out_plane = 0;
-  Flags* out_flags = nullptr;
+  int64_t out_plane = 0;  // kDz, float32: out is three bfloat16 planes, out_plane elements apart
   float* sums = nullptr;  // kDz, may be null: [ceil(m / 32), n], the columns' sums over 32 rows
 };
 

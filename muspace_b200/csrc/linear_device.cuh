@@ -199,12 +199,6 @@ __device__ __forceinline__ void split_pairs(const float* v, uint32_t top, uint32
   }
 }
 
-// 1: an infinity, 2: a NaN, 0: finite
-__device__ __forceinline__ uint32_t flag_of(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? 0u : (b == 0x7f800000u ? 1u : 2u);
-}
-
 // ---- eight neighbouring values ----------------------------------------------------------
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -306,23 +300,6 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, 
   }
 }
 
-// Marks what is not finite among `count` <= 8 values at (r, c).
-__device__ __forceinline__ void mark_flags(const float v[8], int count, Flags* flags, int64_t rows, int64_t r,
-                                           int64_t c) {
-  if (top_bits<8>(v) < 0x7f800000u) return;
-  uint32_t any = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t f = j < count ? flag_of(v[j]) : 0u;
-    if (f) atomicOr(flags->cols(rows) + c + j, f);
-    any |= f;
-  }
-  if (any) {
-    atomicOr(flags->rows() + r, any);
-    atomicOr(&flags->any, any);
-  }
-}
-
 // ---- the epilogue -----------------------------------------------------------------------
 
 template <typename T>
@@ -337,7 +314,7 @@ struct SlopeOf<float> {
 // Eight neighbouring outputs of row m, of sums that were finished apart.
 template <typename T>
 __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], const float x[8], const float b[8], int64_t m,
-                                        int64_t n, int64_t rows, int64_t cols, int count, bool vec) {
+                                        int64_t n, int64_t cols, int count, bool vec) {
   if (e.mode != Epilogue::kStore) {
     float s[8];
 #pragma unroll
@@ -354,7 +331,6 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], const flo
       for (int j = 0; j < 8; ++j) v[j] = x[j] * s[j];
       if (sizeof(T) == 4) {
         store_planes(static_cast<bf16*>(e.out) + m * e.out_ld + n, e.out_plane, count, vec, v);
-        mark_flags(v, count, e.out_flags, rows, m, n);
         return;
       }
     }
@@ -365,12 +341,12 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], const flo
 // The same where vectors do not fit, out of the way.
 template <typename T>
 __device__ __noinline__ void finish_some(const Epilogue& e, const float4 lo, const float4 hi, int64_t m, int64_t n,
-                                         int64_t rows, int64_t cols) {
+                                         int64_t cols) {
   const int count = static_cast<int>(cols - n < 8 ? cols - n : 8);
   float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, x[8] = {}, b[8] = {};
   if (e.extra) load_some(static_cast<const T*>(e.extra) + m * e.extra_ld + n, count, false, x);
   if (e.bias) load_some(static_cast<const T*>(e.bias) + n, count, false, b);
-  finish8<T>(e, v, x, b, m, n, rows, cols, count, false);
+  finish8<T>(e, v, x, b, m, n, cols, count, false);
 }
 
 }  // namespace lin

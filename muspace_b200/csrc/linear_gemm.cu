@@ -302,46 +302,6 @@ __device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
   return t;
 }
 
-// ---- float32: what planes cannot hold -----------------------------------------------
-
-__device__ __forceinline__ float whole(const Operand& o, bool across, int64_t i, int64_t k) {
-  const int64_t at = across ? k * o.ld + i : i * o.ld + k;
-  float v = 0.f;
-  for (int q = o.planes - 1; q >= 0; --q) v += __bfloat162float(o.p[q * o.plane + at]);
-  return v;
-}
-
-// An infinity is all in the first plane, and its product with the other
-// operand's small planes is an infinity of any sign, or a NaN. So outputs
-// whose row or column holds one are summed again, element by element; a NaN
-// there makes them NaN.
-__device__ __noinline__ float repaired(const Product& pr, uint32_t flags, int64_t m, int64_t n) {
-  if (flags & 2u) return __uint_as_float(0x7fc00000u);
-  float s = 0.f;
-  for (int64_t k = 0; k < pr.k; ++k) s = fmaf(whole(pr.a, pr.a_mn, m, k), whole(pr.b, pr.b_mn, n, k), s);
-  return s;
-}
-
-// Flags of output rows / columns: of A's rows or columns, of B's; null where none can be set.
-__device__ __forceinline__ const uint32_t* flags_of(const Operand& o, bool across) {
-  return o.flags == nullptr ? nullptr : across ? o.flags->cols(o.rows) : o.flags->rows();
-}
-__device__ __forceinline__ bool some_flag(const Product& pr) {
-  return (pr.a.flags && pr.a.flags->any) || (pr.b.flags && pr.b.flags->any);
-}
-
-// Outputs [n, n + N) of row m.
-template <int N>
-__device__ __noinline__ void repair(const Product& pr, float* v, int64_t m, int64_t n) {
-  const uint32_t *fa = flags_of(pr.a, pr.a_mn), *fb = flags_of(pr.b, pr.b_mn);
-  if (m >= pr.m) return;
-  const uint32_t row = fa ? fa[m] : 0u;
-  for (int j = 0; j < N && n + j < pr.n; ++j) {
-    const uint32_t f = row | (fb ? fb[n + j] : 0u);
-    if (f) v[j] = repaired(pr, f, m, n + j);
-  }
-}
-
 // ---- the epilogue ------------------------------------------------------------------------
 
 // A warp's box in shared memory: 32 rows of 128 or 64 bytes, whose 16-byte units
@@ -474,20 +434,6 @@ struct Bias16 {
   }
 };
 
-// Marks what is not finite among 16 outputs of row m.
-__device__ __noinline__ void mark16(Flags* flags, int64_t rows, int64_t cols, const float* v, int64_t m, int64_t n) {
-  uint32_t any = 0;
-  for (int j = 0; j < 16 && m < rows && n + j < cols; ++j) {
-    const uint32_t f = flag_of(v[j]);
-    if (f) atomicOr(flags->cols(rows) + n + j, f);
-    any |= f;
-  }
-  if (any) {
-    atomicOr(flags->rows() + m, any);
-    atomicOr(&flags->any, any);
-  }
-}
-
 __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(map), "r"(x),
                "r"(y), "r"(z), "r"(src)
@@ -505,6 +451,13 @@ __device__ __forceinline__ void stores_read() {
 // ---- the kernel ------------------------------------------------------------------------
 
 constexpr int kFwdSlope = 3;  // beside Epilogue::Mode: kFwd that also writes the slope
+
+// float32: what is not finite. An infinity or a NaN is all in an operand's first
+// plane, so the product of first planes answers as float32 would (a factor below
+// 2^-134 counts as 0 there), and so it does where finite products overflow. The
+// small products then are infinities of any sign, or NaNs: a sum of them that is
+// not finite is left out.
+__device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) <= 3.402823466e38f ? v : 0.f; }
 
 struct Maps {
   CUtensorMap a, b, out, extra, slope;
@@ -551,7 +504,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
   const bool extra = kSlope ? e.extra != nullptr : kExtra;
   const bool with_bias = kMode != Epilogue::kStore && e.bias != nullptr;
   const bool bias_vec = reinterpret_cast<uintptr_t>(e.bias) % 16 == 0;
-  const bool repairs = kF32 && !job.apart && some_flag(job.pr);
   const auto row_of = [&](const Item& t) { return t.m + static_cast<int>(rank) * kTileM + quad * 32; };
   const auto col_of = [&](const Item& t) { return t.n + group * S::kCols; };
   // a box on its way out; the next may be written when `read`
@@ -611,7 +563,7 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
             tmem_load16(acc_at + q * 16, r);
             tmem_wait(r);
 #pragma unroll
-            for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
+            for (int x = 0; x < 16; ++x) acc[q][x] += finite_or_zero(__uint_as_float(r[x]));
             if (last) tmem_store16(acc_at + q * 16, acc[q]);  // the tile waits there for its epilogue
           }
         }
@@ -652,14 +604,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           Bias16<T> bias;
           if (with_bias) bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
           tmem_take16(at, v);
-          if (kF32 && repairs) {
-            float w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = v[j];
-            repair<16>(job.pr, w, m + lane, n + c);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = w[j];
-          }
           if (with_bias) bias.add(v);
           activate<kFast, true, true, 16>(kAct, v, s);
           put_aside(at, s, typename SlopeOf<T>::type());
@@ -704,14 +648,6 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           bias.load(static_cast<const T*>(e.bias) + n + c, bias_vec, rows_n - n - c);
         if (kExtra) get16<kRowBytes>(box, lane, c, x, T());
         tmem_take16(at, v);
-        if (kF32 && repairs) {
-          float w[16];
-#pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = v[j];
-          repair<16>(job.pr, w, m + lane, n + c);
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] = w[j];
-        }
         if (kMode != Epilogue::kStore && with_bias) bias.add(v);
         if (kMode == Epilogue::kDz) {
           activate<kFast, false, true, 16>(kAct, v, s);
@@ -749,14 +685,7 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
           float v[16];
           uint32_t part[3][8];
           tmem_take16(acc_at + c, v);
-          const uint32_t top = top_bits<16>(v);
-          if (top >= 0x7f800000u) {
-            float w[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) w[j] = v[j];
-            mark16(e.out_flags, job.pr.m, job.pr.n, w, m + lane, n + c);
-          }
-          split_pairs<16>(v, top, part);
+          split_pairs<16>(v, top_bits<16>(v), part);
 #pragma unroll
           for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -1023,12 +952,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Adds up the ranges of k and runs the epilogue: eight columns to kLanes lanes,
 // which take the ranges in turn. The order of the additions is fixed.
-template <typename T, bool kF32, int kLanes>
+template <typename T, int kLanes>
 __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job job) {
   const Product& pr = job.pr;
   const int64_t per_row = (pr.n + 7) / 8, total = pr.m * per_row, ld = partial_ld(pr.n);
   const int sub = threadIdx.x % kLanes;
-  const bool repairs = kF32 && pr.k > 0 && some_flag(pr);
   for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) / kLanes; i - threadIdx.x % 32 / kLanes < total;
        i += gridDim.x * 256ll / kLanes) {
     const bool some = i < total;
@@ -1049,22 +977,13 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], d);
     if (!some || sub != 0) continue;
-    if (repairs) {
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[j];
-      repair<8>(pr, w, m, n);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = w[j];
-    }
     if (job.vec && n + 8 <= pr.n) {
       float x[8] = {}, b[8] = {};
       if (pr.epi.bias) load_some(static_cast<const T*>(pr.epi.bias) + n, 8, false, b);
       if (pr.epi.extra) load8(static_cast<const T*>(pr.epi.extra) + m * pr.epi.extra_ld + n, x);
-      finish8<T>(pr.epi, v, x, b, m, n, pr.m, pr.n, 8, true);
+      finish8<T>(pr.epi, v, x, b, m, n, pr.n, 8, true);
     } else {
-      finish_some<T>(pr.epi, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), m, n, pr.m,
-                     pr.n);
+      finish_some<T>(pr.epi, make_float4(v[0], v[1], v[2], v[3]), make_float4(v[4], v[5], v[6], v[7]), m, n, pr.n);
     }
   }
 }
@@ -1293,9 +1212,9 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
   const bool spread = job.splits >= 8;
   const int blocks = static_cast<int>(std::min<int64_t>((groups * (spread ? 8 : 1) + 255) / 256, 148 * 8));
   if (f32)
-    (spread ? finish_kernel<float, true, 8> : finish_kernel<float, true, 1>)<<<blocks, 256, 0, stream>>>(job);
+    (spread ? finish_kernel<float, 8> : finish_kernel<float, 1>)<<<blocks, 256, 0, stream>>>(job);
   else
-    (spread ? finish_kernel<bf16, false, 8> : finish_kernel<bf16, false, 1>)<<<blocks, 256, 0, stream>>>(job);
+    (spread ? finish_kernel<bf16, 8> : finish_kernel<bf16, 1>)<<<blocks, 256, 0, stream>>>(job);
   if (pr.epi.mode == Epilogue::kDz && pr.epi.sums) {
     const int count = static_cast<int>(std::min<int64_t>(((pr.m + 31) / 32 * pr.n + 255) / 256, 148 * 8));
     (f32 ? sums_kernel<float> : sums_kernel<bf16>)<<<count, 256, 0, stream>>>(job);

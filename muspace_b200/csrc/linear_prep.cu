@@ -20,14 +20,11 @@ inline int blocks_for(int64_t groups) {
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T>
-__device__ __forceinline__ void put(bf16* dst, int64_t plane, int count, bool vec, const float v[8], Flags* flags,
-                                    int64_t rows, int64_t r, int64_t c) {
-  if (sizeof(T) == 4) {
-    store_planes(dst, plane, count, vec, v);
-    mark_flags(v, count, flags, rows, r, c);
-  } else {
-    store_some(dst, count, vec, v);
-  }
+__device__ __forceinline__ void put(bf16* dst, int64_t plane, const float v[8]) {
+  if (sizeof(T) == 4)
+    store_planes(dst, plane, 8, true, v);
+  else
+    store8(dst, v);
 }
 
 // dst = src, or src * slope. A row of dst is padded to a multiple of eight
@@ -36,7 +33,7 @@ template <typename T, bool kScale>
 __global__ void __launch_bounds__(kThreads)
     operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec,
                    const typename SlopeOf<T>::type* __restrict__ slope, bool slope_vec, bf16* __restrict__ dst,
-                   int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, Flags* flags) {
+                   int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols) {
   const int64_t per_row = (cols + 7) / 8, total = rows * per_row;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kThreads) + threadIdx.x; i < total;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -50,7 +47,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] *= s[j];
     }
-    put<T>(dst + r * dst_ld + c, plane, 8, true, v, flags, rows, r, c);
+    put<T>(dst + r * dst_ld + c, plane, v);
   }
 }
 
@@ -63,7 +60,7 @@ cudaError_t launch_operand(const void* src, int64_t src_ld, const void* slope, c
   const bool slope_vec = aligned16(slope) && (dst.cols * sizeof(S)) % 16 == 0;
   operand_kernel<T, kScale><<<blocks_for(groups), kThreads, 0, stream>>>(
       static_cast<const T*>(src), src_ld, src_vec, static_cast<const S*>(slope), slope_vec, const_cast<bf16*>(dst.p),
-      dst.ld, dst.plane, dst.rows, dst.cols, dst.flags);
+      dst.ld, dst.plane, dst.rows, dst.cols);
   return cudaGetLastError();
 }
 
@@ -132,8 +129,8 @@ template <typename T, bool kScale>
 __global__ void __launch_bounds__(32 * kSumWarps, 4)
     operand_sums_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec,
                         const typename SlopeOf<T>::type* __restrict__ slope, bool slope_vec, bf16* __restrict__ dst,
-                        int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, Flags* flags,
-                        int64_t rows_per_part, float* __restrict__ parts) {
+                        int64_t dst_ld, int64_t plane, int64_t rows, int64_t cols, int64_t rows_per_part,
+                        float* __restrict__ parts) {
   __shared__ float buf[kSumWarps][kSumCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
@@ -153,7 +150,7 @@ __global__ void __launch_bounds__(32 * kSumWarps, 4)
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
-      put<T>(dst + r * dst_ld + c, plane, 8, true, v, flags, rows, r, c);
+      put<T>(dst + r * dst_ld + c, plane, v);
     }
   }
   put_sums(buf, s, cols, parts);
@@ -170,7 +167,7 @@ cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slo
   const dim3 grid(static_cast<unsigned>((dst.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
   operand_sums_kernel<T, kScale><<<grid, 32 * kSumWarps, 0, stream>>>(
       static_cast<const T*>(src), src_ld, src_vec, static_cast<const S*>(slope), slope_vec, const_cast<bf16*>(dst.p),
-      dst.ld, dst.plane, dst.rows, dst.cols, dst.flags, (dst.rows + count - 1) / count, parts);
+      dst.ld, dst.plane, dst.rows, dst.cols, (dst.rows + count - 1) / count, parts);
   return cudaGetLastError();
 }
 

@@ -10,8 +10,11 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
+from muspace_b200.ops import linear_act
 from muspace_b200.runtime import native
+from test_layer_ops import F32, SUM, held64, linear_inputs, near, slope64
 
 
 def workspace_of(name: str, **fields) -> int:
@@ -38,3 +41,87 @@ def test_workspace_holds_the_last_vector_of_partial_sums(n, rows):
     needed = workspace_of("msda_linear_act_backward", dtype=1, rows=rows, in_features=n, out_features=256,
                           weight_stride=n, grad_output_stride=256, weight=p, grad_output=p, grad_input=p)
     assert needed >= rows * -(-n // 8) * 8 * 4
+
+
+# ---- what is not finite in float32 (more rows than the kernel for few rows takes) ---------
+
+
+def same_where_not_finite(got, expected):
+    """The same infinities and NaNs; returns the rest of both, zeros elsewhere."""
+    assert torch.equal(got.isnan(), expected.isnan())
+    assert torch.equal(got.isinf(), expected.isinf())
+    inf = expected.isinf()
+    assert torch.equal(got[inf].double(), expected[inf])
+    zero = expected.isfinite()
+    return torch.where(zero, got, 0), torch.where(zero, expected, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(1100, 64, 96), (1100, 640, 40), (1100, 67, 33), (5000, 2100, 256)])
+def test_float32_products_that_overflow_are_infinities(cuda_device, rows, k, n):
+    """One product of some 1e30 * 1e30 to an output: an infinity of its sign, beside finite sums."""
+    gen = torch.Generator().manual_seed(rows + k)
+    x = torch.randn(rows, k, generator=gen, dtype=torch.float64).clamp(-3, 3)
+    w = torch.randn(n, k, generator=gen, dtype=torch.float64).clamp(-3, 3)
+    sizes = lambda count: 1 + torch.rand(count, generator=gen, dtype=torch.float64)  # noqa: E731
+    x[::3, 5] = 1e30 * (sizes(rows) * torch.randn(rows, generator=gen, dtype=torch.float64).sign())[::3]
+    w[::2, 5] = 1e30 * (sizes(n) * torch.randn(n, generator=gen, dtype=torch.float64).sign())[::2]
+    x, w = x.float().to(cuda_device), w.float().to(cuda_device)
+    exact = x.double() @ w.double().T
+    terms = x.double().abs() @ w.double().abs().T
+    exact = torch.where(exact.abs() > 3.5e38, torch.copysign(torch.full_like(exact, float("inf")), exact), exact)
+    got, expected = same_where_not_finite(linear_act(x, w), exact)
+    near(got, expected, torch.where(exact.isfinite(), terms, 0), F32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("rows,k,n", [(1200, 256, 520), (1300, 300, 259)])
+def test_float32_infinities_in_most_rows_and_columns(cuda_device, rows, k, n, checkpoint):
+    x, w, b, r, g = linear_inputs(rows, k, n, F32, cuda_device, seed=k)
+    gen = torch.Generator().manual_seed(1)
+    pick = lambda t, part: (torch.rand(t.shape, generator=gen) < part).to(t.device)  # noqa: E731
+    g = torch.where(pick(g, 0.5 / n), torch.copysign(torch.full_like(g, float("inf")), g), g)
+    g = torch.where(pick(g, 0.05 / n), torch.full_like(g, float("nan")), g)
+    bad_x = torch.where(pick(x, 0.5 / k), torch.copysign(torch.full_like(x, float("inf")), x), x)
+    bad_w = w.clone()
+    bad_w[3, 7], bad_w[11, 2] = -float("inf"), float("nan")
+    exact = bad_x.double() @ bad_w.double().T + b.double() + r.double()
+    size = torch.nan_to_num(bad_x, 0, 0, 0).double().abs() @ torch.nan_to_num(bad_w, 0, 0, 0).double().abs().T
+    got, expected = same_where_not_finite(linear_act(bad_x, bad_w, b, r), exact)
+    near(got, expected, 2 * size + r.double().abs() + 1, F32)
+    # backward: the gradients of finite inputs for a gradient with infinities and NaNs
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(linear_act(*leaves, activation="silu", checkpoint=checkpoint), leaves, g)
+    x6 = held64(x) if checkpoint else x.double()
+    z = x6 @ w.double().T + b.double()
+    slope, clean = slope64("silu", z), torch.nan_to_num(g, 0, 0, 0).double()
+    dz, part = g.double() * slope, (clean * slope).abs()
+    loose = clean.abs() * 2 * SUM * (x6.abs() @ w.double().abs().T + b.double().abs())
+    for value, exact, terms in zip(
+            grads, (dz @ w.double(), dz.T @ x6, dz.sum(0)),
+            (part @ w.double().abs() + loose @ w.double().abs() / SUM, part.T @ x6.abs() + loose.T @ x6.abs() / SUM,
+             part.sum(0) + loose.sum(0) / SUM)):
+        got, expected = same_where_not_finite(value, exact)
+        near(got, expected, terms, F32)
+
+
+@pytest.mark.gpu
+def test_float32_infinities_cost_no_time(cuda_device):
+    """A gradient that overflowed everywhere takes the time of a finite one (within a factor of three)."""
+    x, w, b, _, g = linear_inputs(1200, 256, 256, F32, cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = linear_act(*leaves)
+    took = []
+    for gradient in (g, torch.full_like(g, float("inf"))):
+        times = []
+        for _ in range(9):
+            start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda._sleep(1000000)  # the launches wait here, so that the host's part is not timed
+            start.record()
+            torch.autograd.grad(y, leaves, gradient, retain_graph=True)
+            end.record()
+            end.synchronize()
+            times.append(start.elapsed_time(end))
+        took.append(sorted(times)[4])
+    assert took[1] <= 3 * took[0], took
