@@ -492,9 +492,14 @@ MSDA_API int msda_layer_norm_backward_workspace(const msda_layer_norm_t *args, s
 MSDA_API int msda_layer_norm_backward(const msda_layer_norm_t *args, void *stream);
 
 /* Waits inside the linear and layer-norm kernels that gave up on the current
- * device since the library loaded. 0 is expected; anything else means that
- * results since then may be wrong. Synchronises with the device. */
+ * device since the library loaded. 0 is expected; anything else means that a
+ * call since then has left NaNs in the part of its results that depended on
+ * such a wait. Synchronises with the device. */
 MSDA_API int msda_layer_wait_timeouts(unsigned int *count);
+
+/* Adds one to that count: a kernel that waits `clocks` (at most 2 * 10^9) of
+ * the device's clock for nothing and returns. For tests of a caller's checks. */
+MSDA_API int msda_layer_wait_probe(int64_t clocks, void *stream);
 
 /* Message of the last failed call on this thread ("" after a success). The
  * reference raised it as a TVM-FFI exception (csrc/ffi/tensor_utils.hpp:13-34). */

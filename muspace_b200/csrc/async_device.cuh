@@ -33,16 +33,17 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// Waits have a limit. One that runs out is counted, and from then on the
-// thread polls each barrier once: the kernel ends, with wrong results and a
-// count that msda_layer_wait_timeouts reports.
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& dead) {
+// Waits have a limit. One that runs out is counted (msda_layer_wait_timeouts)
+// and leaves `dead` set: from then on the thread polls each barrier once, and
+// starts no copies and no products. Its block waits once more, with a limit, for
+// what is in flight, and writes NaNs over all of its results.
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& dead, long long limit = kWaitClocks) {
   if (try_wait(bar, parity)) return;
   if (dead) return;
   const long long start = clock64();
   do {
     if (try_wait(bar, parity)) return;
-  } while (clock64() - start < kWaitClocks);
+  } while (clock64() - start < limit);
   dead = true;
   atomicAdd(&g_wait_timeouts, 1u);
 }
@@ -52,6 +53,12 @@ __device__ __forceinline__ void copy_bytes(uint32_t dst, const void* src, uint32
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// The same once more, whatever ran out before: for copies in flight before their memory goes.
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
+  bool late = false;
+  wait(bar, parity, late);
 }
 
 inline cudaError_t read_timeouts(unsigned int* count) {

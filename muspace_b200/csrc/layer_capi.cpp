@@ -206,6 +206,13 @@ int msda_layer_wait_timeouts(unsigned int* count) {
   });
 }
 
+int msda_layer_wait_probe(int64_t clocks, void* stream) {
+  return guarded([&] {
+    require(clocks >= 0 && clocks <= 2000000000, "clocks must be between 0 and 2000000000");
+    check_launch(lnorm::wait_probe(clocks, static_cast<cudaStream_t>(stream)), "msda_layer_wait_probe");
+  });
+}
+
 int msda_layer_norm_forward(const msda_layer_norm_t* args, void* stream) {
   return guarded([&] {
     check_launch(lnorm::forward(norm_args(args, false), static_cast<cudaStream_t>(stream)),

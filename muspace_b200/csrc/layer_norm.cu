@@ -457,7 +457,9 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncthreads();
+  uint32_t fetched = 0;  // by this thread, into the stages in turn
   const auto fetch = [&](int64_t r, int s) {
+    ++fetched;
     const uint32_t bar = bar0 + 8 * s, dst = ring0 + s * stage_bytes;
     async::expect_bytes(bar, stage_bytes);
     async::copy_bytes(dst, kCodes ? static_cast<const void*>(a.codes_in + r * a.cols)
@@ -550,7 +552,7 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
     }
     const Sums s = row_sums<G, true>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
     // every thread is past the row before: its stage takes the row that comes `stages` after it
-    if (lane == 0 && last >= 0) {
+    if (lane == 0 && last >= 0 && !dead) {
       const int64_t ahead = r + (stages - 1) * step;
       if (ahead < a.rows) fetch(ahead, last);
     }
@@ -573,6 +575,23 @@ __global__ void __launch_bounds__(kRingThreads, 1) backward_ring_kernel(const Ar
     }
     last = stage;
     if (++stage == stages) stage = 0, phase ^= 1;
+  }
+  if (__syncthreads_or(dead)) {  // a wait ran out: NaNs, once no copy is in flight
+    if (lane == 0)
+      for (uint32_t i = fetched > stages ? fetched - stages : 0; i < fetched; ++i)
+        async::settle(bar0 + 8 * (i % stages), i / stages & 1);
+    const float nan = __uint_as_float(~0u);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float all[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) all[j] = nan;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dw[i][j] = db[i][j] = both(nan);
+      if (a.dx)
+        for (int64_t r = first; r < a.rows; r += step)
+          store_chunk<G, true>(static_cast<T*>(a.dx) + r * a.cols, cols, lane, i, all);
+    }
   }
   if (!a.dw && !a.db) return;
   // the groups' sums, in order, over the ring
@@ -735,6 +754,15 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
+// A wait that runs out: nothing ever arrives at its barrier.
+__global__ void wait_probe_kernel(long long clocks) {
+  __shared__ __align__(8) uint64_t bar;
+  if (threadIdx.x != 0) return;
+  async::barrier_init(async::smem_addr(&bar), 1);
+  bool dead = false;
+  async::wait(async::smem_addr(&bar), 0, dead, clocks);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T, typename W>
@@ -875,6 +903,11 @@ int backward_parts(int64_t rows, int64_t cols) {
 }
 
 cudaError_t wait_timeouts(unsigned int* count) { return async::read_timeouts(count); }
+
+cudaError_t wait_probe(int64_t clocks, cudaStream_t stream) {
+  wait_probe_kernel<<<1, 32, 0, stream>>>(clocks);
+  return cudaGetLastError();
+}
 
 cudaError_t forward(const Args& a, cudaStream_t stream) {
   return a.rows == 0 || a.cols == 0 ? cudaSuccess : dispatch_types(a, false, stream);

@@ -36,6 +36,8 @@ int backward_parts(int64_t rows, int64_t cols);
 cudaError_t forward(const Args& a, cudaStream_t stream);
 cudaError_t backward(const Args& a, cudaStream_t stream);
 cudaError_t wait_timeouts(unsigned int* count);
+// A kernel with one wait that runs out after `clocks`, and no copies: what wait_timeouts counts, on purpose.
+cudaError_t wait_probe(int64_t clocks, cudaStream_t stream);
 
 }  // namespace lnorm
 

@@ -46,6 +46,7 @@ namespace {
 
 using async::barrier_init;
 using async::expect_bytes;
+using async::settle;
 using async::smem_addr;
 using async::wait;
 
@@ -472,8 +473,9 @@ struct Place {
 // activation and whether there is a residual, as constants: with branches in
 // here, 16 columns took 170 instructions and more where 50 do, and issuing them
 // was the bound of short products; as one function with all kinds it spilled.
+// Returns whether a wait ran out.
 template <int BN, int CG, typename T, bool kF32, int kKind>
-__device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Place place) {
+__device__ __noinline__ bool epilogue(const Maps& maps, const Job& job, const Place place) {
   using S = Shape<BN, CG, kF32>;
   constexpr int kMode = kKind / 8;
   constexpr Act kAct = static_cast<Act>(kKind / 2 % 4);
@@ -522,7 +524,10 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
     if (lane == 0) stores_read<1>();
     __syncwarp();
   };
+  uint32_t loads = 0;
   const auto load_extra = [&](const Item& t) {
+    if (dead) return;
+    ++loads;
     if constexpr (kSlope) {
       expect_bytes(arrived, kHalves * kBoxBytes / 2);
 #pragma unroll
@@ -736,6 +741,43 @@ __device__ __noinline__ void epilogue(const Maps& maps, const Job& job, const Pl
     }
   }
   if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (lane == 0 && dead && loads > 0) settle(arrived, (loads - 1) & 1);
+  return dead;
+}
+
+// NaNs over all that this block's epilogue writes, by the same boxes: a box of ones in every bit.
+template <int BN, int CG, typename T, bool kF32>
+__device__ __noinline__ void spoil(const Maps& maps, const Job& job, const Place place) {
+  using S = Shape<BN, CG, kF32>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Epilogue& e = job.pr.epi;
+  const int mode = job.apart ? Epilogue::kStore : e.mode;
+  const bool slope = mode == Epilogue::kFwd && e.slope, planes = mode == Epilogue::kDz && sizeof(T) == 4;
+  const int wide = 128 / sizeof(T) < S::kCols ? 128 / sizeof(T) : S::kCols;
+  const int cols = slope ? 64 / sizeof(T) : planes ? 32 : wide;
+  const uint32_t box = place.boxes + warp * kBoxBytes;
+  for (int unit = lane; unit < kBoxBytes / 16; unit += 32) put_unit(box + unit * 16, ~0u, ~0u, ~0u, ~0u);
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+  const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
+  for (uint32_t i = blockIdx.x / CG; i < items; i += gridDim.x / CG) {
+    const Item t = item_of<BN, CG>(job, i);
+    const int m = t.m + static_cast<int>(place.rank) * kTileM + (warp & 3) * 32, n0 = t.n + (warp >> 2) * S::kCols;
+    for (int n = n0; n < n0 + S::kCols; n += cols) {
+      if (m >= job.pr.m || n >= job.pr.n) continue;
+      if (lane == 0) {
+        for (int z = 0; z < (planes ? 3 : 1); ++z) store_box(&maps.out, n, m, job.apart ? t.split : z, box);
+        if (slope) store_box(&maps.slope, n, m, 0, box);
+      }
+      if (mode == Epilogue::kDz && e.sums)
+        for (int c = lane; c < cols && n + c < job.pr.n; c += 32)
+          e.sums[static_cast<int64_t>(m / 32) * job.pr.n + n + c] = __uint_as_float(~0u);
+    }
+  }
+  if (lane == 0) {
+    stores_commit();
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
 }
 
 template <int BN, int CG, typename T, bool kF32>
@@ -745,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ uint8_t raw[];
   const uint32_t ring = (smem_addr(raw) + 1023) & ~1023u;
   const uint32_t bars = ring + S::kStages * S::kStage + kEpiWarps * kBoxBytes;
-  const uint32_t tmem_slot = bars + S::kBarriers * 8;
+  const uint32_t tmem_slot = bars + S::kBarriers * 8, spoilt = tmem_slot + 4;
   const auto full = [&](int s) { return bars + 8 * s; };
   const auto empty = [&](int s) { return bars + 8 * (S::kStages + s); };
   const auto acc_full = [&](int b) { return bars + 8 * (2 * S::kStages + b); };
@@ -767,6 +809,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (kF32) barrier_init(small_empty(b), S::kWarps * CG);
     }
     for (int x = 0; x < kEpiWarps; ++x) barrier_init(bars + 8 * (2 * S::kStages + 4 + x), 1);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(spoilt), "r"(0) : "memory");
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == kIssuer) tmem_alloc<CG>(tmem_slot, S::kColumns);
@@ -786,7 +829,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
     const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
     const uint32_t full0 = CG == 2 ? in_block(full(0), 0) : full(0);  // the pair's copies count in its first block
-    for (uint32_t i = first; i < items; i += step) {
+    for (uint32_t i = first; i < items && !dead; i += step) {
       const Item t = item_of<BN, CG>(job, i);
       // boxes that hold rows of the tile; what a skipped box leaves in its place reaches no row or column that is kept
       const auto boxes = [](int have, int most) { return have <= 0 ? 0 : min(most, (have - 1) / 64 + 1); };
@@ -811,6 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool has_a = !kF32 || p < job.pr.a.planes, has_b = !kF32 || p < job.pr.b.planes;
             const uint32_t bar = full0 + 8 * s, a = ring + s * S::kStage, b = a + kStageA;
             wait(empty(s), phase ^ 1, dead);
+            if (dead) return;
             if (rank == 0) expect_bytes(full(s), (has_a ? from_a : 0) + (has_b ? from_b : 0));
             if (kA) {
 #pragma unroll
@@ -837,14 +881,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       else
         stages(std::false_type(), std::false_type());
     }
-    // the copies that are still in flight land before the block's memory goes
-    dead = false;
+    // the copies have landed, and their products are done, before the block's memory goes
     for (int x = 0; x < S::kStages; ++x) {
-      wait(empty(s), phase ^ 1, dead);
+      if (rank == 0) settle(full(s), phase ^ 1);
+      settle(empty(s), phase ^ 1);
       if (++s == S::kStages) s = 0, phase ^= 1;
     }
   } else if (warp == kIssuer && rank == 0) {
-    // the whole warp walks the loop, one lane issues: the warp stays together for the barriers below
+    // the whole warp walks the loop, one lane issues (nothing more once a wait of its own ran out): the warp
+    // stays together for the barriers below
     const uint32_t idesc = instruction(kTileM * CG, BN, job.pr.a_mn, job.pr.b_mn);
     const uint32_t step_a = k_step(job.pr.a_mn) >> 4, step_b = k_step(job.pr.b_mn) >> 4;
     const uint64_t first_a = tile_descriptor(ring, job.pr.a_mn);
@@ -879,16 +924,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kF32) {
             bool add = x > 0 || !fresh;  // in the small products' accumulator
             const int mid = arrived();
-            if (lane == 0 && more_a && more_b) product(small, mid, mid, add), add = true;
+            if (lane == 0 && !dead && more_a && more_b) product(small, mid, mid, add), add = true;
             const int hi = arrived();
-            if (lane == 0) {
+            if (lane == 0 && !dead) {
               if (more_a) product(small, mid, hi, add), add = true;
               if (more_b) product(small, hi, mid, add);
               commit<CG>(empty(mid));
               product(acc, hi, hi, x > 0);
             }
             const int lo = arrived();
-            if (lane == 0) {
+            if (lane == 0 && !dead) {
               if (more_a) product(small, lo, hi, true);
               if (more_b) product(small, hi, lo, true);
               commit<CG>(empty(hi));
@@ -896,20 +941,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           } else {
             const int at = arrived();
-            if (lane == 0) {
+            if (lane == 0 && !dead) {
               product(acc, at, at, x > 0);
               commit<CG>(empty(at));
             }
           }
           __syncwarp();
         }
-        if (lane == 0) commit<CG>(acc_full(buf));
+        if (lane == 0 && !dead) commit<CG>(acc_full(buf));
         __syncwarp();
         if (kF32 && (c + chunk >= t.kb1 || n % kFold == 0) && (small_buf ^= 1) == 0) small_phase ^= 1;
         buf ^= 1;
         if (buf == 0) acc_phase ^= 1;
       }
     }
+    // the last products are done before their tensor memory goes, also where the epilogue gave up on them
+    wait(acc_full(buf ^ 1), buf == 0 ? acc_phase ^ 1 : acc_phase, dead);
   } else if (warp < S::kWarps) {
     const Epilogue& e = job.pr.epi;
     const int mode = job.apart ? Epilogue::kStore : e.mode;
@@ -919,31 +966,39 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                        : mode * 8 + static_cast<int>(e.act) * 2 + (extra ? 1 : 0);
     const Place at{tmem, ring + S::kStages * S::kStage, bars, rank};
     if constexpr (sizeof(T) == 4 && !kF32) {  // partial sums
-      epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at);
+      dead = epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at);
     } else {
       switch (kind) {
-        case Epilogue::kStore * 8: epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at); break;
-        case Epilogue::kFwd * 8: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 1: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 1>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 2: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 2>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 3: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 3>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 4: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 4>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 5: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 5>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 6: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 6>(maps, job, at); break;
-        case Epilogue::kFwd * 8 + 7: epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 7>(maps, job, at); break;
-        case Epilogue::kDz * 8 + 3: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 3>(maps, job, at); break;
-        case Epilogue::kDz * 8 + 5: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 5>(maps, job, at); break;
-        case Epilogue::kDz * 8 + 7: epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 7>(maps, job, at); break;
-        case kFwdSlope * 8 + 2: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 2>(maps, job, at); break;
-        case kFwdSlope * 8 + 4: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 4>(maps, job, at); break;
-        case kFwdSlope * 8 + 6: epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 6>(maps, job, at); break;
-        default: epilogue<BN, CG, T, kF32, kFwdSlope * 8>(maps, job, at);
+        case Epilogue::kStore * 8: dead = epilogue<BN, CG, T, kF32, Epilogue::kStore * 8>(maps, job, at); break;
+        case Epilogue::kFwd * 8: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 1: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 1>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 2: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 2>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 3: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 3>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 4: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 4>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 5: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 5>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 6: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 6>(maps, job, at); break;
+        case Epilogue::kFwd * 8 + 7: dead = epilogue<BN, CG, T, kF32, Epilogue::kFwd * 8 + 7>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 3: dead = epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 3>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 5: dead = epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 5>(maps, job, at); break;
+        case Epilogue::kDz * 8 + 7: dead = epilogue<BN, CG, T, kF32, Epilogue::kDz * 8 + 7>(maps, job, at); break;
+        case kFwdSlope * 8 + 2: dead = epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 2>(maps, job, at); break;
+        case kFwdSlope * 8 + 4: dead = epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 4>(maps, job, at); break;
+        case kFwdSlope * 8 + 6: dead = epilogue<BN, CG, T, kF32, kFwdSlope * 8 + 6>(maps, job, at); break;
+        default: dead = epilogue<BN, CG, T, kF32, kFwdSlope * 8>(maps, job, at);
       }
     }
+  }
+  if (dead) {
+    for (uint32_t r = 0; r < CG; ++r)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_block(spoilt, r)), "r"(1) : "memory");
   }
   __syncwarp();
   fence_before();
   block_or_pair_sync<CG>();
+  uint32_t bad;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(bad) : "r"(spoilt) : "memory");
+  if (bad && warp < S::kWarps)
+    spoil<BN, CG, T, kF32>(maps, job, Place{tmem, ring + S::kStages * S::kStage, bars, rank});
   if (warp == kIssuer) {
     fence_after();
     tmem_free<CG>(tmem, S::kColumns);

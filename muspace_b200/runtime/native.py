@@ -182,6 +182,18 @@ _PLAIN_SIGNATURES: dict[str, tuple] = {
 }
 
 
+def layer_wait_timeouts(device: torch.device | int | None = None) -> int:
+    """Waits inside the linear and layer-norm kernels that gave up on a CUDA device
+    (the current one by default) since the library loaded. 0 is expected; a call
+    with such a wait leaves NaNs. Synchronises with the device."""
+    module = load_native_module()
+    count = ctypes.c_uint()
+    with torch.cuda.device(device):
+        if module.lib.msda_layer_wait_timeouts(ctypes.byref(count)) != 0:
+            raise RuntimeError(f"msda_layer_wait_timeouts: {module.last_error()}")
+    return count.value
+
+
 _WORKSPACE_CALLS = {"msda_linear_act_forward_workspace", "msda_linear_act_backward_workspace",
                     "msda_layer_norm_backward_workspace"}
 
