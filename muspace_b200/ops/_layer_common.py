@@ -6,6 +6,7 @@ from __future__ import annotations
 from dataclasses import replace
 
 import torch
+from torch.autograd import forward_ad
 
 from ..runtime.kernel_dispatch import (
     DispatchDecision,
@@ -78,6 +79,18 @@ def failed(report: DispatchReport, reason: str) -> RuntimeError:
     """The error of a call that would have been reported as ``report``, after reporting it."""
     record_dispatch_report(replace(report, selected_backend="error", reason=reason))
     return RuntimeError(reason)
+
+
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)  # without the Python around it
+
+
+def autograd_sees(*tensors: torch.Tensor | None) -> bool:
+    """Whether a call on these tensors has to go through its autograd function: for
+    gradients, within forward mode (where the function refuses a tangent, which the
+    kernels would drop), and while tracing (where it is what the trace records).
+    Elsewhere a call spares itself the function's 10 us."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0 or _is_tracing())
 
 
 def rows_of(tensor: torch.Tensor) -> tuple[torch.Tensor, int]:

@@ -21,7 +21,7 @@ import torch
 
 from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import NativeModule
-from ._layer_common import DTYPE_CODES, STORAGE, check_tensor, decide, rows_of
+from ._layer_common import DTYPE_CODES, STORAGE, check_tensor, decide, native_module, rows_of
 
 BLOCK = 32
 
@@ -45,6 +45,43 @@ def pack_rows(module: NativeModule, rows: torch.Tensor, stride: int) -> tuple[to
     return codes, exponents
 
 
+def _unpack(module: NativeModule, codes: torch.Tensor, exponents: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """What contiguous codes and exponents hold, in float32 or bfloat16."""
+    out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
+    width = codes.size(-1)
+    module.plain_call("msda_checkpoint_unpack")(codes.device, DTYPE_CODES[dtype], codes.data_ptr(),
+                                                exponents.data_ptr(), codes.numel() // max(width, 1), width,
+                                                out.data_ptr())
+    return out
+
+
+# Only for tracing, which records a function's call and nothing of what a kernel does.
+
+
+class _PackFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows):
+        outputs = pack_rows(native_module(), *rows_of(rows))
+        ctx.mark_non_differentiable(*outputs)
+        return outputs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return None
+
+
+class _UnpackFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, codes, exponents, dtype):
+        output = _unpack(native_module(), codes, exponents, dtype)
+        ctx.mark_non_differentiable(output)
+        return output
+
+    @staticmethod
+    def backward(ctx, grad):
+        return None, None, None
+
+
 def checkpoint_pack(input: torch.Tensor, *, backend: str = "auto") -> Checkpoint8:
     """The 8-bit checkpoint of a float16, bfloat16 or float32 CUDA tensor."""
     check_tensor(input, "input")
@@ -53,7 +90,10 @@ def checkpoint_pack(input: torch.Tensor, *, backend: str = "auto") -> Checkpoint
     module, report = decide("checkpoint_pack", backend, input)
     source = input.detach()
     rows, stride = rows_of(source.float() if source.dtype == torch.float16 else source)
-    codes, exponents = pack_rows(module, rows, stride)
+    if torch.jit.is_tracing():
+        codes, exponents = _PackFunction.apply(rows)
+    else:
+        codes, exponents = pack_rows(module, rows, stride)
     record_dispatch_report(report)
     return Checkpoint8(codes.view(input.shape), exponents.view(*input.shape[:-1], exponents.size(1)), input.dtype)
 
@@ -73,11 +113,11 @@ def checkpoint_unpack(checkpoint: Checkpoint8, dtype: torch.dtype | None = None,
         raise ValueError("exponents must have the leading shape of codes and one byte for each block of 32")
     module, report = decide("checkpoint_unpack", backend, codes, exponents)
     codes, exponents = codes.contiguous(), exponents.contiguous()
-    out = torch.empty(codes.shape, dtype=torch.float32 if dtype == torch.float16 else dtype, device=codes.device)
-    width = codes.size(-1)
-    module.plain_call("msda_checkpoint_unpack")(codes.device, DTYPE_CODES[out.dtype], codes.data_ptr(),
-                                                exponents.data_ptr(), codes.numel() // max(width, 1), width,
-                                                out.data_ptr())
+    stored = torch.float32 if dtype == torch.float16 else dtype
+    if torch.jit.is_tracing():
+        out = _UnpackFunction.apply(codes, exponents, stored)
+    else:
+        out = _unpack(module, codes, exponents, stored)
     record_dispatch_report(report)
     return out.to(dtype)
 

@@ -12,7 +12,8 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import LayerNormArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of
+from ._layer_common import (
+    DTYPE_CODES, autograd_sees, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of)
 from .checkpoint8 import BLOCK
 
 OPERATOR_NAME = "layer_norm"
@@ -21,7 +22,7 @@ OPERATOR_NAME = "layer_norm"
 def _forward(module: NativeModule, x, weight, bias, eps: float, keep: str | None):
     """``(output, statistics, codes, exponents)``; ``keep``: "statistics", "int8" or None."""
     rows, stride = rows_of(x)
-    count, width = rows.shape
+    count, width = map(int, rows.shape)  # tensors while tracing
     out = x.new_empty(x.shape)
     statistics = codes = exponents = None
     mean = rstd = None
@@ -110,7 +111,7 @@ def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: to
     weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
     tensors = (input, weight, bias)
     try:
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        if autograd_sees(*tensors):
             output = _LayerNormFunction.apply(*tensors, float(eps), checkpoint)
         else:
             output = _forward(module, *tensors, float(eps), None)[0]

@@ -21,7 +21,8 @@ from torch.autograd.function import once_differentiable
 
 from ..runtime.kernel_dispatch import record_dispatch_report
 from ..runtime.native import LinearArgs, NativeModule
-from ._layer_common import DTYPE_CODES, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of
+from ._layer_common import (
+    DTYPE_CODES, autograd_sees, check_checkpoint, check_tensor, decide, failed, native_module, pointer, rows_of)
 from .checkpoint8 import pack_rows
 
 OPERATOR_NAME = "linear_act"
@@ -149,7 +150,7 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         input, weight, bias, residual = (t if t is None else t.float() for t in (input, weight, bias, residual))
     tensors = (input, weight, bias, residual)
     try:
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        if autograd_sees(*tensors):
             output = _LinearActFunction.apply(*tensors, activation, checkpoint)
         else:
             output, _ = _forward(module, *tensors, activation, False)

@@ -8,11 +8,14 @@ says otherwise.
 from __future__ import annotations
 
 import ctypes
+import importlib
+import warnings
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from muspace_b200.ops import linear_act
+from muspace_b200.ops import checkpoint_pack, checkpoint_unpack, layer_norm, linear_act
 from muspace_b200.runtime import native
 from test_layer_ops import F32, SUM, held64, linear_inputs, near, slope64
 
@@ -125,3 +128,82 @@ def test_float32_infinities_cost_no_time(cuda_device):
             times.append(start.elapsed_time(end))
         took.append(sorted(times)[4])
     assert took[1] <= 3 * took[0], took
+
+
+# ---- calls that autograd or a tracer has to see ---------------------------------------------
+
+
+class FakeModule:
+    """A library whose calls write 1 into the outputs' memory, unseen by torch, as kernels do."""
+
+    def plain_call(self, name):
+        def call(device, *args):
+            if name.startswith("msda_checkpoint"):
+                out, count = (args[5], args[2] * args[3]) if name.endswith("_pack") else (args[5], 4 * args[3] * args[4])
+            else:
+                a = args[0]
+                out, count = a.output, 4 * a.rows * (a.out_features if "linear" in name else a.cols)
+            ctypes.memset(out, 1, count)
+        return call
+
+
+OPERATORS = {
+    "linear_act": lambda x: linear_act(x, torch.ones(8, 8, device=x.device), activation="gelu"),
+    "layer_norm": lambda x: layer_norm(x, torch.ones(8, device=x.device)),
+    "checkpoint_pack": lambda x: checkpoint_pack(x).codes,
+    "checkpoint_unpack": lambda x: checkpoint_unpack(checkpoint_pack(x)),
+}
+
+
+@pytest.fixture
+def fake_library(monkeypatch):
+    """The operators on CPU tensors, with their kernels replaced."""
+    for name in ("linear_act", "layer_norm", "checkpoint8"):
+        module = importlib.import_module("muspace_b200.ops." + name)
+        monkeypatch.setattr(module, "decide", lambda *args: (FakeModule(), None))
+        monkeypatch.setattr(module, "record_dispatch_report", lambda report: report)
+        if hasattr(module, "failed"):
+            monkeypatch.setattr(module, "failed", lambda report, reason: RuntimeError(reason))
+        if hasattr(module, "native_module"):
+            monkeypatch.setattr(module, "native_module", lambda: FakeModule())
+
+
+@pytest.mark.parametrize("name", ["linear_act", "layer_norm"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(fake_library, name, grad):
+    """A tangent that the kernels would drop: an error, as from any operator without a forward-mode formula."""
+    x = torch.ones(3, 8)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward AD|jvp"):
+            OPERATORS[name](forward_ad.make_dual(x, torch.ones(3, 8)))
+        assert OPERATORS[name](x).shape == (3, 8)  # no tangent: as outside
+
+
+def traced(name, x):
+    with warnings.catch_warnings(), torch.no_grad():
+        warnings.simplefilter("ignore")  # sizes become constants
+        return torch.jit.trace(OPERATORS[name], (x,), check_trace=False)
+
+
+@pytest.mark.parametrize("name", sorted(OPERATORS))
+def test_a_trace_has_the_call(fake_library, name):
+    kinds = [node.kind() for node in traced(name, torch.ones(3, 8)).graph.nodes()]
+    assert "prim::PythonOp" in kinds and not any("empty" in kind for kind in kinds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", sorted(OPERATORS))
+def test_a_trace_computes_again(cuda_device, name):
+    x, y = torch.randn(3, 8, device=cuda_device), torch.randn(3, 8, device=cuda_device)
+    call = traced(name, x)
+    for t in (x, y):
+        assert torch.equal(call(t), OPERATORS[name](t))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["linear_act", "layer_norm"])
+def test_forward_mode_is_refused_on_the_gpu(cuda_device, name):
+    x = torch.randn(3, 8, device=cuda_device)
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward AD|jvp"):
+            OPERATORS[name](forward_ad.make_dual(x, torch.ones_like(x)))
