@@ -77,6 +77,7 @@ struct Epilogue {
   void* slope = nullptr;  // kFwd, [m, n] contiguous
   int64_t out_plane = 0;  // kDz, float32: out is three bfloat16 planes, out_plane elements apart
   float* sums = nullptr;  // kDz, may be null: [ceil(m / 32), n], the columns' sums over 32 rows
+  float* unrounded = nullptr;  // finished apart with sums: where out is left in float32 for them, rows of partial_ld(n)
 };
 
 // ---- the product (linear_gemm.cu) --------------------------------------------------
@@ -101,8 +102,8 @@ struct Plan {
 
 Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs_of_planes, int sms);
 // Whether the product leaves float32 sums that a second kernel adds up and
-// finishes: ranges of k, and outputs that TMA cannot address (rows off 16-byte
-// boundaries).
+// finishes: ranges of k, outputs that TMA cannot address (rows off 16-byte
+// boundaries), and empty sums.
 bool finished_apart(const Product& pr, const Plan& p);
 // Floats from one row of the sums to the next: they are read in whole eights, the last of a row too.
 __host__ __device__ inline int64_t partial_ld(int64_t n) { return (n + 7) / 8 * 8; }

@@ -329,6 +329,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, float v[8], const flo
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = x[j] * s[j];
+      if (e.unrounded) store8(e.unrounded + m * partial_ld(cols) + n, v);
       if (sizeof(T) == 4) {
         store_planes(static_cast<bf16*>(e.out) + m * e.out_ld + n, e.out_plane, count, vec, v);
         return;

@@ -1043,18 +1043,14 @@ __global__ void __launch_bounds__(256) finish_kernel(const __grid_constant__ Job
   }
 }
 
-// The columns' sums over 32 rows of what a finished epilogue left in `out`.
-template <typename T>
+// The columns' sums over 32 rows of what a finished epilogue left before its rounding.
 __global__ void __launch_bounds__(256) sums_kernel(const __grid_constant__ Job job) {
   const Product& pr = job.pr;
-  const int64_t total = (pr.m + 31) / 32 * pr.n;
+  const int64_t total = (pr.m + 31) / 32 * pr.n, ld = partial_ld(pr.n);
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
     const int64_t part = i / pr.n, n = i - part * pr.n;
     float s = 0.f;
-    for (int64_t m = part * 32; m < min(pr.m, part * 32 + 32); ++m) {
-      const bf16* p = static_cast<const bf16*>(pr.epi.out) + m * pr.epi.out_ld + n;
-      for (int q = sizeof(T) == 4 ? 2 : 0; q >= 0; --q) s += __bfloat162float(p[q * pr.epi.out_plane]);
-    }
+    for (int64_t m = part * 32; m < min(pr.m, part * 32 + 32); ++m) s += pr.epi.unrounded[m * ld + n];
     pr.epi.sums[i] = s;
   }
 }
@@ -1219,7 +1215,7 @@ Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs, int s
   return best;
 }
 
-bool finished_apart(const Product& pr, const Plan& plan) { return plan.splits > 1 || !vectors_fit(pr); }
+bool finished_apart(const Product& pr, const Plan& plan) { return plan.splits > 1 || pr.k == 0 || !vectors_fit(pr); }
 
 cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t stream) {
   if (pr.m == 0 || pr.n == 0) return cudaSuccess;
@@ -1263,6 +1259,9 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
   } else {
     job.splits = 0;  // an empty sum
   }
+  // in the place of the first range's sums, which a thread has read before it writes there
+  const bool sums = pr.epi.mode == Epilogue::kDz && pr.epi.sums;
+  if (sums) job.pr.epi.unrounded = pr.partial;
   const int64_t groups = pr.m * ((pr.n + 7) / 8);
   const bool spread = job.splits >= 8;
   const int blocks = static_cast<int>(std::min<int64_t>((groups * (spread ? 8 : 1) + 255) / 256, 148 * 8));
@@ -1270,9 +1269,9 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
     (spread ? finish_kernel<float, 8> : finish_kernel<float, 1>)<<<blocks, 256, 0, stream>>>(job);
   else
     (spread ? finish_kernel<bf16, 8> : finish_kernel<bf16, 1>)<<<blocks, 256, 0, stream>>>(job);
-  if (pr.epi.mode == Epilogue::kDz && pr.epi.sums) {
+  if (sums) {
     const int count = static_cast<int>(std::min<int64_t>(((pr.m + 31) / 32 * pr.n + 255) / 256, 148 * 8));
-    (f32 ? sums_kernel<float> : sums_kernel<bf16>)<<<count, 256, 0, stream>>>(job);
+    sums_kernel<<<count, 256, 0, stream>>>(job);
   }
   return cudaGetLastError();
 }

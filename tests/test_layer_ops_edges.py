@@ -17,7 +17,7 @@ from torch.autograd import forward_ad
 
 from muspace_b200.ops import checkpoint_pack, checkpoint_unpack, layer_norm, linear_act
 from muspace_b200.runtime import native
-from test_layer_ops import F32, SUM, held64, linear_inputs, near, slope64
+from test_layer_ops import BF16, F32, SUM, held64, linear_inputs, near, slope64
 
 
 def workspace_of(name: str, **fields) -> int:
@@ -128,6 +128,31 @@ def test_float32_infinities_cost_no_time(cuda_device):
             times.append(start.elapsed_time(end))
         took.append(sorted(times)[4])
     assert took[1] <= 3 * took[0], took
+
+
+# ---- sums before their rounding ---------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("rows,k,n", [(300, 72, 200), (300, 72, 77), (2000, 2048, 33), (300, 0, 77)])
+def test_bias_gradient_is_rounded_once(cuda_device, rows, k, n, checkpoint):
+    """Equal rows, so that a rounding of dz before its sum would be the same one in
+    every term: db is within half a unit of its last place (2^-8 of its power of
+    two), and the error of a float32 sum, of the exact sum."""
+    x, w, b, _, g = linear_inputs(1, k, n, BF16, cuda_device, seed=k)
+    x, g = x.expand(rows, k), g.expand(rows, n)
+    bias = b.clone().requires_grad_(True)
+    (db,) = torch.autograd.grad(linear_act(x, w, bias, activation="silu", checkpoint=checkpoint), [bias], g)
+    x6 = held64(x) if checkpoint else x.double()
+    z = x6 @ w.double().T + b.double()
+    dz = g.double() * slope64("silu", z)
+    # the slope: 2^-11 of it where the forward kept it in float16, and what z's error moves it by
+    loose = dz.abs() * (0 if checkpoint else 2.0 ** -11) + 2 * SUM * g.double().abs() * (
+        x6.abs() @ w.double().abs().T + b.double().abs())
+    exact = dz.sum(0)
+    bound = torch.exp2(exact.abs().log2().floor() - 8) + SUM * dz.abs().sum(0) + loose.sum(0)
+    assert bool(((db.double() - exact).abs() <= bound).all()), float(((db.double() - exact).abs() / bound).max())
 
 
 # ---- calls that autograd or a tracer has to see ---------------------------------------------
