@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib
+import math
 import warnings
 
 import pytest
@@ -153,6 +154,25 @@ def test_bias_gradient_is_rounded_once(cuda_device, rows, k, n, checkpoint):
     exact = dz.sum(0)
     bound = torch.exp2(exact.abs().log2().floor() - 8) + SUM * dz.abs().sum(0) + loose.sum(0)
     assert bool(((db.double() - exact).abs() <= bound).all()), float(((db.double() - exact).abs() / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(4, 16), (1300, 64), (1300, 33)])
+def test_gelu_of_large_negative_numbers_in_bfloat16(cuda_device, rows, n):
+    """One term to a sum, so that z is exact: y is within half a unit in its last
+    place, and 2^-12 of it, of z * Phi(z) down to z = -12.5. The approximation of
+    Phi is within 2^-13 of it, its exponential's argument of at most 113 within 2^-17."""
+    z = torch.linspace(-12.5, 12.5, rows * n, dtype=torch.float64).view(rows, n).to(BF16)
+    x = torch.zeros(rows, 8 * n, dtype=BF16)
+    x[:, ::8] = z
+    w = torch.zeros(n, 8 * n, dtype=BF16)
+    w[torch.arange(n), 8 * torch.arange(n)] = 1
+    x, w, z = x.to(cuda_device), w.to(cuda_device), z.to(cuda_device).double()
+    exact = z * 0.5 * torch.erfc(-z / math.sqrt(2))
+    y = linear_act(x, w, activation="gelu").double()
+    bound = torch.exp2(exact.abs().log2().floor().clamp(min=-126) - 8) + 2.0 ** -12 * exact.abs()
+    assert bool(((y - exact).abs() <= bound)[z != 0].all()), float(((y - exact).abs() / bound)[z != 0].max())
+    assert bool((y[z == 0] == 0).all())
 
 
 # ---- calls that autograd or a tracer has to see ---------------------------------------------
