@@ -116,7 +116,8 @@ def layer_norm(input: torch.Tensor, weight: torch.Tensor | None = None, bias: to
         else:
             output = _forward(module, *tensors, float(eps), None)[0]
     except RuntimeError as exc:
-        raise failed(report, str(exc)) from exc
+        failed(report, str(exc))
+        raise
     record_dispatch_report(report)
     return output if dtype != torch.float16 else output.to(dtype)
 

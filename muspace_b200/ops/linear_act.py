@@ -155,7 +155,8 @@ def linear_act(input: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         else:
             output, _ = _forward(module, *tensors, activation, False)
     except RuntimeError as exc:
-        raise failed(report, str(exc)) from exc
+        failed(report, str(exc))
+        raise
     record_dispatch_report(report)
     return output if dtype != torch.float16 else output.to(dtype)
 

@@ -252,3 +252,14 @@ def test_forward_mode_is_refused_on_the_gpu(cuda_device, name):
     with torch.no_grad(), forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward AD|jvp"):
             OPERATORS[name](forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("name", ["linear_act", "layer_norm"])
+def test_errors_keep_their_type(fake_library, monkeypatch, name):
+    """A caller that frees memory and tries again looks for torch's own class."""
+    def full(*args):
+        raise torch.OutOfMemoryError("no memory left")
+
+    monkeypatch.setattr(importlib.import_module("muspace_b200.ops." + name), "_forward", full)
+    with pytest.raises(torch.OutOfMemoryError, match="no memory left"):
+        OPERATORS[name](torch.ones(3, 8))
