@@ -108,12 +108,13 @@ __global__ void __launch_bounds__(32 * kSumWarps)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
   const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
+  const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);  // src may be a caller's: nothing beyond its rows is read
   float s[8] = {};
   if (c < cols) {
 #pragma unroll 4
     for (int64_t r = begin + warp; r < end; r += kSumWarps) {
       float v[8];
-      load8(src + r * ld + c, v);  // rows are padded to eight: what lies beyond is not kept
+      load_some(src + r * ld + c, count, count == 8, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }

@@ -157,6 +157,21 @@ def test_bias_gradient_is_rounded_once(cuda_device, rows, k, n, checkpoint):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [250, 255, 129])
+def test_bias_gradient_of_rows_that_end_with_their_storage(cuda_device, n):
+    """A gradient whose rows are 256 apart and whose last one ends the tensor's memory; what lies between rows is NaN."""
+    rows = 700
+    gen = torch.Generator().manual_seed(n)
+    held = torch.full((256 * (rows - 1) + n,), float("nan"), dtype=BF16, device=cuda_device)
+    g = torch.as_strided(held, (rows, n), (256, 1))
+    g.copy_(torch.randn(rows, n, generator=gen).to(BF16))
+    x, w = torch.ones(rows, 16, device=cuda_device, dtype=BF16), torch.ones(n, 16, device=cuda_device, dtype=BF16)
+    bias = torch.zeros(n, device=cuda_device, dtype=BF16, requires_grad=True)
+    (db,) = torch.autograd.grad(linear_act(x, w, bias), [bias], g)
+    near(db, g.double().sum(0), g.double().abs().sum(0), BF16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,n", [(4, 16), (1300, 64), (1300, 33)])
 def test_gelu_of_large_negative_numbers_in_bfloat16(cuda_device, rows, n):
     """One term to a sum, so that z is exact: y is within half a unit in its last
