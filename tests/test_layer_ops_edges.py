@@ -18,7 +18,8 @@ from torch.autograd import forward_ad
 
 from muspace_b200.ops import checkpoint_pack, checkpoint_unpack, layer_norm, linear_act
 from muspace_b200.runtime import native
-from test_layer_ops import BF16, F32, SUM, held64, linear_inputs, near, slope64
+from test_layer_ops import (
+    BF16, F16, F32, SUM, check_linear, check_norm, held64, linear_inputs, near, norm_inputs, slope64)
 
 
 def workspace_of(name: str, **fields) -> int:
@@ -278,3 +279,24 @@ def test_errors_keep_their_type(fake_library, monkeypatch, name):
     monkeypatch.setattr(importlib.import_module("muspace_b200.ops." + name), "_forward", full)
     with pytest.raises(torch.OutOfMemoryError, match="no memory left"):
         OPERATORS[name](torch.ones(3, 8))
+
+
+# ---- float16 ------------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("activation", ["none", "gelu", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(3, 72, 40), (1100, 72, 200), (1100, 67, 77)])
+def test_linear_in_float16(cuda_device, rows, k, n, activation, checkpoint):
+    check_linear(*linear_inputs(rows, k, n, F16, cuda_device, seed=n), activation, checkpoint)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("checkpoint", [None, "int8"])
+@pytest.mark.parametrize("rows,n", [(1, 4096), (700, 256), (700, 33), (160, 5000)])
+def test_layer_norm_in_float16(cuda_device, rows, n, checkpoint):
+    x, w, b, g = norm_inputs(rows, n, F16, cuda_device, seed=n)
+    check_norm(x, w, b, g, checkpoint)
+    check_norm(x, w.float(), b.float(), g, checkpoint)
+    check_norm(x, None, None, g, checkpoint)
