@@ -101,6 +101,12 @@ __device__ __forceinline__ void put_sums(float (*buf)[kSumCols], const float s[8
   if (c < cols) parts[blockIdx.y * cols + c] = sum;
 }
 
+// kRagged: cols is no multiple of eight. Rows are multiples of eight apart, so a
+// vector that reaches beyond a row ends before the next one, and what it holds
+// there is not kept; but the last row may be the end of a caller's memory, and is
+// read element by element. (In one kernel for both, 8192 x 8192 took 32 us instead
+// of 23: the loop's end then costs it loads on their way.)
+template <bool kRagged>
 __global__ void __launch_bounds__(32 * kSumWarps)
     column_parts_kernel(const bf16* __restrict__ src, int64_t ld, int64_t rows, int64_t cols, int64_t rows_per_part,
                         float* __restrict__ parts) {
@@ -108,13 +114,19 @@ __global__ void __launch_bounds__(32 * kSumWarps)
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
   const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
-  const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);  // src may be a caller's: nothing beyond its rows is read
+  const int64_t whole = kRagged ? min(end, rows - 1) : end;
   float s[8] = {};
   if (c < cols) {
 #pragma unroll 4
-    for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+    for (int64_t r = begin + warp; r < whole; r += kSumWarps) {
       float v[8];
-      load_some(src + r * ld + c, count, count == 8, v);
+      load8(src + r * ld + c, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
+    }
+    if (kRagged && whole < end && (end - 1 - begin) % kSumWarps == warp) {
+      float v[8];
+      load_some(src + (rows - 1) * ld + c, static_cast<int>(cols - c < 8 ? cols - c : 8), false, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
@@ -233,8 +245,8 @@ cudaError_t column_sums(const Operand& src, float* parts, cudaStream_t stream) {
   if (src.cols == 0 || src.rows == 0) return cudaSuccess;
   const int count = column_parts(src.rows, src.cols);
   const dim3 grid(static_cast<unsigned>((src.cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
-  column_parts_kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.rows, src.cols,
-                                                          (src.rows + count - 1) / count, parts);
+  const auto kernel = src.cols % 8 == 0 ? column_parts_kernel<false> : column_parts_kernel<true>;
+  kernel<<<grid, 32 * kSumWarps, 0, stream>>>(src.p, src.ld, src.rows, src.cols, (src.rows + count - 1) / count, parts);
   return cudaGetLastError();
 }
 
