@@ -424,7 +424,8 @@ MSDA_API int msda_checkpoint_unpack(msda_dtype_t dtype, const int8_t *codes, con
  *                  input (or codes), weight and bias.
  *   codes, exponents  backward only: an 8-bit checkpoint of x that takes the
  *                  place of input; the gradients are those at the x it holds.
- *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional
+ *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional;
+ *                  bfloat16: dz is rounded to bfloat16 for dx and dW, not for db
  *
  * workspace: 256-byte aligned, of at least as many bytes as the *_workspace
  * call gives for the same structure (it reads sizes, strides and the
@@ -433,7 +434,9 @@ MSDA_API int msda_checkpoint_unpack(msda_dtype_t dtype, const int8_t *codes, con
  *
  * The matrix products run on the tensor cores: bfloat16 as it stands, float32
  * as three bfloat16 parts of each operand, which keeps 24 bits of every
- * product. Sizes up to 2^31 - 1.
+ * product; infinities, NaNs and sums that overflow come out as in float32
+ * arithmetic, but for factors below 2^-134, which count as 0. Sizes up to
+ * 2^31 - 1.
  */
 typedef struct {
   int32_t dtype;      /* msda_dtype_t */

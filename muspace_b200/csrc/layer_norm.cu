@@ -318,7 +318,9 @@ struct Input<G, NV, kVec, true, T> {
   }
 };
 
-// Blocks that an SM holds; as many are launched, so that all rows are under way at once.
+// Blocks of the register kernels that an SM holds; as many are launched, so that all
+// rows are under way at once. The ring kernel gets the same number, and an SM holds
+// one block of it: for 2049 to 4096 columns that makes two waves.
 constexpr int backward_blocks(int threads) {
   return threads == 32 ? 3 : threads == 128 ? 4 : threads == 256 ? 2 : 1;
 }

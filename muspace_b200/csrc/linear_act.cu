@@ -6,9 +6,12 @@
 // that matter at 2^-24 are added up.
 //
 // Backward: dz = g * act'(z) is one operand of two products (dx = dz W,
-// dW = dz^T x). Where the forward kept the slope act'(z), dz is one
-// elementwise pass; where it kept nothing (a checkpoint of x in 8 bits), z is
-// computed again and dz leaves that product's epilogue.
+// dW = dz^T x). In bfloat16 it is rounded to bfloat16 for them, as the tensor core
+// takes it in one product (two planes would double both): with the output's own
+// rounding the gradients are off by 0.0024 of their size, by 0.0017 without (40000
+// x 256 x 512). db is added up before that rounding. Where the forward kept the
+// slope act'(z), dz is one elementwise pass; where it kept nothing (a checkpoint of
+// x in 8 bits), z is computed again and dz leaves that product's epilogue.
 #include <algorithm>
 
 #include "checkpoint8.cuh"

@@ -148,7 +148,8 @@ cudaError_t launch_rows(const Args& a, cudaStream_t stream) {
 }  // namespace
 
 // Where this kernel is the faster one (B200, us here / on the tensor cores).
-// bfloat16: up to 4 rows (1 x 4096 x 4096 8.2 / 13.9; 4 rows 14.1 / 13.9), and up
+// bfloat16: up to 4 rows (1 x 4096 x 4096 8.2 / 13.9; 4 rows 14.1 / 13.9, as good
+// as even, and here without sums in a workspace or a second launch), and up
 // to 8 of short ones (8 x 256 x 512 4.0 / 6.0; 8 x 1024 x 256 9.1 / 7.0).
 // float32, which the tensor cores get in planes: up to 16 rows of any weight (16
 // x 4096 x 4096 48 / 86), and more while the products are few (64 x 256 x 512

@@ -5,13 +5,15 @@ attention: ``y = act(x W^T + b) + r``. The product runs on the tensor cores,
 bias, activation and residual on its float32 sums before the one rounding.
 
 Backward: ``dz = g * act'(z)``, ``dx = dz W``, ``dW = dz^T x``, ``db`` the sum of
-``dz`` over rows, and ``g`` itself for the residual. ``act'(z)`` comes from the
-forward (in float16 beside bfloat16: 11 bits of a number in [-0.2, 1.2]), which
-holds as much between the passes as ``z`` itself would, or, with a checkpoint, from
-computing ``z`` again in the epilogue that makes ``dz``. Forward and backward,
-kept and computed again, on a B200: 40000 x 256 x 512 bfloat16 108 and 125 us,
-40000 x 2048 x 512 260 and 321; 22223 x 256 x 1024 float32 359 and 418. Kept was
-the faster one at every size from 64 input features on, in both types.
+``dz`` over rows, and ``g`` itself for the residual. In bfloat16 ``dz`` is rounded
+to bfloat16 before the two products, as a tensor core takes it. ``act'(z)`` comes
+from the forward (in float16 beside bfloat16: 11 bits of a number in [-0.2, 1.2],
+and 2^-25 where it is below 2^-14), which holds as much between the passes as ``z``
+itself would, or, with a checkpoint, from computing ``z`` again in the epilogue
+that makes ``dz``. Forward and backward, kept and computed again, on a B200: 40000
+x 256 x 512 bfloat16 108 and 125 us, 40000 x 2048 x 512 260 and 321; 22223 x 256 x
+1024 float32 359 and 418. Kept was the faster one at every size from 64 input
+features on, in both types.
 """
 
 from __future__ import annotations
