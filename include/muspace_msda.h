@@ -93,6 +93,7 @@ typedef enum {
 typedef enum {
   MSDA_DTYPE_FLOAT32 = 0,
   MSDA_DTYPE_BFLOAT16 = 1,
+  MSDA_DTYPE_FLOAT16 = 2, /* msda_dropout and msda_residual_norm_* alone take it */
 } msda_dtype_t;
 
 /* Problem sizes for the plain-pointer entry points. */
@@ -493,6 +494,74 @@ typedef struct {
 MSDA_API int msda_layer_norm_forward(const msda_layer_norm_t *args, void *stream);
 MSDA_API int msda_layer_norm_backward_workspace(const msda_layer_norm_t *args, size_t *bytes);
 MSDA_API int msda_layer_norm_backward(const msda_layer_norm_t *args, void *stream);
+
+/*
+ * Dropout from a counter-based generator. Nothing of a mask is stored: an element's
+ * number follows from the seed, the sequence (one per dropout of a program) and the
+ * element's row and column, by Philox-4x32 with ten rounds: key (seed mod 2^32,
+ * seed / 2^32), counter (column / 8, row, sequence mod 2^32, sequence / 2^32), whose
+ * four words are the 16-bit numbers of eight neighbouring columns, the low half of
+ * the first word first. An element is kept where its number is at least threshold
+ * (0 to 65536), and is multiplied by 65536 / (65536 - threshold) then; else it is 0.
+ * The backward pass is the same call on the gradient.
+ *
+ *   input [rows, cols]; output contiguous; storage float32, bfloat16 or float16.
+ *   seed_at: NULL, or an int64 on the device that takes the place of seed (a captured
+ *   graph then draws another mask whenever it has changed between two replays).
+ */
+MSDA_API int msda_dropout(msda_dtype_t dtype, const void *input, int64_t rows, int64_t cols, int64_t input_stride,
+                          int64_t threshold, int64_t seed, int64_t sequence, const int64_t *seed_at, void *output,
+                          void *stream);
+
+typedef enum {
+  MSDA_NORM_LAYER = 0, /* (x - mean) * rstd, rstd = 1 / sqrt(var + eps) */
+  MSDA_NORM_RMS = 1,   /* x * rstd, rstd = 1 / sqrt(mean(x^2) + eps) */
+} msda_norm_t;
+
+/*
+ * Norms over the last dimension with the residual they belong to; D is dropout as
+ * in msda_dropout, norm(x) = (x - mean) * rstd * weight + bias:
+ *
+ *   msda_add_norm_*   s = residual_scale * residual + gate * D(input), output = norm(s)
+ *   msda_norm_add_*   s = residual_scale * residual + gate * D(norm(input))
+ *
+ *   input, residual [rows, cols]; weight, bias [cols] or NULL, of weight_dtype;
+ *   gate [gate_groups, cols] or NULL, of gate_dtype, rows / gate_groups neighbouring
+ *   rows to a row of it (weight_dtype, gate_dtype: dtype or float32);
+ *   output, sum contiguous; add_norm may leave sum NULL, norm_add has no output;
+ *   mean, rstd [rows] float32, written by the forward where not NULL and read by the
+ *   backward (mean: NULL with MSDA_NORM_RMS); add_norm takes output from the sum
+ *   before its rounding, mean and rstd (for the backward) from the sum as stored;
+ *   backward: grad_output (add_norm) and grad_sum [rows, cols], either may be NULL
+ *   in add_norm, where what reaches the other is 0 then; sum (add_norm) and input
+ *   (norm_add, and add_norm with grad_gate) as in the forward, sum_stride apart;
+ *   grad_input, grad_residual, grad_weight, grad_bias, grad_gate contiguous,
+ *   overwritten, each optional (grad_weight and grad_bias need grad_output in
+ *   add_norm); workspace: 256-byte aligned, of as many bytes as the *_workspace call gives.
+ */
+typedef struct {
+  int32_t dtype, weight_dtype, gate_dtype; /* msda_dtype_t */
+  int32_t kind;                            /* msda_norm_t */
+  int64_t rows, cols, gate_groups;
+  int64_t input_stride, residual_stride, gate_stride, sum_stride, grad_output_stride, grad_sum_stride;
+  float residual_scale, eps;
+  int64_t threshold, seed, sequence;
+  const int64_t *seed_at;
+  const void *input, *residual, *gate, *weight, *bias;
+  void *output, *sum;
+  float *mean, *rstd;
+  const void *grad_output, *grad_sum;
+  void *grad_input, *grad_residual, *grad_weight, *grad_bias, *grad_gate;
+  void *workspace;
+  size_t workspace_bytes;
+} msda_residual_norm_t;
+
+MSDA_API int msda_add_norm_forward(const msda_residual_norm_t *args, void *stream);
+MSDA_API int msda_add_norm_backward_workspace(const msda_residual_norm_t *args, size_t *bytes);
+MSDA_API int msda_add_norm_backward(const msda_residual_norm_t *args, void *stream);
+MSDA_API int msda_norm_add_forward(const msda_residual_norm_t *args, void *stream);
+MSDA_API int msda_norm_add_backward_workspace(const msda_residual_norm_t *args, size_t *bytes);
+MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stream);
 
 /* Waits inside the linear and layer-norm kernels that gave up on the current
  * device since the library loaded. 0 is expected; anything else means that a

@@ -23,6 +23,8 @@ _SUBMODULES = (
     "ops.linear_act",
     "ops.layer_norm",
     "ops.checkpoint8",
+    "ops.dropout",
+    "ops.residual_norm",
     "runtime",
     "runtime.kernel_dispatch",
     "runtime.native",

@@ -1,5 +1,6 @@
 // extern "C" boundary of the layer operators (declared in
-// include/muspace_msda.h): linear_act, layer norm and 8-bit checkpoints.
+// include/muspace_msda.h): linear_act, layer norm, 8-bit checkpoints, dropout and the
+// norms with their residual.
 #include <cuda_runtime.h>
 
 #include <limits>
@@ -7,8 +8,10 @@
 
 #include "../../include/muspace_msda.h"
 #include "capi_common.h"
+#include "dropout.h"
 #include "layer_norm.h"
 #include "linear_act.h"
+#include "residual_norm.h"
 
 namespace {
 
@@ -129,9 +132,148 @@ size_t norm_workspace(const msda_layer_norm_t& in) {
   return static_cast<size_t>(lnorm::backward_parts(in.rows, in.cols)) * 2 * in.cols * sizeof(float);
 }
 
+void check_wide_dtype(int dtype) {
+  require(dtype == MSDA_DTYPE_FLOAT32 || dtype == MSDA_DTYPE_BFLOAT16 || dtype == MSDA_DTYPE_FLOAT16,
+          "dtype must be float32, bfloat16 or float16");
+}
+
+drop::Rule rule_of(int64_t threshold, int64_t seed, int64_t sequence, const int64_t* seed_at) {
+  require(threshold >= 0 && threshold <= 65536, "threshold must be between 0 and 65536");
+  drop::Rule rule;
+  rule.threshold = static_cast<uint32_t>(threshold);
+  rule.scale = drop::scale_of(rule.threshold);
+  rule.seed = static_cast<uint64_t>(seed);
+  rule.sequence = static_cast<uint64_t>(sequence);
+  rule.seed_at = threshold ? seed_at : nullptr;
+  return rule;
+}
+
+resnorm::Args residual_norm_args(const msda_residual_norm_t* in, bool branch, bool backward) {
+  require(in != nullptr, "args is null");
+  check_wide_dtype(in->dtype);
+  require(in->weight_dtype == in->dtype || in->weight_dtype == MSDA_DTYPE_FLOAT32, "weight_dtype must be dtype or float32");
+  require(in->gate_dtype == in->dtype || in->gate_dtype == MSDA_DTYPE_FLOAT32, "gate_dtype must be dtype or float32");
+  require(in->kind == MSDA_NORM_LAYER || in->kind == MSDA_NORM_RMS, "kind must be layer or rms");
+  check_size(in->rows, "rows");
+  check_size(in->cols, "cols");
+  for (int64_t stride : {in->input_stride, in->residual_stride, in->gate_stride, in->sum_stride,
+                         in->grad_output_stride, in->grad_sum_stride})
+    require(stride >= 0, "strides must be non-negative");
+  const bool some = in->rows > 0 && in->cols > 0, gated = in->gate || in->grad_gate;
+  require(in->gate_groups >= 0, "sizes must be non-negative");
+  require(!some || !gated || (in->gate_groups > 0 && in->rows % in->gate_groups == 0),
+          "gate_groups must divide rows");
+  resnorm::Args a{};
+  a.dtype = static_cast<drop::DType>(in->dtype);
+  a.weight_f32 = in->weight_dtype == MSDA_DTYPE_FLOAT32, a.gate_f32 = in->gate_dtype == MSDA_DTYPE_FLOAT32;
+  a.branch = branch, a.rms = in->kind == MSDA_NORM_RMS;
+  a.rows = in->rows, a.cols = in->cols;
+  a.gate_groups = gated ? in->gate_groups : 1;
+  a.gate_rows = a.gate_groups ? a.rows / a.gate_groups : 0;
+  a.h_stride = in->input_stride, a.r_stride = in->residual_stride, a.gate_stride = in->gate_stride;
+  a.gy_stride = in->grad_output_stride, a.gs_stride = in->grad_sum_stride, a.sum_stride = in->sum_stride;
+  a.alpha = in->residual_scale, a.eps = in->eps;
+  a.rule = rule_of(in->threshold, in->seed, in->sequence, in->seed_at);
+  a.gate = in->gate, a.w = in->weight, a.b = in->bias;
+  a.rstd = in->rstd;
+  if (backward) {
+    const bool normed = branch || in->grad_output;
+    require(branch || !some || in->grad_output || in->grad_sum, "grad_output and grad_sum are null");
+    require(normed || !some || (!in->grad_weight && !in->grad_bias), "grad_weight and grad_bias need grad_output");
+    check_pointer(some && branch, in->grad_sum, "grad_sum");
+    check_pointer(some && (branch || in->grad_gate), in->input, "input");
+    check_pointer(some && !branch && normed, in->sum, "sum");
+    check_pointer(some && normed, in->rstd, "rstd");
+    check_pointer(some && normed && !a.rms, in->mean, "mean");
+    a.mean = a.rms ? nullptr : in->mean;
+    a.h = in->input;
+    a.gs = in->grad_sum;
+    if (!branch) a.gy = in->grad_output, a.sum = in->sum;
+    a.dh = in->grad_input, a.dr = in->grad_residual;
+    a.dw = in->grad_weight, a.db = in->grad_bias, a.dgate = in->grad_gate;
+    a.parts = static_cast<float*>(in->workspace);
+  } else {
+    check_pointer(some, in->input, "input");
+    check_pointer(some, in->residual, "residual");
+    check_pointer(some, branch ? in->sum : in->output, branch ? "sum" : "output");
+    a.mean = in->mean;
+    a.h = in->input, a.r = in->residual;
+    if (!branch) a.y = in->output;
+    a.s = in->sum;
+  }
+  return a;
+}
+
+int residual_norm_forward(const msda_residual_norm_t* args, bool branch, const char* name, void* stream) {
+  return guarded([&] {
+    check_launch(resnorm::forward(residual_norm_args(args, branch, false), static_cast<cudaStream_t>(stream)), name);
+  });
+}
+
+size_t residual_norm_workspace(const resnorm::Args& a) {
+  return static_cast<size_t>(resnorm::backward_parts(a)) * sizeof(float);
+}
+
+int residual_norm_workspace(const msda_residual_norm_t* args, bool branch, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "bytes is null");
+    *bytes = residual_norm_workspace(residual_norm_args(args, branch, true));
+  });
+}
+
+int residual_norm_backward(const msda_residual_norm_t* args, bool branch, const char* name, void* stream) {
+  return guarded([&] {
+    const resnorm::Args a = residual_norm_args(args, branch, true);
+    check_workspace(args->workspace, args->workspace_bytes, residual_norm_workspace(a));
+    check_launch(resnorm::backward(a, static_cast<cudaStream_t>(stream)), name);
+  });
+}
+
 }  // namespace
 
 extern "C" {
+
+int msda_dropout(msda_dtype_t dtype, const void* input, int64_t rows, int64_t cols, int64_t input_stride,
+                 int64_t threshold, int64_t seed, int64_t sequence, const int64_t* seed_at, void* output,
+                 void* stream) {
+  return guarded([&] {
+    check_wide_dtype(dtype);
+    check_size(rows, "rows");
+    check_size(cols, "cols");
+    require(input_stride >= 0, "strides must be non-negative");
+    const drop::Rule rule = rule_of(threshold, seed, sequence, seed_at);
+    const bool some = rows > 0 && cols > 0;
+    check_pointer(some, input, "input");
+    check_pointer(some, output, "output");
+    check_launch(drop::dropout(static_cast<drop::DType>(dtype), input, input_stride, rows, cols, rule, output,
+                               static_cast<cudaStream_t>(stream)),
+                 "msda_dropout");
+  });
+}
+
+int msda_add_norm_forward(const msda_residual_norm_t* args, void* stream) {
+  return residual_norm_forward(args, false, "msda_add_norm_forward", stream);
+}
+
+int msda_add_norm_backward_workspace(const msda_residual_norm_t* args, size_t* bytes) {
+  return residual_norm_workspace(args, false, bytes);
+}
+
+int msda_add_norm_backward(const msda_residual_norm_t* args, void* stream) {
+  return residual_norm_backward(args, false, "msda_add_norm_backward", stream);
+}
+
+int msda_norm_add_forward(const msda_residual_norm_t* args, void* stream) {
+  return residual_norm_forward(args, true, "msda_norm_add_forward", stream);
+}
+
+int msda_norm_add_backward_workspace(const msda_residual_norm_t* args, size_t* bytes) {
+  return residual_norm_workspace(args, true, bytes);
+}
+
+int msda_norm_add_backward(const msda_residual_norm_t* args, void* stream) {
+  return residual_norm_backward(args, true, "msda_norm_add_backward", stream);
+}
 
 int msda_checkpoint_pack(msda_dtype_t dtype, const void* input, int64_t rows, int64_t cols, int64_t input_stride,
                          int8_t* codes, uint8_t* exponents, void* stream) {

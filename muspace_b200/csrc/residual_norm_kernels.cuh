@@ -1,0 +1,766 @@
+// Norms with the residual they belong to, forward and backward (formulas in
+// residual_norm.h), for one storage type.
+//
+// Bound by memory: a row is read once into the registers of G threads, 8 NV values
+// each; dropout, gate, residual and norm happen there in float32, and each result is
+// rounded once. A dropout mask is made again from its counter wherever it is needed.
+//
+//   add_norm backward, from what reaches y (gy) and s (gs):
+//     ds = gs + rstd (gy w - mean(gy w) - k mean(gy w k)), k = (s - mean) rstd
+//     dr = alpha ds,  dh = D'(gate ds),  dgate = sum of ds D(h),  dw = sum of gy k,  db = sum of gy
+//   norm_add backward, from what reaches s:
+//     dr = alpha gs,  d = gate D'(gs),  dgate = sum of gs D(norm(h)),  dw = sum of d k,  db = sum of d
+//     dh = rstd (d w - mean(d w) - k mean(d w k)), k = (h - mean) rstd
+//   (kind rms: mean and the mean of d w are 0; D' multiplies as D does)
+//
+// y is the norm of the sum before s is rounded to its type. The backward pass takes s
+// as it was stored, and with it the statistics of what was stored, which the forward
+// takes in the same reductions: the gradients are those at the stored sum. (With the
+// statistics of the unrounded one, k's sum over a row is not 0, nor that of its squares
+// n; where a row's mean is large beside its spread nothing of the gradient is left.)
+//
+// A backward block takes whole units of neighbouring rows, a unit's rows all under
+// one row of the gate: so a thread sums dw, db and dgate of its columns in
+// registers, writes them once, and a second kernel adds the blocks' sums in order.
+#pragma once
+
+#include <algorithm>
+
+#include "dropout_device.cuh"
+#include "residual_norm.h"
+#include "rows_device.cuh"
+
+namespace resnorm {
+namespace {
+
+using lin::add2;
+using lin::both;
+using lin::fma2;
+using lin::mul2;
+using rows::Chunk;
+using rows::column;
+using rows::row_sums;
+using rows::Shape;
+using rows::store_chunk;
+using rows::Sums;
+
+// Eight values of a parameter, of the rows' type or float32.
+template <int G, bool kVec, typename T>
+__device__ __forceinline__ void load_param(const void* p, bool f32, int cols, int lane, int i, float2 v[4]) {
+  if (sizeof(T) == 4 || f32) {
+    Chunk<float, kVec> c;
+    c.template load<G>(static_cast<const float*>(p), cols, lane, i);
+    c.get(v);
+  } else {
+    Chunk<T, kVec> c;
+    c.template load<G>(static_cast<const T*>(p), cols, lane, i);
+    c.get(v);
+  }
+}
+
+// Which of a thread's eight values are kept. Where they are neighbours, they are one
+// call of the generator. Where they are G columns apart, a warp's 256 columns are 32
+// calls, one to a lane, and a lane fetches its bits from the lanes that have them.
+template <int G, bool kVec>
+struct Mask {
+  drop::Words n;
+  __device__ __forceinline__ void make(const drop::Key& key, int64_t row, int lane, int i) {
+    n = drop::numbers(key, static_cast<uint32_t>(row), i * G + lane);
+  }
+  __device__ __forceinline__ bool kept(const drop::Key& key, int j) const { return drop::kept(key, n, j); }
+};
+template <int G>
+struct Mask<G, false> {
+  uint32_t bits;
+  __device__ __forceinline__ void make(const drop::Key& key, int64_t row, int lane, int i) {
+    const int l = lane & 31, group = ((i * 8 + l / 4) * G + lane - l) / 8 + l % 4;
+    const uint32_t mine = drop::bits8(key, drop::numbers(key, static_cast<uint32_t>(row), group));
+    bits = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits |= (__shfl_sync(0xffffffffu, mine, j * 4 + l / 8) >> (l % 8) & 1u) << j;
+  }
+  __device__ __forceinline__ bool kept(const drop::Key&, int j) const { return bits >> j & 1u; }
+};
+
+template <typename M>
+__device__ __forceinline__ void apply(const M& mask, const drop::Key& key, float* v) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = mask.kept(key, j) ? v[j] * key.scale : 0.f;
+}
+
+// The gate's row for a row.
+__device__ __forceinline__ const void* gate_at(const Args& a, int64_t r, int size) {
+  if (!a.gate) return nullptr;
+  const int64_t g = a.gate_rows == a.rows ? 0
+                    : a.gate_rows == 1    ? r
+                                          : static_cast<uint32_t>(r) / static_cast<uint32_t>(a.gate_rows);
+  return static_cast<const char*>(a.gate) + g * a.gate_stride * size;
+}
+
+__device__ __forceinline__ float2 stored(float2 v, float) { return v; }
+__device__ __forceinline__ float2 stored(float2 v, lin::bf16) { return lin::unpack2(lin::pack2(v.x, v.y)); }
+__device__ __forceinline__ float2 stored(float2 v, __half) { return __half22float2(__floats2half2_rn(v.x, v.y)); }
+
+struct Moments {
+  float mean, rstd;
+};
+
+// Mean and rstd of the row whose values lie in v; beyond the row v is 0. kBoth: and
+// those of the values as T stores them, in the same reductions.
+template <int G, int NV, bool kVec, bool kBoth, typename T>
+__device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a, int cols, int lane, Sums* buf,
+                                           int& turn, Moments& of_stored) {
+  const float n = static_cast<float>(cols);
+  const auto over_row = [&](float2 x, float2 y) {
+    if constexpr (kBoth)
+      return row_sums<G>(Sums{x.x + x.y, y.x + y.y}, buf, turn);
+    else
+      return Sums{row_sums<G>(x.x + x.y, buf, turn), 0.f};
+  };
+  Sums mean{0.f, 0.f};
+  if (!a.rms) {
+    float2 t = both(0.f), u = both(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        t = add2(t, v[i][j]);
+        if (kBoth) u = add2(u, stored(v[i][j], T()));
+      }
+    mean = over_row(t, u);
+    mean.a /= n, mean.b /= n;
+  }
+  float2 t = both(0.f), u = both(0.f);
+  const auto square = [&](int i, int j, float2 d, float2 sum) {
+    if (!kVec) {
+      if (column<G, false>(lane, i, 2 * j) >= cols) d.x = 0.f;
+      if (column<G, false>(lane, i, 2 * j + 1) >= cols) d.y = 0.f;
+    }
+    return fma2(d, d, sum);
+  };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (kVec && column<G, true>(lane, i, 0) >= cols) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      t = square(i, j, add2(v[i][j], both(-mean.a)), t);
+      if (kBoth) u = square(i, j, add2(stored(v[i][j], T()), both(-mean.b)), u);
+    }
+  }
+  const Sums var = over_row(t, u);
+  of_stored = Moments{mean.b, rsqrtf(var.b / n + a.eps)};
+  return Moments{mean.a, rsqrtf(var.a / n + a.eps)};
+}
+
+template <int G, int NV, bool kVec, bool kBranch, typename T>
+__global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args a) {
+  __shared__ Sums buf[Shape<G>::kBuf];
+  int turn = 0;
+  const int lane = threadIdx.x % G, cols = static_cast<int>(a.cols);
+  const int gate_size = a.gate_f32 ? 4 : sizeof(T);
+  const int64_t step = static_cast<int64_t>(gridDim.x) * Shape<G>::kRows;
+  const T *h = static_cast<const T*>(a.h), *res = static_cast<const T*>(a.r);
+  const drop::Key key = drop::key_of(a.rule);
+  const float2 alpha = both(a.alpha);
+  int64_t r = blockIdx.x * static_cast<int64_t>(Shape<G>::kRows) + threadIdx.x / G;
+  Chunk<T, kVec> next_h[NV], next_r[NV];
+  const auto load = [&](int64_t row) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      next_h[i].template load<G>(h + row * a.h_stride, cols, lane, i);
+      next_r[i].template load<G>(res + row * a.r_stride, cols, lane, i);
+    }
+  };
+  if (r < a.rows) load(r);
+  for (; r < a.rows; r += step) {
+    float2 v[NV][4], p[4];
+    Chunk<T, kVec> here_r[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      next_h[i].get(v[i]);
+      here_r[i] = next_r[i];
+    }
+    if (r + step < a.rows) load(r + step);
+    const void* gate = gate_at(a, r, gate_size);
+    // D, the gate and the residual, on eight values
+    const auto join = [&](int i) {
+      if (a.rule.threshold) {
+        Mask<G, kVec> mask;
+        mask.make(key, r, lane, i);
+        apply(mask, key, &v[i][0].x);
+      }
+      if (gate) {
+        load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = mul2(v[i][j], p[j]);
+      }
+      here_r[i].get(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = fma2(alpha, p[j], v[i][j]);
+      if (a.s) store_chunk<G, kVec>(static_cast<T*>(a.s) + r * a.cols, cols, lane, i, &v[i][0].x);
+    };
+    if (!kBranch) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) join(i);
+    }
+    Moments m, kept;
+    if (!kBranch && sizeof(T) == 2 && a.rstd) {
+      m = moments<G, NV, kVec, true, T>(v, a, cols, lane, buf, turn, kept);
+    } else {
+      Moments none;
+      kept = m = moments<G, NV, kVec, false, T>(v, a, cols, lane, buf, turn, none);
+    }
+    if (a.rstd && lane == 0) {
+      if (a.mean) a.mean[r] = kept.mean;
+      a.rstd[r] = kept.rstd;
+    }
+    const float2 scale = both(m.rstd), minus = both(-m.mean);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = mul2(add2(v[i][j], minus), scale);
+      if (a.w) {
+        load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = mul2(v[i][j], p[j]);
+      }
+      if (a.b) {
+        load_param<G, kVec, T>(a.b, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = add2(v[i][j], p[j]);
+      }
+      if (kBranch)
+        join(i);
+      else
+        store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, &v[i][0].x);
+    }
+  }
+}
+
+// A unit of a backward block: rows [begin, end), all under the gate's row `group`.
+struct Unit {
+  int64_t begin, end, group;
+};
+__device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
+  const int64_t group = u / grid.group_units, first = group * grid.group_rows;
+  const int64_t begin = first + (u - group * grid.group_units) * grid.unit_rows;
+  return Unit{begin, min(begin + grid.unit_rows, first + grid.group_rows), group};
+}
+
+template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
+__global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
+    backward_kernel(const Args a, const Grid grid) {
+  constexpr int kRows = Shape<G>::kRows;
+  __shared__ Sums buf[Shape<G>::kBuf];
+  __shared__ float fold[kRows > 1 ? kRows * 32 * 8 : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % G, slot = threadIdx.x / G, cols = static_cast<int>(a.cols);
+  const int gate_size = a.gate_f32 ? 4 : sizeof(T);
+  const float n = static_cast<float>(a.cols);
+  const drop::Key key = drop::key_of(a.rule);
+  const float2 alpha = both(a.alpha);
+  float2 dw[NV][4] = {}, db[NV][4] = {}, dg[kGate ? NV : 1][4] = {};
+
+  // Sums over the block's rows, of this thread's columns, into `out`.
+  const auto put_sums = [&](const float2 (*v)[4], float* out) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float* mine = &v[i][0].x;
+      if (kRows > 1) {  // the block's rows, in order
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) fold[(slot * 8 + j) * 32 + lane] = mine[j];
+        __syncthreads();
+        // thread (slot, lane) adds up column j = slot of lane's eight
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + slot) * 32 + lane];
+        const int c = column<G, kVec>(lane, i, slot);
+        if (c < cols) out[c] = sum;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = column<G, kVec>(lane, i, j);
+          if (c < cols) out[c] = mine[j];
+        }
+      }
+    }
+  };
+  // dgate of eight values: added up, or a row of its own
+  const auto put_gate = [&](int64_t r, int i, float2 t[4]) {
+    if (grid.sums_gate) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dg[kGate ? i : 0][j] = add2(dg[kGate ? i : 0][j], t[j]);
+    } else if (a.gate_f32) {
+      store_chunk<G, kVec>(static_cast<float*>(a.dgate) + r * a.cols, cols, lane, i, &t[0].x);
+    } else {
+      store_chunk<G, kVec>(static_cast<T*>(a.dgate) + r * a.cols, cols, lane, i, &t[0].x);
+    }
+  };
+
+  for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
+    const Unit unit = unit_of(grid, u);
+    for (int64_t r = unit.begin + slot; r < unit.end; r += kRows) {
+      const void* gate = gate_at(a, r, gate_size);
+      Chunk<T, kVec> x[NV], g[NV];
+      const T* x_row = kBranch ? static_cast<const T*>(a.h) + r * a.h_stride
+                               : static_cast<const T*>(a.sum) + r * a.sum_stride;
+      const T* g_row = kBranch ? static_cast<const T*>(a.gs) + r * a.gs_stride
+                               : static_cast<const T*>(a.gy) + r * a.gy_stride;
+      const bool normed = kBranch || a.gy;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (normed) {
+          x[i].template load<G>(x_row, cols, lane, i);
+          g[i].template load<G>(g_row, cols, lane, i);
+        }
+      }
+      const float mean = normed && a.mean ? a.mean[r] : 0.f, rstd = normed ? a.rstd[r] : 0.f;
+      const float2 scale = both(rstd), minus = both(-mean);
+      float2 sum = both(0.f), dot = both(0.f);
+      if (!kBranch) {
+        if (normed) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            float2 k[4], d[4], p[4];
+            x[i].get(k);
+            g[i].get(d);
+            if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              k[j] = mul2(add2(k[j], minus), scale);  // beyond the row the gradient is 0, and counts for nothing
+              dw[i][j] = fma2(d[j], k[j], dw[i][j]);
+              db[i][j] = add2(db[i][j], d[j]);
+              if (a.w) d[j] = mul2(d[j], p[j]);
+              sum = add2(sum, d[j]);
+              dot = fma2(d[j], k[j], dot);
+            }
+          }
+        }
+        if (!a.dh && !a.dr && !kGate) continue;
+        float2 c1 = both(0.f), c2 = both(0.f);
+        if (normed) {
+          const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
+          c1 = both(a.rms ? 0.f : -rstd * (s.a / n)), c2 = both(-rstd * rstd * (s.b / n));  // of s - mean
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float2 d[4], p[4];
+          if (normed) {
+            float2 k[4];
+            x[i].get(k);
+            g[i].get(d);
+            if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (a.w) d[j] = mul2(d[j], p[j]);
+              d[j] = fma2(add2(k[j], minus), c2, fma2(d[j], scale, c1));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = both(0.f);
+          }
+          if (a.gs) {
+            Chunk<T, kVec> more;
+            more.template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, cols, lane, i);
+            more.get(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = add2(d[j], p[j]);
+          }
+          if (a.dr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[j]);
+            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, cols, lane, i, &p[0].x);
+          }
+          if (!kGate && !a.dh) continue;
+          Mask<G, kVec> mask;
+          if (a.rule.threshold) mask.make(key, r, lane, i);
+          if (kGate) {
+            Chunk<T, kVec> branch;
+            branch.template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, cols, lane, i);
+            branch.get(p);
+            if (a.rule.threshold) apply(mask, key, &p[0].x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[j]);
+            put_gate(r, i, p);
+          }
+          if (!a.dh) continue;
+          if (a.rule.threshold) apply(mask, key, &d[0].x);
+          if (gate) {
+            load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], p[j]);
+          }
+          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, cols, lane, i, &d[0].x);
+        }
+      } else {
+        float2 d[NV][4];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float2 k[4], p[4], w[4];
+          x[i].get(k);
+          g[i].get(d[i]);
+          if (a.dr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[i][j]);
+            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, cols, lane, i, &p[0].x);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) k[j] = mul2(add2(k[j], minus), scale);
+          if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, w);
+          Mask<G, kVec> mask;
+          if (a.rule.threshold) mask.make(key, r, lane, i);
+          if (kGate) {
+            float2 b[4];
+            if (a.b) load_param<G, kVec, T>(a.b, a.weight_f32, cols, lane, i, b);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              p[j] = a.w ? mul2(k[j], w[j]) : k[j];
+              if (a.b) p[j] = add2(p[j], b[j]);
+            }
+            if (a.rule.threshold) apply(mask, key, &p[0].x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[i][j]);
+            put_gate(r, i, p);
+          }
+          if (a.rule.threshold) apply(mask, key, &d[i][0].x);
+          if (gate) {
+            load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[i][j] = mul2(d[i][j], p[j]);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            dw[i][j] = fma2(d[i][j], k[j], dw[i][j]);
+            db[i][j] = add2(db[i][j], d[i][j]);
+            if (a.w) d[i][j] = mul2(d[i][j], w[j]);
+            sum = add2(sum, d[i][j]);
+            dot = fma2(d[i][j], k[j], dot);
+          }
+        }
+        if (!a.dh) continue;
+        const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
+        const float2 c1 = both(a.rms ? 0.f : -rstd * (s.a / n)), c2 = both(-rstd * rstd * (s.b / n));  // of h - mean
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float2 k[4];
+          x[i].get(k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[i][j] = fma2(add2(k[j], minus), c2, fma2(d[i][j], scale, c1));
+          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, cols, lane, i, &d[i][0].x);
+        }
+      }
+    }
+    if (kGate && grid.sums_gate) {
+      put_sums(dg, a.parts + static_cast<int64_t>(gridDim.x) * 2 * a.cols + u * a.cols);
+#pragma unroll
+      for (int i = 0; i < (kGate ? NV : 1); ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) dg[i][j] = both(0.f);
+    }
+  }
+  if (!a.dw && !a.db) return;
+  float* part = a.parts + blockIdx.x * 2 * a.cols;
+  put_sums(dw, part);
+  put_sums(db, part + a.cols);
+}
+
+// Rows beyond the registers: a block of 1024 threads a row, eight neighbouring columns
+// a thread at a time, the row read again for each pass; sums over rows go to `parts`,
+// whose columns a thread owns.
+constexpr int kLong = 1024;
+
+template <typename T>
+struct LongRow {
+  const Args& a;
+  int64_t r, c;  // c: the first of eight columns
+  int count;
+  __device__ __forceinline__ LongRow(const Args& args, int64_t row, int64_t column)
+      : a(args), r(row), c(column), count(static_cast<int>(args.cols - column < 8 ? args.cols - column : 8)) {}
+  __device__ __forceinline__ void rows_of(const void* p, int64_t stride, float v[8]) const {
+    lin::load_some(static_cast<const T*>(p) + r * stride + c, count, false, v);
+  }
+  __device__ __forceinline__ void param(const void* p, bool f32, float none, float v[8]) const {
+    if (!p) {
+      for (int j = 0; j < 8; ++j) v[j] = none;
+    } else if (f32) {
+      lin::load_some(static_cast<const float*>(p) + c, count, false, v);
+    } else {
+      lin::load_some(static_cast<const T*>(p) + c, count, false, v);
+    }
+  }
+  __device__ __forceinline__ void put(void* p, const float v[8]) const {
+    lin::store_some(static_cast<T*>(p) + r * a.cols + c, count, false, v);
+  }
+  __device__ __forceinline__ drop::Words mask(const drop::Key& key) const {
+    return drop::numbers(key, static_cast<uint32_t>(r), static_cast<uint32_t>(c / 8));
+  }
+  // s of add_norm, from its parts
+  __device__ __forceinline__ void sum(const drop::Key& key, float v[8]) const {
+    float p[8];
+    rows_of(a.h, a.h_stride, v);
+    if (a.rule.threshold) drop::apply8(key, mask(key), v);
+    param(gate_at(a, r, a.gate_f32 ? 4 : sizeof(T)), a.gate_f32, 1.f, p);
+    for (int j = 0; j < 8; ++j) v[j] *= p[j];
+    rows_of(a.r, a.r_stride, p);
+    for (int j = 0; j < 8; ++j) v[j] = fmaf(a.alpha, p[j], v[j]);
+  }
+};
+
+template <bool kBranch, typename T>
+__global__ void __launch_bounds__(kLong) forward_long_kernel(const Args a) {
+  __shared__ Sums buf[2 * kLong / 32];
+  int turn = 0;
+  const drop::Key key = drop::key_of(a.rule);
+  const float n = static_cast<float>(a.cols);
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const auto over = [&](auto&& f) {
+      for (int64_t c = threadIdx.x * 8ll; c < a.cols; c += kLong * 8) {
+        const LongRow<T> at(a, r, c);
+        float v[8];
+        if (kBranch)
+          at.rows_of(a.h, a.h_stride, v);
+        else
+          at.sum(key, v);
+        f(at, v);
+      }
+    };
+    // of the row, and of the row as it is stored
+    Sums mean{0.f, 0.f}, t{0.f, 0.f};
+    const auto as_stored = [](float v) { return kBranch ? v : lin::to_float(lin::from_float<T>(v)); };
+    if (!a.rms) {
+      over([&](const LongRow<T>& at, float* v) {
+        for (int j = 0; j < at.count; ++j) t = t + Sums{v[j], as_stored(v[j])};
+      });
+      mean = row_sums<kLong>(t, buf, turn);
+      mean.a /= n, mean.b /= n;
+    }
+    t = Sums{0.f, 0.f};
+    over([&](const LongRow<T>& at, float* v) {
+      for (int j = 0; j < at.count; ++j) {
+        const float d = v[j] - mean.a, e = as_stored(v[j]) - mean.b;
+        t = Sums{fmaf(d, d, t.a), fmaf(e, e, t.b)};
+      }
+    });
+    t = row_sums<kLong>(t, buf, turn);
+    const float rstd = rsqrtf(t.a / n + a.eps);
+    if (a.rstd && threadIdx.x == 0) {
+      if (a.mean) a.mean[r] = mean.b;
+      a.rstd[r] = rsqrtf(t.b / n + a.eps);
+    }
+    over([&](const LongRow<T>& at, float* v) {
+      float w[8], b[8];
+      if (!kBranch && a.s) at.put(a.s, v);
+      at.param(a.w, a.weight_f32, 1.f, w);
+      at.param(a.b, a.weight_f32, 0.f, b);
+      for (int j = 0; j < 8; ++j) v[j] = fmaf((v[j] - mean.a) * rstd, w[j], b[j]);
+      if (kBranch) {
+        if (a.rule.threshold) drop::apply8(key, at.mask(key), v);
+        at.param(gate_at(a, r, a.gate_f32 ? 4 : sizeof(T)), a.gate_f32, 1.f, w);
+        at.rows_of(a.r, a.r_stride, b);
+        for (int j = 0; j < 8; ++j) v[j] = fmaf(a.alpha, b[j], v[j] * w[j]);
+        at.put(a.s, v);
+      } else {
+        at.put(a.y, v);
+      }
+    });
+  }
+}
+
+template <bool kBranch, typename T>
+__global__ void __launch_bounds__(kLong) backward_long_kernel(const Args a, const Grid grid) {
+  __shared__ Sums buf[2 * kLong / 32];
+  int turn = 0;
+  const drop::Key key = drop::key_of(a.rule);
+  const float n = static_cast<float>(a.cols);
+  const bool normed = kBranch || a.gy;
+  float* part = a.parts + blockIdx.x * 2 * a.cols;
+  bool first = true;  // of the block's rows
+  for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
+    const Unit unit = unit_of(grid, u);
+    float* gate_part = a.parts + static_cast<int64_t>(gridDim.x) * 2 * a.cols + u * a.cols;
+    for (int64_t r = unit.begin; r < unit.end; ++r, first = false) {
+      const float mean = normed && a.mean ? a.mean[r] : 0.f, rstd = normed ? a.rstd[r] : 0.f;
+      const void* gate = gate_at(a, r, a.gate_f32 ? 4 : sizeof(T));
+      // eight normalised values k and what reaches the norm's output, d
+      const auto inputs = [&](const LongRow<T>& at, float k[8], float d[8]) {
+        at.rows_of(kBranch ? a.h : a.sum, kBranch ? a.h_stride : a.sum_stride, k);
+        for (int j = 0; j < 8; ++j) k[j] = (k[j] - mean) * rstd;
+        at.rows_of(kBranch ? a.gs : a.gy, kBranch ? a.gs_stride : a.gy_stride, d);
+        if (kBranch) {
+          float p[8];
+          if (a.rule.threshold) drop::apply8(key, at.mask(key), d);
+          at.param(gate, a.gate_f32, 1.f, p);
+          for (int j = 0; j < 8; ++j) d[j] *= p[j];
+        }
+      };
+      const auto put_gate = [&](const LongRow<T>& at, const float t[8]) {
+        if (grid.sums_gate) {
+          for (int j = 0; j < at.count; ++j) gate_part[at.c + j] = t[j] + (r == unit.begin ? 0.f : gate_part[at.c + j]);
+        } else if (a.gate_f32) {
+          lin::store_some(static_cast<float*>(a.dgate) + r * a.cols + at.c, at.count, false, t);
+        } else {
+          at.put(a.dgate, t);
+        }
+      };
+      Sums s = {0.f, 0.f};
+      if (normed) {
+        for (int64_t c = threadIdx.x * 8ll; c < a.cols; c += kLong * 8) {
+          const LongRow<T> at(a, r, c);
+          float k[8], d[8], w[8];
+          inputs(at, k, d);
+          at.param(a.w, a.weight_f32, 1.f, w);
+          for (int j = 0; j < at.count; ++j) {
+            if (a.dw || a.db) {
+              part[c + j] = fmaf(d[j], k[j], first ? 0.f : part[c + j]);
+              part[a.cols + c + j] = d[j] + (first ? 0.f : part[a.cols + c + j]);
+            }
+            s.a = fmaf(d[j], w[j], s.a);
+            s.b = fmaf(d[j] * w[j], k[j], s.b);
+          }
+        }
+        s = row_sums<kLong>(s, buf, turn);
+      }
+      const float c1 = a.rms ? 0.f : s.a / n, c2 = s.b / n;
+      for (int64_t c = threadIdx.x * 8ll; c < a.cols; c += kLong * 8) {
+        const LongRow<T> at(a, r, c);
+        float k[8] = {}, d[8] = {}, p[8], t[8];
+        if (normed) {
+          inputs(at, k, d);
+          at.param(a.w, a.weight_f32, 1.f, p);
+          if (kBranch && a.dgate) {
+            at.param(a.b, a.weight_f32, 0.f, t);
+            for (int j = 0; j < 8; ++j) t[j] = fmaf(k[j], p[j], t[j]);
+            if (a.rule.threshold) drop::apply8(key, at.mask(key), t);
+            float g[8];
+            at.rows_of(a.gs, a.gs_stride, g);
+            for (int j = 0; j < 8; ++j) t[j] *= g[j];
+            put_gate(at, t);
+          }
+          for (int j = 0; j < 8; ++j) d[j] = rstd * (d[j] * p[j] - c1 - k[j] * c2);
+        }
+        if (kBranch) {
+          if (a.dh) at.put(a.dh, d);
+          if (a.dr) {
+            at.rows_of(a.gs, a.gs_stride, t);
+            for (int j = 0; j < 8; ++j) t[j] *= a.alpha;
+            at.put(a.dr, t);
+          }
+          continue;
+        }
+        if (a.gs) {
+          at.rows_of(a.gs, a.gs_stride, t);
+          for (int j = 0; j < 8; ++j) d[j] += t[j];
+        }
+        if (a.dr) {
+          for (int j = 0; j < 8; ++j) t[j] = a.alpha * d[j];
+          at.put(a.dr, t);
+        }
+        if (a.dgate) {
+          at.rows_of(a.h, a.h_stride, t);
+          if (a.rule.threshold) drop::apply8(key, at.mask(key), t);
+          for (int j = 0; j < 8; ++j) t[j] *= d[j];
+          put_gate(at, t);
+        }
+        if (a.dh) {
+          if (a.rule.threshold) drop::apply8(key, at.mask(key), d);
+          at.param(gate, a.gate_f32, 1.f, p);
+          for (int j = 0; j < 8; ++j) d[j] *= p[j];
+          at.put(a.dh, d);
+        }
+      }
+    }
+  }
+}
+
+// ---- host --------------------------------------------------------------------------
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+bool vectors_fit(const Args& a) {
+  const auto rows_fit = [](const void* p, int64_t stride, size_t size) {
+    return !p || (aligned16(p) && (stride * size) % 16 == 0);
+  };
+  bool ok = a.cols % 8 == 0;
+  ok = ok && rows_fit(a.h, a.h_stride, sizeof(T)) && rows_fit(a.r, a.r_stride, sizeof(T));
+  ok = ok && rows_fit(a.gate, a.gate_stride, a.gate_f32 ? 4 : sizeof(T));
+  ok = ok && rows_fit(a.gy, a.gy_stride, sizeof(T)) && rows_fit(a.gs, a.gs_stride, sizeof(T));
+  ok = ok && rows_fit(a.sum, a.sum_stride, sizeof(T));
+  for (const void* p : {a.w, a.b, static_cast<const void*>(a.y), static_cast<const void*>(a.s),
+                        static_cast<const void*>(a.dh), static_cast<const void*>(a.dr),
+                        static_cast<const void*>(a.dgate)})
+    ok = ok && aligned16(p);
+  return ok;
+}
+
+template <int G, int NV, bool kVec, bool kBranch, typename T>
+cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
+  // as many blocks as are under way together
+  static const int per_sm = [] {
+    int n = 0;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, forward_kernel<G, NV, kVec, kBranch, T>,
+                                                         Shape<G>::kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
+  }();
+  const int64_t groups = (a.rows + Shape<G>::kRows - 1) / Shape<G>::kRows;
+  const int blocks = static_cast<int>(std::min<int64_t>(groups, 148ll * per_sm));
+  forward_kernel<G, NV, kVec, kBranch, T><<<blocks, Shape<G>::kThreads, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <bool kVec, bool kBranch, typename T>
+cudaError_t forward_form(const Args& a, cudaStream_t stream) {
+  if (a.cols <= 1024) {
+    if (kVec && a.cols <= 256) return launch_forward<32, kVec ? 1 : 4, kVec, kBranch, T>(a, stream);
+    if (kVec && a.cols <= 512) return launch_forward<32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
+    return launch_forward<32, 4, kVec, kBranch, T>(a, stream);
+  }
+  // few rows: short ones in time, not many in flight
+  if (a.cols <= 4096 && a.rows < 296) return launch_forward<512, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 4096) return launch_forward<256, 2, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 8192) return launch_forward<512, 2, kVec, kBranch, T>(a, stream);
+  const int blocks = static_cast<int>(std::min<int64_t>(a.rows, 148 * 2));
+  forward_long_kernel<kBranch, T><<<blocks, kLong, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t forward_of(const Args& a, cudaStream_t stream) {
+  if (vectors_fit<T>(a))
+    return a.branch ? forward_form<true, true, T>(a, stream) : forward_form<true, false, T>(a, stream);
+  return a.branch ? forward_form<false, true, T>(a, stream) : forward_form<false, false, T>(a, stream);
+}
+
+template <bool kVec, bool kBranch, bool kGate, typename T>
+cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) {
+  if (kVec && a.cols <= 256)
+    backward_kernel<32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+  else if (a.cols <= 512)
+    backward_kernel<32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+  else if (a.cols <= 2048)
+    backward_kernel<128, 2, kVec, kBranch, kGate, T><<<grid.blocks, 128, 0, stream>>>(a, grid);
+  else if (a.cols <= 4096)
+    backward_kernel<256, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+  else if (a.cols <= 8192)
+    backward_kernel<512, 2, kVec, kBranch, kGate, T><<<grid.blocks, 512, 0, stream>>>(a, grid);
+  else
+    backward_long_kernel<kBranch, T><<<grid.blocks, kLong, 0, stream>>>(a, grid);
+  return cudaGetLastError();
+}
+
+template <bool kVec, typename T>
+cudaError_t backward_kind(const Args& a, const Grid& grid, cudaStream_t stream) {
+  if (a.branch)
+    return a.dgate ? backward_form<kVec, true, true, T>(a, grid, stream)
+                   : backward_form<kVec, true, false, T>(a, grid, stream);
+  return a.dgate ? backward_form<kVec, false, true, T>(a, grid, stream)
+                 : backward_form<kVec, false, false, T>(a, grid, stream);
+}
+
+template <typename T>
+cudaError_t backward_of(const Args& a, const Grid& grid, cudaStream_t stream) {
+  return vectors_fit<T>(a) ? backward_kind<true, T>(a, grid, stream) : backward_kind<false, T>(a, grid, stream);
+}
+
+}  // namespace
+}  // namespace resnorm

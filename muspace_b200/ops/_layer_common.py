@@ -1,5 +1,5 @@
-"""What the layer operators (``linear_act``, ``layer_norm``, 8-bit checkpoints)
-share: storage types, rows of a tensor, dispatch reports."""
+"""What the layer operators (``linear_act``, ``layer_norm``, 8-bit checkpoints, dropout,
+norms with their residual) share: storage types, rows of a tensor, dispatch reports."""
 
 from __future__ import annotations
 
@@ -17,6 +17,7 @@ from ..runtime.kernel_dispatch import (
 from ..runtime.native import NativeModule, NativeModuleUnavailable, load_native_module
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1}  # msda_dtype_t
+WIDE_DTYPE_CODES = {**DTYPE_CODES, torch.float16: 2}  # of the operators that store float16 as it is
 STORAGE = (torch.float16, torch.bfloat16, torch.float32)
 CHECKPOINTS = (None, "int8")
 

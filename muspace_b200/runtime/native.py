@@ -171,6 +171,23 @@ class LayerNormArgs(ctypes.Structure):
     )
 
 
+class ResidualNormArgs(ctypes.Structure):
+    """``msda_residual_norm_t`` of include/muspace_msda.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("dtype", "weight_dtype", "gate_dtype", "kind")]
+        + [(name, ctypes.c_int64) for name in
+           ("rows", "cols", "gate_groups", "input_stride", "residual_stride", "gate_stride", "sum_stride",
+            "grad_output_stride", "grad_sum_stride")]
+        + [(name, ctypes.c_float) for name in ("residual_scale", "eps")]
+        + [(name, ctypes.c_int64) for name in ("threshold", "seed", "sequence")]
+        + [(name, ctypes.c_void_p) for name in
+           ("seed_at", "input", "residual", "gate", "weight", "bias", "output", "sum", "mean", "rstd", "grad_output",
+            "grad_sum", "grad_input", "grad_residual", "grad_weight", "grad_bias", "grad_gate", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+    )
+
+
 # the plain-pointer entry points of the layer operators: argument types before the stream
 _PLAIN_SIGNATURES: dict[str, tuple] = {
     "msda_linear_act_forward": (ctypes.POINTER(LinearArgs),),
@@ -179,6 +196,11 @@ _PLAIN_SIGNATURES: dict[str, tuple] = {
     "msda_layer_norm_backward": (ctypes.POINTER(LayerNormArgs),),
     "msda_checkpoint_pack": (ctypes.c_int, ctypes.c_void_p) + (ctypes.c_int64,) * 3 + (ctypes.c_void_p,) * 2,
     "msda_checkpoint_unpack": (ctypes.c_int,) + (ctypes.c_void_p,) * 2 + (ctypes.c_int64,) * 2 + (ctypes.c_void_p,),
+    "msda_dropout": (ctypes.c_int, ctypes.c_void_p) + (ctypes.c_int64,) * 6 + (ctypes.c_void_p,) * 2,
+    "msda_add_norm_forward": (ctypes.POINTER(ResidualNormArgs),),
+    "msda_add_norm_backward": (ctypes.POINTER(ResidualNormArgs),),
+    "msda_norm_add_forward": (ctypes.POINTER(ResidualNormArgs),),
+    "msda_norm_add_backward": (ctypes.POINTER(ResidualNormArgs),),
 }
 
 
@@ -195,7 +217,8 @@ def layer_wait_timeouts(device: torch.device | int | None = None) -> int:
 
 
 _WORKSPACE_CALLS = {"msda_linear_act_forward_workspace", "msda_linear_act_backward_workspace",
-                    "msda_layer_norm_backward_workspace"}
+                    "msda_layer_norm_backward_workspace", "msda_add_norm_backward_workspace",
+                    "msda_norm_add_backward_workspace"}
 
 
 class NativeModule:
