@@ -563,6 +563,41 @@ MSDA_API int msda_norm_add_forward(const msda_residual_norm_t *args, void *strea
 MSDA_API int msda_norm_add_backward_workspace(const msda_residual_norm_t *args, size_t *bytes);
 MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stream);
 
+/*
+ * The gated product y = D(act(x Wg^T + bg) * (x Wu^T + bu)) and its gradients, D being
+ * dropout as in msda_dropout, and Wg, bg the first out_features rows of weight and bias,
+ * Wu, bu the others. With factors P = D'(act'(zg) * zu) and Q = D'(act(zg)) (D' multiplies
+ * as D does), dz = [g * P, g * Q], dx = dz W, dW = dz^T x, db = sum of dz over rows.
+ *
+ *   input x  [rows, in_features]               weight W [2 out_features, in_features]
+ *   bias b   [2 out_features] or NULL          output y, grad_output g [rows, out_features]
+ *   factors  [rows, 2 out_features] contiguous, of dtype, P before Q: the forward writes
+ *            them where it is not NULL, the backward reads them
+ *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional;
+ *            bfloat16: dz is rounded to bfloat16 for dx and dW, not for db
+ *
+ * storage, products and workspace as with msda_linear_t; 2 out_features up to 2^31 - 1.
+ */
+typedef struct {
+  int32_t dtype;      /* msda_dtype_t */
+  int32_t activation; /* msda_activation_t */
+  int64_t rows, in_features, out_features;
+  int64_t input_stride, weight_stride, output_stride, grad_output_stride;
+  int64_t threshold, seed, sequence;
+  const int64_t *seed_at;
+  const void *input, *weight, *bias;
+  void *output, *factors;
+  const void *grad_output;
+  void *grad_input, *grad_weight, *grad_bias;
+  void *workspace;
+  size_t workspace_bytes;
+} msda_gated_linear_t;
+
+MSDA_API int msda_gated_linear_forward_workspace(const msda_gated_linear_t *args, size_t *bytes);
+MSDA_API int msda_gated_linear_forward(const msda_gated_linear_t *args, void *stream);
+MSDA_API int msda_gated_linear_backward_workspace(const msda_gated_linear_t *args, size_t *bytes);
+MSDA_API int msda_gated_linear_backward(const msda_gated_linear_t *args, void *stream);
+
 /* Waits inside the linear and layer-norm kernels that gave up on the current
  * device since the library loaded. 0 is expected; anything else means that a
  * call since then has left NaNs in the part of its results that depended on

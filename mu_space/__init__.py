@@ -25,6 +25,7 @@ _SUBMODULES = (
     "ops.checkpoint8",
     "ops.dropout",
     "ops.residual_norm",
+    "ops.gated_linear",
     "runtime",
     "runtime.kernel_dispatch",
     "runtime.native",

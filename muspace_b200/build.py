@@ -23,7 +23,7 @@ INCLUDE = PACKAGE.parent / "include"
 LIBRARY = PACKAGE / "native" / "libmuspace_ops.so"
 SOURCES = ("msda_capi.cpp", "msda_forward.cu", "msda_staged.cu", "msda_backward.cu", "msda_bucketed.cu", "msda_noalloc.cu",
            "msda_deterministic.cu", "deform_agg.cu", "flash_sca.cu", "layer_capi.cpp", "linear_act.cu", "linear_prep.cu",
-           "linear_gemm.cu", "linear_gemv.cu", "layer_norm.cu", "checkpoint8.cu",
+           "linear_gemm.cu", "linear_gemv.cu", "linear_gated.cu", "layer_norm.cu", "checkpoint8.cu",
            "dropout.cu", "residual_norm.cu", "residual_norm_f32.cu", "residual_norm_bf16.cu", "residual_norm_f16.cu")
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")
 

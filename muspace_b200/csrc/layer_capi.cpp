@@ -1,6 +1,6 @@
 // extern "C" boundary of the layer operators (declared in
-// include/muspace_msda.h): linear_act, layer norm, 8-bit checkpoints, dropout and the
-// norms with their residual.
+// include/muspace_msda.h): linear_act, layer norm, 8-bit checkpoints, dropout, the
+// norms with their residual and the gated product.
 #include <cuda_runtime.h>
 
 #include <limits>
@@ -204,6 +204,48 @@ resnorm::Args residual_norm_args(const msda_residual_norm_t* in, bool branch, bo
   return a;
 }
 
+lin::GatedArgs gated_args(const msda_gated_linear_t* in, bool backward) {
+  require(in != nullptr, "args is null");
+  check_dtype(in->dtype);
+  require(in->activation >= MSDA_ACTIVATION_NONE && in->activation <= MSDA_ACTIVATION_SILU,
+          "activation must be none, relu, gelu or silu");
+  check_size(in->rows, "rows");
+  check_size(in->in_features, "in_features");
+  check_size(in->out_features, "out_features");
+  require(2 * in->out_features <= kMax, "out_features exceeds the supported range (< 2^30)");
+  require(in->input_stride >= 0 && in->weight_stride >= 0 && in->output_stride >= 0 && in->grad_output_stride >= 0,
+          "strides must be non-negative");
+  const bool some_x = in->rows > 0 && in->in_features > 0, some_w = in->out_features > 0 && in->in_features > 0;
+  const bool some_y = in->rows > 0 && in->out_features > 0;
+  lin::GatedArgs a{};
+  a.dtype = static_cast<lin::DType>(in->dtype);
+  a.act = static_cast<lin::Act>(in->activation);
+  a.rows = in->rows, a.in = in->in_features, a.out = in->out_features;
+  a.x_stride = in->input_stride, a.w_stride = in->weight_stride;
+  a.y_stride = in->output_stride, a.g_stride = in->grad_output_stride;
+  a.factors = in->factors;
+  if (backward) {
+    check_pointer(some_w && in->grad_input, in->weight, "weight");
+    check_pointer(some_x && in->grad_weight, in->input, "input");
+    check_pointer(some_y, in->grad_output, "grad_output");
+    check_pointer(some_y, in->factors, "factors");
+    a.g = in->grad_output;
+    a.dx = in->grad_input, a.dw = in->grad_weight, a.db = in->grad_bias;
+  } else {
+    check_pointer(some_w, in->weight, "weight");
+    check_pointer(some_x, in->input, "input");
+    check_pointer(some_y, in->output, "output");
+    require(in->rows <= 1 || in->output_stride >= in->out_features, "output rows must not overlap");
+    a.rule = rule_of(in->threshold, in->seed, in->sequence, in->seed_at);
+    a.bias = in->bias;
+    a.y = in->output;
+  }
+  a.x = in->input, a.w = in->weight;
+  a.workspace = in->workspace;
+  a.workspace_bytes = in->workspace_bytes;
+  return a;
+}
+
 int residual_norm_forward(const msda_residual_norm_t* args, bool branch, const char* name, void* stream) {
   return guarded([&] {
     check_launch(resnorm::forward(residual_norm_args(args, branch, false), static_cast<cudaStream_t>(stream)), name);
@@ -248,6 +290,36 @@ int msda_dropout(msda_dtype_t dtype, const void* input, int64_t rows, int64_t co
     check_launch(drop::dropout(static_cast<drop::DType>(dtype), input, input_stride, rows, cols, rule, output,
                                static_cast<cudaStream_t>(stream)),
                  "msda_dropout");
+  });
+}
+
+int msda_gated_linear_forward_workspace(const msda_gated_linear_t* args, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "bytes is null");
+    *bytes = lin::gated_forward_workspace(gated_args(args, false));
+  });
+}
+
+int msda_gated_linear_forward(const msda_gated_linear_t* args, void* stream) {
+  return guarded([&] {
+    const lin::GatedArgs a = gated_args(args, false);
+    check_workspace(a.workspace, a.workspace_bytes, lin::gated_forward_workspace(a));
+    check_launch(lin::gated_forward(a, static_cast<cudaStream_t>(stream)), "msda_gated_linear_forward");
+  });
+}
+
+int msda_gated_linear_backward_workspace(const msda_gated_linear_t* args, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "bytes is null");
+    *bytes = lin::gated_backward_workspace(gated_args(args, true));
+  });
+}
+
+int msda_gated_linear_backward(const msda_gated_linear_t* args, void* stream) {
+  return guarded([&] {
+    const lin::GatedArgs a = gated_args(args, true);
+    check_workspace(a.workspace, a.workspace_bytes, lin::gated_backward_workspace(a));
+    check_launch(lin::gated_backward(a, static_cast<cudaStream_t>(stream)), "msda_gated_linear_backward");
   });
 }
 
@@ -341,10 +413,11 @@ int msda_linear_act_backward(const msda_linear_t* args, void* stream) {
 int msda_layer_wait_timeouts(unsigned int* count) {
   return guarded([&] {
     require(count != nullptr, "count is null");
-    unsigned int linear = 0, norm = 0;
+    unsigned int linear = 0, gated = 0, norm = 0;
     check_launch(lin::wait_timeouts(&linear), "msda_layer_wait_timeouts");
+    check_launch(lin::gated_wait_timeouts(&gated), "msda_layer_wait_timeouts");
     check_launch(lnorm::wait_timeouts(&norm), "msda_layer_wait_timeouts");
-    *count = linear + norm;
+    *count = linear + gated + norm;
   });
 }
 

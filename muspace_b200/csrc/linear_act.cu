@@ -1,5 +1,5 @@
-// The fused linear operator: lays its operands out where that is needed and
-// strings the products of linear_gemm.cu together.
+// The fused linear operators: lay their operands out where that is needed and
+// string the products of linear_gemm.cu and linear_gated.cu together.
 //
 // float32 runs on the same bfloat16 tensor-core product: every operand is
 // split into three bfloat16 planes (24 bits), and the six products of planes
@@ -12,6 +12,9 @@
 // x 256 x 512). db is added up before that rounding. Where the forward kept the
 // slope act'(z), dz is one elementwise pass; where it kept nothing (a checkpoint of
 // x in 8 bits), z is computed again and dz leaves that product's epilogue.
+//
+// The gated operator's backward is the same with dz = [g P, g Q], whose factors the
+// forward kept: one elementwise pass, then products over all 2 n rows of the weight.
 #include <algorithm>
 
 #include "checkpoint8.cuh"
@@ -103,6 +106,29 @@ cudaError_t forward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   return run_product(pr, arena, stream);
 }
 
+// dx = dz W and dW = dz^T x, each where it is asked for.
+cudaError_t products_of(DType dtype, int64_t rows, int64_t in, int64_t out, const Operand& dz, const Operand& w,
+                        const Operand& x, void* dx, void* dw, Arena& arena, cudaStream_t stream) {
+  if (dx && rows && in) {
+    Product pr;
+    pr.a = dz, pr.b = w, pr.b_mn = true;
+    pr.m = rows, pr.n = in, pr.k = out, pr.dtype = dtype;
+    pr.epi.out = dx;
+    pr.epi.out_ld = in;
+    LIN_TRY(run_product(pr, arena, stream));
+  }
+  if (dw && out && in) {
+    Product pr;
+    pr.a = dz, pr.a_mn = true;
+    pr.b = x, pr.b_mn = true;
+    pr.m = out, pr.n = in, pr.k = rows, pr.dtype = dtype;
+    pr.epi.out = dw;
+    pr.epi.out_ld = in;
+    LIN_TRY(run_product(pr, arena, stream));
+  }
+  return cudaSuccess;
+}
+
 cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
   const bool f32 = a.dtype == DType::kF32;
   const bool recompute = a.act != Act::kNone && a.slope == nullptr;
@@ -153,30 +179,48 @@ cudaError_t backward_in(const Args& a, Arena& arena, cudaStream_t stream) {
     }
   }
   if (need_b && !arena.measuring) LIN_TRY(add_parts(a.dtype, parts, parts_count, a.out, a.db, stream));
-  if (a.dx && a.rows && a.in) {
-    Product pr;
-    pr.a = dz, pr.b = w, pr.b_mn = true;
-    pr.m = a.rows, pr.n = a.in, pr.k = a.out, pr.dtype = a.dtype;
-    pr.epi.out = a.dx;
-    pr.epi.out_ld = a.in;
-    LIN_TRY(run_product(pr, arena, stream));
-  }
-  if (a.dw && a.out && a.in) {
-    Product pr;
-    pr.a = dz, pr.a_mn = true;
-    pr.b = x, pr.b_mn = true;
-    pr.m = a.out, pr.n = a.in, pr.k = a.rows, pr.dtype = a.dtype;
-    pr.epi.out = a.dw;
-    pr.epi.out_ld = a.in;
-    LIN_TRY(run_product(pr, arena, stream));
-  }
-  return cudaSuccess;
+  return products_of(a.dtype, a.rows, a.in, a.out, dz, w, x, a.dx, a.dw, arena, stream);
 }
 
-Arena arena_of(const Args& a) {
+cudaError_t gated_forward_in(const GatedArgs& a, Arena& arena, cudaStream_t stream) {
+  if (a.rows == 0 || a.out == 0) return cudaSuccess;
+  if (gated_few_rows(a)) return arena.measuring ? cudaSuccess : gated_forward_few_rows(a, stream);
+  Product pr;
+  LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &pr.a, stream));
+  LIN_TRY(operand_of(a.dtype, a.w, 2 * a.out, a.in, a.w_stride, arena, &pr.b, stream));
+  pr.m = a.rows, pr.n = a.out, pr.k = a.in, pr.dtype = a.dtype;
+  pr.epi.act = a.act;
+  pr.epi.bias = a.bias;
+  pr.epi.out = a.y;
+  pr.epi.out_ld = a.y_stride;
+  pr.epi.slope = a.factors;
+  pr.epi.rule = a.rule;
+  const Plan plan = plan_product(pr.dtype, pr.m, 2 * pr.n, pr.k, plane_pairs(pr.a, pr.b), multiprocessors());
+  if (gated_apart(pr, plan)) pr.partial = static_cast<float*>(arena.take(partial_bytes(plan, pr.m, 2 * pr.n)));
+  return arena.measuring ? cudaSuccess : launch_gated(pr, plan, stream);
+}
+
+cudaError_t gated_backward_in(const GatedArgs& a, Arena& arena, cudaStream_t stream) {
+  const int64_t both = 2 * a.out;
+  Operand x, w, dz;
+  if (a.dx) LIN_TRY(operand_of(a.dtype, a.w, both, a.in, a.w_stride, arena, &w, stream));
+  if (a.dw) LIN_TRY(operand_of(a.dtype, a.x, a.rows, a.in, a.x_stride, arena, &x, stream));
+  const bool need_b = a.db != nullptr && a.out > 0;
+  const int64_t parts_count = a.rows == 0 ? 0 : column_parts(a.rows, a.out);
+  float* parts = nullptr;
+  if (need_b) parts = static_cast<float*>(arena.take(static_cast<size_t>(parts_count) * both * sizeof(float)));
+  dz = fresh(a.dtype, a.rows, both, a.dtype == DType::kF32 ? 3 : 1, arena);
+  if (!arena.measuring) {
+    LIN_TRY(gate_operand(a.dtype, a.g, a.g_stride, a.factors, dz, parts, stream));
+    if (need_b) LIN_TRY(add_parts(a.dtype, parts, parts_count, both, a.db, stream));
+  }
+  return products_of(a.dtype, a.rows, a.in, both, dz, w, x, a.dx, a.dw, arena, stream);
+}
+
+Arena arena_of(void* workspace, size_t bytes) {
   Arena arena;
-  arena.base = static_cast<char*>(a.workspace);
-  arena.size = a.workspace_bytes;
+  arena.base = static_cast<char*>(workspace);
+  arena.size = bytes;
   arena.measuring = false;
   return arena;
 }
@@ -196,13 +240,35 @@ size_t backward_workspace(const Args& a) {
 }
 
 cudaError_t forward(const Args& a, cudaStream_t stream) {
-  Arena arena = arena_of(a);
+  Arena arena = arena_of(a.workspace, a.workspace_bytes);
   return forward_in(a, arena, stream);
 }
 
 cudaError_t backward(const Args& a, cudaStream_t stream) {
-  Arena arena = arena_of(a);
+  Arena arena = arena_of(a.workspace, a.workspace_bytes);
   return backward_in(a, arena, stream);
+}
+
+size_t gated_forward_workspace(const GatedArgs& a) {
+  Arena arena;
+  (void)gated_forward_in(a, arena, nullptr);
+  return arena.used;
+}
+
+size_t gated_backward_workspace(const GatedArgs& a) {
+  Arena arena;
+  (void)gated_backward_in(a, arena, nullptr);
+  return arena.used;
+}
+
+cudaError_t gated_forward(const GatedArgs& a, cudaStream_t stream) {
+  Arena arena = arena_of(a.workspace, a.workspace_bytes);
+  return gated_forward_in(a, arena, stream);
+}
+
+cudaError_t gated_backward(const GatedArgs& a, cudaStream_t stream) {
+  Arena arena = arena_of(a.workspace, a.workspace_bytes);
+  return gated_backward_in(a, arena, stream);
 }
 
 }  // namespace lin

@@ -1,8 +1,13 @@
 // Host-side interface of the fused linear kernels: linear_gemm.cu (tensor-core
-// product), linear_prep.cu (operand layouts) and linear_act.cu (the operator).
+// product), linear_gated.cu (the gated one), linear_prep.cu (operand layouts) and
+// linear_act.cu (the operators).
 //
 //   forward   z = x W^T + b,  y = act(z) + r
 //   backward  dz = g * act'(z),  dx = dz W,  dW = dz^T x,  db = sum over rows of dz
+//
+//   gated: W [2 n, k] and b [2 n], the gate's rows above up's
+//   forward   z = x W^T + b,  y = D(act(z_gate) * z_up)
+//   backward  dz = [g * P, g * Q], P = D'(act'(z_gate) * z_up), Q = D'(act(z_gate)), and dx, dW, db as above
 //
 // x [rows, in], W [out, in], y / r / g [rows, out]; rows may be apart
 // (a row stride in elements), elements of a row are adjacent.
@@ -12,6 +17,8 @@
 #include <cuda_runtime.h>
 #include <stddef.h>
 #include <stdint.h>
+
+#include "dropout.h"
 
 namespace lin {
 
@@ -40,6 +47,31 @@ struct Args {
   void* workspace;
   size_t workspace_bytes;
 };
+
+// The gated operator: out is n, the weight and the bias have 2 n rows, act is the
+// gate's, dropout the rule's.
+struct GatedArgs {
+  DType dtype;
+  Act act;
+  int64_t rows, in, out;
+  int64_t x_stride, w_stride, y_stride, g_stride;
+  drop::Rule rule;     // forward
+  const void* x;       // forward; backward with dw
+  const void* w;       // forward; backward with dx
+  const void* bias;    // forward, may be null
+  void* y;             // forward
+  void* factors;       // [rows, 2 out] contiguous, P and Q; forward: may be null
+  const void* g;       // backward
+  void* dx;            // [rows, in] contiguous, may be null
+  void* dw;            // [2 out, in] contiguous, may be null
+  void* db;            // [2 out], may be null
+  void* workspace;
+  size_t workspace_bytes;
+};
+size_t gated_forward_workspace(const GatedArgs& a);
+size_t gated_backward_workspace(const GatedArgs& a);
+cudaError_t gated_forward(const GatedArgs& a, cudaStream_t stream);
+cudaError_t gated_backward(const GatedArgs& a, cudaStream_t stream);
 
 // Bytes of workspace that forward / backward need for these arguments (the
 // pointers' alignment counts, their contents do not); 0 for many calls.
@@ -77,6 +109,7 @@ struct Epilogue {
   void* slope = nullptr;  // kFwd, [m, n] contiguous
   int64_t out_plane = 0;  // kDz, float32: out is three bfloat16 planes, out_plane elements apart
   float* sums = nullptr;  // kDz, may be null: [ceil(m / 32), n], the columns' sums over 32 rows
+  drop::Rule rule;         // gated
   float* unrounded = nullptr;  // finished apart with sums: where out is left in float32 for them, rows of partial_ld(n)
 };
 
@@ -112,6 +145,16 @@ inline size_t partial_bytes(const Plan& p, int64_t m, int64_t n) {
 }
 cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t stream);
 cudaError_t wait_timeouts(unsigned int* count);
+// The first part of a product that is finished apart: its sums in pr.partial.
+cudaError_t launch_sums(const Product& pr, const Plan& plan, cudaStream_t stream);
+
+// ---- the gated product (linear_gated.cu) -------------------------------------------
+
+// pr.n columns of the output, from b's rows n and pr.n + n; epi: act, bias, out, rule,
+// and in `slope` the factors or null. The plan is that of a product of 2 pr.n columns.
+bool gated_apart(const Product& pr, const Plan& plan);
+cudaError_t launch_gated(const Product& pr, const Plan& plan, cudaStream_t stream);
+cudaError_t gated_wait_timeouts(unsigned int* count);
 
 // ---- operand layouts and column sums (linear_prep.cu) ------------------------------
 
@@ -124,6 +167,10 @@ cudaError_t scale_operand(DType dtype, const void* g, int64_t g_ld, const void* 
 // ranges of rows on the way: parts [column_parts(rows, cols), cols].
 cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const void* slope, const Operand& dst,
                              float* parts, cudaStream_t stream);
+// dst [rows, 2 n] = [g * P, g * Q] of the factors [rows, 2 n], with the sums of its columns
+// on the way where parts is not null: parts [column_parts(rows, n), 2 n].
+cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const Operand& dst,
+                         float* parts, cudaStream_t stream);
 cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream);
 // The sums of src's columns over ranges of rows; and of parts [count, cols], in order.
 int column_parts(int64_t rows, int64_t cols);
@@ -135,5 +182,7 @@ cudaError_t add_parts(DType out_dtype, const float* parts, int64_t count, int64_
 
 bool few_rows(const Args& a);
 cudaError_t forward_few_rows(const Args& a, cudaStream_t stream);
+bool gated_few_rows(const GatedArgs& a);
+cudaError_t gated_forward_few_rows(const GatedArgs& a, cudaStream_t stream);
 
 }  // namespace lin

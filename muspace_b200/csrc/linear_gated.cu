@@ -1,0 +1,360 @@
+// The gated product: z = x W^T + b with W's rows [0, n) the gate's and [n, 2 n) up's,
+// and of every pair of neighbours in it, y = D(act(z_gate) * z_up), in one kernel.
+//
+// A tile's columns are a range of the gate's and, behind them, the same range of up's:
+// one tcgen05.mma multiplies both, and the lane that holds a row's gate sums in tensor
+// memory holds its up sums too, BN / 2 columns on. In a pair of SMs each copies the
+// half of the weight's rows that it would anyway: the first the gate's, the second
+// up's. So the product is that of linear_gemm.cu, and nothing of size rows x 2 n is
+// written in inference. For training the epilogue also writes the factors P = D'(act'(z_gate)
+// z_up) and Q = D'(act(z_gate)) (D' multiplies as D does), by which a gradient of y becomes
+// those of the gate's and of up's columns: the backward pass needs no generator, no
+// exponential and no product for them.
+#include <algorithm>
+
+#include "dropout_device.cuh"
+#include "linear_tile.cuh"
+
+namespace lin {
+namespace {
+
+// 16 columns of a warp's rows, gate and up, without waiting for them.
+__device__ __forceinline__ void take_both(uint32_t gate_at, uint32_t up_at, float g[16], float u[16]) {
+  uint32_t a[16], b[16];
+  tmem_load16(gate_at, a);
+  tmem_load16(up_at, b);
+  tmem_wait(a);
+  tmem_wait(b);
+#pragma unroll
+  for (int j = 0; j < 16; ++j) g[j] = __uint_as_float(a[j]), u[j] = __uint_as_float(b[j]);
+}
+
+// Of N values (whole eights) gate sums g and up sums u, both with their bias: the
+// output in g, and with kTrain P in s and Q in u.
+template <bool kFast, bool kTrain, int N>
+__device__ __forceinline__ void gate_values(Act act, const drop::Rule& rule, const drop::Key& key, uint32_t row,
+                                            uint32_t group, float* g, float* u, float* s) {
+  activate<kFast, true, kTrain, N>(act, g, s);
+  if (rule.threshold) {
+#pragma unroll
+    for (int h = 0; h < N / 8; ++h) {
+      const drop::Words words = drop::numbers(key, row, group + h);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool kept = drop::kept(key, words, j);
+        g[8 * h + j] = kept ? g[8 * h + j] : 0.f;
+        u[8 * h + j] = kept ? u[8 * h + j] * rule.scale : 0.f;
+        if (kTrain) s[8 * h + j] = kept ? s[8 * h + j] : 0.f;
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float y = g[j] * u[j];
+    if (kTrain) s[j] *= u[j], u[j] = g[j] * rule.scale;
+    g[j] = y;
+  }
+}
+
+// kKind: the activation, twice, and one more in training.
+template <int BN, int CG, typename T, bool kF32, int kKind>
+__device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, const Place place) {
+  using S = Shape<BN, CG, kF32, true>;
+  constexpr Act kAct = static_cast<Act>(kKind / 2);
+  constexpr bool kTrain = kKind % 2, kFast = sizeof(T) == 2;
+  constexpr int kOut = S::kCols / 2;  // columns of the output that a warp takes
+  constexpr int kRowBytes = kOut * sizeof(T), kPart = 32 * kRowBytes;
+  static_assert(kRowBytes == 32 || kRowBytes == 64, "three boxes to a warp");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t tmem = place.tmem, rank = place.rank;
+  const auto acc_full = [&](int b) { return place.bars + 8 * (2 * S::kStages + b); };
+  const auto acc_empty = [&](int b) { return place.bars + 8 * (2 * S::kStages + 2 + b); };
+  const auto small_empty = [&](int b) { return place.bars + 8 * (2 * S::kStages + 4 + kEpiWarps + b); };
+  const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
+  const uint32_t first = blockIdx.x / CG, step = gridDim.x / CG;
+  const int chunk = kF32 ? kPromote : job.kblocks;
+  const int quad = warp & 3, group = warp >> 2;
+  const uint32_t box = place.boxes + warp * S::kBox;
+  const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
+  const int rows_m = static_cast<int>(job.pr.m), rows_n = static_cast<int>(job.pr.n);
+  const Epilogue& e = job.pr.epi;
+  const T* bias_gate = static_cast<const T*>(e.bias);
+  const T* bias_up = bias_gate + rows_n;
+  const bool with_bias = bias_gate != nullptr;
+  const bool bias_vec = reinterpret_cast<uintptr_t>(bias_gate) % 16 == 0 && rows_n * sizeof(T) % 16 == 0;
+  const drop::Key key = drop::key_of(e.rule);
+  // the warp's q-th sixteen columns of an accumulator: first the gate's, then up's
+  const auto sixteen = [&](int q) {
+    return q < kOut / 16 ? group * kOut + q * 16 : BN / 2 + group * kOut + (q - kOut / 16) * 16;
+  };
+  bool dead = false;
+  int buf = 0, small = 0, part = 0;
+  uint32_t acc_phase = 0;
+  for (uint32_t i = first; i < items; i += step) {
+    const Item t = item_of<S::kTileN, CG>(job, i);
+    const int m = t.m + static_cast<int>(rank) * kTileM + quad * 32, n0 = t.n + group * kOut;
+    uint32_t acc_at = tmem + lanes + buf * BN;
+    if (kF32) {  // as in linear_gemm.cu's epilogue
+      float acc[S::kCols / 16][16] = {};
+      for (int c = t.kb0, n = 1; c < t.kb1; c += chunk, ++n) {
+        wait(acc_full(buf), acc_phase, dead);
+        fence_after();
+        const bool last = c + chunk >= t.kb1, fold = last || n % kFold == 0;
+        const uint32_t main_at = tmem + lanes + buf * BN;
+        acc_at = tmem + lanes + S::kSmall + small * BN;
+#pragma unroll
+        for (int q = 0; q < S::kCols / 16; ++q) {
+          uint32_t r[16];
+          tmem_load16(main_at + sixteen(q), r);
+          tmem_wait(r);
+#pragma unroll
+          for (int x = 0; x < 16; ++x) acc[q][x] += __uint_as_float(r[x]);
+        }
+        if (fold) {
+#pragma unroll
+          for (int q = 0; q < S::kCols / 16; ++q) {
+            uint32_t r[16];
+            tmem_load16(acc_at + sixteen(q), r);
+            tmem_wait(r);
+#pragma unroll
+            for (int x = 0; x < 16; ++x) acc[q][x] += finite_or_zero(__uint_as_float(r[x]));
+            if (last) tmem_store16(acc_at + sixteen(q), acc[q]);  // the tile waits there for its epilogue
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          arrive_in(in_block(acc_empty(buf), 0));
+          if (fold && !last) arrive_in(in_block(small_empty(small), 0));
+        }
+        if (fold && !last) small ^= 1;
+        buf ^= 1;
+        if (buf == 0) acc_phase ^= 1;
+      }
+      tmem_stored();
+    } else {
+      wait(acc_full(buf), acc_phase, dead);
+      fence_after();
+    }
+    // training: the three boxes at once; inference: one after the other, two on their way out meanwhile
+    if (lane == 0) stores_read<kTrain ? 0 : 2>();
+    __syncwarp();
+    const uint32_t out = kTrain ? box : box + part * kPart;
+#pragma unroll 1
+    for (int c = 0; c < kOut; c += 16) {
+      float g[16], u[16], s[16];
+      Bias16<T> bias, more;
+      if (with_bias) {
+        bias.load(bias_gate + n0 + c, bias_vec, rows_n - n0 - c);
+        more.load(bias_up + n0 + c, bias_vec, rows_n - n0 - c);
+      }
+      take_both(acc_at + group * kOut + c, acc_at + BN / 2 + group * kOut + c, g, u);
+      if (with_bias) bias.add(g), more.add(u);
+      gate_values<kFast, kTrain, 16>(kAct, e.rule, key, m + lane, (n0 + c) / 8, g, u, s);
+      put16<kRowBytes>(out, lane, c, g, T());
+      if (kTrain) {
+        put16<kRowBytes>(box + kPart, lane, c, s, T());
+        put16<kRowBytes>(box + 2 * kPart, lane, c, u, T());
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    fence_before();
+    __syncwarp();
+    if (lane == 0) {
+      if (m < rows_m && n0 < rows_n) {
+        store_box(&maps.out, n0, m, 0, out);
+        if (kTrain) {
+          store_box(&maps.extra, n0, m, 0, box + kPart);
+          store_box(&maps.slope, n0, m, 0, box + 2 * kPart);
+        }
+      }
+      stores_commit();
+      arrive_in(in_block(kF32 ? small_empty(small) : acc_empty(buf), 0));
+    }
+    if (kF32) {
+      small ^= 1;
+    } else {
+      buf ^= 1;
+      if (buf == 0) acc_phase ^= 1;
+    }
+    if (++part == 3) part = 0;
+  }
+  if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  return dead;
+}
+
+struct GatedEpilogue {
+  static constexpr bool kGated = true;
+
+  template <int BN, int CG, typename T, bool kF32>
+  static __device__ __forceinline__ bool run(const Maps& maps, const Job& job, const Place place) {
+    const Epilogue& e = job.pr.epi;
+    switch (static_cast<int>(e.act) * 2 + (e.slope ? 1 : 0)) {
+      case 0: return gated_epilogue<BN, CG, T, kF32, 0>(maps, job, place);
+      case 1: return gated_epilogue<BN, CG, T, kF32, 1>(maps, job, place);
+      case 2: return gated_epilogue<BN, CG, T, kF32, 2>(maps, job, place);
+      case 3: return gated_epilogue<BN, CG, T, kF32, 3>(maps, job, place);
+      case 4: return gated_epilogue<BN, CG, T, kF32, 4>(maps, job, place);
+      case 5: return gated_epilogue<BN, CG, T, kF32, 5>(maps, job, place);
+      case 6: return gated_epilogue<BN, CG, T, kF32, 6>(maps, job, place);
+      default: return gated_epilogue<BN, CG, T, kF32, 7>(maps, job, place);
+    }
+  }
+
+  template <int BN, int CG, typename T, bool kF32>
+  static __device__ __noinline__ void spoil(const Maps& maps, const Job& job, const Place place) {
+    using S = Shape<BN, CG, kF32, true>;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t box = place.boxes + warp * S::kBox;
+    for (int unit = lane; unit < S::kBox / 16; unit += 32) put_unit(box + unit * 16, ~0u, ~0u, ~0u, ~0u);
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if (lane != 0) return;
+    const uint32_t items = job.tiles_m * job.tiles_n * job.splits;
+    for (uint32_t i = blockIdx.x / CG; i < items; i += gridDim.x / CG) {
+      const Item t = item_of<S::kTileN, CG>(job, i);
+      const int m = t.m + static_cast<int>(place.rank) * kTileM + (warp & 3) * 32, n = t.n + (warp >> 2) * (S::kCols / 2);
+      if (m >= job.pr.m || n >= job.pr.n) continue;
+      store_box(&maps.out, n, m, 0, box);
+      if (job.pr.epi.slope) {
+        store_box(&maps.extra, n, m, 0, box);
+        store_box(&maps.slope, n, m, 0, box);
+      }
+    }
+    stores_commit();
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+};
+
+// The same from sums that were finished apart, [splits, m, partial_ld(2 n)]: eight
+// columns to kLanes lanes, which take the ranges of k in turn, in a fixed order.
+template <typename T, int kLanes>
+__global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant__ Job job) {
+  const Product& pr = job.pr;
+  const Epilogue& e = pr.epi;
+  const int64_t per_row = (pr.n + 7) / 8, total = pr.m * per_row, ld = partial_ld(2 * pr.n);
+  const int sub = threadIdx.x % kLanes;
+  const bool up_vec = pr.n % 4 == 0;
+  const drop::Key key = drop::key_of(e.rule);
+  for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) / kLanes; i - threadIdx.x % 32 / kLanes < total;
+       i += gridDim.x * 256ll / kLanes) {
+    const bool some = i < total;
+    const int64_t m = some ? i / per_row : 0, n = some ? (i - m * per_row) * 8 : 0;
+    const int count = static_cast<int>(pr.n - n < 8 ? pr.n - n : 8);
+    float g[8] = {}, u[8] = {}, s[8];
+    if (some) {
+      const float* p = pr.partial + m * ld + n;  // rows are padded to eight
+#pragma unroll 2
+      for (int split = sub; split < job.splits; split += kLanes) {
+        float w[8], x[8];
+        load8(p + split * pr.m * ld, w);
+        load_some(p + split * pr.m * ld + pr.n, count, up_vec && count == 8, x);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) g[j] += w[j], u[j] += x[j];
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < kLanes; d <<= 1)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        g[j] += __shfl_xor_sync(0xffffffffu, g[j], d);
+        u[j] += __shfl_xor_sync(0xffffffffu, u[j], d);
+      }
+    if (!some || sub != 0) continue;
+    const bool vec = job.vec && count == 8;
+    if (e.bias) {
+      float b[8];
+      load_some(static_cast<const T*>(e.bias) + n, count, false, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] += b[j];
+      load_some(static_cast<const T*>(e.bias) + pr.n + n, count, false, b);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[j] += b[j];
+    }
+    gate_values<sizeof(T) == 2, true, 8>(e.act, e.rule, key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8), g, u,
+                                         s);
+    store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, g);
+    if (e.slope) {
+      T* factors = static_cast<T*>(e.slope) + m * 2 * pr.n + n;
+      store_some(factors, count, vec, s);
+      store_some(factors + pr.n, count, vec, u);
+    }
+  }
+}
+
+// Whether rows of out and of both halves of the factors are what TMA and vectors of eight columns can address.
+bool gated_fits(const Product& pr) {
+  const Epilogue& e = pr.epi;
+  const int64_t size = pr.dtype == DType::kF32 ? 4 : 2;
+  bool ok = aligned16(e.out) && (e.out_ld * size) % 16 == 0;
+  if (e.slope) ok = ok && aligned16(e.slope) && (pr.n * size) % 16 == 0;
+  return ok;
+}
+
+template <typename T, bool kF32>
+cudaError_t launch_gated_tile(const Plan& plan, const Maps& maps, const Job& job, int sms, cudaStream_t stream) {
+  if constexpr (kF32) {
+    if (plan.bn == 128) return launch<128, 2, T, kF32, GatedEpilogue>(maps, job, sms, stream);
+  } else {
+    if (plan.bn == 256)
+      return plan.pair == 2 ? launch<256, 2, T, kF32, GatedEpilogue>(maps, job, sms, stream)
+                            : launch<256, 1, T, kF32, GatedEpilogue>(maps, job, sms, stream);
+    if (plan.bn == 128) return launch<128, 1, T, kF32, GatedEpilogue>(maps, job, sms, stream);
+  }
+  return launch<64, 1, T, kF32, GatedEpilogue>(maps, job, sms, stream);
+}
+
+}  // namespace
+
+bool gated_apart(const Product& pr, const Plan& plan) { return plan.splits > 1 || pr.k == 0 || !gated_fits(pr); }
+
+cudaError_t launch_gated(const Product& pr, const Plan& plan, cudaStream_t stream) {
+  if (pr.m == 0 || pr.n == 0) return cudaSuccess;
+  const bool f32 = pr.dtype == DType::kF32;
+  Job job{};
+  job.pr = pr;
+  job.vec = gated_fits(pr);
+  job.splits = plan.splits;
+  if (!gated_apart(pr, plan)) {
+    int sms = 148;
+    const cudaError_t err = prepare(job, plan, plan.bn / 2, &sms);
+    if (err != cudaSuccess) return err;
+    job.box_a = static_cast<int>(std::min<int64_t>(kTileM, ceil_div(pr.m, 8) * 8));
+    job.box_b = static_cast<int>(std::min<int64_t>(plan.bn / 2, ceil_div(pr.n, 8) * 8));
+    const Epilogue& e = pr.epi;
+    const auto type = f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const int64_t size = f32 ? 4 : 2;
+    const int cols = std::max(32, plan.bn / 4) / 2, row_bytes = cols * static_cast<int>(size);
+    Maps maps{};
+    bool ok = operand_map(&maps.a, pr.a, job.box_a) && operand_map(&maps.b, pr.b, job.box_b) &&
+              make_map(&maps.out, type, e.out, pr.n, pr.m, 1, e.out_ld * size, 0, cols, 32, row_bytes);
+    if (e.slope)
+      ok = ok &&
+           make_map(&maps.extra, type, e.slope, pr.n, pr.m, 1, 2 * pr.n * size, 0, cols, 32, row_bytes) &&
+           make_map(&maps.slope, type, static_cast<char*>(e.slope) + pr.n * size, pr.n, pr.m, 1, 2 * pr.n * size, 0, cols,
+                    32, row_bytes);
+    if (!ok) return cudaErrorInvalidValue;
+    return f32 ? launch_gated_tile<float, true>(plan, maps, job, sms, stream)
+               : launch_gated_tile<bf16, false>(plan, maps, job, sms, stream);
+  }
+  if (pr.k > 0) {
+    Product sums = pr;
+    sums.n = 2 * pr.n;
+    const cudaError_t err = launch_sums(sums, plan, stream);
+    if (err != cudaSuccess) return err;
+  } else {
+    job.splits = 0;  // an empty sum
+  }
+  const int64_t groups = pr.m * ((pr.n + 7) / 8);
+  const bool spread = job.splits >= 8;
+  const int blocks = static_cast<int>(std::min<int64_t>((groups * (spread ? 8 : 1) + 255) / 256, 148 * 8));
+  if (f32)
+    (spread ? gated_finish_kernel<float, 8> : gated_finish_kernel<float, 1>)<<<blocks, 256, 0, stream>>>(job);
+  else
+    (spread ? gated_finish_kernel<bf16, 8> : gated_finish_kernel<bf16, 1>)<<<blocks, 256, 0, stream>>>(job);
+  return cudaGetLastError();
+}
+
+cudaError_t gated_wait_timeouts(unsigned int* count) { return async::read_timeouts(count); }
+
+}  // namespace lin

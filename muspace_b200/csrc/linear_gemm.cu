@@ -530,6 +530,35 @@ Plan plan_product(DType dtype, int64_t m, int64_t n, int64_t k, int pairs, int s
 
 bool finished_apart(const Product& pr, const Plan& plan) { return plan.splits > 1 || pr.k == 0 || !vectors_fit(pr); }
 
+namespace {
+
+cudaError_t launch_tiles(Job& job, const Plan& plan, cudaStream_t stream) {
+  const Product& pr = job.pr;
+  int sms = 148;
+  const cudaError_t err = prepare(job, plan, plan.bn, &sms);
+  if (err != cudaSuccess) return err;
+  const int64_t rows_b = plan.bn / plan.pair;
+  job.box_a = pr.a_mn ? 64 : static_cast<int>(std::min<int64_t>(kTileM, ceil_div(pr.m, 8) * 8));
+  job.box_b = pr.b_mn ? 64 : static_cast<int>(std::min<int64_t>(rows_b, ceil_div(pr.n, 8) * 8));
+  Maps maps{};
+  if (!operand_map(&maps.a, pr.a, job.box_a) || !operand_map(&maps.b, pr.b, job.box_b) ||
+      !epilogue_maps(maps, pr, plan, job.apart))
+    return cudaErrorInvalidValue;
+  if (pr.dtype == DType::kF32) return launch_tile<float, true>(plan, maps, job, sms, stream);
+  return job.apart ? launch_tile<float, false>(plan, maps, job, sms, stream)
+                   : launch_tile<bf16, false>(plan, maps, job, sms, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_sums(const Product& pr, const Plan& plan, cudaStream_t stream) {
+  Job job{};
+  job.pr = pr;
+  job.splits = plan.splits;
+  job.apart = true;
+  return launch_tiles(job, plan, stream);
+}
+
 cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t stream) {
   if (pr.m == 0 || pr.n == 0) return cudaSuccess;
   Job job{};
@@ -538,23 +567,8 @@ cudaError_t launch_product(const Product& pr, const Plan& plan, cudaStream_t str
   job.splits = plan.splits;
   const bool f32 = pr.dtype == DType::kF32;
   if (pr.k > 0) {
-    int sms = 148;
-    cudaError_t err = prepare(job, plan, plan.bn, &sms);
-    if (err != cudaSuccess) return err;
     job.apart = finished_apart(pr, plan);
-    const int64_t rows_b = plan.bn / plan.pair;
-    job.box_a = pr.a_mn ? 64 : static_cast<int>(std::min<int64_t>(kTileM, ceil_div(pr.m, 8) * 8));
-    job.box_b = pr.b_mn ? 64 : static_cast<int>(std::min<int64_t>(rows_b, ceil_div(pr.n, 8) * 8));
-    Maps maps{};
-    if (!operand_map(&maps.a, pr.a, job.box_a) || !operand_map(&maps.b, pr.b, job.box_b) ||
-        !epilogue_maps(maps, pr, plan, job.apart))
-      return cudaErrorInvalidValue;
-    if (f32)
-      err = launch_tile<float, true>(plan, maps, job, sms, stream);
-    else if (job.apart)
-      err = launch_tile<float, false>(plan, maps, job, sms, stream);
-    else
-      err = launch_tile<bf16, false>(plan, maps, job, sms, stream);
+    const cudaError_t err = launch_tiles(job, plan, stream);
     if (err != cudaSuccess || !job.apart) return err;
   } else {
     job.splits = 0;  // an empty sum

@@ -6,6 +6,7 @@
 // float32 first lays the weight out in planes. 1 x 4096 x 4096 in bfloat16: 8.2
 // us, 4.1 TB/s; see few_rows for where the one or the other is the faster.
 
+#include "dropout_device.cuh"
 #include "linear_device.cuh"
 
 namespace lin {
@@ -25,33 +26,78 @@ __device__ __forceinline__ void load_vec<float>(const float* p, float v[4]) {
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
 }
 
-// kRows rows of x (from blockIdx.y * kRows on) against kCols rows of the weight,
-// whose columns `split` neighbouring warps share: few rows of a long weight are
-// work for many warps, and their sums are added in order.
-template <typename T, int kRows, int kCols, int kUnroll, int split, bool kVec>
-__global__ void __launch_bounds__(32 * kWarps) gemv_kernel(const Args a) {
+// What becomes of a sum of the plain operator, and of the two of the gated one.
+template <typename T>
+__device__ __forceinline__ void finish(const Args& a, int64_t m, int64_t n, const float sums[1]) {
+  float z[2] = {sums[0], 0.f}, s[2];
+  if (a.bias) z[0] += to_float(static_cast<const T*>(a.bias)[n]);
+  activate<sizeof(T) == 2, true, true, 2>(a.act, z, s);
+  if (a.slope)
+    static_cast<typename SlopeOf<T>::type*>(a.slope)[m * a.out + n] = from_float<typename SlopeOf<T>::type>(s[0]);
+  if (a.r) z[0] += to_float(static_cast<const T*>(a.r)[m * a.r_stride + n]);
+  static_cast<T*>(a.y)[m * a.y_stride + n] = from_float<T>(z[0]);
+}
+template <typename T>
+__device__ __forceinline__ void finish(const GatedArgs& a, int64_t m, int64_t n, const float sums[2]) {
+  float g[2] = {sums[0], 0.f}, s[2], u = sums[1];
+  if (a.bias) {
+    g[0] += to_float(static_cast<const T*>(a.bias)[n]);
+    u += to_float(static_cast<const T*>(a.bias)[a.out + n]);
+  }
+  activate<sizeof(T) == 2, true, true, 2>(a.act, g, s);
+  if (a.rule.threshold) {
+    const drop::Key key = drop::key_of(a.rule);
+    const drop::Words words = drop::numbers(key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8));
+    uint32_t word = words.w[0];  // of column n % 8, without an index into registers
+    if (n % 8 >= 2) word = words.w[1];
+    if (n % 8 >= 4) word = words.w[2];
+    if (n % 8 >= 6) word = words.w[3];
+    const bool kept = n % 2 ? word > key.high : (word << 16) > key.low;
+    g[0] = kept ? g[0] : 0.f, s[0] = kept ? s[0] : 0.f, u = kept ? u * a.rule.scale : 0.f;
+  }
+  if (a.factors) {
+    T* factors = static_cast<T*>(a.factors) + m * 2 * a.out + n;
+    factors[0] = from_float<T>(s[0] * u);
+    factors[a.out] = from_float<T>(g[0] * a.rule.scale);
+  }
+  static_cast<T*>(a.y)[m * a.y_stride + n] = from_float<T>(g[0] * u);
+}
+
+// Rows of the weight to a column of the output.
+template <typename A>
+constexpr int kHalves = 1;
+template <>
+constexpr int kHalves<GatedArgs> = 2;
+
+// kRows rows of x (from blockIdx.y * kRows on) against kCols rows of the weight (of
+// each half, in the gated operator), whose columns `split` neighbouring warps share:
+// few rows of a long weight are work for many warps, and their sums are added in order.
+template <typename T, int kRows, int kCols, int kUnroll, int split, bool kVec, typename A>
+__global__ void __launch_bounds__(32 * kWarps) gemv_kernel(const A a) {
   constexpr int kPer = kVec ? 16 / sizeof(T) : 1, kOut = kCols * kRows, step = 32 * kPer * split;
-  __shared__ float parts[split > 1 ? kWarps : 1][kOut];
+  constexpr int kH = kHalves<A>, kW = kH * kCols;  // rows of the weight
+  __shared__ float parts[split > 1 ? kWarps : 1][kH * kOut];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t n0 = (blockIdx.x * static_cast<int64_t>(kWarps / split) + warp / split) * kCols;
   const int64_t m0 = blockIdx.y * static_cast<int64_t>(kRows);
   const int cols = static_cast<int>(a.out - n0 < kCols ? a.out - n0 : kCols);
   const int rows = static_cast<int>(a.rows - m0 < kRows ? a.rows - m0 : kRows);
-  float acc[kCols][kRows] = {};
+  float acc[kW][kRows] = {};
   if (cols > 0) {
     const T* w = static_cast<const T*>(a.w) + n0 * a.w_stride;
     const T* x = static_cast<const T*>(a.x) + m0 * a.x_stride;
-    const auto load_w = [&](int64_t k, float u[kCols][kPer]) {
+    const auto load_w = [&](int64_t k, float u[kW][kPer]) {
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const T* p = w + (c < cols ? c : 0) * a.w_stride + k;  // a row that is not there repeats the first
+      for (int c = 0; c < kW; ++c) {
+        // a row that is not there repeats the first
+        const T* p = w + ((c % kCols < cols ? c % kCols : 0) + (c < kCols ? 0 : a.out)) * a.w_stride + k;
         if constexpr (kVec)
           load_vec<T>(p, u[c]);
         else
           u[c][0] = to_float(*p);
       }
     };
-    const auto multiply = [&](int64_t k, const float u[kCols][kPer]) {
+    const auto multiply = [&](int64_t k, const float u[kW][kPer]) {
 #pragma unroll
       for (int m = 0; m < kRows; ++m) {
         if (m < rows) {
@@ -61,7 +107,7 @@ __global__ void __launch_bounds__(32 * kWarps) gemv_kernel(const Args a) {
           else
             v[0] = to_float(x[m * a.x_stride + k]);
 #pragma unroll
-          for (int c = 0; c < kCols; ++c)
+          for (int c = 0; c < kW; ++c)
 #pragma unroll
             for (int j = 0; j < kPer; ++j) acc[c][m] = fmaf(u[c][j], v[j], acc[c][m]);
         }
@@ -69,54 +115,53 @@ __global__ void __launch_bounds__(32 * kWarps) gemv_kernel(const Args a) {
     };
     int64_t k = (warp % split * 32 + lane) * kPer;
     for (; k + (kUnroll - 1) * step < a.in; k += kUnroll * step) {  // this many loads on their way together
-      float u[kUnroll][kCols][kPer];
+      float u[kUnroll][kW][kPer];
 #pragma unroll
       for (int q = 0; q < kUnroll; ++q) load_w(k + q * step, u[q]);
 #pragma unroll
       for (int q = 0; q < kUnroll; ++q) multiply(k + q * step, u[q]);
     }
     for (; k < a.in; k += step) {
-      float u[kCols][kPer];
+      float u[kW][kPer];
       load_w(k, u);
       multiply(k, u);
     }
   }
-  const auto finish = [&](int o, float z0) {
+  const auto put = [&](int o, const float sums[kH]) {
     const int c = o / kRows;
-    if (c >= cols || o % kRows >= rows) return;
-    float z[2] = {z0, 0.f}, s[2];
-    const int64_t m = m0 + o % kRows, n = n0 + c;
-    if (a.bias) z[0] += to_float(static_cast<const T*>(a.bias)[n]);
-    activate<sizeof(T) == 2, true, true, 2>(a.act, z, s);
-    if (a.slope)
-      static_cast<typename SlopeOf<T>::type*>(a.slope)[m * a.out + n] = from_float<typename SlopeOf<T>::type>(s[0]);
-    if (a.r) z[0] += to_float(static_cast<const T*>(a.r)[m * a.r_stride + n]);
-    static_cast<T*>(a.y)[m * a.y_stride + n] = from_float<T>(z[0]);
+    if (c < cols && o % kRows < rows) finish<T>(a, m0 + o % kRows, n0 + c, sums);
   };
-  float mine = 0.f;  // lane o % 32 keeps output o
+  float mine[kH] = {};  // lane o % 32 keeps output o
 #pragma unroll
-  for (int o = 0; o < kOut; ++o) {
-    float t = acc[o / kRows][o % kRows];
+  for (int o = 0; o < kOut; ++o)
 #pragma unroll
-    for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-    if (lane == o % 32) mine = t;
-  }
+    for (int h = 0; h < kH; ++h) {
+      float t = acc[h * kCols + o / kRows][o % kRows];
+#pragma unroll
+      for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+      if (lane == o % 32) mine[h] = t;
+    }
   static_assert(kOut <= 32, "an output to a lane");
   if (split == 1) {
-    if (lane < kOut) finish(lane, mine);
+    if (lane < kOut) put(lane, mine);
     return;
   }
-  if (lane < kOut) parts[warp][lane] = mine;
+  if (lane < kOut) {
+#pragma unroll
+    for (int h = 0; h < kH; ++h) parts[warp][h * kOut + lane] = mine[h];
+  }
   __syncthreads();
   if (warp % split != 0 || lane >= kOut) return;  // the first of the warps finishes
-  float sum = 0.f;
+  float sums[kH] = {};
 #pragma unroll
-  for (int q = 0; q < split; ++q) sum += parts[warp + q][lane];
-  finish(lane, sum);
+  for (int q = 0; q < split; ++q)
+#pragma unroll
+    for (int h = 0; h < kH; ++h) sums[h] += parts[warp + q][h * kOut + lane];
+  put(lane, sums);
 }
 
-template <typename T, int kRows, int kCols, int kUnroll>
-cudaError_t launch(const Args& a, bool vec, cudaStream_t stream) {
+template <typename T, int kRows, int kCols, int kUnroll, typename A>
+cudaError_t launch(const A& a, bool vec, cudaStream_t stream) {
   const int64_t steps = a.in / (32 * (vec ? 16 / sizeof(T) : 1)), groups = (a.out + kCols - 1) / kCols;
   // Four warps to a weight row where one each would leave half of the GPU's
   // warps idle over rows of eight steps or more (bfloat16, one row of 8192:
@@ -125,24 +170,24 @@ cudaError_t launch(const Args& a, bool vec, cudaStream_t stream) {
   const int64_t per_block = (shared ? kWarps / 4 : kWarps) * kCols;
   const dim3 grid(static_cast<unsigned>((a.out + per_block - 1) / per_block),
                   static_cast<unsigned>((a.rows + kRows - 1) / kRows));
-  const auto kernel = shared ? (vec ? gemv_kernel<T, kRows, kCols, kUnroll, 4, true>
-                                    : gemv_kernel<T, kRows, kCols, kUnroll, 4, false>)
-                             : (vec ? gemv_kernel<T, kRows, kCols, kUnroll, 1, true>
-                                    : gemv_kernel<T, kRows, kCols, kUnroll, 1, false>);
+  const auto kernel = shared ? (vec ? gemv_kernel<T, kRows, kCols, kUnroll, 4, true, A>
+                                    : gemv_kernel<T, kRows, kCols, kUnroll, 4, false, A>)
+                             : (vec ? gemv_kernel<T, kRows, kCols, kUnroll, 1, true, A>
+                                    : gemv_kernel<T, kRows, kCols, kUnroll, 1, false, A>);
   kernel<<<grid, 32 * kWarps, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t launch_rows(const Args& a, cudaStream_t stream) {
+template <typename T, typename A>
+cudaError_t launch_rows(const A& a, cudaStream_t stream) {
   const auto aligned = [](const void* p, int64_t stride) {
     return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * sizeof(T)) % 16 == 0;
   };
-  const bool vec = aligned(a.x, a.rows == 1 ? 0 : a.x_stride) && aligned(a.w, a.out == 1 ? 0 : a.w_stride) &&
+  const bool vec = aligned(a.x, a.rows == 1 ? 0 : a.x_stride) && aligned(a.w, kHalves<A> * a.out == 1 ? 0 : a.w_stride) &&
                    (a.in * sizeof(T)) % 16 == 0;
   if (a.rows == 1) return launch<T, 1, 1, 4>(a, vec, stream);
   if (a.rows <= 4) return launch<T, 4, 1, 2>(a, vec, stream);
-  return launch<T, 8, 2, 2>(a, vec, stream);
+  return launch<T, 8, 2 / kHalves<A>, 2>(a, vec, stream);
 }
 
 }  // namespace
@@ -160,6 +205,16 @@ bool few_rows(const Args& a) {
 }
 
 cudaError_t forward_few_rows(const Args& a, cudaStream_t stream) {
+  return a.dtype == DType::kF32 ? launch_rows<float>(a, stream) : launch_rows<bf16>(a, stream);
+}
+
+bool gated_few_rows(const GatedArgs& a) {
+  Args as{};  // a product of twice the columns
+  as.dtype = a.dtype, as.rows = a.rows, as.in = a.in, as.out = 2 * a.out;
+  return few_rows(as);
+}
+
+cudaError_t gated_forward_few_rows(const GatedArgs& a, cudaStream_t stream) {
   return a.dtype == DType::kF32 ? launch_rows<float>(a, stream) : launch_rows<bf16>(a, stream);
 }
 

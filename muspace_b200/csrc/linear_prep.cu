@@ -184,6 +184,69 @@ cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slo
   return cudaGetLastError();
 }
 
+// dst = [g * P, g * Q] with the sums of both halves' columns, before the rounding: a
+// lane takes eight columns of g and the same of either half.
+template <typename T>
+__global__ void __launch_bounds__(32 * kSumWarps, 4)
+    gate_operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec, const T* __restrict__ factors,
+                        bool factors_vec, bf16* __restrict__ dst, int64_t dst_ld, int64_t plane, bool dst_vec,
+                        int64_t rows, int64_t cols, int64_t rows_per_part, float* __restrict__ parts) {
+  __shared__ float buf[kSumWarps][kSumCols];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
+  const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
+  const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);
+  const bool vec = dst_vec && count == 8;
+  float s[2][8] = {};
+  if (c < cols) {
+    for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+      float v[8], f[8];
+      load_some(src + r * src_ld + c, count, src_vec && count == 8, v);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        load_some(factors + (2 * r + half) * cols + c, count, factors_vec && count == 8, f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          f[j] *= v[j];
+          s[half][j] += f[j];
+        }
+        bf16* at = dst + r * dst_ld + half * cols + c;
+        if (sizeof(T) == 4)
+          store_planes(at, plane, count, vec, f);
+        else
+          store_some(at, count, vec, f);
+      }
+    }
+  }
+  if (!parts) return;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (half) __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) buf[warp][lane + 32 * j] = s[half][j];
+    __syncthreads();
+    const int64_t at = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8 + warp;  // column `warp` of the lane's eight
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kSumWarps; ++w) sum += buf[w][lane + 32 * warp];
+    if (at < cols) parts[(2ll * blockIdx.y + half) * cols + at] = sum;
+  }
+}
+
+template <typename T>
+cudaError_t launch_gate_operand(const void* g, int64_t g_ld, const void* factors, const Operand& dst, float* parts,
+                                cudaStream_t stream) {
+  const int64_t cols = dst.cols / 2, count = column_parts(dst.rows, cols);
+  if (dst.rows == 0 || cols == 0) return cudaSuccess;
+  const bool g_vec = aligned16(g) && (g_ld * sizeof(T)) % 16 == 0;
+  const bool factors_vec = aligned16(factors) && (cols * sizeof(T)) % 16 == 0;
+  const dim3 grid(static_cast<unsigned>((cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
+  gate_operand_kernel<T><<<grid, 32 * kSumWarps, 0, stream>>>(
+      static_cast<const T*>(g), g_ld, g_vec, static_cast<const T*>(factors), factors_vec, const_cast<bf16*>(dst.p),
+      dst.ld, dst.plane, cols % 8 == 0, dst.rows, cols, (dst.rows + count - 1) / count, parts);
+  return cudaGetLastError();
+}
+
 template <typename T>
 __global__ void __launch_bounds__(1024)
     add_parts_kernel(const float* __restrict__ parts, int64_t count, int64_t cols, T* __restrict__ sums) {
@@ -239,6 +302,12 @@ cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const voi
                  : launch_operand_sums<float, false>(g, g_ld, nullptr, dst, parts, stream);
   return slope ? launch_operand_sums<bf16, true>(g, g_ld, slope, dst, parts, stream)
                : launch_operand_sums<bf16, false>(g, g_ld, nullptr, dst, parts, stream);
+}
+
+cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const Operand& dst,
+                         float* parts, cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_gate_operand<float>(g, g_ld, factors, dst, parts, stream)
+                              : launch_gate_operand<bf16>(g, g_ld, factors, dst, parts, stream);
 }
 
 cudaError_t column_sums(const Operand& src, float* parts, cudaStream_t stream) {

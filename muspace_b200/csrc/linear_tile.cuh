@@ -282,13 +282,14 @@ __device__ __forceinline__ Item item_of(const Job& j, uint32_t i) {
 
 // ---- the epilogue ------------------------------------------------------------------------
 
-// A warp's box in shared memory: 32 rows of 128 or 64 bytes, whose 16-byte units
-// are exchanged by the row's number as TMA's swizzle has it; eight neighbouring
+// A warp's box in shared memory: 32 rows of 128, 64 or 32 bytes, whose 16-byte units
+// (of the first two) are exchanged by the row's number as TMA's swizzle has it; eight neighbouring
 // rows' units at one place then lie in different banks.
 template <int kRowBytes>
 __device__ __forceinline__ uint32_t unit_at(uint32_t box, int row, int unit) {
-  return kRowBytes == 128 ? box + row * 128 + ((unit ^ (row & 7)) << 4)
-                          : box + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4);
+  return kRowBytes == 128  ? box + row * 128 + ((unit ^ (row & 7)) << 4)
+         : kRowBytes == 64 ? box + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4)
+                           : box + row * 32 + (unit << 4);
 }
 
 __device__ __forceinline__ void put_unit(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

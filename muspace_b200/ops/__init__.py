@@ -1,7 +1,8 @@
 """Canonical operator exports of the B200 build: the MSDA operator, the fused
 spatial-cross-attention scatter built on it, FlashSCA, SparseDrive's deformable
-aggregation, and the layer around them: the linear product with its epilogue, layer
-norm, 8-bit activation checkpoints, dropout and norms with their residual."""
+aggregation, and the layer around them: the linear product with its epilogue, the gated
+feed-forward product, layer norm, norms with their residual, dropout and 8-bit
+activation checkpoints."""
 
 from .checkpoint8 import Checkpoint8, checkpoint_pack, checkpoint_unpack
 from .deformable_aggregation import (
@@ -16,6 +17,7 @@ from .multi_scale_deformable_attn import (
     multi_scale_deformable_attn_pytorch_compat,
 )
 from .flash_sca import flash_bevpool_sca
+from .gated_linear import gated_linear
 from .layer_norm import layer_norm
 from .linear_act import linear_act
 from .residual_norm import add_norm, norm_add
@@ -32,6 +34,7 @@ __all__ = [
     "explain_dispatch",
     "feature_maps_format",
     "flash_bevpool_sca",
+    "gated_linear",
     "layer_norm",
     "linear_act",
     "ms_deform_attn_scatter_div",

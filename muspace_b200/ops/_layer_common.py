@@ -1,5 +1,5 @@
 """What the layer operators (``linear_act``, ``layer_norm``, 8-bit checkpoints, dropout,
-norms with their residual) share: storage types, rows of a tensor, dispatch reports."""
+norms with their residual, ``gated_linear``) share: storage types, rows of a tensor, dispatch reports."""
 
 from __future__ import annotations
 

@@ -89,7 +89,8 @@ def _is_cuda_tensor(tensor: torch.Tensor) -> bool:
 _KERNEL_NAMES = {"multi_scale_deformable_attn": "MSDA", "deformable_aggregation": "deformable aggregation",
                  "flash_bevpool_sca": "FlashSCA", "linear_act": "linear", "layer_norm": "layer norm",
                  "checkpoint_pack": "checkpoint", "checkpoint_unpack": "checkpoint",
-                 "dropout": "dropout", "add_norm": "residual norm", "norm_add": "residual norm"}
+                 "dropout": "dropout", "add_norm": "residual norm", "norm_add": "residual norm",
+                 "gated_linear": "gated linear"}
 
 
 def explain_dispatch(

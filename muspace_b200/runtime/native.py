@@ -188,6 +188,21 @@ class ResidualNormArgs(ctypes.Structure):
     )
 
 
+class GatedLinearArgs(ctypes.Structure):
+    """``msda_gated_linear_t`` of include/muspace_msda.h."""
+
+    _fields_ = (
+        [(name, ctypes.c_int32) for name in ("dtype", "activation")]
+        + [(name, ctypes.c_int64) for name in
+           ("rows", "in_features", "out_features", "input_stride", "weight_stride", "output_stride",
+            "grad_output_stride", "threshold", "seed", "sequence")]
+        + [(name, ctypes.c_void_p) for name in
+           ("seed_at", "input", "weight", "bias", "output", "factors", "grad_output", "grad_input", "grad_weight",
+            "grad_bias", "workspace")]
+        + [("workspace_bytes", ctypes.c_size_t)]
+    )
+
+
 # the plain-pointer entry points of the layer operators: argument types before the stream
 _PLAIN_SIGNATURES: dict[str, tuple] = {
     "msda_linear_act_forward": (ctypes.POINTER(LinearArgs),),
@@ -197,6 +212,8 @@ _PLAIN_SIGNATURES: dict[str, tuple] = {
     "msda_checkpoint_pack": (ctypes.c_int, ctypes.c_void_p) + (ctypes.c_int64,) * 3 + (ctypes.c_void_p,) * 2,
     "msda_checkpoint_unpack": (ctypes.c_int,) + (ctypes.c_void_p,) * 2 + (ctypes.c_int64,) * 2 + (ctypes.c_void_p,),
     "msda_dropout": (ctypes.c_int, ctypes.c_void_p) + (ctypes.c_int64,) * 6 + (ctypes.c_void_p,) * 2,
+    "msda_gated_linear_forward": (ctypes.POINTER(GatedLinearArgs),),
+    "msda_gated_linear_backward": (ctypes.POINTER(GatedLinearArgs),),
     "msda_add_norm_forward": (ctypes.POINTER(ResidualNormArgs),),
     "msda_add_norm_backward": (ctypes.POINTER(ResidualNormArgs),),
     "msda_norm_add_forward": (ctypes.POINTER(ResidualNormArgs),),
@@ -218,7 +235,8 @@ def layer_wait_timeouts(device: torch.device | int | None = None) -> int:
 
 _WORKSPACE_CALLS = {"msda_linear_act_forward_workspace", "msda_linear_act_backward_workspace",
                     "msda_layer_norm_backward_workspace", "msda_add_norm_backward_workspace",
-                    "msda_norm_add_backward_workspace"}
+                    "msda_norm_add_backward_workspace", "msda_gated_linear_forward_workspace",
+                    "msda_gated_linear_backward_workspace"}
 
 
 class NativeModule:
