@@ -207,14 +207,13 @@ def _groups_of(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int]:
     gradients that are then summed to its own shape are not rounded before."""
     lead = shape[:-1]
     own = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
-    full = _expanded("gate", gate.float(), shape)
     if own[-1] == shape[-1]:
         upto = len(lead)
         while upto and own[upto - 1] == 1:
             upto -= 1
         if own[:upto] == tuple(lead[:upto]):
             return gate, prod(lead[:upto])
-    return full, prod(lead)
+    return _expanded("gate", gate.float(), shape), prod(lead)
 
 
 def _call(operator: str, input, residual, weight, bias, gate, residual_scale, kind, eps, p, seed, sequence, want_sum,

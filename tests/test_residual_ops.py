@@ -190,7 +190,8 @@ def check(op, data, kind="layer", p=0.25, alpha=1.5, want_sum=True, use=("y", "s
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
-@pytest.mark.parametrize("rows,n", [(1, 1), (1, 256), (3, 7), (1, 4099), (129, 64), (1000, 257), (40, 1000), (3000, 512)])
+@pytest.mark.parametrize("rows,n", [(1, 1), (1, 256), (3, 7), (1, 4099), (129, 64), (1000, 257), (40, 1000), (3000, 512),
+                                    (2, 2500007), (1, 2500008), (100000, 3)])
 def test_dropout_is_the_generator(cuda_device, rows, n, dtype):
     gen = torch.Generator().manual_seed(n)
     x, g = (torch.randn(rows, n, generator=gen).to(dtype).to(cuda_device) for _ in range(2))
