@@ -64,17 +64,17 @@ __device__ __forceinline__ void load_param(const void* p, bool f32, int cols, in
 template <int G, bool kVec>
 struct Mask {
   drop::Words n;
-  __device__ __forceinline__ void make(const drop::Key& key, int64_t row, int lane, int i) {
-    n = drop::numbers(key, static_cast<uint32_t>(row), i * G + lane);
+  __device__ __forceinline__ void make(const drop::Key& key, uint32_t row, int lane, int i) {
+    n = drop::numbers(key, row, i * G + lane);
   }
   __device__ __forceinline__ bool kept(const drop::Key& key, int j) const { return drop::kept(key, n, j); }
 };
 template <int G>
 struct Mask<G, false> {
   uint32_t bits;
-  __device__ __forceinline__ void make(const drop::Key& key, int64_t row, int lane, int i) {
+  __device__ __forceinline__ void make(const drop::Key& key, uint32_t row, int lane, int i) {
     const int l = lane & 31, group = ((i * 8 + l / 4) * G + lane - l) / 8 + l % 4;
-    const uint32_t mine = drop::bits8(key, drop::numbers(key, static_cast<uint32_t>(row), group));
+    const uint32_t mine = drop::bits8(key, drop::numbers(key, row, group));
     bits = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) bits |= (__shfl_sync(0xffffffffu, mine, j * 4 + l / 8) >> (l % 8) & 1u) << j;
@@ -89,11 +89,9 @@ __device__ __forceinline__ void apply(const M& mask, const drop::Key& key, float
 }
 
 // The gate's row for a row.
-__device__ __forceinline__ const void* gate_at(const Args& a, int64_t r, int size) {
+__device__ __forceinline__ const void* gate_at(const Args& a, uint32_t r, int size) {
   if (!a.gate) return nullptr;
-  const int64_t g = a.gate_rows == a.rows ? 0
-                    : a.gate_rows == 1    ? r
-                                          : static_cast<uint32_t>(r) / static_cast<uint32_t>(a.gate_rows);
+  const int64_t g = a.gate_rows == a.rows ? 0 : a.gate_rows == 1 ? r : r / static_cast<uint32_t>(a.gate_rows);
   return static_cast<const char*>(a.gate) + g * a.gate_stride * size;
 }
 
@@ -152,27 +150,33 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
   return Moments{mean.a, rsqrtf(var.a / n + a.eps)};
 }
 
+// With fewer than 32 threads to a row, a warp has several rows under way, of which the
+// last may not be there: its loads give 0, and it stores nothing.
 template <int G, int NV, bool kVec, bool kBranch, typename T>
 __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args a) {
+  constexpr int kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
   int turn = 0;
   const int lane = threadIdx.x % G, cols = static_cast<int>(a.cols);
   const int gate_size = a.gate_f32 ? 4 : sizeof(T);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * Shape<G>::kRows;
+  const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * Shape<G>::kRows;
   const T *h = static_cast<const T*>(a.h), *res = static_cast<const T*>(a.r);
   const drop::Key key = drop::key_of(a.rule);
   const float2 alpha = both(a.alpha);
-  int64_t r = blockIdx.x * static_cast<int64_t>(Shape<G>::kRows) + threadIdx.x / G;
+  const uint32_t offset = threadIdx.x / G % kTogether;
+  uint32_t r = blockIdx.x * Shape<G>::kRows + threadIdx.x / G;
   Chunk<T, kVec> next_h[NV], next_r[NV];
-  const auto load = [&](int64_t row) {
+  const auto load = [&](uint32_t row) {
+    const int there = row < rows ? cols : 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      next_h[i].template load<G>(h + row * a.h_stride, cols, lane, i);
-      next_r[i].template load<G>(res + row * a.r_stride, cols, lane, i);
+      next_h[i].template load<G>(h + row * a.h_stride, there, lane, i);
+      next_r[i].template load<G>(res + row * a.r_stride, there, lane, i);
     }
   };
-  if (r < a.rows) load(r);
-  for (; r < a.rows; r += step) {
+  load(r);
+  for (; r - offset < rows; r += step) {
+    const int there = r < rows ? cols : 0;
     float2 v[NV][4], p[4];
     Chunk<T, kVec> here_r[NV];
 #pragma unroll
@@ -180,7 +184,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       next_h[i].get(v[i]);
       here_r[i] = next_r[i];
     }
-    if (r + step < a.rows) load(r + step);
+    if (r - offset + step < rows) load(r + step);
     const void* gate = gate_at(a, r, gate_size);
     // D, the gate and the residual, on eight values
     const auto join = [&](int i) {
@@ -197,7 +201,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       here_r[i].get(p);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = fma2(alpha, p[j], v[i][j]);
-      if (a.s) store_chunk<G, kVec>(static_cast<T*>(a.s) + r * a.cols, cols, lane, i, &v[i][0].x);
+      if (a.s) store_chunk<G, kVec>(static_cast<T*>(a.s) + r * a.cols, there, lane, i, &v[i][0].x);
     };
     if (!kBranch) {
 #pragma unroll
@@ -210,7 +214,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       Moments none;
       kept = m = moments<G, NV, kVec, false, T>(v, a, cols, lane, buf, turn, none);
     }
-    if (a.rstd && lane == 0) {
+    if (a.rstd && lane == 0 && r < rows) {
       if (a.mean) a.mean[r] = kept.mean;
       a.rstd[r] = kept.rstd;
     }
@@ -232,7 +236,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       if (kBranch)
         join(i);
       else
-        store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, &v[i][0].x);
+        store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, there, lane, i, &v[i][0].x);
     }
   }
 }
@@ -250,9 +254,9 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
 __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
     backward_kernel(const Args a, const Grid grid) {
-  constexpr int kRows = Shape<G>::kRows;
+  constexpr int kRows = Shape<G>::kRows, kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
-  __shared__ float fold[kRows > 1 ? kRows * 32 * 8 : 1];
+  __shared__ float fold[kRows > 1 ? kRows * G * 8 : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, slot = threadIdx.x / G, cols = static_cast<int>(a.cols);
   const int gate_size = a.gate_f32 ? 4 : sizeof(T);
@@ -269,14 +273,16 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
       if (kRows > 1) {  // the block's rows, in order
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) fold[(slot * 8 + j) * 32 + lane] = mine[j];
+        for (int j = 0; j < 8; ++j) fold[(slot * 8 + j) * G + lane] = mine[j];
         __syncthreads();
         // thread (slot, lane) adds up column j = slot of lane's eight
-        float sum = 0.f;
+        if (slot < 8) {
+          float sum = 0.f;
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + slot) * 32 + lane];
-        const int c = column<G, kVec>(lane, i, slot);
-        if (c < cols) out[c] = sum;
+          for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + slot) * G + lane];
+          const int c = column<G, kVec>(lane, i, slot);
+          if (c < cols) out[c] = sum;
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -287,20 +293,23 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
     }
   };
   // dgate of eight values: added up, or a row of its own
-  const auto put_gate = [&](int64_t r, int i, float2 t[4]) {
+  const auto put_gate = [&](uint32_t r, int there, int i, float2 t[4]) {
     if (grid.sums_gate) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) dg[kGate ? i : 0][j] = add2(dg[kGate ? i : 0][j], t[j]);
     } else if (a.gate_f32) {
-      store_chunk<G, kVec>(static_cast<float*>(a.dgate) + r * a.cols, cols, lane, i, &t[0].x);
+      store_chunk<G, kVec>(static_cast<float*>(a.dgate) + r * a.cols, there, lane, i, &t[0].x);
     } else {
-      store_chunk<G, kVec>(static_cast<T*>(a.dgate) + r * a.cols, cols, lane, i, &t[0].x);
+      store_chunk<G, kVec>(static_cast<T*>(a.dgate) + r * a.cols, there, lane, i, &t[0].x);
     }
   };
 
   for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
     const Unit unit = unit_of(grid, u);
-    for (int64_t r = unit.begin + slot; r < unit.end; r += kRows) {
+    const uint32_t end = static_cast<uint32_t>(unit.end), offset = slot % kTogether;
+    for (uint32_t r = static_cast<uint32_t>(unit.begin) + slot; r - offset < end; r += kRows) {
+      const bool valid = r < end;
+      const int there = valid ? cols : 0;
       const void* gate = gate_at(a, r, gate_size);
       Chunk<T, kVec> x[NV], g[NV];
       const T* x_row = kBranch ? static_cast<const T*>(a.h) + r * a.h_stride
@@ -311,11 +320,11 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         if (normed) {
-          x[i].template load<G>(x_row, cols, lane, i);
-          g[i].template load<G>(g_row, cols, lane, i);
+          x[i].template load<G>(x_row, there, lane, i);
+          g[i].template load<G>(g_row, there, lane, i);
         }
       }
-      const float mean = normed && a.mean ? a.mean[r] : 0.f, rstd = normed ? a.rstd[r] : 0.f;
+      const float mean = normed && valid && a.mean ? a.mean[r] : 0.f, rstd = normed && valid ? a.rstd[r] : 0.f;
       const float2 scale = both(rstd), minus = both(-mean);
       float2 sum = both(0.f), dot = both(0.f);
       if (!kBranch) {
@@ -362,7 +371,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
           }
           if (a.gs) {
             Chunk<T, kVec> more;
-            more.template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, cols, lane, i);
+            more.template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, there, lane, i);
             more.get(p);
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[j] = add2(d[j], p[j]);
@@ -370,19 +379,19 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
           if (a.dr) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[j]);
-            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, cols, lane, i, &p[0].x);
+            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, there, lane, i, &p[0].x);
           }
           if (!kGate && !a.dh) continue;
           Mask<G, kVec> mask;
           if (a.rule.threshold) mask.make(key, r, lane, i);
           if (kGate) {
             Chunk<T, kVec> branch;
-            branch.template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, cols, lane, i);
+            branch.template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, there, lane, i);
             branch.get(p);
             if (a.rule.threshold) apply(mask, key, &p[0].x);
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[j]);
-            put_gate(r, i, p);
+            put_gate(r, there, i, p);
           }
           if (!a.dh) continue;
           if (a.rule.threshold) apply(mask, key, &d[0].x);
@@ -391,7 +400,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], p[j]);
           }
-          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, cols, lane, i, &d[0].x);
+          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, there, lane, i, &d[0].x);
         }
       } else {
         float2 d[NV][4];
@@ -403,7 +412,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
           if (a.dr) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[i][j]);
-            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, cols, lane, i, &p[0].x);
+            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, there, lane, i, &p[0].x);
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) k[j] = mul2(add2(k[j], minus), scale);
@@ -421,7 +430,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
             if (a.rule.threshold) apply(mask, key, &p[0].x);
 #pragma unroll
             for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[i][j]);
-            put_gate(r, i, p);
+            put_gate(r, there, i, p);
           }
           if (a.rule.threshold) apply(mask, key, &d[i][0].x);
           if (gate) {
@@ -447,7 +456,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
           x[i].get(k);
 #pragma unroll
           for (int j = 0; j < 4; ++j) d[i][j] = fma2(add2(k[j], minus), c2, fma2(d[i][j], scale, c1));
-          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, cols, lane, i, &d[i][0].x);
+          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, there, lane, i, &d[i][0].x);
         }
       }
     }
@@ -711,7 +720,8 @@ cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
 template <bool kVec, bool kBranch, typename T>
 cudaError_t forward_form(const Args& a, cudaStream_t stream) {
   if (a.cols <= 1024) {
-    if (kVec && a.cols <= 256) return launch_forward<32, kVec ? 1 : 4, kVec, kBranch, T>(a, stream);
+    if (kVec && a.cols <= 128) return launch_forward<kVec ? 16 : 32, kVec ? 1 : 4, kVec, kBranch, T>(a, stream);
+    if (kVec && a.cols <= 256) return launch_forward<kVec ? 16 : 32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
     if (kVec && a.cols <= 512) return launch_forward<32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
     return launch_forward<32, 4, kVec, kBranch, T>(a, stream);
   }
@@ -733,8 +743,10 @@ cudaError_t forward_of(const Args& a, cudaStream_t stream) {
 
 template <bool kVec, bool kBranch, bool kGate, typename T>
 cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) {
-  if (kVec && a.cols <= 256)
-    backward_kernel<32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+  if (kVec && a.cols <= 128)
+    backward_kernel<kVec ? 16 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+  else if (kVec && a.cols <= 256)
+    backward_kernel<kVec ? 16 : 32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (a.cols <= 512)
     backward_kernel<32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (a.cols <= 2048)

@@ -15,17 +15,20 @@ struct Sums {
   float a, b;
 };
 
+// Over N neighbouring lanes.
+template <int N = 32>
 __device__ __forceinline__ Sums warp_sums(Sums s) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) {
+  for (int d = N / 2; d; d >>= 1) {
     s.a += __shfl_xor_sync(0xffffffffu, s.a, d);
     s.b += __shfl_xor_sync(0xffffffffu, s.b, d);
   }
   return s;
 }
+template <int N = 32>
 __device__ __forceinline__ float warp_sums(float s) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  for (int d = N / 2; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   return s;
 }
 __device__ __forceinline__ Sums operator+(Sums s, Sums t) { return Sums{s.a + t.a, s.b + t.b}; }
@@ -34,9 +37,9 @@ __device__ __forceinline__ Sums operator+(Sums s, Sums t) { return Sums{s.a + t.
 // between two halves, so one barrier per sum is enough.
 template <int G, bool kNamed = false, typename S>
 __device__ __forceinline__ S row_sums(S s, Sums* buf, int& turn) {
-  s = warp_sums(s);
-  if (G == 32) return s;
-  constexpr int kWarps = G / 32;
+  s = warp_sums<(G < 32 ? G : 32)>(s);
+  if (G <= 32) return s;
+  constexpr int kWarps = G <= 32 ? 1 : G / 32;
   S* half = reinterpret_cast<S*>(buf + turn * kWarps);
   turn ^= 1;
   if ((threadIdx.x & 31) == 0) half[(threadIdx.x % G) >> 5] = s;
@@ -116,9 +119,9 @@ __device__ __forceinline__ void store_chunk(T* row, int cols, int lane, int i, c
 // Rows per block and block size for G threads a row.
 template <int G>
 struct Shape {
-  static constexpr int kRows = G == 32 ? 8 : 1;
+  static constexpr int kRows = G <= 32 ? 256 / G : 1;
   static constexpr int kThreads = G * kRows;
-  static constexpr int kBuf = G == 32 ? 1 : 2 * (G / 32);
+  static constexpr int kBuf = G <= 32 ? 1 : 2 * (G / 32);
 };
 
 }  // namespace rows
