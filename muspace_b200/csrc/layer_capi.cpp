@@ -173,6 +173,7 @@ resnorm::Args residual_norm_args(const msda_residual_norm_t* in, bool branch, bo
   a.h_stride = in->input_stride, a.r_stride = in->residual_stride, a.gate_stride = in->gate_stride;
   a.gy_stride = in->grad_output_stride, a.gs_stride = in->grad_sum_stride, a.sum_stride = in->sum_stride;
   a.alpha = in->residual_scale, a.eps = in->eps;
+  a.share = a.cols ? 1.f / static_cast<float>(a.cols) : 0.f;
   a.rule = rule_of(in->threshold, in->seed, in->sequence, in->seed_at);
   a.gate = in->gate, a.w = in->weight, a.b = in->bias;
   a.rstd = in->rstd;

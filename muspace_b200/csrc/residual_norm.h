@@ -26,6 +26,7 @@ struct Args {
   int64_t gate_groups;       // rows of the gate
   int64_t gate_rows;         // neighbouring rows that share one: rows / gate_groups
   float alpha, eps;
+  float share;               // 1 / cols
   drop::Rule rule;
   const void* h;             // forward; backward: norm_add, and with dgate
   const void* r;             // forward

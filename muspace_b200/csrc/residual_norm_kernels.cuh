@@ -103,18 +103,31 @@ struct Moments {
   float mean, rstd;
 };
 
+// Whether the warp has columns in its i-th chunk: what has none is skipped.
+template <int G, bool kVec>
+__device__ __forceinline__ bool any(int cols, int i) {
+  return i == 0 || i * G * 8 < cols;
+}
+
 // Mean and rstd of the row whose values lie in v; beyond the row v is 0. kBoth: and
 // those of the values as T stores them, in the same reductions.
 template <int G, int NV, bool kVec, bool kBoth, typename T>
 __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a, int cols, int lane, Sums* buf,
                                            int& turn, Moments& of_stored) {
-  const float n = static_cast<float>(cols);
+  const float share = a.share;
   const auto over_row = [&](float2 x, float2 y) {
     if constexpr (kBoth)
       return row_sums<G>(Sums{x.x + x.y, y.x + y.y}, buf, turn);
     else
       return Sums{row_sums<G>(x.x + x.y, buf, turn), 0.f};
   };
+  float2 w[kBoth ? NV : 1][4];
+  if (kBoth) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[kBoth ? i : 0][j] = stored(v[i][j], T());
+  }
   Sums mean{0.f, 0.f};
   if (!a.rms) {
     float2 t = both(0.f), u = both(0.f);
@@ -123,10 +136,10 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         t = add2(t, v[i][j]);
-        if (kBoth) u = add2(u, stored(v[i][j], T()));
+        if (kBoth) u = add2(u, w[kBoth ? i : 0][j]);
       }
     mean = over_row(t, u);
-    mean.a /= n, mean.b /= n;
+    mean.a *= share, mean.b *= share;
   }
   float2 t = both(0.f), u = both(0.f);
   const auto square = [&](int i, int j, float2 d, float2 sum) {
@@ -142,12 +155,35 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       t = square(i, j, add2(v[i][j], both(-mean.a)), t);
-      if (kBoth) u = square(i, j, add2(stored(v[i][j], T()), both(-mean.b)), u);
+      if (kBoth) u = square(i, j, add2(w[kBoth ? i : 0][j], both(-mean.b)), u);
     }
   }
   const Sums var = over_row(t, u);
-  of_stored = Moments{mean.b, rsqrtf(var.b / n + a.eps)};
-  return Moments{mean.a, rsqrtf(var.a / n + a.eps)};
+  of_stored = Moments{mean.b, rsqrtf(fmaf(var.b, share, a.eps))};
+  return Moments{mean.a, rsqrtf(fmaf(var.a, share, a.eps))};
+}
+
+// v times, or plus, a parameter's values, chunk by chunk of the row.
+template <int G, int NV, bool kVec, bool kAdd, typename T>
+__device__ __forceinline__ void with_param(const void* p, bool f32, int cols, int lane, float2 v[NV][4]) {
+  const auto each = [&](auto type) {
+    using P = decltype(type);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!any<G, kVec>(cols, i)) continue;
+      float2 w[4];
+      Chunk<P, kVec> c;
+      c.template load<G>(static_cast<const P*>(p), cols, lane, i);
+      c.get(w);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[i][j] = kAdd ? add2(v[i][j], w[j]) : mul2(v[i][j], w[j]);
+    }
+  };
+  if (!p) return;
+  if (sizeof(T) == 4 || f32)
+    each(float());
+  else
+    each(T());
 }
 
 // With fewer than 32 threads to a row, a warp has several rows under way, of which the
@@ -177,7 +213,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
   load(r);
   for (; r - offset < rows; r += step) {
     const int there = r < rows ? cols : 0;
-    float2 v[NV][4], p[4];
+    float2 v[NV][4];
     Chunk<T, kVec> here_r[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -185,28 +221,32 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
       here_r[i] = next_r[i];
     }
     if (r - offset + step < rows) load(r + step);
-    const void* gate = gate_at(a, r, gate_size);
-    // D, the gate and the residual, on eight values
-    const auto join = [&](int i) {
+    const int64_t at = r * a.cols;
+    // D, the gate and the residual
+    const auto join = [&] {
       if (a.rule.threshold) {
-        Mask<G, kVec> mask;
-        mask.make(key, r, lane, i);
-        apply(mask, key, &v[i][0].x);
-      }
-      if (gate) {
-        load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = mul2(v[i][j], p[j]);
+        for (int i = 0; i < NV; ++i) {
+          if (!any<G, kVec>(cols, i)) continue;
+          Mask<G, kVec> mask;
+          mask.make(key, r, lane, i);
+          apply(mask, key, &v[i][0].x);
+        }
       }
-      here_r[i].get(p);
+      with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, v);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[i][j] = fma2(alpha, p[j], v[i][j]);
-      if (a.s) store_chunk<G, kVec>(static_cast<T*>(a.s) + r * a.cols, there, lane, i, &v[i][0].x);
+      for (int i = 0; i < NV; ++i) {
+        float2 p[4];
+        here_r[i].get(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[i][j] = fma2(alpha, p[j], v[i][j]);
+      }
+      if (a.s) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store_chunk<G, kVec>(static_cast<T*>(a.s) + at, there, lane, i, &v[i][0].x);
+      }
     };
-    if (!kBranch) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) join(i);
-    }
+    if (!kBranch) join();
     Moments m, kept;
     if (!kBranch && sizeof(T) == 2 && a.rstd) {
       m = moments<G, NV, kVec, true, T>(v, a, cols, lane, buf, turn, kept);
@@ -220,23 +260,16 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
     }
     const float2 scale = both(m.rstd), minus = both(-m.mean);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
+    for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = mul2(add2(v[i][j], minus), scale);
-      if (a.w) {
-        load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+    with_param<G, NV, kVec, false, T>(a.w, a.weight_f32, cols, lane, v);
+    with_param<G, NV, kVec, true, T>(a.b, a.weight_f32, cols, lane, v);
+    if (kBranch) {
+      join();
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = mul2(v[i][j], p[j]);
-      }
-      if (a.b) {
-        load_param<G, kVec, T>(a.b, a.weight_f32, cols, lane, i, p);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = add2(v[i][j], p[j]);
-      }
-      if (kBranch)
-        join(i);
-      else
-        store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, there, lane, i, &v[i][0].x);
+      for (int i = 0; i < NV; ++i) store_chunk<G, kVec>(static_cast<T*>(a.y) + at, there, lane, i, &v[i][0].x);
     }
   }
 }
@@ -251,8 +284,11 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
   return Unit{begin, min(begin + grid.unit_rows, first + grid.group_rows), group};
 }
 
+// Blocks to an SM: as many as leave the sums of NV chunks in registers.
+constexpr int backward_blocks(int threads, int chunks) { return threads > 256 ? 1 : (chunks == 1 ? 768 : 512) / threads; }
+
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
-__global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
+__global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::kThreads, NV))
     backward_kernel(const Args a, const Grid grid) {
   constexpr int kRows = Shape<G>::kRows, kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
@@ -260,9 +296,9 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
   int turn = 0;
   const int lane = threadIdx.x % G, slot = threadIdx.x / G, cols = static_cast<int>(a.cols);
   const int gate_size = a.gate_f32 ? 4 : sizeof(T);
-  const float n = static_cast<float>(a.cols);
   const drop::Key key = drop::key_of(a.rule);
   const float2 alpha = both(a.alpha);
+  const bool normed = kBranch || a.gy;
   float2 dw[NV][4] = {}, db[NV][4] = {}, dg[kGate ? NV : 1][4] = {};
 
   // Sums over the block's rows, of this thread's columns, into `out`.
@@ -292,172 +328,187 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, 512 / Shape<G>::kThreads)
       }
     }
   };
-  // dgate of eight values: added up, or a row of its own
-  const auto put_gate = [&](uint32_t r, int there, int i, float2 t[4]) {
-    if (grid.sums_gate) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) dg[kGate ? i : 0][j] = add2(dg[kGate ? i : 0][j], t[j]);
-    } else if (a.gate_f32) {
-      store_chunk<G, kVec>(static_cast<float*>(a.dgate) + r * a.cols, there, lane, i, &t[0].x);
-    } else {
-      store_chunk<G, kVec>(static_cast<T*>(a.dgate) + r * a.cols, there, lane, i, &t[0].x);
-    }
-  };
 
   for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
     const Unit unit = unit_of(grid, u);
     const uint32_t end = static_cast<uint32_t>(unit.end), offset = slot % kTogether;
-    for (uint32_t r = static_cast<uint32_t>(unit.begin) + slot; r - offset < end; r += kRows) {
-      const bool valid = r < end;
-      const int there = valid ? cols : 0;
-      const void* gate = gate_at(a, r, gate_size);
-      Chunk<T, kVec> x[NV], g[NV];
-      const T* x_row = kBranch ? static_cast<const T*>(a.h) + r * a.h_stride
-                               : static_cast<const T*>(a.sum) + r * a.sum_stride;
-      const T* g_row = kBranch ? static_cast<const T*>(a.gs) + r * a.gs_stride
-                               : static_cast<const T*>(a.gy) + r * a.gy_stride;
-      const bool normed = kBranch || a.gy;
+    uint32_t r = static_cast<uint32_t>(unit.begin) + slot;
+    // the norm's rows and what reaches its output, one row ahead
+    Chunk<T, kVec> next_x[NV], next_g[NV];
+    float next_mean = 0.f, next_rstd = 0.f;
+    const auto load = [&](uint32_t row) {
+      if (!normed) return;
+      const int there = row < end ? cols : 0;
+      const T* x = kBranch ? static_cast<const T*>(a.h) + row * a.h_stride : static_cast<const T*>(a.sum) + row * a.sum_stride;
+      const T* g = kBranch ? static_cast<const T*>(a.gs) + row * a.gs_stride : static_cast<const T*>(a.gy) + row * a.gy_stride;
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        if (normed) {
-          x[i].template load<G>(x_row, there, lane, i);
-          g[i].template load<G>(g_row, there, lane, i);
+        next_x[i].template load<G>(x, there, lane, i);
+        next_g[i].template load<G>(g, there, lane, i);
+      }
+      next_mean = there && a.mean ? a.mean[row] : 0.f;
+      next_rstd = there ? a.rstd[row] : 0.f;
+    };
+    load(r);
+    for (; r - offset < end; r += kRows) {
+      const int there = r < end ? cols : 0;
+      const int64_t at = r * a.cols;
+      Chunk<T, kVec> x[NV], g[NV];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[i] = next_x[i], g[i] = next_g[i];
+      const float rstd = next_rstd;
+      const float2 scale = both(rstd), minus = both(-next_mean);
+      // what else the row needs, on its way while the sums are taken
+      Chunk<T, kVec> more[kBranch ? 1 : NV], branch[kGate && !kBranch ? NV : 1];
+      if (!kBranch) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (a.gs) more[kBranch ? 0 : i].template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, there, lane, i);
+          if (kGate) branch[kGate && !kBranch ? i : 0].template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, there, lane, i);
         }
       }
-      const float mean = normed && valid && a.mean ? a.mean[r] : 0.f, rstd = normed && valid ? a.rstd[r] : 0.f;
-      const float2 scale = both(rstd), minus = both(-mean);
-      float2 sum = both(0.f), dot = both(0.f);
-      if (!kBranch) {
-        if (normed) {
+      if (r - offset + kRows < end) load(r + kRows);
+      float2 sum = both(0.f), dot = both(0.f), d[NV][4];
+      // x - mean of eight values
+      const auto centred = [&](int i, float2 k[4]) {
+        x[i].get(k);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) k[j] = add2(k[j], minus);
+      };
+      // from d, what reaches the norm's output: dw, db, and d times the weight with its sums
+      const auto take_sums = [&] {
+        const auto add = [&](bool weighted) {
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
-            float2 k[4], d[4], p[4];
-            x[i].get(k);
-            g[i].get(d);
-            if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+            if (!any<G, kVec>(cols, i)) continue;
+            float2 k[4], w[4];
+            centred(i, k);
+            if (weighted) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, w);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              k[j] = mul2(add2(k[j], minus), scale);  // beyond the row the gradient is 0, and counts for nothing
-              dw[i][j] = fma2(d[j], k[j], dw[i][j]);
-              db[i][j] = add2(db[i][j], d[j]);
-              if (a.w) d[j] = mul2(d[j], p[j]);
-              sum = add2(sum, d[j]);
-              dot = fma2(d[j], k[j], dot);
+              k[j] = mul2(k[j], scale);  // beyond the row d is 0, and counts for nothing
+              dw[i][j] = fma2(d[i][j], k[j], dw[i][j]);
+              db[i][j] = add2(db[i][j], d[i][j]);
+              if (weighted) d[i][j] = mul2(d[i][j], w[j]);
+              sum = add2(sum, d[i][j]);
+              dot = fma2(d[i][j], k[j], dot);
             }
           }
-        }
-        if (!a.dh && !a.dr && !kGate) continue;
-        float2 c1 = both(0.f), c2 = both(0.f);
-        if (normed) {
-          const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
-          c1 = both(a.rms ? 0.f : -rstd * (s.a / n)), c2 = both(-rstd * rstd * (s.b / n));  // of s - mean
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float2 d[4], p[4];
-          if (normed) {
-            float2 k[4];
-            x[i].get(k);
-            g[i].get(d);
-            if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (a.w) d[j] = mul2(d[j], p[j]);
-              d[j] = fma2(add2(k[j], minus), c2, fma2(d[j], scale, c1));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = both(0.f);
-          }
-          if (a.gs) {
-            Chunk<T, kVec> more;
-            more.template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, there, lane, i);
-            more.get(p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = add2(d[j], p[j]);
-          }
-          if (a.dr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[j]);
-            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, there, lane, i, &p[0].x);
-          }
-          if (!kGate && !a.dh) continue;
-          Mask<G, kVec> mask;
-          if (a.rule.threshold) mask.make(key, r, lane, i);
-          if (kGate) {
-            Chunk<T, kVec> branch;
-            branch.template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, there, lane, i);
-            branch.get(p);
-            if (a.rule.threshold) apply(mask, key, &p[0].x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[j]);
-            put_gate(r, there, i, p);
-          }
-          if (!a.dh) continue;
-          if (a.rule.threshold) apply(mask, key, &d[0].x);
-          if (gate) {
-            load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = mul2(d[j], p[j]);
-          }
-          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, there, lane, i, &d[0].x);
-        }
-      } else {
-        float2 d[NV][4];
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float2 k[4], p[4], w[4];
-          x[i].get(k);
-          g[i].get(d[i]);
-          if (a.dr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[i][j]);
-            store_chunk<G, kVec>(static_cast<T*>(a.dr) + r * a.cols, there, lane, i, &p[0].x);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) k[j] = mul2(add2(k[j], minus), scale);
-          if (a.w) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, w);
-          Mask<G, kVec> mask;
-          if (a.rule.threshold) mask.make(key, r, lane, i);
-          if (kGate) {
-            float2 b[4];
-            if (a.b) load_param<G, kVec, T>(a.b, a.weight_f32, cols, lane, i, b);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              p[j] = a.w ? mul2(k[j], w[j]) : k[j];
-              if (a.b) p[j] = add2(p[j], b[j]);
-            }
-            if (a.rule.threshold) apply(mask, key, &p[0].x);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = mul2(p[j], d[i][j]);
-            put_gate(r, there, i, p);
-          }
-          if (a.rule.threshold) apply(mask, key, &d[i][0].x);
-          if (gate) {
-            load_param<G, kVec, T>(gate, a.gate_f32, cols, lane, i, p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[i][j] = mul2(d[i][j], p[j]);
-          }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            dw[i][j] = fma2(d[i][j], k[j], dw[i][j]);
-            db[i][j] = add2(db[i][j], d[i][j]);
-            if (a.w) d[i][j] = mul2(d[i][j], w[j]);
-            sum = add2(sum, d[i][j]);
-            dot = fma2(d[i][j], k[j], dot);
-          }
-        }
-        if (!a.dh) continue;
-        const Sums s = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
-        const float2 c1 = both(a.rms ? 0.f : -rstd * (s.a / n)), c2 = both(-rstd * rstd * (s.b / n));  // of h - mean
+        };
+        a.w ? add(true) : add(false);
+      };
+      // the gradient of the norm's input in the place of d
+      const auto through_norm = [&] {
+        const Sums t = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
+        const float2 c1 = both(a.rms ? 0.f : -rstd * (t.a * a.share)), c2 = both(-rstd * rstd * (t.b * a.share));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           float2 k[4];
-          x[i].get(k);
+          centred(i, k);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[i][j] = fma2(add2(k[j], minus), c2, fma2(d[i][j], scale, c1));
-          store_chunk<G, kVec>(static_cast<T*>(a.dh) + r * a.cols, there, lane, i, &d[i][0].x);
+          for (int j = 0; j < 4; ++j) d[i][j] = fma2(k[j], c2, fma2(d[i][j], scale, c1));
         }
+      };
+      const auto put_rows = [&](void* p, float2 v[NV][4]) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) store_chunk<G, kVec>(static_cast<T*>(p) + at, there, lane, i, &v[i][0].x);
+      };
+      const auto put_residual = [&] {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          float2 p[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = mul2(alpha, d[i][j]);
+          store_chunk<G, kVec>(static_cast<T*>(a.dr) + at, there, lane, i, &p[0].x);
+        }
+      };
+      // dgate of eight values, what reaches the sum times the branch's t: added up, or a row of its own
+      const auto put_gate = [&](int i, float2 t[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = mul2(t[j], d[i][j]);
+        if (grid.sums_gate) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) dg[kGate ? i : 0][j] = add2(dg[kGate ? i : 0][j], t[j]);
+        } else if (a.gate_f32) {
+          store_chunk<G, kVec>(static_cast<float*>(a.dgate) + at, there, lane, i, &t[0].x);
+        } else {
+          store_chunk<G, kVec>(static_cast<T*>(a.dgate) + at, there, lane, i, &t[0].x);
+        }
+      };
+      // d through dropout; the gate's gradient on the way, from D of the branch
+      const auto through_dropout = [&](auto&& branch_of) {
+        const auto each = [&](bool some) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            if (!any<G, kVec>(cols, i)) continue;
+            Mask<G, kVec> mask;
+            if (some) mask.make(key, r, lane, i);
+            if (kGate) {
+              float2 t[4];
+              branch_of(i, t);
+              if (some) apply(mask, key, &t[0].x);
+              put_gate(i, t);
+            }
+            if (some) apply(mask, key, &d[i][0].x);
+          }
+        };
+        if (a.rule.threshold)
+          each(true);
+        else if (kGate)
+          each(false);
+      };
+      if (!kBranch) {
+        if (normed) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) g[i].get(d[i]);
+          take_sums();
+          if (!a.dh && !a.dr && !kGate) continue;
+          through_norm();
+        } else {
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[i][j] = both(0.f);
+        }
+        if (a.gs) {
+#pragma unroll
+          for (int i = 0; i < NV; ++i) {
+            float2 p[4];
+            more[kBranch ? 0 : i].get(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[i][j] = add2(d[i][j], p[j]);
+          }
+        }
+        if (a.dr) put_residual();
+        through_dropout([&](int i, float2 t[4]) { branch[kGate && !kBranch ? i : 0].get(t); });
+        if (!a.dh) continue;
+        with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, d);
+        put_rows(a.dh, d);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) g[i].get(d[i]);
+        if (a.dr) put_residual();
+        through_dropout([&](int i, float2 t[4]) {  // norm(h)
+          centred(i, t);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[j] = mul2(t[j], scale);
+          float2 p[4];
+          if (a.w) {
+            load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = mul2(t[j], p[j]);
+          }
+          if (a.b) {
+            load_param<G, kVec, T>(a.b, a.weight_f32, cols, lane, i, p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = add2(t[j], p[j]);
+          }
+        });
+        with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, d);
+        take_sums();
+        if (!a.dh) continue;
+        through_norm();
+        put_rows(a.dh, d);
       }
     }
     if (kGate && grid.sums_gate) {
@@ -746,7 +797,7 @@ cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) 
   if (kVec && a.cols <= 128)
     backward_kernel<kVec ? 16 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (kVec && a.cols <= 256)
-    backward_kernel<kVec ? 16 : 32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+    backward_kernel<32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (a.cols <= 512)
     backward_kernel<32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (a.cols <= 2048)
