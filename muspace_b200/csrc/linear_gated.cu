@@ -18,15 +18,45 @@
 namespace lin {
 namespace {
 
-// 16 columns of a warp's rows, gate and up, without waiting for them.
-__device__ __forceinline__ void take_both(uint32_t gate_at, uint32_t up_at, float g[16], float u[16]) {
-  uint32_t a[16], b[16];
-  tmem_load16(gate_at, a);
-  tmem_load16(up_at, b);
-  tmem_wait(a);
-  tmem_wait(b);
+// Eight columns of this warp's 32 lanes of tensor memory, without waiting for them.
+__device__ __forceinline__ void ask8(uint32_t addr, uint32_t r[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(addr)
+               : "memory");
+}
+
+// The loads so far have arrived; the registers pass through, so none is read before.
+__device__ __forceinline__ void arrived8(uint32_t r[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+
+// Bias of eight columns, the same for all lanes.
+template <typename T>
+__device__ __forceinline__ void add_bias8(const T* p, bool vec, int count, float v[8]) {
+  float b[8];
+  load_some(p, count, vec && count >= 8, b);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) g[j] = __uint_as_float(a[j]), u[j] = __uint_as_float(b[j]);
+  for (int j = 0; j < 8; j += 2) {
+    const float2 s = add2(make_float2(v[j], v[j + 1]), make_float2(b[j], b[j + 1]));
+    v[j] = s.x, v[j + 1] = s.y;
+  }
+}
+
+// Eight values of a row into the box from column `col` on.
+template <int kRowBytes>
+__device__ __forceinline__ void put8(uint32_t box, int row, int col, const float v[8], bf16) {
+  put_unit(unit_at<kRowBytes>(box, row, col / 8), pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+}
+template <int kRowBytes>
+__device__ __forceinline__ void put8(uint32_t box, int row, int col, const float v[8], float) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    put_unit(unit_at<kRowBytes>(box, row, col / 4 + u), __float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]),
+             __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3]));
 }
 
 // Of N values (whole eights) gate sums g and up sums u, both with their bias: the
@@ -140,23 +170,33 @@ __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, co
     if (lane == 0) stores_read<kTrain ? 0 : 2>();
     __syncwarp();
     const uint32_t out = kTrain ? box : box + part * kPart;
+    const uint32_t gate_at = acc_at + group * kOut, up_at = gate_at + BN / 2;
+    uint32_t next_g[8], next_u[8];
+    ask8(gate_at, next_g);
+    ask8(up_at, next_u);
 #pragma unroll 1
-    for (int c = 0; c < kOut; c += 16) {
-      float g[16], u[16], s[16];
-      Bias16<T> bias, more;
+    for (int c = 0; c < kOut; c += 8) {  // sixteen columns at a time spilled: KKK
+      float g[8], u[8], s[8];
+      arrived8(next_g);
+      arrived8(next_u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = __uint_as_float(next_g[j]), u[j] = __uint_as_float(next_u[j]);
+      const int ahead = c + 8 < kOut ? c + 8 : c;  // the last eight are asked for again
+      ask8(gate_at + ahead, next_g);
+      ask8(up_at + ahead, next_u);
       if (with_bias) {
-        bias.load(bias_gate + n0 + c, bias_vec, rows_n - n0 - c);
-        more.load(bias_up + n0 + c, bias_vec, rows_n - n0 - c);
+        add_bias8(bias_gate + n0 + c, bias_vec, rows_n - n0 - c, g);
+        add_bias8(bias_up + n0 + c, bias_vec, rows_n - n0 - c, u);
       }
-      take_both(acc_at + group * kOut + c, acc_at + BN / 2 + group * kOut + c, g, u);
-      if (with_bias) bias.add(g), more.add(u);
-      gate_values<kFast, kTrain, 16>(kAct, e.rule, key, m + lane, (n0 + c) / 8, g, u, s);
-      put16<kRowBytes>(out, lane, c, g, T());
+      gate_values<kFast, kTrain, 8>(kAct, e.rule, key, m + lane, (n0 + c) / 8, g, u, s);
+      put8<kRowBytes>(out, lane, c, g, T());
       if (kTrain) {
-        put16<kRowBytes>(box + kPart, lane, c, s, T());
-        put16<kRowBytes>(box + 2 * kPart, lane, c, u, T());
+        put8<kRowBytes>(box + kPart, lane, c, s, T());
+        put8<kRowBytes>(box + 2 * kPart, lane, c, u, T());
       }
     }
+    arrived8(next_g);
+    arrived8(next_u);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     fence_before();
     __syncwarp();

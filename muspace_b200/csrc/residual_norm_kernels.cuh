@@ -285,7 +285,7 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
 }
 
 // Blocks to an SM: as many as leave the sums of NV chunks in registers.
-constexpr int backward_blocks(int threads, int chunks) { return threads > 256 ? 1 : (chunks == 1 ? 768 : 512) / threads; }
+constexpr int backward_blocks(int threads, int chunks) { return chunks == 1 ? (threads > 256 ? 1 : 768 / threads) : threads > 256 ? 1 : 512 / threads; }
 
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
 __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::kThreads, NV))
@@ -770,6 +770,15 @@ cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
 
 template <bool kVec, bool kBranch, typename T>
 cudaError_t forward_form(const Args& a, cudaStream_t stream) {
+  if constexpr (kVec) {
+    if (a.cols <= 128) return launch_forward<16, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 256) return launch_forward<32, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 512) return launch_forward<64, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 1024) return launch_forward<128, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 2048) return launch_forward<256, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 4096) return launch_forward<512, 1, true, kBranch, T>(a, stream);
+    if (a.cols <= 8192) return launch_forward<1024, 1, true, kBranch, T>(a, stream);
+  }
   if (a.cols <= 1024) {
     if (kVec && a.cols <= 128) return launch_forward<kVec ? 16 : 32, kVec ? 1 : 4, kVec, kBranch, T>(a, stream);
     if (kVec && a.cols <= 256) return launch_forward<kVec ? 16 : 32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
@@ -794,7 +803,16 @@ cudaError_t forward_of(const Args& a, cudaStream_t stream) {
 
 template <bool kVec, bool kBranch, bool kGate, typename T>
 cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) {
-  if (kVec && a.cols <= 128)
+  if (kVec && a.cols > 256 && a.cols <= 4096) {
+    if (a.cols <= 512)
+      backward_kernel<kVec ? 64 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 64, 0, stream>>>(a, grid);
+    else if (a.cols <= 1024)
+      backward_kernel<kVec ? 128 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 128, 0, stream>>>(a, grid);
+    else if (a.cols <= 2048)
+      backward_kernel<kVec ? 256 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
+    else
+      backward_kernel<kVec ? 512 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 512, 0, stream>>>(a, grid);
+  } else if (kVec && a.cols <= 128)
     backward_kernel<kVec ? 16 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
   else if (kVec && a.cols <= 256)
     backward_kernel<32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
