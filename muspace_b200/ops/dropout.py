@@ -24,7 +24,7 @@ OPERATOR_NAME = "dropout"
 def check_rule(p, seed, sequence, needed: bool = False) -> tuple[int, int, int, torch.Tensor | None]:
     """``(threshold, seed, sequence, seed tensor)`` of a dropout; the seed is needed
     where something is dropped, or always."""
-    if isinstance(p, bool) or not isinstance(p, Real):
+    if p.__class__ is not float and (isinstance(p, bool) or not isinstance(p, Real)):
         raise TypeError("the dropout probability must be a number")
     if not 0.0 <= p <= 1.0:  # NaN is outside too
         raise ValueError(f"the dropout probability must be between 0 and 1, got {p}")
@@ -33,7 +33,7 @@ def check_rule(p, seed, sequence, needed: bool = False) -> tuple[int, int, int, 
         if threshold or needed:
             raise ValueError("dropout needs a seed")
         return 0, 0, 0, None
-    if isinstance(sequence, bool) or not isinstance(sequence, Integral):
+    if sequence.__class__ is not int and (isinstance(sequence, bool) or not isinstance(sequence, Integral)):
         raise TypeError("sequence must be an integer")
     if not 0 <= sequence < 2 ** 63:
         raise ValueError(f"sequence must be between 0 and 2^63 - 1, got {sequence}")
@@ -43,7 +43,7 @@ def check_rule(p, seed, sequence, needed: bool = False) -> tuple[int, int, int, 
         if seed.numel() != 1:
             raise ValueError(f"a seed tensor must have one element, got shape {tuple(seed.shape)}")
         return threshold, 0, int(sequence), seed
-    if isinstance(seed, bool) or not isinstance(seed, Integral):
+    if seed.__class__ is not int and (isinstance(seed, bool) or not isinstance(seed, Integral)):
         raise TypeError("seed must be an integer or an int64 tensor")
     if not 0 <= seed < 2 ** 63:
         raise ValueError(f"seed must be between 0 and 2^63 - 1, got {seed}")
@@ -53,7 +53,7 @@ def check_rule(p, seed, sequence, needed: bool = False) -> tuple[int, int, int, 
 def _apply(module: NativeModule, x, threshold, seed, sequence, seed_tensor):
     rows, stride = rows_of(x)
     count, width = map(int, rows.shape)  # tensors while tracing
-    out = x.new_empty(x.shape)
+    out = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     module.plain_call("msda_dropout")(x.device, WIDE_DTYPE_CODES[x.dtype], rows.data_ptr(), count, width, stride,
                                       threshold, seed, sequence, pointer(seed_tensor), out.data_ptr())
     return out

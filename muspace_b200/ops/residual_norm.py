@@ -29,60 +29,43 @@ from .dropout import check_rule
 KINDS = {"layer": 0, "rms": 1}
 
 
-class _Rule:
-    """What a call has beside its tensors."""
-
-    __slots__ = ("branch", "kind", "scale", "eps", "threshold", "seed", "sequence", "groups", "want_sum")
-
-    def __init__(self, branch, kind, scale, eps, threshold, seed, sequence, groups, want_sum):
-        self.branch, self.kind, self.scale, self.eps = branch, kind, scale, eps
-        self.threshold, self.seed, self.sequence = threshold, seed, sequence
-        self.groups, self.want_sum = groups, want_sum
+# What a call has beside its tensors, as a tuple: branch, kind, residual scale, eps,
+# threshold, seed, sequence, groups of the gate, whether the sum is asked for.
+#
+# Both passes below are written for few Python steps: in training, the host's part of a
+# call with short rows takes longer than its kernels.
 
 
-def _args(rule: _Rule, dtype, weight, bias, gate, count: int, width: int, seed_tensor) -> ResidualNormArgs:
-    code = WIDE_DTYPE_CODES[dtype]
-    kind = weight if weight is not None else bias
-    args = ResidualNormArgs(code, code if kind is None else WIDE_DTYPE_CODES[kind.dtype],
-                            code if gate is None else WIDE_DTYPE_CODES[gate.dtype], rule.kind, count, width,
-                            rule.groups)
-    args.residual_scale, args.eps = rule.scale, rule.eps
-    args.threshold, args.seed, args.sequence = rule.threshold, rule.seed, rule.sequence
-    args.seed_at = pointer(seed_tensor)
-    args.weight, args.bias = pointer(weight), pointer(bias)
-    return args
+def _fresh(like: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of the same shape and kind."""
+    return torch.empty_like(like) if like.is_contiguous() else like.new_empty(like.shape)
 
 
-def _gate_rows(args, gate, width: int):
-    """Lays the gate out as rows, one to a group, and notes them; the tensor to hold."""
-    if gate is not None:
-        gate, args.gate_stride = rows_of(gate)
-        args.gate = gate.data_ptr()
-    return gate
-
-
-def _forward(module: NativeModule, rule: _Rule, x, residual, weight, bias, gate, seed_tensor, keep: bool):
+def _forward(module: NativeModule, rule, x, residual, weight, bias, gate, seed_tensor, keep: bool):
     """``(output or None, sum or None, statistics or None)``."""
+    branch, kind, scale, eps, threshold, seed, sequence, groups, want_sum = rule
     rows, x_stride = rows_of(x)
     residual, r_stride = rows_of(residual)
     count, width = map(int, rows.shape)  # tensors while tracing
-    args = _args(rule, x.dtype, weight, bias, gate, count, width, seed_tensor)
-    gate = _gate_rows(args, gate, width)
-    args.input, args.input_stride = rows.data_ptr(), x_stride
-    args.residual, args.residual_stride = residual.data_ptr(), r_stride
-    out = total = statistics = None
-    if not rule.branch:
-        out = x.new_empty(x.shape)
-        args.output = out.data_ptr()
-    if rule.branch or rule.want_sum or keep:
-        total = x.new_empty(x.shape)
-        args.sum = total.data_ptr()
+    code = WIDE_DTYPE_CODES[x.dtype]
+    param = weight if weight is not None else bias
+    gate_code = code
+    gate_stride = 0
+    if gate is not None:
+        gate_code = WIDE_DTYPE_CODES[gate.dtype]
+        gate, gate_stride = rows_of(gate)
+    out = None if branch else _fresh(x)
+    total = _fresh(x) if branch or want_sum or keep else None
+    statistics = mean = rstd = None
     if keep:
-        statistics = torch.empty((2 - rule.kind, count), dtype=torch.float32, device=x.device)
-        args.rstd = statistics.data_ptr()
-        if rule.kind == 0:
-            args.mean = args.rstd + 4 * count if count else args.rstd
-    module.plain_call("msda_norm_add_forward" if rule.branch else "msda_add_norm_forward")(x.device, args)
+        statistics = torch.empty((2, count), dtype=torch.float32, device=x.device)
+        mean = statistics.data_ptr()
+        rstd = mean + 4 * count
+    module.plain_call("msda_norm_add_forward" if branch else "msda_add_norm_forward")(x.device, ResidualNormArgs(
+        code, code if param is None else WIDE_DTYPE_CODES[param.dtype], gate_code, kind, count, width, groups,
+        x_stride, r_stride, gate_stride, 0, 0, 0, scale, eps, threshold, seed, sequence, pointer(seed_tensor),
+        rows.data_ptr(), residual.data_ptr(), pointer(gate), pointer(weight), pointer(bias), pointer(out),
+        pointer(total), mean, rstd))
     return out, total, statistics
 
 
@@ -90,24 +73,21 @@ class _ResidualNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, bias, gate, seed_tensor, rule):
         ctx.set_materialize_grads(False)
-        keep = any(ctx.needs_input_grad)
-        out, total, statistics = _forward(native_module(), rule, x, residual, weight, bias, gate, seed_tensor, keep)
-        need_x, need_r, need_w, need_b, need_gate = ctx.needs_input_grad[:5]
-        if rule.branch:
-            # the residual's gradient alone needs nothing of the norm
-            some = need_x or need_w or need_b or need_gate
-            kept = (x if some else None, weight if need_x or need_gate else None, bias if need_gate else None,
-                    gate, statistics if some else None, seed_tensor)
-        else:
-            kept = (x if need_gate else None, weight, None, gate, statistics, seed_tensor)
+        needs = ctx.needs_input_grad
+        out, total, statistics = _forward(native_module(), rule, x, residual, weight, bias, gate, seed_tensor,
+                                          any(needs))
+        need_x, _, need_w, need_b, need_gate = needs[:5]
         ctx.rule = rule
-        ctx.width = x.size(-1)
         ctx.kinds = (x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype,
                      gate if gate is None else (gate.dtype, gate.shape))
-        ctx.save_for_backward(*kept, None if rule.branch else total)
-        if rule.branch:
+        if rule[0]:
+            # the residual's gradient alone needs nothing of the norm
+            some = need_x or need_w or need_b or need_gate
+            ctx.save_for_backward(x if some else None, weight if need_x or need_gate else None,
+                                  bias if need_gate else None, gate, statistics if some else None, seed_tensor, None)
             return total
-        return (out, total) if rule.want_sum else out
+        ctx.save_for_backward(x if need_gate else None, weight, None, gate, statistics, seed_tensor, total)
+        return (out, total) if rule[-1] else out
 
     @staticmethod
     def backward(ctx, *grads):
@@ -116,70 +96,66 @@ class _ResidualNormFunction(torch.autograd.Function):
 
 
 def _backward(ctx, *grads):
-    rule = ctx.rule
-    grad_y, grad_s = (None, grads[0]) if rule.branch else (grads[0], grads[1] if rule.want_sum else None)
+    branch, kind, scale, eps, threshold, seed, sequence, groups, want_sum = rule = ctx.rule
+    grad_y, grad_s = (None, grads[0]) if branch else (grads[0], grads[1] if want_sum else None)
     first = grad_s if grad_y is None else grad_y
     if first is None:
         return (None,) * 7
     x, weight, bias, gate, statistics, seed_tensor, total = ctx.saved_tensors
     need_x, need_r, need_w, need_b, need_gate = ctx.needs_input_grad[:5]
-    normed = rule.branch or grad_y is not None
-    need_w, need_b = need_w and normed, need_b and normed
-    shape, width = first.shape, ctx.width
-    plain = rule.scale == 1.0
+    if not branch and grad_y is None:
+        need_w = need_b = False
     dx = dr = dw = db = dgate = None
-    if rule.branch:
-        if need_r and (plain or not (need_x or need_w or need_b or need_gate)):
-            dr, need_r = grad_s if plain else grad_s * rule.scale, False  # nothing of the norm is in it
-        same = False
-    else:
+    same = False
+    if branch:
+        if need_r and (scale == 1.0 or not (need_x or need_w or need_b or need_gate)):
+            dr, need_r = grad_s if scale == 1.0 else grad_s * scale, False  # nothing of the norm is in it
+    elif need_x and need_r:
         # without gate and dropout both parts of the sum have one gradient
-        same = need_x and need_r and plain and gate is None and rule.threshold == 0
+        same = scale == 1.0 and gate is None and threshold == 0
     if not (need_x or need_r or need_w or need_b or need_gate):
         return None, dr, None, None, None, None, None
-    kind, gate_kind = ctx.kinds
-    count = first.numel() // width if width else prod(shape[:-1])
-    args = _args(rule, first.dtype, weight, bias, gate, count, width, seed_tensor)
-    args.weight_dtype = WIDE_DTYPE_CODES[kind]
-    gate = _gate_rows(args, gate, width)
-    hold = []
+    param, gate_kind = ctx.kinds
+    device, dtype = first.device, first.dtype
+    code = WIDE_DTYPE_CODES[dtype]
+    rows, stride = rows_of(first)
+    count, width = rows.shape
+    y_stride = s_stride = x_stride = total_stride = gate_stride = 0
+    y_at = s_at = total_at = mean = rstd = None
     if grad_y is not None:
-        g, args.grad_output_stride = rows_of(grad_y)
-        args.grad_output = g.data_ptr()
-        hold.append(g)
-    if grad_s is not None:
-        g, args.grad_sum_stride = rows_of(grad_s)
-        args.grad_sum = g.data_ptr()
-        hold.append(g)
+        y_at, y_stride = rows.data_ptr(), stride
+        if grad_s is not None and (need_x or need_r or need_gate):  # what reaches the sum reaches no weight or bias
+            more, s_stride = rows_of(grad_s)
+            s_at = more.data_ptr()
+    else:
+        s_at, s_stride = rows.data_ptr(), stride
     if x is not None:
-        x, args.input_stride = rows_of(x)
-        args.input = x.data_ptr()
+        x, x_stride = rows_of(x)
     if total is not None:
-        total, args.sum_stride = rows_of(total)
-        args.sum = total.data_ptr()
+        total_at, total_stride = total.data_ptr(), width  # laid out by the forward
+    gate_code = code
+    if gate_kind is not None:
+        gate_code = WIDE_DTYPE_CODES[gate_kind[0]]
+        gate, gate_stride = rows_of(gate)
     if statistics is not None:
-        args.rstd = statistics.data_ptr()
-        if rule.kind == 0:
-            args.mean = args.rstd + 4 * count if count else args.rstd
+        mean = statistics.data_ptr()
+        rstd = mean + 4 * count
     if need_x:
-        dx = first.new_empty(shape)
-        args.grad_input = dx.data_ptr()
+        dx = _fresh(first)
     if need_r and not same:
-        dr = first.new_empty(shape)
-        args.grad_residual = dr.data_ptr()
+        dr = _fresh(first)
     if need_w:
-        dw = torch.empty(width, dtype=kind, device=first.device)
-        args.grad_weight = dw.data_ptr()
+        dw = torch.empty(width, dtype=param, device=device)
     if need_b:
-        db = torch.empty(width, dtype=kind, device=first.device)
-        args.grad_bias = db.data_ptr()
+        db = torch.empty(width, dtype=param, device=device)
     if need_gate:
-        dgate = torch.empty(gate_kind[1], dtype=gate_kind[0], device=first.device)
-        args.grad_gate = dgate.data_ptr()
-    if not rule.branch and not (need_x or need_r or need_gate):
-        args.grad_sum = None  # what reaches the sum does not reach weight and bias
-    native_module().plain_call("msda_norm_add_backward" if rule.branch else "msda_add_norm_backward")(
-        first.device, args)
+        dgate = torch.empty(gate_kind[1], dtype=gate_kind[0], device=device)
+    native_module().plain_call("msda_norm_add_backward" if branch else "msda_add_norm_backward")(
+        device, ResidualNormArgs(
+            code, WIDE_DTYPE_CODES[param], gate_code, kind, count, width, groups, x_stride, 0, gate_stride,
+            total_stride, y_stride, s_stride, scale, eps, threshold, seed, sequence, pointer(seed_tensor), pointer(x),
+            None, pointer(gate), pointer(weight), pointer(bias), None, total_at, mean, rstd, y_at, s_at, pointer(dx),
+            pointer(dr), pointer(dw), pointer(db), pointer(dgate)))
     return dx, dx if same else dr, dw, db, dgate, None, None
 
 
@@ -241,15 +217,15 @@ def _call(operator: str, input, residual, weight, bias, gate, residual_scale, ki
         gate, groups = _groups_of(gate, input.shape)
     module, report = decide(operator, backend, input, residual, weight, bias, gate, seed_tensor)
     weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
-    rule = _Rule(operator == "norm_add", KINDS[kind], float(residual_scale), float(eps), threshold, number, sequence,
-                 groups, want_sum)
+    rule = (operator == "norm_add", KINDS[kind], float(residual_scale), float(eps), threshold, number, sequence, groups,
+            want_sum)
     tensors = (input, residual, weight, bias, gate)
     try:
         if autograd_sees(*tensors):
             output = _ResidualNormFunction.apply(*tensors, seed_tensor, rule)
         else:
             out, total, _ = _forward(module, rule, *tensors, seed_tensor, False)
-            output = total if rule.branch else (out, total) if want_sum else out
+            output = total if rule[0] else (out, total) if want_sum else out
     except RuntimeError as exc:
         failed(report, str(exc))
         raise
