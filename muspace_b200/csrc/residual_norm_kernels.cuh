@@ -82,6 +82,25 @@ struct Mask<G, false> {
   __device__ __forceinline__ bool kept(const drop::Key&, int j) const { return bits >> j & 1u; }
 };
 
+// A parameter's values of a thread's columns, held in registers through all rows where
+// a thread has but one chunk; where there is no parameter, `none`.
+template <int G, bool kVec, typename T>
+struct Held {
+  float2 v[4];
+  __device__ __forceinline__ void set(const void* p, bool f32, int there, int lane, float none) {
+    if (p) {
+      load_param<G, kVec, T>(p, f32, there, lane, 0, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = both(none);
+    }
+  }
+};
+// Rows of one chunk a thread are bound by issue, and loads and conversions of
+// parameters were a fifth of it.
+template <int G, int NV>
+constexpr bool kHolds = NV == 1;
+
 template <typename M>
 __device__ __forceinline__ void apply(const M& mask, const drop::Key& key, float* v) {
 #pragma unroll
@@ -163,9 +182,10 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
   return Moments{mean.a, rsqrtf(fmaf(var.a, share, a.eps))};
 }
 
-// v times, or plus, a parameter's values, chunk by chunk of the row.
+// v times, or plus, a parameter's values, chunk by chunk of the row; `there`: cols, or
+// 0 where the row is not there, and nothing may be loaded for it.
 template <int G, int NV, bool kVec, bool kAdd, typename T>
-__device__ __forceinline__ void with_param(const void* p, bool f32, int cols, int lane, float2 v[NV][4]) {
+__device__ __forceinline__ void with_param(const void* p, bool f32, int cols, int there, int lane, float2 v[NV][4]) {
   const auto each = [&](auto type) {
     using P = decltype(type);
 #pragma unroll
@@ -173,7 +193,7 @@ __device__ __forceinline__ void with_param(const void* p, bool f32, int cols, in
       if (!any<G, kVec>(cols, i)) continue;
       float2 w[4];
       Chunk<P, kVec> c;
-      c.template load<G>(static_cast<const P*>(p), cols, lane, i);
+      c.template load<G>(static_cast<const P*>(p), there, lane, i);
       c.get(w);
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = kAdd ? add2(v[i][j], w[j]) : mul2(v[i][j], w[j]);
@@ -199,6 +219,14 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
   const T *h = static_cast<const T*>(a.h), *res = static_cast<const T*>(a.r);
   const drop::Key key = drop::key_of(a.rule);
   const float2 alpha = both(a.alpha);
+  constexpr bool kHold = kHolds<G, NV>;
+  Held<G, kVec, T> held_w, held_b, held_gate;
+  const bool one_gate = !a.gate || a.gate_rows == a.rows;
+  if (kHold) {
+    held_w.set(a.w, a.weight_f32, cols, lane, 1.f);
+    held_b.set(a.b, a.weight_f32, cols, lane, 0.f);
+    held_gate.set(one_gate ? a.gate : nullptr, a.gate_f32, cols, lane, 1.f);
+  }
   const uint32_t offset = threadIdx.x / G % kTogether;
   uint32_t r = blockIdx.x * Shape<G>::kRows + threadIdx.x / G;
   Chunk<T, kVec> next_h[NV], next_r[NV];
@@ -233,7 +261,13 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
           apply(mask, key, &v[i][0].x);
         }
       }
-      with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, v);
+      if (kHold) {
+        if (!one_gate) held_gate.set(gate_at(a, r, gate_size), a.gate_f32, there, lane, 1.f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[0][j] = mul2(v[0][j], held_gate.v[j]);
+      } else {
+        with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, there, lane, v);
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         float2 p[4];
@@ -263,8 +297,13 @@ __global__ void __launch_bounds__(Shape<G>::kThreads) forward_kernel(const Args 
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = mul2(add2(v[i][j], minus), scale);
-    with_param<G, NV, kVec, false, T>(a.w, a.weight_f32, cols, lane, v);
-    with_param<G, NV, kVec, true, T>(a.b, a.weight_f32, cols, lane, v);
+    if (kHold) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[0][j] = fma2(v[0][j], held_w.v[j], held_b.v[j]);
+    } else {
+      with_param<G, NV, kVec, false, T>(a.w, a.weight_f32, cols, cols, lane, v);
+      with_param<G, NV, kVec, true, T>(a.b, a.weight_f32, cols, cols, lane, v);
+    }
     if (kBranch) {
       join();
     } else {
@@ -284,11 +323,11 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
   return Unit{begin, min(begin + grid.unit_rows, first + grid.group_rows), group};
 }
 
-// Blocks to an SM: as many as leave the sums of NV chunks in registers.
-constexpr int backward_blocks(int threads, int chunks) { return chunks == 1 ? (threads > 256 ? 1 : 768 / threads) : threads > 256 ? 1 : 512 / threads; }
+// Blocks to an SM: 128 registers a thread, for the sums, the parameters and a row ahead.
+constexpr int backward_blocks(int threads) { return 512 / threads; }
 
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
-__global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::kThreads, NV))
+__global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::kThreads))
     backward_kernel(const Args a, const Grid grid) {
   constexpr int kRows = Shape<G>::kRows, kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
@@ -299,6 +338,15 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
   const drop::Key key = drop::key_of(a.rule);
   const float2 alpha = both(a.alpha);
   const bool normed = kBranch || a.gy;
+  constexpr bool kHold = kHolds<G, NV>;
+  Held<G, kVec, T> held_w, held_b, held_gate;
+  // a unit's rows share a row of the gate, or else each looks its own up
+  const bool one_gate = !a.gate || a.gate_rows == a.rows || grid.sums_gate;
+  if (kHold) {
+    held_w.set(a.w, a.weight_f32, cols, lane, 1.f);
+    if (kBranch && kGate) held_b.set(a.b, a.weight_f32, cols, lane, 0.f);
+    if (!one_gate) held_gate.set(nullptr, false, cols, lane, 1.f);
+  }
   float2 dw[NV][4] = {}, db[NV][4] = {}, dg[kGate ? NV : 1][4] = {};
 
   // Sums over the block's rows, of this thread's columns, into `out`.
@@ -333,6 +381,8 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
     const Unit unit = unit_of(grid, u);
     const uint32_t end = static_cast<uint32_t>(unit.end), offset = slot % kTogether;
     uint32_t r = static_cast<uint32_t>(unit.begin) + slot;
+    if (kHold && one_gate)
+      held_gate.set(gate_at(a, static_cast<uint32_t>(unit.begin), gate_size), a.gate_f32, cols, lane, 1.f);
     // the norm's rows and what reaches its output, one row ahead
     Chunk<T, kVec> next_x[NV], next_g[NV];
     float next_mean = 0.f, next_rstd = 0.f;
@@ -383,7 +433,12 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
             if (!any<G, kVec>(cols, i)) continue;
             float2 k[4], w[4];
             centred(i, k);
-            if (weighted) load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, w);
+            if (kHold) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[j] = held_w.v[j];
+            } else if (weighted) {
+              load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, w);
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               k[j] = mul2(k[j], scale);  // beyond the row d is 0, and counts for nothing
@@ -395,7 +450,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
             }
           }
         };
-        a.w ? add(true) : add(false);
+        kHold || a.w ? add(true) : add(false);
       };
       // the gradient of the norm's input in the place of d
       const auto through_norm = [&] {
@@ -433,6 +488,15 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
           store_chunk<G, kVec>(static_cast<float*>(a.dgate) + at, there, lane, i, &t[0].x);
         } else {
           store_chunk<G, kVec>(static_cast<T*>(a.dgate) + at, there, lane, i, &t[0].x);
+        }
+      };
+      const auto through_gate = [&] {
+        if (kHold) {
+          if (!one_gate) held_gate.set(gate_at(a, r, gate_size), a.gate_f32, there, lane, 1.f);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[0][j] = mul2(d[0][j], held_gate.v[j]);
+        } else {
+          with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, there, lane, d);
         }
       };
       // d through dropout; the gate's gradient on the way, from D of the branch
@@ -482,7 +546,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
         if (a.dr) put_residual();
         through_dropout([&](int i, float2 t[4]) { branch[kGate && !kBranch ? i : 0].get(t); });
         if (!a.dh) continue;
-        with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, d);
+        through_gate();
         put_rows(a.dh, d);
       } else {
 #pragma unroll
@@ -492,6 +556,11 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
           centred(i, t);
 #pragma unroll
           for (int j = 0; j < 4; ++j) t[j] = mul2(t[j], scale);
+          if (kHold) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = fma2(t[j], held_w.v[j], held_b.v[j]);
+            return;
+          }
           float2 p[4];
           if (a.w) {
             load_param<G, kVec, T>(a.w, a.weight_f32, cols, lane, i, p);
@@ -504,7 +573,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
             for (int j = 0; j < 4; ++j) t[j] = add2(t[j], p[j]);
           }
         });
-        with_param<G, NV, kVec, false, T>(gate_at(a, r, gate_size), a.gate_f32, cols, lane, d);
+        through_gate();
         take_sums();
         if (!a.dh) continue;
         through_norm();
@@ -770,24 +839,12 @@ cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
 
 template <bool kVec, bool kBranch, typename T>
 cudaError_t forward_form(const Args& a, cudaStream_t stream) {
-  if constexpr (kVec) {
-    if (a.cols <= 128) return launch_forward<16, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 256) return launch_forward<32, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 512) return launch_forward<64, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 1024) return launch_forward<128, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 2048) return launch_forward<256, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 4096) return launch_forward<512, 1, true, kBranch, T>(a, stream);
-    if (a.cols <= 8192) return launch_forward<1024, 1, true, kBranch, T>(a, stream);
-  }
-  if (a.cols <= 1024) {
-    if (kVec && a.cols <= 128) return launch_forward<kVec ? 16 : 32, kVec ? 1 : 4, kVec, kBranch, T>(a, stream);
-    if (kVec && a.cols <= 256) return launch_forward<kVec ? 16 : 32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
-    if (kVec && a.cols <= 512) return launch_forward<32, kVec ? 2 : 4, kVec, kBranch, T>(a, stream);
-    return launch_forward<32, 4, kVec, kBranch, T>(a, stream);
-  }
-  // few rows: short ones in time, not many in flight
-  if (a.cols <= 4096 && a.rows < 296) return launch_forward<512, 1, kVec, kBranch, T>(a, stream);
-  if (a.cols <= 4096) return launch_forward<256, 2, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 128) return launch_forward<kVec ? 16 : 32, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 256) return launch_forward<32, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 512) return launch_forward<64, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 1024) return launch_forward<128, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 2048) return launch_forward<256, 1, kVec, kBranch, T>(a, stream);
+  if (a.cols <= 4096) return launch_forward<512, 1, kVec, kBranch, T>(a, stream);
   if (a.cols <= 8192) return launch_forward<512, 2, kVec, kBranch, T>(a, stream);
   const int blocks = static_cast<int>(std::min<int64_t>(a.rows, 148 * 2));
   forward_long_kernel<kBranch, T><<<blocks, kLong, 0, stream>>>(a);
@@ -801,31 +858,22 @@ cudaError_t forward_of(const Args& a, cudaStream_t stream) {
   return a.branch ? forward_form<false, true, T>(a, stream) : forward_form<false, false, T>(a, stream);
 }
 
+template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
+cudaError_t launch_backward(const Args& a, const Grid& grid, cudaStream_t stream) {
+  backward_kernel<G, NV, kVec, kBranch, kGate, T><<<grid.blocks, Shape<G>::kThreads, 0, stream>>>(a, grid);
+  return cudaGetLastError();
+}
+
 template <bool kVec, bool kBranch, bool kGate, typename T>
 cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) {
-  if (kVec && a.cols > 256 && a.cols <= 4096) {
-    if (a.cols <= 512)
-      backward_kernel<kVec ? 64 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 64, 0, stream>>>(a, grid);
-    else if (a.cols <= 1024)
-      backward_kernel<kVec ? 128 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 128, 0, stream>>>(a, grid);
-    else if (a.cols <= 2048)
-      backward_kernel<kVec ? 256 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
-    else
-      backward_kernel<kVec ? 512 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 512, 0, stream>>>(a, grid);
-  } else if (kVec && a.cols <= 128)
-    backward_kernel<kVec ? 16 : 32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
-  else if (kVec && a.cols <= 256)
-    backward_kernel<32, kVec ? 1 : 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
-  else if (a.cols <= 512)
-    backward_kernel<32, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
-  else if (a.cols <= 2048)
-    backward_kernel<128, 2, kVec, kBranch, kGate, T><<<grid.blocks, 128, 0, stream>>>(a, grid);
-  else if (a.cols <= 4096)
-    backward_kernel<256, 2, kVec, kBranch, kGate, T><<<grid.blocks, 256, 0, stream>>>(a, grid);
-  else if (a.cols <= 8192)
-    backward_kernel<512, 2, kVec, kBranch, kGate, T><<<grid.blocks, 512, 0, stream>>>(a, grid);
-  else
-    backward_long_kernel<kBranch, T><<<grid.blocks, kLong, 0, stream>>>(a, grid);
+  if (a.cols <= 128) return launch_backward<kVec ? 16 : 32, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 256) return launch_backward<32, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 512) return launch_backward<64, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 1024) return launch_backward<128, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 2048) return launch_backward<256, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 4096) return launch_backward<512, 1, kVec, kBranch, kGate, T>(a, grid, stream);
+  if (a.cols <= 8192) return launch_backward<512, 2, kVec, kBranch, kGate, T>(a, grid, stream);
+  backward_long_kernel<kBranch, T><<<grid.blocks, kLong, 0, stream>>>(a, grid);
   return cudaGetLastError();
 }
 
