@@ -166,7 +166,10 @@ cudaError_t launch(const A& a, bool vec, cudaStream_t stream) {
   // Four warps to a weight row where one each would leave half of the GPU's
   // warps idle over rows of eight steps or more (bfloat16, one row of 8192:
   // 1024 weight rows 16 us with one warp, 7 with four; 4096 x 4096 8.4 and 10).
-  const bool shared = steps >= 8 && groups < 148 * 16;
+  // The gated operator's warp has two rows to read at a time, and four warps to them
+  // are the faster ones up to where each has several (1 x 4096, 2 x 4096 weight rows:
+  // 13.2 us, in turn of one step; with one warp to both rows 14.6, in turns of eight 18).
+  const bool shared = steps >= 8 && groups < 148 * (kHalves<A> == 2 ? 64 : 16);
   const int64_t per_block = (shared ? kWarps / 4 : kWarps) * kCols;
   const dim3 grid(static_cast<unsigned>((a.out + per_block - 1) / per_block),
                   static_cast<unsigned>((a.rows + kRows - 1) / kRows));
@@ -185,7 +188,7 @@ cudaError_t launch_rows(const A& a, cudaStream_t stream) {
   };
   const bool vec = aligned(a.x, a.rows == 1 ? 0 : a.x_stride) && aligned(a.w, kHalves<A> * a.out == 1 ? 0 : a.w_stride) &&
                    (a.in * sizeof(T)) % 16 == 0;
-  if (a.rows == 1) return launch<T, 1, 1, 4>(a, vec, stream);
+  if (a.rows == 1) return launch<T, 1, 1, kHalves<A> == 2 ? 1 : 4>(a, vec, stream);
   if (a.rows <= 4) return launch<T, 4, 1, 2>(a, vec, stream);
   return launch<T, 8, 2 / kHalves<A>, 2>(a, vec, stream);
 }
@@ -208,8 +211,13 @@ cudaError_t forward_few_rows(const Args& a, cudaStream_t stream) {
   return a.dtype == DType::kF32 ? launch_rows<float>(a, stream) : launch_rows<bf16>(a, stream);
 }
 
+// The same of the gated operator. bfloat16: 1 x 4096 x 2 x 4096 13.2 / 20.2, 4 rows 22.0
+// / 20.2, and 4 x 4096 x 2 x 1024 8.2 / 11.6; 8 rows of up to 2^21 weights 6.4 / 7.4, of
+// 2^23 16.5 / 11.7. float32 as the plain operator of twice the columns: 16 x 4096 x 2 x
+// 4096 103 / 149, 64 x 256 x 2 x 512 7.5 / 15.4, 64 x 1024 x 2 x 1024 35 / 21.
 bool gated_few_rows(const GatedArgs& a) {
-  Args as{};  // a product of twice the columns
+  if (a.dtype == DType::kBF16) return a.rows <= 4 || (a.rows <= 8 && 2 * a.out * a.in <= 1ll << 21);
+  Args as{};
   as.dtype = a.dtype, as.rows = a.rows, as.in = a.in, as.out = 2 * a.out;
   return few_rows(as);
 }

@@ -185,7 +185,9 @@ cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slo
 }
 
 // dst = [g * P, g * Q] with the sums of both halves' columns, before the rounding: a
-// lane takes eight columns of g and the same of either half.
+// lane takes eight columns of g and the same of either half. Bound by memory: 40000 x
+// 512 bfloat16 (205 MB) 36 us, 5.6 TB/s; two rows unrolled 46, more blocks to an SM 52
+// to 66 (spills).
 template <typename T>
 __global__ void __launch_bounds__(32 * kSumWarps, 4)
     gate_operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec, const T* __restrict__ factors,
@@ -200,21 +202,23 @@ __global__ void __launch_bounds__(32 * kSumWarps, 4)
   float s[2][8] = {};
   if (c < cols) {
     for (int64_t r = begin + warp; r < end; r += kSumWarps) {
-      float v[8], f[8];
+      float v[8], f[2][8];
       load_some(src + r * src_ld + c, count, src_vec && count == 8, v);
 #pragma unroll
+      for (int half = 0; half < 2; ++half)
+        load_some(factors + (2 * r + half) * cols + c, count, factors_vec && count == 8, f[half]);
+#pragma unroll
       for (int half = 0; half < 2; ++half) {
-        load_some(factors + (2 * r + half) * cols + c, count, factors_vec && count == 8, f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          f[j] *= v[j];
-          s[half][j] += f[j];
+          f[half][j] *= v[j];
+          s[half][j] += f[half][j];
         }
         bf16* at = dst + r * dst_ld + half * cols + c;
         if (sizeof(T) == 4)
-          store_planes(at, plane, count, vec, f);
+          store_planes(at, plane, count, vec, f[half]);
         else
-          store_some(at, count, vec, f);
+          store_some(at, count, vec, f[half]);
       }
     }
   }
