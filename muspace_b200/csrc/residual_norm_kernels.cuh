@@ -206,17 +206,18 @@ __device__ __forceinline__ void with_param(const void* p, bool f32, int cols, in
     each(T());
 }
 
-// Blocks to an SM, where 64 registers a thread do: not for short rows of float32 (44446
-// x 256: 36 us in 64 registers, 30 in 78), nor where columns are apart.
+// Blocks to an SM that 64 registers a thread allow, where they do: not for short rows of
+// float32 (44446 x 256: 36 us in 64 registers, 30 in 78), nor where columns are apart
+// (30000 x 260 bfloat16: 64 and 47 us). 0: as the compiler likes.
 template <typename T>
-constexpr int forward_blocks(int threads, int chunks, bool vec) {
-  return vec && chunks == 1 && (sizeof(T) == 2 || threads == 512) ? 1024 / (threads < 256 && threads > 32 ? threads : threads == 512 ? 512 : 256) : 1;
+constexpr int forward_blocks(int row_threads, int threads, bool one_vector) {
+  return one_vector && (sizeof(T) == 2 || row_threads == 512) ? 1024 / threads : 0;
 }
 
 // With fewer than 32 threads to a row, a warp has several rows under way, of which the
 // last may not be there: its loads give 0, and it stores nothing.
 template <int G, int NV, bool kVec, bool kBranch, typename T>
-__global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, NV, kVec)) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, Shape<G>::kThreads, kVec && NV == 1)) forward_kernel(const Args a) {
   constexpr int kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
   int turn = 0;
