@@ -414,12 +414,11 @@ int msda_linear_act_backward(const msda_linear_t* args, void* stream) {
 int msda_layer_wait_timeouts(unsigned int* count) {
   return guarded([&] {
     require(count != nullptr, "count is null");
-    unsigned int linear = 0, gated = 0, norm = 0, residual = 0;
+    unsigned int linear = 0, gated = 0, norm = 0;
     check_launch(lin::wait_timeouts(&linear), "msda_layer_wait_timeouts");
     check_launch(lin::gated_wait_timeouts(&gated), "msda_layer_wait_timeouts");
     check_launch(lnorm::wait_timeouts(&norm), "msda_layer_wait_timeouts");
-    check_launch(resnorm::wait_timeouts(&residual), "msda_layer_wait_timeouts");
-    *count = linear + gated + norm + residual;
+    *count = linear + gated + norm;
   });
 }
 

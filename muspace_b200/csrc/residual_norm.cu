@@ -61,37 +61,8 @@ cudaError_t join(const Args& a, const Grid& grid, cudaStream_t stream) {
 
 }  // namespace
 
-bool vectors_fit(const Args& a) {
-  const int64_t size = a.dtype == DType::kF32 ? 4 : 2;
-  const auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
-  const auto rows_fit = [&](const void* p, int64_t stride, int64_t bytes) {
-    return !p || (aligned(p) && stride * bytes % 16 == 0);
-  };
-  bool ok = a.cols % 8 == 0;
-  ok = ok && rows_fit(a.h, a.h_stride, size) && rows_fit(a.r, a.r_stride, size);
-  ok = ok && rows_fit(a.gate, a.gate_stride, a.gate_f32 ? 4 : size);
-  ok = ok && rows_fit(a.gy, a.gy_stride, size) && rows_fit(a.gs, a.gs_stride, size);
-  ok = ok && rows_fit(a.sum, a.sum_stride, size);
-  for (const void* p : {a.w, a.b, static_cast<const void*>(a.y), static_cast<const void*>(a.s),
-                        static_cast<const void*>(a.dh), static_cast<const void*>(a.dr),
-                        static_cast<const void*>(a.dgate)})
-    ok = ok && aligned(p);
-  return ok;
-}
-
-int ring_stages(const Args& a, int tensors, bool two_blocks) {
-  if (a.cols <= 1024 || a.cols > 8192 || a.rows < 148 * 8) return 0;
-  const int64_t groups = a.cols <= 2048 ? 2 : 1, memory = two_blocks ? kRingBytes / 2 : kRingBytes;
-  const int64_t stages = memory / (a.cols * (a.dtype == DType::kF32 ? 4 : 2) * tensors * groups);
-  return stages < 2 ? 0 : static_cast<int>(std::min<int64_t>(stages, kMaxStages));
-}
-
 Grid backward_grid(const Args& a) {
   Grid grid;
-  // the ring's stages are free again at a row's sums, so there have to be some
-  grid.tensors = 2 + (!a.branch && a.gs ? 1 : 0) + (!a.branch && a.dgate ? 1 : 0);
-  if (vectors_fit(a) && (a.branch ? a.dh != nullptr : a.gy && (a.dh || a.dr || a.dgate)))
-    grid.stages = ring_stages(a, grid.tensors, false);
   grid.sums_gate = a.dgate && a.gate_rows != 1;
   grid.group_rows = grid.sums_gate ? a.gate_rows : a.rows;
   const int64_t groups = a.rows / grid.group_rows;
@@ -100,7 +71,7 @@ Grid backward_grid(const Args& a) {
   const int64_t most = 148ll * (a.cols <= 256    ? 2
                                 : a.cols <= 512  ? 8
                                 : a.cols <= 1024 ? 4
-                                : a.cols <= 2048 ? (grid.stages ? 1 : 2)
+                                : a.cols <= 2048 ? 2
                                                  : 1);
   const int64_t wanted = std::max<int64_t>(1, most / groups);
   grid.unit_rows = (grid.group_rows + wanted - 1) / wanted;
@@ -115,15 +86,6 @@ int64_t backward_parts(const Args& a) {
   if (a.rows == 0 || a.cols == 0 || (!a.dw && !a.db && !a.dgate)) return 0;
   const Grid grid = backward_grid(a);
   return (2 * grid.blocks + (grid.sums_gate ? grid.units : 0)) * a.cols;
-}
-
-cudaError_t wait_timeouts(unsigned int* count) {
-  unsigned int f32 = 0, b16 = 0, f16 = 0;
-  cudaError_t err = wait_timeouts_f32(&f32);
-  if (err == cudaSuccess) err = wait_timeouts_bf16(&b16);
-  if (err == cudaSuccess) err = wait_timeouts_f16(&f16);
-  *count = f32 + b16 + f16;
-  return err;
 }
 
 cudaError_t forward(const Args& a, cudaStream_t stream) {

@@ -53,23 +53,12 @@ struct Args {
 int64_t backward_parts(const Args& a);
 cudaError_t forward(const Args& a, cudaStream_t stream);
 cudaError_t backward(const Args& a, cudaStream_t stream);
-cudaError_t wait_timeouts(unsigned int* count);
-
-// Rows of whole eights at 16-byte boundaries.
-bool vectors_fit(const Args& a);
-
-// Rows of 1025 to 8192 columns, so many of them that a ring in shared memory pays: its
-// stages, of a row of `tensors` tensors for each of a block's groups, for one block or
-// two of an SM. 0: no ring.
-constexpr int kRingThreads = 512, kMaxStages = 8, kRingBytes = 200 * 1024;
-int ring_stages(const Args& a, int tensors, bool two_blocks);
 
 // Of one storage type (residual_norm_<type>.cu).
 struct Grid {
   int blocks = 0;
   int64_t units = 0, unit_rows = 0, group_units = 0, group_rows = 0;
   bool sums_gate = false;  // the gate's gradient is a sum over rows
-  int tensors = 0, stages = 0;  // of the ring
 };
 Grid backward_grid(const Args& a);
 cudaError_t forward_f32(const Args& a, cudaStream_t stream);
@@ -78,8 +67,5 @@ cudaError_t forward_f16(const Args& a, cudaStream_t stream);
 cudaError_t backward_f32(const Args& a, const Grid& grid, cudaStream_t stream);
 cudaError_t backward_bf16(const Args& a, const Grid& grid, cudaStream_t stream);
 cudaError_t backward_f16(const Args& a, const Grid& grid, cudaStream_t stream);
-cudaError_t wait_timeouts_f32(unsigned int* count);
-cudaError_t wait_timeouts_bf16(unsigned int* count);
-cudaError_t wait_timeouts_f16(unsigned int* count);
 
 }  // namespace resnorm

@@ -9,6 +9,4 @@ cudaError_t backward_bf16(const Args& a, const Grid& grid, cudaStream_t stream) 
   return backward_of<lin::bf16>(a, grid, stream);
 }
 
-cudaError_t wait_timeouts_bf16(unsigned int* count) { return async::read_timeouts(count); }
-
 }  // namespace resnorm

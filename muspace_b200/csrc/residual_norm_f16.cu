@@ -9,6 +9,4 @@ cudaError_t backward_f16(const Args& a, const Grid& grid, cudaStream_t stream) {
   return backward_of<__half>(a, grid, stream);
 }
 
-cudaError_t wait_timeouts_f16(unsigned int* count) { return async::read_timeouts(count); }
-
 }  // namespace resnorm

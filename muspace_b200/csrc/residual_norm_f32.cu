@@ -9,6 +9,4 @@ cudaError_t backward_f32(const Args& a, const Grid& grid, cudaStream_t stream) {
   return backward_of<float>(a, grid, stream);
 }
 
-cudaError_t wait_timeouts_f32(unsigned int* count) { return async::read_timeouts(count); }
-
 }  // namespace resnorm

@@ -19,10 +19,6 @@
 // statistics of the unrounded one, k's sum over a row is not 0, nor that of its squares
 // n; where a row's mean is large beside its spread nothing of the gradient is left.)
 //
-// Rows of more than 1024 columns come to shared memory by bulk copies, several rows
-// ahead: their sums need barriers, and registers hold no more than one more row
-// meanwhile. KKK
-//
 // A backward block takes whole units of neighbouring rows, a unit's rows all under
 // one row of the gate: so a thread sums dw, db and dgate of its columns in
 // registers, writes them once, and a second kernel adds the blocks' sums in order.
@@ -30,7 +26,6 @@
 
 #include <algorithm>
 
-#include "async_device.cuh"
 #include "dropout_device.cuh"
 #include "residual_norm.h"
 #include "rows_device.cuh"
@@ -135,15 +130,15 @@ __device__ __forceinline__ bool any(int cols, int i) {
 
 // Mean and rstd of the row whose values lie in v; beyond the row v is 0. kBoth: and
 // those of the values as T stores them, in the same reductions.
-template <int G, int NV, bool kVec, bool kBoth, bool kNamed, typename T>
+template <int G, int NV, bool kVec, bool kBoth, typename T>
 __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a, int cols, int lane, Sums* buf,
                                            int& turn, Moments& of_stored) {
   const float share = a.share;
   const auto over_row = [&](float2 x, float2 y) {
     if constexpr (kBoth)
-      return row_sums<G, kNamed>(Sums{x.x + x.y, y.x + y.y}, buf, turn);
+      return row_sums<G>(Sums{x.x + x.y, y.x + y.y}, buf, turn);
     else
-      return Sums{row_sums<G, kNamed>(x.x + x.y, buf, turn), 0.f};
+      return Sums{row_sums<G>(x.x + x.y, buf, turn), 0.f};
   };
   float2 w[kBoth ? NV : 1][4];
   if (kBoth) {
@@ -211,75 +206,6 @@ __device__ __forceinline__ void with_param(const void* p, bool f32, int cols, in
     each(T());
 }
 
-// A group of G threads' rows on their way into shared memory. A stage holds one row of
-// each of a few tensors; its barrier counts their bytes. One thread (`fetcher`) starts
-// the copies; everyone waits for them.
-struct Ring {
-  uint32_t at, bars;  // shared memory: this group's first stage, its barriers
-  uint32_t row_bytes, tensors;
-  int stages;
-  int stage = 0, fill = 0;  // of the row at hand, and the one to be filled next
-  uint32_t phase = 0, fetched = 0, taken = 0;
-  bool fetcher, dead = false;
-
-  __device__ __forceinline__ Ring(uint8_t* memory, uint64_t (*barriers)[kMaxStages], int group, int lane, uint32_t bytes,
-                                  uint32_t count, int depth)
-      : at(async::smem_addr(memory) + group * depth * bytes * count),
-        bars(async::smem_addr(barriers[group])),
-        row_bytes(bytes),
-        tensors(count),
-        stages(depth),
-        fetcher(lane == 0) {
-    if (fetcher) {
-      for (int i = 0; i < stages; ++i) async::barrier_init(bars + 8 * i, 1);
-      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (stages) __syncthreads();
-  }
-  __device__ __forceinline__ bool room() const { return fetched - taken < static_cast<uint32_t>(stages) && !dead; }
-  // One row of each tensor, by the fetcher, where there is room.
-  template <typename... P>
-  __device__ __forceinline__ void fetch(const P*... rows) {
-    const uint32_t bar = bars + 8 * fill;
-    uint32_t to = at + fill * tensors * row_bytes;
-    async::expect_bytes(bar, tensors * row_bytes);
-    const auto copy = [&](const void* row) {
-      if (row) async::copy_bytes(to, row, row_bytes, bar), to += row_bytes;
-    };
-    (copy(rows), ...);
-    ++fetched;
-    if (++fill == stages) fill = 0;
-  }
-  __device__ __forceinline__ void wait() { async::wait(bars + 8 * stage, phase, dead); }
-  // Eight values of the row at hand, of its n-th tensor.
-  template <typename T>
-  __device__ __forceinline__ void get(int n, int c, float2 v[4]) const {
-    uint32_t u[2 * sizeof(T)];
-    raw<T>(n, c, u);
-    lin::load8(reinterpret_cast<const T*>(u), &v[0].x);
-  }
-  template <typename T>
-  __device__ __forceinline__ void raw(int n, int c, uint32_t* u) const {
-    const uint32_t from = at + (stage * tensors + n) * row_bytes + c * sizeof(T);
-#pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k)
-      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(u[4 * k]), "=r"(u[4 * k + 1]), "=r"(u[4 * k + 2]), "=r"(u[4 * k + 3])
-                   : "r"(from + 16 * k)
-                   : "memory");
-  }
-  __device__ __forceinline__ void next() {
-    ++taken;
-    if (++stage == stages) stage = 0, phase ^= 1;
-  }
-  // Copies in flight land before their memory goes.
-  __device__ __forceinline__ void settle() const {
-    if (!fetcher) return;
-    for (uint32_t i = fetched > stages ? fetched - stages : 0; i < fetched; ++i)
-      async::settle(bars + 8 * (i % stages), i / stages & 1);
-  }
-};
-
 // Blocks to an SM that 64 registers a thread allow, where they do: not for short rows of
 // float32 (44446 x 256: 36 us in 64 registers, 30 in 78), nor where columns are apart
 // (30000 x 260 bfloat16: 64 and 47 us). 0: as the compiler likes.
@@ -290,21 +216,14 @@ constexpr int forward_blocks(int row_threads, int threads, bool one_vector) {
 
 // With fewer than 32 threads to a row, a warp has several rows under way, of which the
 // last may not be there: its loads give 0, and it stores nothing.
-template <int G, bool kRing>
-constexpr int kThreads = kRing ? kRingThreads : Shape<G>::kThreads;
-
-template <int G, int NV, bool kVec, bool kRing, bool kBranch, typename T>
-__global__ void __launch_bounds__(kThreads<G, kRing>, forward_blocks<T>(G, kThreads<G, kRing>, kVec && NV == 1))
-    forward_kernel(const Args a, int stages) {
-  constexpr int kTogether = G < 32 ? 32 / G : 1, kRows = kThreads<G, kRing> / G;
-  extern __shared__ __align__(16) uint8_t memory[];
-  __shared__ Sums bufs[kRing ? kRows : 1][Shape<G>::kBuf];
-  __shared__ __align__(8) uint64_t barriers[kRing ? kRows : 1][kMaxStages];
-  Sums* buf = bufs[kRing ? threadIdx.x / G : 0];
+template <int G, int NV, bool kVec, bool kBranch, typename T>
+__global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, Shape<G>::kThreads, kVec && NV == 1)) forward_kernel(const Args a) {
+  constexpr int kTogether = G < 32 ? 32 / G : 1;
+  __shared__ Sums buf[Shape<G>::kBuf];
   int turn = 0;
   const int lane = threadIdx.x % G, cols = static_cast<int>(a.cols);
   const int gate_size = a.gate_f32 ? 4 : sizeof(T);
-  const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * kRows;
+  const uint32_t rows = static_cast<uint32_t>(a.rows), step = gridDim.x * Shape<G>::kRows;
   const T *h = static_cast<const T*>(a.h), *res = static_cast<const T*>(a.r);
   const drop::Key key = drop::key_of(a.rule);
   const float2 alpha = both(a.alpha);
@@ -317,17 +236,9 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, forward_blocks<T>(G, kThre
     held_gate.set(one_gate ? a.gate : nullptr, a.gate_f32, cols, lane, 1.f);
   }
   const uint32_t offset = threadIdx.x / G % kTogether;
-  uint32_t r = blockIdx.x * kRows + threadIdx.x / G, ahead = r;
-  Ring ring(memory, barriers, kRing ? threadIdx.x / G : 0, kRing ? lane : 1, cols * sizeof(T), 2, kRing ? stages : 0);
-  const auto fetch = [&] {
-    if (kRing && ring.fetcher && ahead < rows && ring.room()) {
-      ring.fetch(h + ahead * a.h_stride, res + ahead * a.r_stride);
-      ahead += step;
-    }
-  };
+  uint32_t r = blockIdx.x * Shape<G>::kRows + threadIdx.x / G;
   Chunk<T, kVec> next_h[NV], next_r[NV];
   const auto load = [&](uint32_t row) {
-    if (kRing) return;
     const int there = row < rows ? cols : 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -336,31 +247,14 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, forward_blocks<T>(G, kThre
     }
   };
   load(r);
-  if (kRing)
-    for (int i = 0; i < stages; ++i) fetch();
   for (; r - offset < rows; r += step) {
     const int there = r < rows ? cols : 0;
     float2 v[NV][4];
     Chunk<T, kVec> here_r[NV];
-    if constexpr (kRing) {
-      ring.wait();
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = column<G, true>(lane, i, 0);
-        here_r[i].zero();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[i][j] = both(0.f);
-        if (c < cols) {
-          ring.template get<T>(0, c, v[i]);
-          ring.template raw<T>(1, c, &here_r[i].u[0].x);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        next_h[i].get(v[i]);
-        here_r[i] = next_r[i];
-      }
+    for (int i = 0; i < NV; ++i) {
+      next_h[i].get(v[i]);
+      here_r[i] = next_r[i];
     }
     if (r - offset + step < rows) load(r + step);
     const int64_t at = r * a.cols;
@@ -397,14 +291,10 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, forward_blocks<T>(G, kThre
     if (!kBranch) join();
     Moments m, kept;
     if (!kBranch && sizeof(T) == 2 && a.rstd) {
-      m = moments<G, NV, kVec, true, kRing, T>(v, a, cols, lane, buf, turn, kept);
+      m = moments<G, NV, kVec, true, T>(v, a, cols, lane, buf, turn, kept);
     } else {
       Moments none;
-      kept = m = moments<G, NV, kVec, false, kRing, T>(v, a, cols, lane, buf, turn, none);
-    }
-    if (kRing) {  // the group is past its reads of the row
-      ring.next();
-      fetch();
+      kept = m = moments<G, NV, kVec, false, T>(v, a, cols, lane, buf, turn, none);
     }
     if (a.rstd && lane == 0 && r < rows) {
       if (a.mean) a.mean[r] = kept.mean;
@@ -429,18 +319,6 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, forward_blocks<T>(G, kThre
       for (int i = 0; i < NV; ++i) store_chunk<G, kVec>(static_cast<T*>(a.y) + at, there, lane, i, &v[i][0].x);
     }
   }
-  if (kRing && __syncthreads_or(ring.dead)) {  // a wait ran out: NaNs, once no copy is in flight
-    ring.settle();
-    float nans[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) nans[j] = __uint_as_float(~0u);
-    for (r = blockIdx.x * kRows + threadIdx.x / G; r < rows; r += step)
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (a.y) store_chunk<G, kVec>(static_cast<T*>(a.y) + r * a.cols, cols, lane, i, nans);
-        if (a.s) store_chunk<G, kVec>(static_cast<T*>(a.s) + r * a.cols, cols, lane, i, nans);
-      }
-  }
 }
 
 // A unit of a backward block: rows [begin, end), all under the gate's row `group`.
@@ -456,14 +334,11 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
 // Blocks to an SM: 128 registers a thread, for the sums, the parameters and a row ahead.
 constexpr int backward_blocks(int threads) { return 512 / threads; }
 
-template <int G, int NV, bool kVec, bool kRing, bool kBranch, bool kGate, typename T>
-__global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G, kRing>))
-    backward_kernel(const Args a, const Grid grid, int stages) {
-  constexpr int kRows = kThreads<G, kRing> / G, kTogether = G < 32 ? 32 / G : 1;
-  extern __shared__ __align__(16) uint8_t memory[];
-  __shared__ Sums bufs[kRing ? kRows : 1][Shape<G>::kBuf];
-  __shared__ __align__(8) uint64_t barriers[kRing ? kRows : 1][kMaxStages];
-  Sums* buf = bufs[kRing ? threadIdx.x / G : 0];
+template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
+__global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::kThreads))
+    backward_kernel(const Args a, const Grid grid) {
+  constexpr int kRows = Shape<G>::kRows, kTogether = G < 32 ? 32 / G : 1;
+  __shared__ Sums buf[Shape<G>::kBuf];
   __shared__ float fold[kRows > 1 ? kRows * G * 8 : 1];
   int turn = 0;
   const int lane = threadIdx.x % G, slot = threadIdx.x / G, cols = static_cast<int>(a.cols);
@@ -492,12 +367,12 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
 #pragma unroll
         for (int j = 0; j < 8; ++j) fold[(slot * 8 + j) * G + lane] = mine[j];
         __syncthreads();
-        // thread (slot, lane) adds up column j = slot of lane's eight, and every kRows-th after it
-        for (int j = slot; j < 8; j += kRows) {
+        // thread (slot, lane) adds up column j = slot of lane's eight
+        if (slot < 8) {
           float sum = 0.f;
 #pragma unroll
-          for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + j) * G + lane];
-          const int c = column<G, kVec>(lane, i, j);
+          for (int k = 0; k < kRows; ++k) sum += fold[(k * 8 + slot) * G + lane];
+          const int c = column<G, kVec>(lane, i, slot);
           if (c < cols) out[c] = sum;
         }
       } else {
@@ -510,29 +385,10 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
     }
   };
 
-  // tensors of a row in the ring: x, g, and what add_norm needs besides
-  const bool with_sum = !kBranch && a.gs, with_branch = !kBranch && kGate;
-  Ring ring(memory, barriers, kRing ? slot : 0, kRing ? lane : 1, cols * sizeof(T), 2 + with_sum + with_branch,
-            kRing ? stages : 0);
   for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
     const Unit unit = unit_of(grid, u);
     const uint32_t end = static_cast<uint32_t>(unit.end), offset = slot % kTogether;
-    uint32_t r = static_cast<uint32_t>(unit.begin) + slot, ahead = r;
-    const auto fetch = [&] {
-      if (kRing && ring.fetcher && ahead < end && ring.room()) {
-        ring.fetch(kBranch ? static_cast<const T*>(a.h) + ahead * a.h_stride
-                           : static_cast<const T*>(a.sum) + ahead * a.sum_stride,
-                   kBranch ? static_cast<const T*>(a.gs) + ahead * a.gs_stride
-                           : static_cast<const T*>(a.gy) + ahead * a.gy_stride,
-                   with_sum ? static_cast<const T*>(a.gs) + ahead * a.gs_stride : nullptr,
-                   with_branch ? static_cast<const T*>(a.h) + ahead * a.h_stride : nullptr);
-        ahead += kRows;
-      }
-    };
-    if (kRing) {
-      if (u != blockIdx.x) __syncthreads();  // every group is past its last unit's rows
-      for (int i = 0; i < stages; ++i) fetch();
-    }
+    uint32_t r = static_cast<uint32_t>(unit.begin) + slot;
     if (kHold && one_gate)
       held_gate.set(gate_at(a, static_cast<uint32_t>(unit.begin), gate_size), a.gate_f32, cols, lane, 1.f);
     // the norm's rows and what reaches its output, one row ahead
@@ -544,7 +400,7 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
       const T* x = kBranch ? static_cast<const T*>(a.h) + row * a.h_stride : static_cast<const T*>(a.sum) + row * a.sum_stride;
       const T* g = kBranch ? static_cast<const T*>(a.gs) + row * a.gs_stride : static_cast<const T*>(a.gy) + row * a.gy_stride;
 #pragma unroll
-      for (int i = 0; i < (kRing ? 0 : NV); ++i) {
+      for (int i = 0; i < NV; ++i) {
         next_x[i].template load<G>(x, there, lane, i);
         next_g[i].template load<G>(g, there, lane, i);
       }
@@ -556,31 +412,13 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
       const int there = r < end ? cols : 0;
       const int64_t at = r * a.cols;
       Chunk<T, kVec> x[NV], g[NV];
-      if constexpr (kRing) {
-        ring.wait();
-      } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) x[i] = next_x[i], g[i] = next_g[i];
-      }
-      // eight values of a tensor of the row: from the ring, or from the registers
-      const auto take = [&](int n, const Chunk<T, kVec>& held, int i, float2 k[4]) {
-        if constexpr (kRing) {
-          const int c = column<G, true>(lane, i, 0);
-          if (c < cols) {
-            ring.template get<T>(n, c, k);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) k[j] = both(0.f);
-          }
-        } else {
-          held.get(k);
-        }
-      };
+      for (int i = 0; i < NV; ++i) x[i] = next_x[i], g[i] = next_g[i];
       const float rstd = next_rstd;
       const float2 scale = both(rstd), minus = both(-next_mean);
       // what else the row needs, on its way while the sums are taken
       Chunk<T, kVec> more[kBranch ? 1 : NV], branch[kGate && !kBranch ? NV : 1];
-      if (!kBranch && !kRing) {
+      if (!kBranch) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           if (a.gs) more[kBranch ? 0 : i].template load<G>(static_cast<const T*>(a.gs) + r * a.gs_stride, there, lane, i);
@@ -591,7 +429,7 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
       float2 sum = both(0.f), dot = both(0.f), d[NV][4];
       // x - mean of eight values
       const auto centred = [&](int i, float2 k[4]) {
-        take(0, x[i], i, k);
+        x[i].get(k);
 #pragma unroll
         for (int j = 0; j < 4; ++j) k[j] = add2(k[j], minus);
       };
@@ -624,8 +462,7 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
       };
       // the gradient of the norm's input in the place of d
       const auto through_norm = [&] {
-        const Sums t = row_sums<G, kRing>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
-        fetch();  // everyone is past the row before
+        const Sums t = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
         const float2 c1 = both(a.rms ? 0.f : -rstd * (t.a * a.share)), c2 = both(-rstd * rstd * (t.b * a.share));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -695,7 +532,7 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
       if (!kBranch) {
         if (normed) {
 #pragma unroll
-          for (int i = 0; i < NV; ++i) take(1, g[i], i, d[i]);
+          for (int i = 0; i < NV; ++i) g[i].get(d[i]);
           take_sums();
           if (!a.dh && !a.dr && !kGate) continue;
           through_norm();
@@ -709,20 +546,19 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
 #pragma unroll
           for (int i = 0; i < NV; ++i) {
             float2 p[4];
-            take(2, more[kBranch ? 0 : i], i, p);
+            more[kBranch ? 0 : i].get(p);
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[i][j] = add2(d[i][j], p[j]);
           }
         }
         if (a.dr) put_residual();
-        through_dropout([&](int i, float2 t[4]) { take(2 + with_sum, branch[kGate && !kBranch ? i : 0], i, t); });
-        if (a.dh) {
-          through_gate();
-          put_rows(a.dh, d);
-        }
+        through_dropout([&](int i, float2 t[4]) { branch[kGate && !kBranch ? i : 0].get(t); });
+        if (!a.dh) continue;
+        through_gate();
+        put_rows(a.dh, d);
       } else {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) take(1, g[i], i, d[i]);
+        for (int i = 0; i < NV; ++i) g[i].get(d[i]);
         if (a.dr) put_residual();
         through_dropout([&](int i, float2 t[4]) {  // norm(h)
           centred(i, t);
@@ -751,7 +587,6 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
         through_norm();
         put_rows(a.dh, d);
       }
-      if (kRing) ring.next();
     }
     if (kGate && grid.sums_gate) {
       put_sums(dg, a.parts + static_cast<int64_t>(gridDim.x) * 2 * a.cols + u * a.cols);
@@ -760,36 +595,6 @@ __global__ void __launch_bounds__(kThreads<G, kRing>, backward_blocks(kThreads<G
 #pragma unroll
         for (int j = 0; j < 4; ++j) dg[i][j] = both(0.f);
     }
-  }
-  if (kRing && __syncthreads_or(ring.dead)) {  // a wait ran out: NaNs, once no copy is in flight
-    ring.settle();
-    float nans[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) nans[j] = __uint_as_float(~0u);
-    const auto spoil = [&](void* p, uint32_t r) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (p) store_chunk<G, kVec>(static_cast<T*>(p) + r * a.cols, cols, lane, i, nans);
-    };
-    for (int64_t u = blockIdx.x; u < grid.units; u += gridDim.x) {
-      const Unit unit = unit_of(grid, u);
-      for (uint32_t r = static_cast<uint32_t>(unit.begin) + slot; r < unit.end; r += kRows) {
-        spoil(a.dh, r);
-        spoil(a.dr, r);
-        if (kGate && !grid.sums_gate && !a.gate_f32) spoil(a.dgate, r);
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
-          if (kGate && !grid.sums_gate && a.gate_f32)
-            store_chunk<G, kVec>(static_cast<float*>(a.dgate) + r * a.cols, cols, lane, i, nans);
-      }
-      if (kGate && grid.sums_gate)
-        for (int c = threadIdx.x; c < cols; c += kThreads<G, kRing>)
-          a.parts[static_cast<int64_t>(gridDim.x) * 2 * a.cols + u * a.cols + c] = nans[0];
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) dw[i][j] = db[i][j] = both(nans[0]);
   }
   if (!a.dw && !a.db) return;
   float* part = a.parts + blockIdx.x * 2 * a.cols;
@@ -1007,30 +812,36 @@ __global__ void __launch_bounds__(kLong) backward_long_kernel(const Args a, cons
 
 // ---- host --------------------------------------------------------------------------
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+bool vectors_fit(const Args& a) {
+  const auto rows_fit = [](const void* p, int64_t stride, size_t size) {
+    return !p || (aligned16(p) && (stride * size) % 16 == 0);
+  };
+  bool ok = a.cols % 8 == 0;
+  ok = ok && rows_fit(a.h, a.h_stride, sizeof(T)) && rows_fit(a.r, a.r_stride, sizeof(T));
+  ok = ok && rows_fit(a.gate, a.gate_stride, a.gate_f32 ? 4 : sizeof(T));
+  ok = ok && rows_fit(a.gy, a.gy_stride, sizeof(T)) && rows_fit(a.gs, a.gs_stride, sizeof(T));
+  ok = ok && rows_fit(a.sum, a.sum_stride, sizeof(T));
+  for (const void* p : {a.w, a.b, static_cast<const void*>(a.y), static_cast<const void*>(a.s),
+                        static_cast<const void*>(a.dh), static_cast<const void*>(a.dr),
+                        static_cast<const void*>(a.dgate)})
+    ok = ok && aligned16(p);
+  return ok;
+}
+
 template <int G, int NV, bool kVec, bool kBranch, typename T>
 cudaError_t launch_forward(const Args& a, cudaStream_t stream) {
-  const auto kernel = forward_kernel<G, NV, kVec, false, kBranch, T>;
   // as many blocks as are under way together
-  static const int per_sm = [&] {
+  static const int per_sm = [] {
     int n = 0;
-    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, Shape<G>::kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
+    return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, forward_kernel<G, NV, kVec, kBranch, T>,
+                                                         Shape<G>::kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
   }();
   const int64_t groups = (a.rows + Shape<G>::kRows - 1) / Shape<G>::kRows;
   const int blocks = static_cast<int>(std::min<int64_t>(groups, 148ll * per_sm));
-  kernel<<<blocks, Shape<G>::kThreads, 0, stream>>>(a, 0);
-  return cudaGetLastError();
-}
-
-template <int G, int NV, bool kBranch, typename T>
-cudaError_t launch_forward_ring(const Args& a, int stages, cudaStream_t stream) {
-  const auto kernel = forward_kernel<G, NV, true, true, kBranch, T>;
-  const int bytes = static_cast<int>(stages * a.cols * sizeof(T) * 2 * (kRingThreads / G));
-  // the most that any call asks for: another thread's launch may come between
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-  if (err != cudaSuccess) return err;
-  const int64_t groups = (a.rows + kRingThreads / G - 1) / (kRingThreads / G);
-  const int blocks = static_cast<int>(std::min<int64_t>(groups, 148ll * (NV == 1 ? 2 : 1)));
-  kernel<<<blocks, kRingThreads, bytes, stream>>>(a, stages);
+  forward_kernel<G, NV, kVec, kBranch, T><<<blocks, Shape<G>::kThreads, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -1040,13 +851,6 @@ cudaError_t forward_form(const Args& a, cudaStream_t stream) {
   if (a.cols <= 256) return launch_forward<32, 1, kVec, kBranch, T>(a, stream);
   if (a.cols <= 512) return launch_forward<64, 1, kVec, kBranch, T>(a, stream);
   if (a.cols <= 1024) return launch_forward<128, 1, kVec, kBranch, T>(a, stream);
-  if constexpr (kVec) {
-    if (const int stages = ring_stages(a, 2, a.cols <= 4096)) {
-      if (a.cols <= 2048) return launch_forward_ring<256, 1, kBranch, T>(a, stages, stream);
-      if (a.cols <= 4096) return launch_forward_ring<512, 1, kBranch, T>(a, stages, stream);
-      return launch_forward_ring<512, 2, kBranch, T>(a, stages, stream);
-    }
-  }
   if (a.cols <= 2048) return launch_forward<256, 1, kVec, kBranch, T>(a, stream);
   if (a.cols <= 4096) return launch_forward<512, 1, kVec, kBranch, T>(a, stream);
   if (a.cols <= 8192) return launch_forward<512, 2, kVec, kBranch, T>(a, stream);
@@ -1057,24 +861,14 @@ cudaError_t forward_form(const Args& a, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t forward_of(const Args& a, cudaStream_t stream) {
-  if (vectors_fit(a))
+  if (vectors_fit<T>(a))
     return a.branch ? forward_form<true, true, T>(a, stream) : forward_form<true, false, T>(a, stream);
   return a.branch ? forward_form<false, true, T>(a, stream) : forward_form<false, false, T>(a, stream);
 }
 
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>
 cudaError_t launch_backward(const Args& a, const Grid& grid, cudaStream_t stream) {
-  backward_kernel<G, NV, kVec, false, kBranch, kGate, T><<<grid.blocks, Shape<G>::kThreads, 0, stream>>>(a, grid, 0);
-  return cudaGetLastError();
-}
-
-template <int G, int NV, bool kBranch, bool kGate, typename T>
-cudaError_t launch_backward_ring(const Args& a, const Grid& grid, cudaStream_t stream) {
-  const auto kernel = backward_kernel<G, NV, true, true, kBranch, kGate, T>;
-  const int bytes = static_cast<int>(grid.stages * a.cols * sizeof(T) * grid.tensors * (kRingThreads / G));
-  const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
-  if (err != cudaSuccess) return err;
-  kernel<<<grid.blocks, kRingThreads, bytes, stream>>>(a, grid, grid.stages);
+  backward_kernel<G, NV, kVec, kBranch, kGate, T><<<grid.blocks, Shape<G>::kThreads, 0, stream>>>(a, grid);
   return cudaGetLastError();
 }
 
@@ -1084,13 +878,6 @@ cudaError_t backward_form(const Args& a, const Grid& grid, cudaStream_t stream) 
   if (a.cols <= 256) return launch_backward<32, 1, kVec, kBranch, kGate, T>(a, grid, stream);
   if (a.cols <= 512) return launch_backward<64, 1, kVec, kBranch, kGate, T>(a, grid, stream);
   if (a.cols <= 1024) return launch_backward<128, 1, kVec, kBranch, kGate, T>(a, grid, stream);
-  if constexpr (kVec) {
-    if (grid.stages) {
-      if (a.cols <= 2048) return launch_backward_ring<256, 1, kBranch, kGate, T>(a, grid, stream);
-      if (a.cols <= 4096) return launch_backward_ring<512, 1, kBranch, kGate, T>(a, grid, stream);
-      return launch_backward_ring<512, 2, kBranch, kGate, T>(a, grid, stream);
-    }
-  }
   if (a.cols <= 2048) return launch_backward<256, 1, kVec, kBranch, kGate, T>(a, grid, stream);
   if (a.cols <= 4096) return launch_backward<512, 1, kVec, kBranch, kGate, T>(a, grid, stream);
   if (a.cols <= 8192) return launch_backward<512, 2, kVec, kBranch, kGate, T>(a, grid, stream);
@@ -1109,7 +896,7 @@ cudaError_t backward_kind(const Args& a, const Grid& grid, cudaStream_t stream) 
 
 template <typename T>
 cudaError_t backward_of(const Args& a, const Grid& grid, cudaStream_t stream) {
-  return vectors_fit(a) ? backward_kind<true, T>(a, grid, stream) : backward_kind<false, T>(a, grid, stream);
+  return vectors_fit<T>(a) ? backward_kind<true, T>(a, grid, stream) : backward_kind<false, T>(a, grid, stream);
 }
 
 }  // namespace
