@@ -68,11 +68,8 @@ Grid backward_grid(const Args& a) {
   const int64_t groups = a.rows / grid.group_rows;
   // rows that a block has under way, and blocks that are under way together
   const int rows = a.cols <= 256 ? 8 : 1;
-  const int64_t most = 148ll * (a.cols <= 256    ? 2
-                                : a.cols <= 512  ? 8
-                                : a.cols <= 1024 ? 4
-                                : a.cols <= 2048 ? 2
-                                                 : 1);
+  const int threads = a.cols <= 256 ? 256 : a.cols <= 512 ? 64 : a.cols <= 1024 ? 128 : a.cols <= 2048 ? 256 : 512;
+  const int64_t most = 148ll * (512 / threads);
   const int64_t wanted = std::max<int64_t>(1, most / groups);
   grid.unit_rows = (grid.group_rows + wanted - 1) / wanted;
   grid.unit_rows = (grid.unit_rows + rows - 1) / rows * rows;

@@ -140,13 +140,6 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
     else
       return Sums{row_sums<G>(x.x + x.y, buf, turn), 0.f};
   };
-  float2 w[kBoth ? NV : 1][4];
-  if (kBoth) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) w[kBoth ? i : 0][j] = stored(v[i][j], T());
-  }
   Sums mean{0.f, 0.f};
   if (!a.rms) {
     float2 t = both(0.f), u = both(0.f);
@@ -155,7 +148,7 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         t = add2(t, v[i][j]);
-        if (kBoth) u = add2(u, w[kBoth ? i : 0][j]);
+        if (kBoth) u = add2(u, stored(v[i][j], T()));
       }
     mean = over_row(t, u);
     mean.a *= share, mean.b *= share;
@@ -174,7 +167,7 @@ __device__ __forceinline__ Moments moments(const float2 v[NV][4], const Args& a,
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       t = square(i, j, add2(v[i][j], both(-mean.a)), t);
-      if (kBoth) u = square(i, j, add2(w[kBoth ? i : 0][j], both(-mean.b)), u);
+      if (kBoth) u = square(i, j, add2(stored(v[i][j], T()), both(-mean.b)), u);
     }
   }
   const Sums var = over_row(t, u);
@@ -206,18 +199,20 @@ __device__ __forceinline__ void with_param(const void* p, bool f32, int cols, in
     each(T());
 }
 
-// Blocks to an SM that 64 registers a thread allow, where they do: not for short rows of
-// float32 (44446 x 256: 36 us in 64 registers, 30 in 78), nor where columns are apart
-// (30000 x 260 bfloat16: 64 and 47 us). 0: as the compiler likes.
+// Blocks to an SM that 64 registers a thread allow, where they do (8192 x 8192 bfloat16
+// 100 us, in 124 registers 138): not for short rows of float32 (44446 x 256: 36 us in 64
+// registers, 30 in 78), nor where columns are apart (30000 x 260 bfloat16: 64 and 47
+// us). 0: as the compiler likes. Fewer registers spill (40000 x 256 in 51: 25 us, 22).
 template <typename T>
-constexpr int forward_blocks(int row_threads, int threads, bool one_vector) {
-  return one_vector && (sizeof(T) == 2 || row_threads == 512) ? 1024 / threads : 0;
+constexpr int forward_blocks(int row_threads, int threads, bool vec) {
+  return vec && (sizeof(T) == 2 || row_threads == 512) ? 1024 / threads : 0;
 }
 
 // With fewer than 32 threads to a row, a warp has several rows under way, of which the
 // last may not be there: its loads give 0, and it stores nothing.
 template <int G, int NV, bool kVec, bool kBranch, typename T>
-__global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, Shape<G>::kThreads, kVec && NV == 1)) forward_kernel(const Args a) {
+__global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, Shape<G>::kThreads, kVec))
+    forward_kernel(const Args a) {
   constexpr int kTogether = G < 32 ? 32 / G : 1;
   __shared__ Sums buf[Shape<G>::kBuf];
   int turn = 0;
@@ -332,6 +327,8 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
 }
 
 // Blocks to an SM: 128 registers a thread, for the sums, the parameters and a row ahead.
+// In 80, 20000 x 1024 with a gate takes 53 us instead of 61, 40000 x 512 53 instead of
+// 51, 44446 x 256 float32 39 instead of 32.
 constexpr int backward_blocks(int threads) { return 512 / threads; }
 
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>

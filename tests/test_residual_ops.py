@@ -344,6 +344,23 @@ def test_norms_match_the_formulas(cuda_device, shape, op, kind, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("op", ["add_norm", "norm_add"])
+@pytest.mark.parametrize("shape,gate", [((1300, 1032), None), ((2369, 2048), (2048,)), ((1250, 4096), (4096,)),
+                                        ((1190, 8192), None), ((6, 400, 2000), (6, 1, 2000)), ((5, 301, 4104), (5, 301, 4104)),
+                                        ((300, 5, 1040), (300, 1, 1040)), ((1185, 5000), (5000,))])
+def test_many_long_rows(cuda_device, shape, gate, op, dtype):
+    """Several rows to each block, and several blocks to a sample."""
+    data = inputs(shape, dtype, cuda_device, gate=gate)
+    check(op, data)
+    check(op, data, kind="rms", p=0.0, alpha=1.0)
+    if op == "add_norm":
+        check(op, data, use=("y",), need="hrwb")
+        check(op, data, use=("s",))
+        check(op, data, use=("y",), need="wb")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("op", ["add_norm", "norm_add"])
 @pytest.mark.parametrize("n", [64, 100, 513, 1024, 2500, 9000])
 def test_gates(cuda_device, n, op, dtype):
     """Per channel, per sample, per row, one per element, one per row, and broadcast along the first dimension."""
