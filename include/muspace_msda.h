@@ -571,8 +571,12 @@ MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stre
  *
  *   input x  [rows, in_features]               weight W [2 out_features, in_features]
  *   bias b   [2 out_features] or NULL          output y, grad_output g [rows, out_features]
- *   factors  [rows, 2 out_features] contiguous, of dtype, P before Q: the forward writes
- *            them where it is not NULL, the backward reads them
+ *   factors  [rows, 2 out_features] contiguous, P before Q, float32 beside float32,
+ *            float16 beside bfloat16: the forward writes them where it is not NULL, the
+ *            backward reads them
+ *   exponents  beside bfloat16, with factors: 4-byte aligned, [2, ceil(out_features / 32),
+ *            rows, 4] bytes (P before Q; column / 32; row; column % 32 / 8), a byte e (15 to
+ *            254) to eight factors, which are their halves times 2^(e - 141)
  *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional;
  *            bfloat16: dz is rounded to bfloat16 for dx and dW, not for db
  *
@@ -587,6 +591,7 @@ typedef struct {
   const int64_t *seed_at;
   const void *input, *weight, *bias;
   void *output, *factors;
+  uint8_t *exponents;
   const void *grad_output;
   void *grad_input, *grad_weight, *grad_bias;
   void *workspace;

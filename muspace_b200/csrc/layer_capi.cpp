@@ -225,6 +225,9 @@ lin::GatedArgs gated_args(const msda_gated_linear_t* in, bool backward) {
   a.x_stride = in->input_stride, a.w_stride = in->weight_stride;
   a.y_stride = in->output_stride, a.g_stride = in->grad_output_stride;
   a.factors = in->factors;
+  a.exponents = in->dtype == MSDA_DTYPE_BFLOAT16 ? in->exponents : nullptr;
+  check_pointer(some_y && in->factors && in->dtype == MSDA_DTYPE_BFLOAT16, in->exponents, "exponents");
+  require((reinterpret_cast<uintptr_t>(a.exponents) & 3) == 0, "exponents must be 4-byte aligned");
   if (backward) {
     check_pointer(some_w && in->grad_input, in->weight, "weight");
     check_pointer(some_x && in->grad_weight, in->input, "input");

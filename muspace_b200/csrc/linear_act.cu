@@ -15,6 +15,9 @@
 //
 // The gated operator's backward is the same with dz = [g P, g Q], whose factors the
 // forward kept: one elementwise pass, then products over all 2 n rows of the weight.
+// In bfloat16 the factors are kept in float16, eight under one exponent: 11 bits of
+// them, where bfloat16's 8 added as much to the gradients' error as dz's rounding does
+// (40000 x 256 x 512: 0.0029 of their size instead of 0.0024).
 #include <algorithm>
 
 #include "checkpoint8.cuh"
@@ -194,6 +197,7 @@ cudaError_t gated_forward_in(const GatedArgs& a, Arena& arena, cudaStream_t stre
   pr.epi.out = a.y;
   pr.epi.out_ld = a.y_stride;
   pr.epi.slope = a.factors;
+  pr.epi.exponents = a.exponents;
   pr.epi.rule = a.rule;
   const Plan plan = plan_product(pr.dtype, pr.m, 2 * pr.n, pr.k, plane_pairs(pr.a, pr.b), multiprocessors());
   if (gated_apart(pr, plan)) pr.partial = static_cast<float*>(arena.take(partial_bytes(plan, pr.m, 2 * pr.n)));
@@ -211,7 +215,7 @@ cudaError_t gated_backward_in(const GatedArgs& a, Arena& arena, cudaStream_t str
   if (need_b) parts = static_cast<float*>(arena.take(static_cast<size_t>(parts_count) * both * sizeof(float)));
   dz = fresh(a.dtype, a.rows, both, a.dtype == DType::kF32 ? 3 : 1, arena);
   if (!arena.measuring) {
-    LIN_TRY(gate_operand(a.dtype, a.g, a.g_stride, a.factors, dz, parts, stream));
+    LIN_TRY(gate_operand(a.dtype, a.g, a.g_stride, a.factors, a.exponents, dz, parts, stream));
     if (need_b) LIN_TRY(add_parts(a.dtype, parts, parts_count, both, a.db, stream));
   }
   return products_of(a.dtype, a.rows, a.in, both, dz, w, x, a.dx, a.dw, arena, stream);

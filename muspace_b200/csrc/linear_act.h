@@ -60,7 +60,8 @@ struct GatedArgs {
   const void* w;       // forward; backward with dx
   const void* bias;    // forward, may be null
   void* y;             // forward
-  void* factors;       // [rows, 2 out] contiguous, P and Q; forward: may be null
+  void* factors;       // [rows, 2 out] contiguous, P and Q: float16 beside bfloat16, float32; forward: may be null
+  uint8_t* exponents;  // beside bfloat16: of each eight factors, [2, ceil(out / 32), rows, 4]
   const void* g;       // backward
   void* dx;            // [rows, in] contiguous, may be null
   void* dw;            // [2 out, in] contiguous, may be null
@@ -110,6 +111,7 @@ struct Epilogue {
   int64_t out_plane = 0;  // kDz, float32: out is three bfloat16 planes, out_plane elements apart
   float* sums = nullptr;  // kDz, may be null: [ceil(m / 32), n], the columns' sums over 32 rows
   drop::Rule rule;         // gated
+  uint8_t* exponents = nullptr;  // gated, bfloat16: of the factors in `slope`
   float* unrounded = nullptr;  // finished apart with sums: where out is left in float32 for them, rows of partial_ld(n)
 };
 
@@ -169,8 +171,8 @@ cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const voi
                              float* parts, cudaStream_t stream);
 // dst [rows, 2 n] = [g * P, g * Q] of the factors [rows, 2 n], with the sums of its columns
 // on the way where parts is not null: parts [column_parts(rows, n), 2 n].
-cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const Operand& dst,
-                         float* parts, cudaStream_t stream);
+cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const uint8_t* exponents,
+                         const Operand& dst, float* parts, cudaStream_t stream);
 cudaError_t unpack_operand(const int8_t* codes, const uint8_t* exps, const Operand& dst, cudaStream_t stream);
 // The sums of src's columns over ranges of rows; and of parts [count, cols], in order.
 int column_parts(int64_t rows, int64_t cols);

@@ -306,6 +306,48 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, 
   }
 }
 
+// ---- eight float16 under one exponent ---------------------------------------------------
+
+// Factors of any size in 11 bits. Eight whose largest lies in [2^-10, 65504] are halves
+// as they are. Others are scaled by a power of two that brings the largest finite one
+// into [2^14, 2^15); it is kept as that one's float32 exponent (15 at least: what is
+// below 2^-112 loses digits). Infinities and NaNs are kept as they are.
+constexpr uint32_t kFactorShift = 141;  // the exponent of 2^14, and of no scale
+
+// Eight factors as halves; their exponent.
+__device__ __forceinline__ uint32_t pack_factors8(const float v[8], uint32_t w[4]) {
+  __half2 h[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+  const float2 m = __half22float2(__hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
+  const float most = fmaxf(m.x, m.y);
+  uint32_t e = kFactorShift;
+  if (!(most >= 0x1p-10f && most <= 65504.f)) {  // rare: no call here, whose registers every other eight would pay for
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = __float_as_uint(v[j]) & 0x7fffffffu;
+      top = max(top, bits < 0x7f800000u ? bits : 0u);
+    }
+    e = max(top >> 23, 15u);
+    const float scale = __uint_as_float((127u + kFactorShift - e) << 23);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j] * scale, v[2 * j + 1] * scale);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(&h[j]);
+  return e;
+}
+
+// Where the exponent of P (half 0) or Q in row m, columns c to c + 7 lies: neighbouring
+// rows' four of 32 columns are neighbours, as a warp of the epilogue writes them (by rows
+// of all columns, 40000 x 256 x 512 took 90 us instead of 76: parts of sectors).
+__device__ __forceinline__ int64_t exponent_at(int64_t rows, int64_t cols, int half, int64_t m, int64_t c) {
+  return ((half * ((cols + 31) / 32) + c / 32) * rows + m) * 4 + c % 32 / 8;
+}
+
+__device__ __forceinline__ float factor_scale(uint32_t e) { return __uint_as_float((e + 127u - kFactorShift) << 23); }
+
 // ---- the epilogue -----------------------------------------------------------------------
 
 template <typename T>

@@ -55,10 +55,10 @@ __device__ __forceinline__ void finish(const GatedArgs& a, int64_t m, int64_t n,
     const bool kept = n % 2 ? word > key.high : (word << 16) > key.low;
     g[0] = kept ? g[0] : 0.f, s[0] = kept ? s[0] : 0.f, u = kept ? u * a.rule.scale : 0.f;
   }
-  if (a.factors) {
-    T* factors = static_cast<T*>(a.factors) + m * 2 * a.out + n;
-    factors[0] = from_float<T>(s[0] * u);
-    factors[a.out] = from_float<T>(g[0] * a.rule.scale);
+  if (sizeof(T) == 4 && a.factors) {  // float32; the others' need eight neighbours
+    float* factors = static_cast<float*>(a.factors) + m * 2 * a.out + n;
+    factors[0] = s[0] * u;
+    factors[a.out] = g[0] * a.rule.scale;
   }
   static_cast<T*>(a.y)[m * a.y_stride + n] = from_float<T>(g[0] * u);
 }
@@ -215,7 +215,9 @@ cudaError_t forward_few_rows(const Args& a, cudaStream_t stream) {
 // / 20.2, and 4 x 4096 x 2 x 1024 8.2 / 11.6; 8 rows of up to 2^21 weights 6.4 / 7.4, of
 // 2^23 16.5 / 11.7. float32 as the plain operator of twice the columns: 16 x 4096 x 2 x
 // 4096 103 / 149, 64 x 256 x 2 x 512 7.5 / 15.4, 64 x 1024 x 2 x 1024 35 / 21.
+// In training, bfloat16's factors share exponents with their neighbours, which other warps hold here.
 bool gated_few_rows(const GatedArgs& a) {
+  if (a.dtype == DType::kBF16 && a.factors) return false;
   if (a.dtype == DType::kBF16) return a.rows <= 4 || (a.rows <= 8 && 2 * a.out * a.in <= 1ll << 21);
   Args as{};
   as.dtype = a.dtype, as.rows = a.rows, as.in = a.in, as.out = 2 * a.out;

@@ -186,39 +186,44 @@ cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slo
 
 // dst = [g * P, g * Q] with the sums of both halves' columns, before the rounding: a
 // lane takes eight columns of g and the same of either half. Bound by memory: 40000 x
-// 512 bfloat16 (205 MB) 36 us, 5.6 TB/s; two rows unrolled 46, more blocks to an SM 52
+// 512 bfloat16 (210 MB) 35 us, 6.0 TB/s; two rows unrolled 46, more blocks to an SM 52
 // to 66 (spills).
-template <typename T>
+// kVec: whole eights at 16-byte boundaries.
+template <typename T, bool kVec>
 __global__ void __launch_bounds__(32 * kSumWarps, 4)
-    gate_operand_kernel(const T* __restrict__ src, int64_t src_ld, bool src_vec, const T* __restrict__ factors,
-                        bool factors_vec, bf16* __restrict__ dst, int64_t dst_ld, int64_t plane, bool dst_vec,
+    gate_operand_kernel(const T* __restrict__ src, int64_t src_ld, const typename SlopeOf<T>::type* __restrict__ factors,
+                        const uint8_t* __restrict__ exponents, bf16* __restrict__ dst, int64_t dst_ld, int64_t plane,
                         int64_t rows, int64_t cols, int64_t rows_per_part, float* __restrict__ parts) {
   __shared__ float buf[kSumWarps][kSumCols];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = blockIdx.x * static_cast<int64_t>(kSumCols) + lane * 8;
   const int64_t begin = blockIdx.y * rows_per_part, end = min(rows, begin + rows_per_part);
-  const int count = static_cast<int>(cols - c < 8 ? cols - c : 8);
-  const bool vec = dst_vec && count == 8;
+  const int count = kVec ? 8 : static_cast<int>(cols - c < 8 ? cols - c : 8);
   float s[2][8] = {};
   if (c < cols) {
+    const uint8_t *exps_p = nullptr, *exps_q = nullptr;
+    if (sizeof(T) == 2)
+      exps_p = exponents + exponent_at(rows, cols, 0, 0, c), exps_q = exponents + exponent_at(rows, cols, 1, 0, c);
     for (int64_t r = begin + warp; r < end; r += kSumWarps) {
+      uint32_t e[2] = {};
+      if (sizeof(T) == 2) e[0] = __ldg(exps_p + 4 * r), e[1] = __ldg(exps_q + 4 * r);
       float v[8], f[2][8];
-      load_some(src + r * src_ld + c, count, src_vec && count == 8, v);
+      load_some(src + r * src_ld + c, count, kVec, v);
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        load_some(factors + (2 * r + half) * cols + c, count, factors_vec && count == 8, f[half]);
+      for (int half = 0; half < 2; ++half) load_some(factors + (2 * r + half) * cols + c, count, kVec, f[half]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
+          if (sizeof(T) == 2) f[half][j] *= factor_scale(e[half]);
           f[half][j] *= v[j];
           s[half][j] += f[half][j];
         }
         bf16* at = dst + r * dst_ld + half * cols + c;
         if (sizeof(T) == 4)
-          store_planes(at, plane, count, vec, f[half]);
+          store_planes(at, plane, count, kVec, f[half]);
         else
-          store_some(at, count, vec, f[half]);
+          store_some(at, count, kVec, f[half]);
       }
     }
   }
@@ -238,16 +243,17 @@ __global__ void __launch_bounds__(32 * kSumWarps, 4)
 }
 
 template <typename T>
-cudaError_t launch_gate_operand(const void* g, int64_t g_ld, const void* factors, const Operand& dst, float* parts,
-                                cudaStream_t stream) {
+cudaError_t launch_gate_operand(const void* g, int64_t g_ld, const void* factors, const uint8_t* exponents,
+                                const Operand& dst, float* parts, cudaStream_t stream) {
+  using S = typename SlopeOf<T>::type;
   const int64_t cols = dst.cols / 2, count = column_parts(dst.rows, cols);
   if (dst.rows == 0 || cols == 0) return cudaSuccess;
-  const bool g_vec = aligned16(g) && (g_ld * sizeof(T)) % 16 == 0;
-  const bool factors_vec = aligned16(factors) && (cols * sizeof(T)) % 16 == 0;
+  const bool vec = aligned16(g) && (g_ld * sizeof(T)) % 16 == 0 && aligned16(factors) && cols % 8 == 0;
   const dim3 grid(static_cast<unsigned>((cols + kSumCols - 1) / kSumCols), static_cast<unsigned>(count));
-  gate_operand_kernel<T><<<grid, 32 * kSumWarps, 0, stream>>>(
-      static_cast<const T*>(g), g_ld, g_vec, static_cast<const T*>(factors), factors_vec, const_cast<bf16*>(dst.p),
-      dst.ld, dst.plane, cols % 8 == 0, dst.rows, cols, (dst.rows + count - 1) / count, parts);
+  const auto kernel = vec ? gate_operand_kernel<T, true> : gate_operand_kernel<T, false>;
+  kernel<<<grid, 32 * kSumWarps, 0, stream>>>(static_cast<const T*>(g), g_ld, static_cast<const S*>(factors), exponents,
+                                              const_cast<bf16*>(dst.p), dst.ld, dst.plane, dst.rows, cols,
+                                              (dst.rows + count - 1) / count, parts);
   return cudaGetLastError();
 }
 
@@ -308,10 +314,10 @@ cudaError_t operand_and_sums(DType dtype, const void* g, int64_t g_ld, const voi
                : launch_operand_sums<bf16, false>(g, g_ld, nullptr, dst, parts, stream);
 }
 
-cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const Operand& dst,
-                         float* parts, cudaStream_t stream) {
-  return dtype == DType::kF32 ? launch_gate_operand<float>(g, g_ld, factors, dst, parts, stream)
-                              : launch_gate_operand<bf16>(g, g_ld, factors, dst, parts, stream);
+cudaError_t gate_operand(DType dtype, const void* g, int64_t g_ld, const void* factors, const uint8_t* exponents,
+                         const Operand& dst, float* parts, cudaStream_t stream) {
+  return dtype == DType::kF32 ? launch_gate_operand<float>(g, g_ld, factors, exponents, dst, parts, stream)
+                              : launch_gate_operand<bf16>(g, g_ld, factors, exponents, dst, parts, stream);
 }
 
 cudaError_t column_sums(const Operand& src, float* parts, cudaStream_t stream) {

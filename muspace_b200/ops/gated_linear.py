@@ -3,9 +3,10 @@ dropout in one kernel, forward and backward.
 
 ``y = D(act(x Wg^T + bg) * (x Wu^T + bu))``; the weight holds ``Wg`` above ``Wu``, so
 both products are one, and what it is made of never reaches memory in inference. In
-training the forward keeps, in the dtype of the rows, the factors ``P = D'(act'(zg)
-zu)`` and ``Q = D'(act(zg))`` (``D'`` multiplies as ``D`` does): two numbers per output
-element, as many as ``zg`` and ``zu`` would be, and the mask is in them.
+training the forward keeps the factors ``P = D'(act'(zg) zu)`` and ``Q = D'(act(zg))``
+(``D'`` multiplies as ``D`` does): two numbers per output element, as many as ``zg`` and
+``zu`` would be, and the mask is in them. Beside bfloat16 they are float16, each eight
+neighbours under an exponent of their own (11 bits of numbers of any size).
 
 Backward: ``dz = [g P, g Q]``, ``dx = dz W``, ``dW = dz^T x``, ``db`` the sum of ``dz``
 over rows. In bfloat16 ``dz`` is rounded to bfloat16 before the two products, as a
@@ -32,12 +33,17 @@ def _forward(module: NativeModule, x, weight, bias, seed_tensor, activation: str
     weight, w_stride = rows_of(weight)
     count, features, width = rows.size(0), weight.size(1), weight.size(0) // 2
     out = x.new_empty((*x.shape[:-1], width))
-    factors = x.new_empty((count, 2 * width)) if keep else None
+    factors = exponents = None
+    if keep and x.dtype == torch.bfloat16:  # halves, and behind them the bytes
+        factors = torch.empty(4 * count * width + 8 * count * -(-width // 32), dtype=torch.uint8, device=x.device)
+        exponents = factors.data_ptr() + 4 * count * width
+    elif keep:
+        factors = x.new_empty((count, 2 * width))
     if bias is not None:
         bias = bias.contiguous()
     args = GatedLinearArgs(DTYPE_CODES[x.dtype], ACTIVATIONS[activation], count, features, width, x_stride, w_stride,
                            width, 0, *rule, pointer(seed_tensor), rows.data_ptr(), weight.data_ptr(), pointer(bias),
-                           out.data_ptr(), pointer(factors))
+                           out.data_ptr(), pointer(factors), exponents)
     module.plain_call("msda_gated_linear_forward")(x.device, args)
     return out, factors
 
@@ -71,8 +77,10 @@ def _backward(ctx, grad):
         x, x_stride = rows_of(x)
     if weight is not None:
         weight, w_stride = rows_of(weight)
-    args = GatedLinearArgs(DTYPE_CODES[grad.dtype], 0, g.size(0), w_shape[1], w_shape[0] // 2, x_stride, w_stride, 0,
-                           g_stride, 0, 0, 0, None, pointer(x), pointer(weight), None, None, factors.data_ptr(),
+    count, width = g.shape
+    exponents = factors.data_ptr() + 4 * count * width if grad.dtype == torch.bfloat16 else None
+    args = GatedLinearArgs(DTYPE_CODES[grad.dtype], 0, count, w_shape[1], width, x_stride, w_stride, 0, g_stride, 0, 0,
+                           0, None, pointer(x), pointer(weight), None, None, factors.data_ptr(), exponents,
                            g.data_ptr(), pointer(dx), pointer(dw), pointer(db))
     native_module().plain_call("msda_gated_linear_backward")(grad.device, args)
     return dx, dw, db, None, None, None

@@ -197,8 +197,8 @@ class GatedLinearArgs(ctypes.Structure):
            ("rows", "in_features", "out_features", "input_stride", "weight_stride", "output_stride",
             "grad_output_stride", "threshold", "seed", "sequence")]
         + [(name, ctypes.c_void_p) for name in
-           ("seed_at", "input", "weight", "bias", "output", "factors", "grad_output", "grad_input", "grad_weight",
-            "grad_bias", "workspace")]
+           ("seed_at", "input", "weight", "bias", "output", "factors", "exponents", "grad_output", "grad_input",
+            "grad_weight", "grad_bias", "workspace")]
         + [("workspace_bytes", ctypes.c_size_t)]
     )
 

@@ -4,8 +4,8 @@ Tolerances, per element, from the arithmetic, on top of one rounding of the resu
 (in `near`): a pre-activation is a float32 sum, off by 2^-20 of the sum of its terms'
 magnitudes; an activation passes that on with a slope of at most 1.2, its slope with
 one of at most 1. The bfloat16 kernels' activations are off by 2^-12 of their terms'
-size besides. In training the factors are rounded to the rows' type (2^-8 in
-bfloat16), and dz again, but for db.
+size besides. In training the factors are rounded (beside bfloat16 to float16 under an
+exponent of eight, 2^-11), and dz to the rows' type (2^-8 in bfloat16), but for db.
 """
 
 from __future__ import annotations
@@ -22,7 +22,8 @@ from muspace_b200.runtime import native
 from test_layer_ops import BF16, F16, F32, SUM, act64, near, slope64
 from test_residual_ops import SEED, SEQUENCE, factors
 
-STEP = {BF16: 2.0 ** -8, F32: 2.0 ** -24}  # of a factor or dz in storage
+STEP = {BF16: 2.0 ** -8, F32: 2.0 ** -24}  # half a step of dz in storage
+FACTOR = {BF16: 2.0 ** -11, F32: 2.0 ** -24}  # and of a factor
 FAST = {BF16: 2.0 ** -12, F32: 0.0}  # of an activation
 
 
@@ -55,7 +56,7 @@ def check(x, w, b, g, activation="silu", p=0.0, need="xwb", seed=SEED):
     grads = dict(zip(wanted, torch.autograd.grad(y, [leaves[m] for m in wanted], g)))
     dz = torch.cat([g6 * f * slope * zu, g6 * f * act], 1)
     loose = SUM * torch.cat([g6.abs() * f * (off_slope * zu.abs() + slope.abs() * size_u), g6.abs() * f * off_act], 1)
-    loose = loose + STEP[dtype] * dz.abs()
+    loose = loose + FACTOR[dtype] * dz.abs()
     rounded = loose + STEP[dtype] * dz.abs() * 1.01
     for name, value, error, terms in (("x", dz @ w6, rounded @ w6.abs(), dz.abs() @ w6.abs()),
                                       ("w", dz.T @ x6, rounded.T @ x6.abs(), dz.abs().T @ x6.abs()),
@@ -106,7 +107,40 @@ def test_gated_inference_and_training_agree(cuda_device, dtype):
         x, w, b, _ = inputs(rows, k, n, dtype, cuda_device)
         for activation in ("none", "relu", "gelu", "silu"):
             kept = gated_linear(x, w.clone().requires_grad_(True), b, activation=activation, dropout=0.2, seed=5)
-            assert torch.equal(kept.detach(), gated_linear(x, w, b, activation=activation, dropout=0.2, seed=5))
+            got = gated_linear(x, w, b, activation=activation, dropout=0.2, seed=5)
+            if dtype == BF16 and rows <= 8:  # inference takes few rows in another order: two roundings of one sum
+                assert torch.allclose(kept.double(), got.double(), rtol=2.0 ** -7, atol=2.0 ** -12)
+            else:
+                assert torch.equal(kept.detach(), got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(40, 64), (40, 67), (3000, 512), (3000, 520)])
+@pytest.mark.parametrize("scale", [2.0 ** -60, 2.0 ** -12, 2.0 ** 20, 2.0 ** 60])
+def test_gated_factors_of_any_size(cuda_device, rows, n, scale):
+    """Bfloat16's factors are halves under an exponent: pre-activations far outside of
+    float16's range lose no more than others, whatever their neighbours in other eights are."""
+    x, w, b, g = inputs(rows, 64, n, BF16, cuda_device)
+    w[n:] *= scale  # up, and with it the gate's gradient
+    b[n:] *= scale
+    w[n + 16:n + 24] /= scale
+    b[n + 16:n + 24] /= scale
+    check(x, w, b, g, "silu", 0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(40, 72), (3000, 512)])
+def test_gated_infinite_factors_leave_their_neighbours(cuda_device, rows, n):
+    x, w, b, g = inputs(rows, 64, n, BF16, cuda_device)
+    clean = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    expected = torch.autograd.grad(gated_linear(*clean), clean, g)
+    bad = w.clone()
+    bad[n + 3] = math.inf  # one column of up: its factor P is not finite
+    leaves = [x.clone().requires_grad_(True), bad.requires_grad_(True), b.clone().requires_grad_(True)]
+    dw, db = torch.autograd.grad(gated_linear(*leaves), leaves, g)[1:]
+    keep = [i for i in range(2 * n) if i != 3]
+    assert torch.equal(dw[keep], expected[1][keep]) and torch.equal(db[keep], expected[2][keep])
+    assert not bool(dw[3].isfinite().all())
 
 
 @pytest.mark.gpu
