@@ -567,7 +567,8 @@ MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stre
  * The gated product y = D(act(x Wg^T + bg) * (x Wu^T + bu)) and its gradients, D being
  * dropout as in msda_dropout, and Wg, bg the first out_features rows of weight and bias,
  * Wu, bu the others. With factors P = D'(act'(zg) * zu) and Q = D'(act(zg)) (D' multiplies
- * as D does), dz = [g * P, g * Q], dx = dz W, dW = dz^T x, db = sum of dz over rows.
+ * as D does), dz = [g * P, g * Q] (0 where the factor is, whatever g), dx = dz W, dW =
+ * dz^T x, db = sum of dz over rows.
  *
  *   input x  [rows, in_features]               weight W [2 out_features, in_features]
  *   bias b   [2 out_features] or NULL          output y, grad_output g [rows, out_features]

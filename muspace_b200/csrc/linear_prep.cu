@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * kSumWarps, 4)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (sizeof(T) == 2) f[half][j] *= factor_scale(e[half]);
-          f[half][j] *= v[j];
+          f[half][j] = f[half][j] == 0.f ? 0.f : f[half][j] * v[j];  // a dropped element passes no infinity on
           s[half][j] += f[half][j];
         }
         bf16* at = dst + r * dst_ld + half * cols + c;

@@ -9,7 +9,7 @@ training the forward keeps the factors ``P = D'(act'(zg) zu)`` and ``Q = D'(act(
 neighbours under an exponent of their own (11 bits of numbers of any size).
 
 Backward: ``dz = [g P, g Q]``, ``dx = dz W``, ``dW = dz^T x``, ``db`` the sum of ``dz``
-over rows. In bfloat16 ``dz`` is rounded to bfloat16 before the two products, as a
+over rows; ``dz`` is 0 where its factor is (a dropped element), whatever ``g``. In bfloat16 ``dz`` is rounded to bfloat16 before the two products, as a
 tensor core takes it.
 """
 

@@ -119,7 +119,7 @@ def _backward(ctx, *grads):
     device, dtype = first.device, first.dtype
     code = WIDE_DTYPE_CODES[dtype]
     rows, stride = rows_of(first)
-    count, width = rows.shape
+    count, width = map(int, rows.shape)
     y_stride = s_stride = x_stride = total_stride = gate_stride = 0
     y_at = s_at = total_at = mean = rstd = None
     if grad_y is not None:
@@ -188,8 +188,8 @@ def _groups_of(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int]:
         while upto and own[upto - 1] == 1:
             upto -= 1
         if own[:upto] == tuple(lead[:upto]):
-            return gate, prod(lead[:upto])
-    return _expanded("gate", gate.float(), shape), prod(lead)
+            return gate, int(prod(lead[:upto]))  # tensors while tracing
+    return _expanded("gate", gate.float(), shape), int(prod(lead))
 
 
 def _call(operator: str, input, residual, weight, bias, gate, residual_scale, kind, eps, p, seed, sequence, want_sum,

@@ -326,6 +326,33 @@ def test_gated_feed_forward_block(cuda_device):
         assert float((a.double() - e).norm()) <= 2.0 ** -20 * float(e.norm())
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("n", [64, 67])
+def test_gated_dropped_elements_pass_no_infinity_on(cuda_device, n, dtype):
+    x, w, b, g = inputs(50, 32, n, dtype, cuda_device)
+    f = factors(50, n, 0.5, SEED, 0).to(cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    run = lambda grad: torch.autograd.grad(gated_linear(*leaves, dropout=0.5, seed=SEED), leaves, grad)  # noqa: E731
+    clean = run(torch.where(f > 0, g, torch.zeros_like(g)))
+    for value in (math.inf, math.nan):
+        for a, e in zip(run(torch.where(f > 0, g, torch.full_like(g, value))), clean):
+            assert torch.equal(a, e)
+
+
+@pytest.mark.gpu
+def test_gated_is_differentiable_once(cuda_device):
+    from torch.autograd import forward_ad
+
+    x, w, b, _ = inputs(6, 16, 8, F32, cuda_device)
+    x.requires_grad_(True)
+    (d,) = torch.autograd.grad(gated_linear(x, w, b).square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        d.sum().backward()
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError):
+        gated_linear(forward_ad.make_dual(x.detach(), torch.ones_like(x)), w, b)
+
+
 def test_gated_refusals():
     x, w, b = torch.randn(4, 8), torch.randn(12, 8), torch.randn(12)
     for error, args, how in (

@@ -19,7 +19,7 @@ import pytest
 import torch
 
 from muspace_b200 import clear_dispatch_report, get_last_dispatch_report
-from muspace_b200.ops import add_norm, dropout, layer_norm, norm_add
+from muspace_b200.ops import add_norm, dropout, gated_linear, layer_norm, norm_add
 from muspace_b200.runtime import native
 import test_layer_ops
 from test_layer_ops import BF16, F16, F32, SUM
@@ -587,6 +587,22 @@ def test_double_backward_and_tangents_are_refused(cuda_device):
             call(forward_ad.make_dual(x.detach(), torch.ones_like(x)))
 
 
+@pytest.mark.gpu
+@pytest.mark.filterwarnings("ignore")
+def test_traces_record_the_calls(cuda_device):
+    data = inputs((3, 20, 48), F32, cuda_device, gate=(3, 1, 48))
+    w2, b2 = torch.randn(128, 48, device=cuda_device), torch.randn(128, device=cuda_device)
+
+    def block(h, r, w, b, gate):
+        y, s = add_norm(dropout(h, 0.2, seed=1), r, w, b, gate=gate, dropout=0.1, seed=2, return_sum=True)
+        return gated_linear(norm_add(y, s, w, b, dropout=0.1, seed=3), w2, b2, dropout=0.1, seed=4)
+
+    args = tuple(data[m] for m in ("h", "r", "w", "b", "gate"))
+    traced = torch.jit.trace(block, args, check_trace=False)
+    other = tuple(torch.randn_like(t) for t in args)
+    assert torch.equal(traced(*other), block(*other))
+
+
 # ---- refusals, on the CPU ---------------------------------------------------------------------
 
 
@@ -652,6 +668,8 @@ def test_c_entry_refusals():
         entry.restype, entry.argtypes = ctypes.c_int, [ctypes.POINTER(native.ResidualNormArgs), ctypes.c_void_p]
         assert entry(args, None) == 1 and message in module.last_error()
 
+    for name in ("msda_add_norm_forward", "msda_norm_add_backward"):
+        assert getattr(module.lib, name)(None, None) == 1 and "args is null" in module.last_error()
     good = dict(rows=4, cols=8, gate_groups=1, input=p, residual=p, output=p, sum=p)
     for name in ("msda_add_norm_forward", "msda_norm_add_forward"):
         fails(name, "dtype must be", **{**good, "dtype": 3})
