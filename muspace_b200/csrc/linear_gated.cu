@@ -35,17 +35,30 @@ __device__ __forceinline__ void arrived8(uint32_t r[8]) {
                : "memory");
 }
 
-// Bias of eight columns, the same for all lanes.
+// Bias of eight columns, the same for all lanes: asked for before the sums it is added to have come.
 template <typename T>
-__device__ __forceinline__ void add_bias8(const T* p, bool vec, int count, float v[8]) {
-  float b[8];
-  load_some(p, count, vec && count >= 8, b);
+struct Bias8 {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p, bool vec, int count) {
+    if (vec && count >= 8) {
 #pragma unroll
-  for (int j = 0; j < 8; j += 2) {
-    const float2 s = add2(make_float2(v[j], v[j + 1]), make_float2(b[j], b[j + 1]));
-    v[j] = s.x, v[j + 1] = s.y;
+      for (int k = 0; k < static_cast<int>(sizeof(T) / 2); ++k) u[k] = __ldg(reinterpret_cast<const uint4*>(p) + k);
+    } else {
+      float b[8];
+      load_some(p, count, false, b);
+      store8(reinterpret_cast<T*>(u), b);
+    }
   }
-}
+  __device__ __forceinline__ void add(float v[8]) const {
+    float b[8];
+    load8(reinterpret_cast<const T*>(u), b);
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      const float2 s = add2(make_float2(v[j], v[j + 1]), make_float2(b[j], b[j + 1]));
+      v[j] = s.x, v[j + 1] = s.y;
+    }
+  }
+};
 
 // Eight values of a row into the box from column `col` on.
 template <int kRowBytes>
@@ -60,27 +73,23 @@ __device__ __forceinline__ void put8(uint32_t box, int row, int col, const float
              __float_as_uint(v[4 * u + 2]), __float_as_uint(v[4 * u + 3]));
 }
 
-// Of N values (whole eights) gate sums g and up sums u, both with their bias: the
-// output in g, and with kTrain P in s and Q in u.
-template <bool kFast, bool kTrain, int N>
-__device__ __forceinline__ void gate_values(Act act, const drop::Rule& rule, const drop::Key& key, uint32_t row,
-                                            uint32_t group, float* g, float* u, float* s) {
-  activate<kFast, true, kTrain, N>(act, g, s);
+// Of eight gate sums g and up sums u, both with their bias: the output in g, and with
+// kTrain P in s and Q in u. `words`: the eight's random numbers, with dropout.
+template <bool kFast, bool kTrain>
+__device__ __forceinline__ void gate_values(Act act, const drop::Rule& rule, const drop::Key& key,
+                                            const drop::Words& words, float g[8], float u[8], float s[8]) {
+  activate<kFast, true, kTrain, 8>(act, g, s);
   if (rule.threshold) {
 #pragma unroll
-    for (int h = 0; h < N / 8; ++h) {
-      const drop::Words words = drop::numbers(key, row, group + h);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool kept = drop::kept(key, words, j);
-        g[8 * h + j] = kept ? g[8 * h + j] : 0.f;
-        u[8 * h + j] = kept ? u[8 * h + j] * rule.scale : 0.f;
-        if (kTrain) s[8 * h + j] = kept ? s[8 * h + j] : 0.f;
-      }
+    for (int j = 0; j < 8; ++j) {
+      const bool kept = drop::kept(key, words, j);
+      g[j] = kept ? g[j] : 0.f;
+      u[j] = kept ? u[j] * rule.scale : 0.f;
+      if (kTrain) s[j] = kept ? s[j] : 0.f;
     }
   }
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
+  for (int j = 0; j < 8; ++j) {
     const float y = g[j] * u[j];
     if (kTrain) s[j] *= u[j], u[j] = g[j] * rule.scale;
     g[j] = y;
@@ -179,6 +188,13 @@ __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, co
 #pragma unroll 1
     for (int c = 0; c < kOut; c += 8) {  // sixteen at a time spill: 83 us and 75 without exponents, float32 22223 x 256 x 512 122 and 92
       float g[8], u[8], s[8];
+      Bias8<T> here_g, here_u;
+      if (with_bias) {
+        here_g.load(bias_gate + n0 + c, bias_vec, rows_n - n0 - c);
+        here_u.load(bias_up + n0 + c, bias_vec, rows_n - n0 - c);
+      }
+      drop::Words words;
+      if (e.rule.threshold) words = drop::numbers(key, m + lane, (n0 + c) / 8);
       arrived8(next_g);
       arrived8(next_u);
 #pragma unroll
@@ -186,11 +202,8 @@ __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, co
       const int ahead = c + 8 < kOut ? c + 8 : c;  // the last eight are asked for again
       ask8(gate_at + ahead, next_g);
       ask8(up_at + ahead, next_u);
-      if (with_bias) {
-        add_bias8(bias_gate + n0 + c, bias_vec, rows_n - n0 - c, g);
-        add_bias8(bias_up + n0 + c, bias_vec, rows_n - n0 - c, u);
-      }
-      gate_values<kFast, kTrain, 8>(kAct, e.rule, key, m + lane, (n0 + c) / 8, g, u, s);
+      if (with_bias) here_g.add(g), here_u.add(u);
+      gate_values<kFast, kTrain>(kAct, e.rule, key, words, g, u, s);
       put8<kRowBytes>(out, lane, c, g, T());
       if constexpr (kTrain && sizeof(T) == 2) {
         uint32_t w[4];
@@ -340,8 +353,9 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant
 #pragma unroll
       for (int j = 0; j < 8; ++j) u[j] += b[j];
     }
-    gate_values<sizeof(T) == 2, true, 8>(e.act, e.rule, key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8), g, u,
-                                         s);
+    drop::Words words;
+    if (e.rule.threshold) words = drop::numbers(key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8));
+    gate_values<sizeof(T) == 2, true>(e.act, e.rule, key, words, g, u, s);
     store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, g);
     if (e.slope && sizeof(T) == 4) {
       float* factors = static_cast<float*>(e.slope) + m * 2 * pr.n + n;
