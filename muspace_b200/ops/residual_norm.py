@@ -183,7 +183,7 @@ def _groups_of(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int]:
     gradients that are then summed to its own shape are not rounded before."""
     lead = shape[:-1]
     own = (1,) * (len(shape) - gate.dim()) + tuple(gate.shape)
-    if own[-1] == shape[-1]:
+    if len(own) == len(shape) and own[-1] == shape[-1]:
         upto = len(lead)
         while upto and own[upto - 1] == 1:
             upto -= 1

@@ -635,7 +635,8 @@ def test_residual_norm_refusals(op):
         (ValueError, (h, h[None]), {}), (ValueError, (h[0, 0], h[0, 0]), {}),
         (ValueError, (h, h), dict(kind="batch")), (TypeError, (h, h), dict(gate=0.5)),
         (TypeError, (h, h), dict(gate=w.bfloat16())), (ValueError, (h, h), dict(gate=w[:4])),
-        (ValueError, (h, h), dict(gate=torch.ones(2, 4, 8))), (ValueError, (h, h), dict(gate=torch.ones(3, 8))),
+        (ValueError, (h, h), dict(gate=torch.ones(2, 4, 8))), (ValueError, (h, h), dict(gate=torch.ones(1, 4, 8))),
+        (ValueError, (h, h), dict(gate=torch.ones(1, 1, 8))), (ValueError, (h, h), dict(gate=torch.ones(3, 8))),
         (ValueError, (h, h), dict(dropout=0.1)), (ValueError, (h, h), dict(dropout=1.5, seed=1)),
         (TypeError, (h, h), dict(dropout=0.1, seed="x")),
         (RuntimeError, (h, h), {}), (RuntimeError, (h, h), dict(backend="reference")))
