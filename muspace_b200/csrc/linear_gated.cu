@@ -11,6 +11,11 @@
 // those of the gate's and of up's columns: the backward pass needs no generator, no
 // exponential and no product for them. Beside bfloat16 they are kept in float16, each
 // eight neighbours under an exponent of their own.
+//
+// 8192 x 4096 x 4096 bfloat16 380 us (1.45 PFLOP/s), with factors 410. Where k is short the
+// epilogue is the bound, by issue (51 % of the slots) and latencies: 40000 x 256 x 512
+// bfloat16 gelu 47 us, with factors and dropout 76; 22223 x 256 x 512 float32 silu with
+// factors 92, where products of 128 columns take the time of 256.
 #include <algorithm>
 
 #include "dropout_device.cuh"

@@ -1,9 +1,10 @@
 // Norms with the residual they belong to, forward and backward (formulas in
 // residual_norm.h), for one storage type.
 //
-// Bound by memory: a row is read once into the registers of G threads, 8 NV values
-// each; dropout, gate, residual and norm happen there in float32, and each result is
-// rounded once. A dropout mask is made again from its counter wherever it is needed.
+// A row is read once into the registers of G threads, 8 NV values each; dropout, gate,
+// residual and norm happen there in float32, and each result is rounded once. A dropout
+// mask is made again from its counter wherever it is needed. Short rows in 16 bits are
+// bound by issue, long rows by memory and its latency.
 //
 //   add_norm backward, from what reaches y (gy) and s (gs):
 //     ds = gs + rstd (gy w - mean(gy w) - k mean(gy w k)), k = (s - mean) rstd
