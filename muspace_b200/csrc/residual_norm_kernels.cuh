@@ -23,7 +23,7 @@
 // Times, forward and backward: 40000 x 256 bfloat16 with dropout 21.7 and 20.6 us (82 MB
 // each, 3.9 TB/s; bound by issue, 58 to 63 % of the slots), 184950 x 256 float16 norm_add
 // with dropout and a gate 80 and 124 (the same, 67 and 48 %), 8192 x 8192 bfloat16 with a
-// gate and both outputs 95 and 175 (537 and 805 MB, 5.7 and 4.6 TB/s).
+// gate and both outputs 95 and 166 (537 and 805 MB, 5.7 and 4.8 TB/s).
 //
 // A backward block takes whole units of neighbouring rows, a unit's rows all under
 // one row of the gate: so a thread sums dw, db and dgate of its columns in
@@ -427,8 +427,12 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
       next_mean = there && a.mean ? a.mean[row] : 0.f;
       next_rstd = there ? a.rstd[row] : 0.f;
     };
-    load(r);
+    // The longest rows, one to an SM, come from L2 when their turn comes, without registers
+    // for the next one: 8192 x 8192 176 -> 166 us, 8192 x 4096 100 -> 95; 2048 columns 47 -> 52.
+    constexpr bool kEarly = !(kPrefetches<G, kVec, T> && G == 512);
+    if (kEarly) load(r);
     for (; r - offset < end; r += kRows) {
+      if (!kEarly) load(r);
       const int there = r < end ? cols : 0;
       const int64_t at = r * a.cols;
       Chunk<T, kVec> x[NV], g[NV];
@@ -445,7 +449,7 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
           if (kGate) branch[kGate && !kBranch ? i : 0].template load<G>(static_cast<const T*>(a.h) + r * a.h_stride, there, lane, i);
         }
       }
-      if (r - offset + kRows < end) load(r + kRows);
+      if (kEarly && r - offset + kRows < end) load(r + kRows);
       if (kPrefetches<G, kVec, T> && lane == 0 && r + kDistance * kRows < end) {
         const uint32_t row = r + kDistance * kRows, bytes = cols * sizeof(T);
         if (kBranch || kGate) prefetch_row(static_cast<const T*>(a.h) + row * a.h_stride, bytes);
