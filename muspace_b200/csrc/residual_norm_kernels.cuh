@@ -22,7 +22,7 @@
 //
 // Times, forward and backward: 40000 x 256 bfloat16 with dropout 21.7 and 20.6 us (82 MB
 // each, 3.9 TB/s; bound by issue, 58 to 63 % of the slots), 184950 x 256 float16 norm_add
-// with dropout and a gate 80 and 124 (the same, 67 and 48 %), 8192 x 8192 bfloat16 with a
+// with dropout and a gate 80 and 112 (the same, 67 and 48 %), 8192 x 8192 bfloat16 with a
 // gate and both outputs 95 and 166 (537 and 805 MB, 5.7 and 4.8 TB/s).
 //
 // A backward block takes whole units of neighbouring rows, a unit's rows all under
@@ -450,6 +450,21 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
         }
       }
       if (kEarly && r - offset + kRows < end) load(r + kRows);
+      // Short rows with the gate's gradient, whose kernels wait for loads more than the others:
+      // the block's next rows, neighbours, by one request to a tensor (184950 x 256 float16
+      // norm_add 124 -> 112 us, 180000 x 256 add_norm with both outputs 111 -> 95; without a
+      // gate, 40000 x 256, 20.7 -> 23).
+      if (kVec && kGate && G <= 32 && threadIdx.x == 0 && r + kDistance * kRows < end) {
+        const uint32_t row = r + kDistance * kRows, count = min(static_cast<uint32_t>(kRows), end - row);
+        const auto ask = [&](const void* p, int64_t stride) {
+          if (stride <= 2 * cols)  // not where other columns lie between
+            prefetch_row(static_cast<const T*>(p) + row * stride,
+                         static_cast<uint32_t>(((count - 1) * stride + cols) * sizeof(T)));
+        };
+        ask(a.h, a.h_stride);
+        if (!kBranch && normed) ask(a.sum, a.sum_stride), ask(a.gy, a.gy_stride);
+        if (a.gs) ask(a.gs, a.gs_stride);
+      }
       if (kPrefetches<G, kVec, T> && lane == 0 && r + kDistance * kRows < end) {
         const uint32_t row = r + kDistance * kRows, bytes = cols * sizeof(T);
         if (kBranch || kGate) prefetch_row(static_cast<const T*>(a.h) + row * a.h_stride, bytes);
