@@ -27,7 +27,6 @@ struct Key {
   float scale;
 };
 
-
 __device__ __forceinline__ Key key_of(const Rule& rule) {
   const uint64_t seed = rule.seed_at ? static_cast<uint64_t>(__ldg(rule.seed_at)) : rule.seed;
   const uint32_t last = (rule.threshold - 1u) << 16;

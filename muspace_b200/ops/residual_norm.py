@@ -10,8 +10,8 @@ a root-mean-square norm; ``D`` is ``dropout``, with the same mask for the same s
 sequence, rows and columns.
 
 The backward pass of ``add_norm`` takes the sum as it was stored, and gives the
-gradients there; that of ``norm_add`` takes the input. Masks are made again. Gradients of weight, bias and gate are
-added up in an order that does not depend on scheduling.
+gradients there; that of ``norm_add`` takes the input. Masks are made again. Gradients
+of weight, bias and gate are added up in an order that does not depend on scheduling.
 """
 
 from __future__ import annotations
