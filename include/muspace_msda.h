@@ -577,7 +577,8 @@ MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stre
  *            backward reads them
  *   exponents  beside bfloat16, with factors: 4-byte aligned, [2, ceil(out_features / 32),
  *            rows, 4] bytes (P before Q; column / 32; row; column % 32 / 8), a byte e (15 to
- *            254) to eight factors, which are their halves times 2^(e - 141)
+ *            254) to eight factors, which are their halves times 2^(e - 141); the forward
+ *            brings the eight's largest into [2^14, 2^15)
  *   grad_input, grad_weight, grad_bias   contiguous, overwritten, each optional;
  *            bfloat16: dz is rounded to bfloat16 for dx and dW, not for db
  *

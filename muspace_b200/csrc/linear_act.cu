@@ -15,8 +15,8 @@
 //
 // The gated operator's backward is the same with dz = [g P, g Q], whose factors the
 // forward kept: one elementwise pass, then products over all 2 n rows of the weight.
-// In bfloat16 the factors are kept in float16, eight under one exponent: 11 bits of
-// them, where bfloat16's 8 added as much to the gradients' error as dz's rounding does
+// In bfloat16 the factors are kept in float16, eight under one exponent: 11 bits down to
+// 2^-28 of the largest, where bfloat16's 8 added as much to the gradients' error as dz's rounding does
 // (40000 x 256 x 512: 0.0029 of their size instead of 0.0024).
 #include <algorithm>
 

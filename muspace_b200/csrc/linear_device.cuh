@@ -308,34 +308,34 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, 
 
 // ---- eight float16 under one exponent ---------------------------------------------------
 
-// Factors of any size in 11 bits. Eight whose largest lies in [2^-10, 65504] are halves
-// as they are. Others are scaled by a power of two that brings the largest finite one
-// into [2^14, 2^15); it is kept as that one's float32 exponent (15 at least: what is
-// below 2^-112 loses digits). Infinities and NaNs are kept as they are.
-constexpr uint32_t kFactorShift = 141;  // the exponent of 2^14, and of no scale
+// Factors of any size, eight at a time: scaled by the power of two that brings the largest
+// finite one into [2^14, 2^15), as halves. Down to 2^-28 of that one they keep 11 bits; below
+// that they are off by up to 2^-39 of it, half of the halves' smallest step. The exponent kept
+// is the largest one's float32 exponent (15 at least: what is below 2^-112 loses digits).
+// Infinities and NaNs are kept as they are.
+constexpr uint32_t kFactorShift = 141;  // the exponent of 2^14
 
 // Eight factors as halves; their exponent.
 __device__ __forceinline__ uint32_t pack_factors8(const float v[8], uint32_t w[4]) {
-  __half2 h[4];
+  float most = fabsf(v[0]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-  const float2 m = __half22float2(__hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3]))));
-  const float most = fmaxf(m.x, m.y);
-  uint32_t e = kFactorShift;
-  if (!(most >= 0x1p-10f && most <= 65504.f)) {  // rare: no call here, whose registers every other eight would pay for
-    uint32_t top = 0;
+  for (int j = 1; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));  // of a NaN and a number it is the number
+  uint32_t top = __float_as_uint(most);
+  if (top >= 0x7f800000u) {  // rare: no call here, whose registers every other eight would pay for
+    top = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const uint32_t bits = __float_as_uint(v[j]) & 0x7fffffffu;
       top = max(top, bits < 0x7f800000u ? bits : 0u);
     }
-    e = max(top >> 23, 15u);
-    const float scale = __uint_as_float((127u + kFactorShift - e) << 23);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) h[j] = __floats2half2_rn(v[2 * j] * scale, v[2 * j + 1] * scale);
   }
+  const uint32_t e = max(top >> 23, 15u);
+  const float2 scale = both(__uint_as_float((127u + kFactorShift - e) << 23));
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = *reinterpret_cast<const uint32_t*>(&h[j]);
+  for (int j = 0; j < 4; ++j) {
+    const __half2 h = __float22half2_rn(mul2(make_float2(v[2 * j], v[2 * j + 1]), scale));
+    w[j] = *reinterpret_cast<const uint32_t*>(&h);
+  }
   return e;
 }
 

@@ -6,7 +6,8 @@ both products are one, and what it is made of never reaches memory in inference.
 training the forward keeps the factors ``P = D'(act'(zg) zu)`` and ``Q = D'(act(zg))``
 (``D'`` multiplies as ``D`` does): two numbers per output element, as many as ``zg`` and
 ``zu`` would be, and the mask is in them. Beside bfloat16 they are float16, each eight
-neighbours under an exponent of their own (11 bits of numbers of any size).
+neighbours under an exponent of their own (11 bits down to 2^-28 of the largest of the eight;
+smaller ones are off by up to 2^-39 of it).
 
 Backward: ``dz = [g P, g Q]``, ``dx = dz W``, ``dW = dz^T x``, ``db`` the sum of ``dz``
 over rows; ``dz`` is 0 where its factor is (a dropped element), whatever ``g``. In

@@ -406,3 +406,51 @@ def test_gated_c_entry_refusals():
     fails("msda_gated_linear_backward", "factors is null", **{**back, "factors": None})
     fails("msda_gated_linear_backward", "input is null", **{**back, "grad_weight": p})
     fails("msda_gated_linear_backward", "workspace has 0 bytes", **back)
+
+
+# ---- factors of one eight that are far apart ----------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(40, 64), (40, 67), (3000, 512), (3000, 520)])
+@pytest.mark.parametrize("spread", [2.0 ** -10, 2.0 ** -18, 2.0 ** -25])
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -10, 1.0, 2.0 ** 20])
+def test_gated_factors_beside_larger_ones(cuda_device, rows, n, spread, size):
+    """One column in eight far smaller than its neighbours keeps its gradients' digits: with the
+    eight's largest brought to 2^14, factors down to 2^-28 of it are normal halves. Up's column makes
+    its P small, and without an activation the gate's makes its Q small."""
+    x, w, b, g = inputs(rows, 64, n, BF16, cuda_device, seed=3)
+    up, gate = w.clone(), w.clone()
+    up[n:] *= size
+    up[n + 3::8] *= spread
+    b_up = b.clone()
+    b_up[n:] *= size
+    b_up[n + 3::8] *= spread
+    check(x, up, b_up, g, "silu", 0.1)
+    gate[:n] *= size
+    gate[3:n:8] *= spread
+    b_gate = b.clone()
+    b_gate[:n] *= size
+    b_gate[3:n:8] *= spread
+    check(x, gate, b_gate, g, "none", 0.1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(40, 64), (40, 67), (3000, 512)])
+def test_gated_factors_far_below_their_neighbours(cuda_device, rows, n):
+    """Below 2^-28 of the eight's largest a factor is off by up to 2^-39 of that one: half of float16's
+    smallest step, 2^-24, beside a largest of at least 2^14."""
+    x, w, b, g = inputs(rows, 64, n, BF16, cuda_device, seed=4)
+    w[n + 3::8] *= 2.0 ** -45
+    b[n + 3::8] *= 2.0 ** -45
+    leaf = b.clone().requires_grad_(True)
+    (db,) = torch.autograd.grad(gated_linear(x, w, leaf), [leaf], g)
+    x6, w6, b6, g6 = (t.double() for t in (x, w, b, g.abs()))
+    z, size = x6 @ w6.T + b6, x6.abs() @ w6.abs().T + b6.abs()
+    zu, slope = z[:, n:], slope64("silu", z[:, :n])
+    p = slope * zu
+    most = torch.nn.functional.pad(p.abs(), (0, -n % 8)).view(rows, -1, 8).amax(-1).repeat_interleave(8, 1)[:, :n]
+    loose = SUM * ((size[:, :n] + 1.2 * FAST[BF16] / SUM) * zu.abs() + slope.abs() * size[:, n:]) + FACTOR[BF16] * p.abs()
+    loose = loose + 2 * 2.0 ** -39 * most  # twice, as the largest itself is off by a little
+    expected, terms = (g.double() * p).sum(0), (g6 * (p.abs() + loose / SUM)).sum(0)
+    near(db[3:n:8], expected[3::8], terms[3::8], BF16)
