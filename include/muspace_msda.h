@@ -567,14 +567,15 @@ MSDA_API int msda_norm_add_backward(const msda_residual_norm_t *args, void *stre
  * The gated product y = D(act(x Wg^T + bg) * (x Wu^T + bu)) and its gradients, D being
  * dropout as in msda_dropout, and Wg, bg the first out_features rows of weight and bias,
  * Wu, bu the others. With factors P = D'(act'(zg) * zu) and Q = D'(act(zg)) (D' multiplies
- * as D does), dz = [g * P, g * Q] (0 where the factor is, whatever g), dx = dz W, dW =
+ * as D does), dz = [g * P, g * Q] (0 where dropped, whatever g), dx = dz W, dW =
  * dz^T x, db = sum of dz over rows.
  *
  *   input x  [rows, in_features]               weight W [2 out_features, in_features]
  *   bias b   [2 out_features] or NULL          output y, grad_output g [rows, out_features]
  *   factors  [rows, 2 out_features] contiguous, P before Q, float32 beside float32,
  *            float16 beside bfloat16: the forward writes them where it is not NULL, the
- *            backward reads them
+ *            backward reads them; a dropped element's P is 0, and its Q a NaN by which it is
+ *            told from a kept one's 0 (0xfffe in float16, 0xfffffffe in float32)
  *   exponents  beside bfloat16, with factors: 4-byte aligned, [2, ceil(out_features / 32),
  *            rows, 4] bytes (P before Q; column / 32; row; column % 32 / 8), a byte e (15 to
  *            254) to eight factors, which are their halves times 2^(e - 141); the forward

@@ -315,6 +315,10 @@ __device__ __forceinline__ void store_planes(bf16* p, int64_t plane, int count, 
 // Infinities and NaNs are kept as they are.
 constexpr uint32_t kFactorShift = 141;  // the exponent of 2^14
 
+// What stands in the place of a dropped element's Q: a NaN that no arithmetic leaves (its NaNs
+// are 0x7fff and 0x7fffffff), nor a wait that ran out (all ones).
+constexpr uint32_t kDroppedHalf = 0xfffe, kDroppedFloat = 0xfffffffe;
+
 // Eight factors as halves; their exponent.
 __device__ __forceinline__ uint32_t pack_factors8(const float v[8], uint32_t w[4]) {
   float most = fabsf(v[0]);

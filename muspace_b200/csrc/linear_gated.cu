@@ -10,11 +10,12 @@
 // z_up) and Q = D'(act(z_gate)) (D' multiplies as D does), by which a gradient of y becomes
 // those of the gate's and of up's columns: the backward pass needs no generator, no
 // exponential and no product for them. Beside bfloat16 they are kept in float16, each
-// eight neighbours under an exponent of their own.
+// eight neighbours under an exponent of their own. A dropped element's Q is a NaN of its own, so
+// that a gradient that is not finite is left out there and nowhere else.
 //
 // 8192 x 4096 x 4096 bfloat16 380 us (1.45 PFLOP/s), with factors 410. Where k is short the
-// epilogue is the bound, by issue (51 % of the slots) and latencies: 40000 x 256 x 512
-// bfloat16 gelu 47 us, with factors and dropout 76; 22223 x 256 x 512 float32 silu with
+// epilogue is the bound, by issue and latencies: 40000 x 256 x 512
+// bfloat16 gelu 43 us, with factors and dropout 68; 22223 x 256 x 512 float32 silu with
 // factors 92, where products of 128 columns take the time of 256.
 #include <algorithm>
 
@@ -67,11 +68,11 @@ struct Bias8 {
 
 // Eight values of a row into the box from column `col` on.
 template <int kRowBytes>
-__device__ __forceinline__ void put8(uint32_t box, int row, int col, const float v[8], bf16) {
-  put_unit(unit_at<kRowBytes>(box, row, col / 8), pack2(v[0], v[1]), pack2(v[2], v[3]), pack2(v[4], v[5]), pack2(v[6], v[7]));
+__device__ __forceinline__ void put8(uint32_t box, int row, int col, const uint32_t w[4]) {
+  put_unit(unit_at<kRowBytes>(box, row, col / 8), w[0], w[1], w[2], w[3]);
 }
 template <int kRowBytes>
-__device__ __forceinline__ void put8(uint32_t box, int row, int col, const float v[8], float) {
+__device__ __forceinline__ void put8(uint32_t box, int row, int col, const float v[8]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u)
     put_unit(unit_at<kRowBytes>(box, row, col / 4 + u), __float_as_uint(v[4 * u]), __float_as_uint(v[4 * u + 1]),
@@ -79,11 +80,12 @@ __device__ __forceinline__ void put8(uint32_t box, int row, int col, const float
 }
 
 // Of eight gate sums g and up sums u, both with their bias: the output in g, and with
-// kTrain P in s and Q in u. `words`: the eight's random numbers, with dropout.
-template <bool kFast, bool kTrain>
+// kTrain P in s and Q in u, where what is dropped is marked. `words`: the eight's random
+// numbers, with dropout. float32.
+template <bool kTrain>
 __device__ __forceinline__ void gate_values(Act act, const drop::Rule& rule, const drop::Key& key,
                                             const drop::Words& words, float g[8], float u[8], float s[8]) {
-  activate<kFast, true, kTrain, 8>(act, g, s);
+  activate<false, true, kTrain, 8>(act, g, s);
   if (rule.threshold) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -99,6 +101,44 @@ __device__ __forceinline__ void gate_values(Act act, const drop::Rule& rule, con
     if (kTrain) s[j] *= u[j], u[j] = g[j] * rule.scale;
     g[j] = y;
   }
+  if (kTrain && rule.threshold) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) u[j] = drop::kept(key, words, j) ? u[j] : __uint_as_float(kDroppedFloat);
+  }
+}
+
+// The same in bfloat16, packed: two columns to a word, and what is dropped is masked there
+// (40000 x 256 x 512 gelu 68 us; with three selects a column and the mark by itself 79). Returns P's exponent and, from bit
+// 16 on, Q's; the largest of eight, to which they are scaled, may be one that is dropped.
+template <bool kTrain>
+__device__ __forceinline__ uint32_t gate_words(Act act, const drop::Rule& rule, const drop::Key& key,
+                                               const drop::Words& words, float g[8], float u[8], uint32_t y[4],
+                                               uint32_t p[4], uint32_t q[4]) {
+  float s[8];
+  uint32_t exps = 0;
+  activate<true, true, kTrain, 8>(act, g, s);
+  const float2 scale = both(rule.scale);
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 a = make_float2(g[j], g[j + 1]), b = mul2(make_float2(u[j], u[j + 1]), scale), v = mul2(a, b);
+    y[j / 2] = pack2(v.x, v.y);
+    if (kTrain) {
+      const float2 to_gate = mul2(make_float2(s[j], s[j + 1]), b), to_up = mul2(a, scale);
+      s[j] = to_gate.x, s[j + 1] = to_gate.y;
+      g[j] = to_up.x, g[j + 1] = to_up.y;
+    }
+  }
+  if (kTrain) exps = pack_factors8(s, p) | pack_factors8(g, q) << 16;
+  if (rule.threshold) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t low = drop::kept(key, words, 2 * j) ? 0xffffu : 0u;
+      const uint32_t keep = drop::kept(key, words, 2 * j + 1) ? low | 0xffff0000u : low;
+      y[j] &= keep;
+      if (kTrain) p[j] &= keep, q[j] = (q[j] & keep) | (~keep & (kDroppedHalf | kDroppedHalf << 16));
+    }
+  }
+  return exps;
 }
 
 // kKind: the activation, twice, and one more in training.
@@ -106,7 +146,7 @@ template <int BN, int CG, typename T, bool kF32, int kKind>
 __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, const Place place) {
   using S = Shape<BN, CG, kF32, true>;
   constexpr Act kAct = static_cast<Act>(kKind / 2);
-  constexpr bool kTrain = kKind % 2, kFast = sizeof(T) == 2;
+  constexpr bool kTrain = kKind % 2;
   constexpr int kOut = S::kCols / 2;  // columns of the output that a warp takes
   constexpr int kRowBytes = kOut * sizeof(T), kPart = 32 * kRowBytes;
   static_assert(kRowBytes == 32 || kRowBytes == 64, "three boxes to a warp");
@@ -192,7 +232,7 @@ __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, co
     uint32_t exps_p = 0, exps_q = 0;  // a byte to eight columns, the first one lowest
 #pragma unroll 1
     for (int c = 0; c < kOut; c += 8) {  // sixteen at a time spill: 83 us and 75 without exponents, float32 22223 x 256 x 512 122 and 92
-      float g[8], u[8], s[8];
+      float g[8], u[8];
       Bias8<T> here_g, here_u;
       if (with_bias) {
         here_g.load(bias_gate + n0 + c, bias_vec, rows_n - n0 - c);
@@ -208,17 +248,23 @@ __device__ __noinline__ bool gated_epilogue(const Maps& maps, const Job& job, co
       ask8(gate_at + ahead, next_g);
       ask8(up_at + ahead, next_u);
       if (with_bias) here_g.add(g), here_u.add(u);
-      gate_values<kFast, kTrain>(kAct, e.rule, key, words, g, u, s);
-      put8<kRowBytes>(out, lane, c, g, T());
-      if constexpr (kTrain && sizeof(T) == 2) {
-        uint32_t w[4];
-        exps_p |= pack_factors8(s, w) << c;
-        put_unit(unit_at<kRowBytes>(box + kPart, lane, c / 8), w[0], w[1], w[2], w[3]);
-        exps_q |= pack_factors8(u, w) << c;
-        put_unit(unit_at<kRowBytes>(box + 2 * kPart, lane, c / 8), w[0], w[1], w[2], w[3]);
-      } else if (kTrain) {
-        put8<kRowBytes>(box + kPart, lane, c, s, T());
-        put8<kRowBytes>(box + 2 * kPart, lane, c, u, T());
+      if constexpr (sizeof(T) == 2) {
+        uint32_t y[4], p[4], q[4];
+        const uint32_t exps = gate_words<kTrain>(kAct, e.rule, key, words, g, u, y, p, q);
+        put8<kRowBytes>(out, lane, c, y);
+        if (kTrain) {
+          exps_p |= (exps & 0xffffu) << c, exps_q |= (exps >> 16) << c;
+          put8<kRowBytes>(box + kPart, lane, c, p);
+          put8<kRowBytes>(box + 2 * kPart, lane, c, q);
+        }
+      } else {
+        float s[8];
+        gate_values<kTrain>(kAct, e.rule, key, words, g, u, s);
+        put8<kRowBytes>(out, lane, c, g);
+        if (kTrain) {
+          put8<kRowBytes>(box + kPart, lane, c, s);
+          put8<kRowBytes>(box + 2 * kPart, lane, c, u);
+        }
       }
     }
     if (kTrain && sizeof(T) == 2 && m + lane < rows_m && n0 < rows_n) {
@@ -300,16 +346,14 @@ struct GatedEpilogue {
   }
 };
 
-// Up to eight factors and their exponent.
-__device__ __forceinline__ void put_factors8(__half* at, int count, bool vec, const float v[8], uint8_t* exponent) {
-  uint32_t w[4];
-  *exponent = static_cast<uint8_t>(pack_factors8(v, w));
+// Up to eight packed values of 16 bits.
+__device__ __forceinline__ void put_words(void* at, int count, bool vec, const uint32_t w[4]) {
   if (vec) {
-    *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+    *static_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < count) at[j] = __ushort_as_half(static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2))));
+      if (j < count) static_cast<unsigned short*>(at)[j] = static_cast<unsigned short>(w[j / 2] >> (16 * (j % 2)));
   }
 }
 
@@ -360,19 +404,29 @@ __global__ void __launch_bounds__(256) gated_finish_kernel(const __grid_constant
     }
     drop::Words words;
     if (e.rule.threshold) words = drop::numbers(key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8));
-    gate_values<sizeof(T) == 2, true>(e.act, e.rule, key, words, g, u, s);
-    store_some(static_cast<T*>(e.out) + m * e.out_ld + n, count, vec, g);
-    if (e.slope && sizeof(T) == 4) {
-      float* factors = static_cast<float*>(e.slope) + m * 2 * pr.n + n;
-      store_some(factors, count, vec, s);
-      store_some(factors + pr.n, count, vec, u);
-    } else if (e.slope) {
-      __half* factors = static_cast<__half*>(e.slope) + m * 2 * pr.n + n;
+    T* out = static_cast<T*>(e.out) + m * e.out_ld + n;
+    if constexpr (sizeof(T) == 4) {
+      gate_values<true>(e.act, e.rule, key, words, g, u, s);
+      store_some(out, count, vec, g);
+      if (e.slope) {
+        float* factors = static_cast<float*>(e.slope) + m * 2 * pr.n + n;
+        store_some(factors, count, vec, s);
+        store_some(factors + pr.n, count, vec, u);
+      }
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (j >= count) s[j] = u[j] = 0.f;  // beyond the row
-      put_factors8(factors, count, vec, s, e.exponents + exponent_at(pr.m, pr.n, 0, m, n));
-      put_factors8(factors + pr.n, count, vec, u, e.exponents + exponent_at(pr.m, pr.n, 1, m, n));
+        if (j >= count) g[j] = u[j] = 0.f;  // beyond the row
+      uint32_t y[4], p[4], q[4];
+      const uint32_t exps = gate_words<true>(e.act, e.rule, key, words, g, u, y, p, q);
+      put_words(out, count, vec, y);
+      if (e.slope) {
+        __half* factors = static_cast<__half*>(e.slope) + m * 2 * pr.n + n;
+        put_words(factors, count, vec, p);
+        put_words(factors + pr.n, count, vec, q);
+        e.exponents[exponent_at(pr.m, pr.n, 0, m, n)] = static_cast<uint8_t>(exps);
+        e.exponents[exponent_at(pr.m, pr.n, 1, m, n)] = static_cast<uint8_t>(exps >> 16);
+      }
     }
   }
 }

@@ -45,6 +45,7 @@ __device__ __forceinline__ void finish(const GatedArgs& a, int64_t m, int64_t n,
     u += to_float(static_cast<const T*>(a.bias)[a.out + n]);
   }
   activate<sizeof(T) == 2, true, true, 2>(a.act, g, s);
+  bool kept = true;
   if (a.rule.threshold) {
     const drop::Key key = drop::key_of(a.rule);
     const drop::Words words = drop::numbers(key, static_cast<uint32_t>(m), static_cast<uint32_t>(n / 8));
@@ -52,13 +53,13 @@ __device__ __forceinline__ void finish(const GatedArgs& a, int64_t m, int64_t n,
     if (n % 8 >= 2) word = words.w[1];
     if (n % 8 >= 4) word = words.w[2];
     if (n % 8 >= 6) word = words.w[3];
-    const bool kept = n % 2 ? word > key.high : (word << 16) > key.low;
+    kept = n % 2 ? word > key.high : (word << 16) > key.low;
     g[0] = kept ? g[0] : 0.f, s[0] = kept ? s[0] : 0.f, u = kept ? u * a.rule.scale : 0.f;
   }
   if (sizeof(T) == 4 && a.factors) {  // float32; the others' need eight neighbours
     float* factors = static_cast<float*>(a.factors) + m * 2 * a.out + n;
     factors[0] = s[0] * u;
-    factors[a.out] = g[0] * a.rule.scale;
+    factors[a.out] = kept ? g[0] * a.rule.scale : __uint_as_float(kDroppedFloat);
   }
   static_cast<T*>(a.y)[m * a.y_stride + n] = from_float<T>(g[0] * u);
 }

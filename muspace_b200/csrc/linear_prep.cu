@@ -184,6 +184,47 @@ cudaError_t launch_operand_sums(const void* src, int64_t src_ld, const void* slo
   return cudaGetLastError();
 }
 
+// Eight values of 16 bits as they lie in memory.
+__device__ __forceinline__ void load_words(const void* p, int count, bool vec, uint32_t w[4]) {
+  if (vec) {
+    const uint4 u = *static_cast<const uint4*>(p);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t bits = j < count ? static_cast<const unsigned short*>(p)[j] : 0u;
+      w[j / 2] = j % 2 ? w[j / 2] | bits << 16 : bits;
+    }
+  }
+}
+
+// Eight gradients g and their Q, both 0 where the element was dropped: there Q is
+// kDroppedHalf, and the difference of its bits from that 0 (or -0, of 0x7ffe, which is
+// no number that is kept). Two elements at a time: 35 us for 40000 x 512, 38 one by one.
+__device__ __forceinline__ void load_kept(const bf16* g_at, const __half* q_at, int count, bool vec, float g[8],
+                                          float q[8]) {
+  uint32_t gw[4], qw[4];
+  load_words(g_at, count, vec, gw);
+  load_words(q_at, count, vec, qw);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t apart = qw[j] ^ (kDroppedHalf | kDroppedHalf << 16);
+    const uint32_t keep = ~__heq2_mask(*reinterpret_cast<const __half2*>(&apart), __half2half2(__ushort_as_half(0)));
+    gw[j] &= keep, qw[j] &= keep;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qw[j])), v = unpack2(gw[j]);
+    g[2 * j] = v.x, g[2 * j + 1] = v.y;
+    q[2 * j] = f.x, q[2 * j + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load_kept(const float* g_at, const float* q_at, int count, bool vec, float g[8],
+                                          float q[8]) {
+  load_some(g_at, count, vec, g);
+  load_some(q_at, count, vec, q);
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (__float_as_uint(q[j]) == kDroppedFloat) g[j] = q[j] = 0.f;
+}
+
 // dst = [g * P, g * Q] with the sums of both halves' columns, before the rounding: a
 // lane takes eight columns of g and the same of either half. Bound by memory: 40000 x
 // 512 bfloat16 (210 MB) 35 us, 6.0 TB/s; two rows unrolled 46, more blocks to an SM 52
@@ -208,15 +249,14 @@ __global__ void __launch_bounds__(32 * kSumWarps, 4)
       uint32_t e[2] = {};
       if (sizeof(T) == 2) e[0] = __ldg(exps_p + 4 * r), e[1] = __ldg(exps_q + 4 * r);
       float v[8], f[2][8];
-      load_some(src + r * src_ld + c, count, kVec, v);
-#pragma unroll
-      for (int half = 0; half < 2; ++half) load_some(factors + (2 * r + half) * cols + c, count, kVec, f[half]);
+      load_some(factors + 2 * r * cols + c, count, kVec, f[0]);
+      load_kept(src + r * src_ld + c, factors + (2 * r + 1) * cols + c, count, kVec, v, f[1]);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (sizeof(T) == 2) f[half][j] *= factor_scale(e[half]);
-          f[half][j] = f[half][j] == 0.f ? 0.f : f[half][j] * v[j];  // a dropped element passes no infinity on
+          f[half][j] *= v[j];
           s[half][j] += f[half][j];
         }
         bf16* at = dst + r * dst_ld + half * cols + c;

@@ -454,3 +454,37 @@ def test_gated_factors_far_below_their_neighbours(cuda_device, rows, n):
     loose = loose + 2 * 2.0 ** -39 * most  # twice, as the largest itself is off by a little
     expected, terms = (g.double() * p).sum(0), (g6 * (p.abs() + loose / SUM)).sum(0)
     near(db[3:n:8], expected[3::8], terms[3::8], BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("rows,n", [(3, 64), (50, 64), (50, 67), (2000, 512), (2000, 516)])
+def test_gated_zero_factors_hide_no_gradient(cuda_device, rows, n, p, dtype):
+    """Where relu is off both factors are 0, of either sign; a gradient there that is not finite gives
+    NaN, as 0 times it is. Dropped elements alone pass nothing on."""
+    gen = torch.Generator().manual_seed(3)
+    x, w, b, g = (torch.randint(-2, 3, s, generator=gen).to(dtype).to(cuda_device)
+                  for s in ((rows, 64), (2 * n, 64), (2 * n,), (rows, n)))
+    f = factors(rows, n, p, SEED, SEQUENCE).to(cuda_device) if p else torch.ones(rows, n, device=cuda_device)
+    off = (x.double() @ w[:n].double().T + b[:n].double()) <= 0
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    run = lambda grad: torch.autograd.grad(  # noqa: E731
+        gated_linear(*leaves, activation="relu", dropout=p, seed=SEED, sequence=SEQUENCE), leaves, grad)
+    clean = run(g)
+    columns, lines = [2, n - 1], []
+    for c in columns:
+        kept = (off[:, c] & (f[:, c] > 0)).nonzero()
+        assert len(kept)
+        lines.append(int(kept[0]))
+    for value in (math.inf, math.nan):
+        bad = torch.where(f > 0, g, torch.full_like(g, value))  # every dropped element too
+        for r, c in zip(lines, columns):
+            bad[r, c] = value
+        dx, dw, db = run(bad)
+        hit = torch.zeros(2 * n, dtype=torch.bool, device=cuda_device)
+        hit[columns + [n + c for c in columns]] = True
+        assert torch.equal(db.isnan(), hit) and bool(dw[hit].isnan().all()) and torch.equal(db[~hit], clean[2][~hit])
+        assert torch.equal(dw[~hit], clean[1][~hit])
+        rest = [r for r in range(rows) if r not in lines]
+        assert bool(dx[lines].isnan().all()) and torch.equal(dx[rest], clean[0][rest])
