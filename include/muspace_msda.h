@@ -516,6 +516,7 @@ MSDA_API int msda_dropout(msda_dtype_t dtype, const void *input, int64_t rows, i
 typedef enum {
   MSDA_NORM_LAYER = 0, /* (x - mean) * rstd, rstd = 1 / sqrt(var + eps) */
   MSDA_NORM_RMS = 1,   /* x * rstd, rstd = 1 / sqrt(mean(x^2) + eps) */
+  MSDA_NORM_KEEP = 16, /* with either, in msda_add_norm_forward: sum is for the backward alone */
 } msda_norm_t;
 
 /*
@@ -531,7 +532,10 @@ typedef enum {
  *   output, sum contiguous; add_norm may leave sum NULL, norm_add has no output;
  *   mean, rstd [rows] float32, written by the forward where not NULL and read by the
  *   backward (mean: NULL with MSDA_NORM_RMS); add_norm takes output from the sum
- *   before its rounding, mean and rstd (for the backward) from the sum as stored;
+ *   before its rounding, mean and rstd (for the backward) from the sum as stored, at
+ *   which the backward gives the gradients; with MSDA_NORM_KEEP a row of 16 bits whose
+ *   mean is more than four times its spread, or whose sum is beyond the type, has k =
+ *   (s - mean) * rstd in sum, mean 0 and -rstd, from which the backward tells it;
  *   backward: grad_output (add_norm) and grad_sum [rows, cols], either may be NULL
  *   in add_norm, where what reaches the other is 0 then; sum (add_norm) and input
  *   (norm_add, and add_norm with grad_gate) as in the forward, sum_stride apart;
@@ -541,7 +545,7 @@ typedef enum {
  */
 typedef struct {
   int32_t dtype, weight_dtype, gate_dtype; /* msda_dtype_t */
-  int32_t kind;                            /* msda_norm_t */
+  int32_t kind;                            /* msda_norm_t, MSDA_NORM_KEEP added to it or not */
   int64_t rows, cols, gate_groups;
   int64_t input_stride, residual_stride, gate_stride, sum_stride, grad_output_stride, grad_sum_stride;
   float residual_scale, eps;

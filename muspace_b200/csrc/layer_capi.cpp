@@ -153,20 +153,24 @@ resnorm::Args residual_norm_args(const msda_residual_norm_t* in, bool branch, bo
   check_wide_dtype(in->dtype);
   require(in->weight_dtype == in->dtype || in->weight_dtype == MSDA_DTYPE_FLOAT32, "weight_dtype must be dtype or float32");
   require(in->gate_dtype == in->dtype || in->gate_dtype == MSDA_DTYPE_FLOAT32, "gate_dtype must be dtype or float32");
-  require(in->kind == MSDA_NORM_LAYER || in->kind == MSDA_NORM_RMS, "kind must be layer or rms");
+  const int kind = in->kind & ~MSDA_NORM_KEEP;
+  const bool keep = kind != in->kind;
+  require(kind == MSDA_NORM_LAYER || kind == MSDA_NORM_RMS, "kind must be layer or rms");
   check_size(in->rows, "rows");
   check_size(in->cols, "cols");
   for (int64_t stride : {in->input_stride, in->residual_stride, in->gate_stride, in->sum_stride,
                          in->grad_output_stride, in->grad_sum_stride})
     require(stride >= 0, "strides must be non-negative");
   const bool some = in->rows > 0 && in->cols > 0, gated = in->gate || in->grad_gate;
+  require(!keep || (!branch && !backward && (!some || (in->sum && in->rstd))),
+          "MSDA_NORM_KEEP goes with add_norm's forward, sum and rstd");
   require(in->gate_groups >= 0, "sizes must be non-negative");
   require(!some || !gated || (in->gate_groups > 0 && in->rows % in->gate_groups == 0),
           "gate_groups must divide rows");
   resnorm::Args a{};
   a.dtype = static_cast<drop::DType>(in->dtype);
   a.weight_f32 = in->weight_dtype == MSDA_DTYPE_FLOAT32, a.gate_f32 = in->gate_dtype == MSDA_DTYPE_FLOAT32;
-  a.branch = branch, a.rms = in->kind == MSDA_NORM_RMS;
+  a.branch = branch, a.rms = kind == MSDA_NORM_RMS, a.keep = keep;
   a.rows = in->rows, a.cols = in->cols;
   a.gate_groups = gated ? in->gate_groups : 1;
   a.gate_rows = a.gate_groups ? a.rows / a.gate_groups : 0;

@@ -21,6 +21,7 @@ struct Args {
   bool weight_f32, gate_f32;  // w, b, dw, db; gate, dgate: float32, or dtype
   bool branch;               // norm_add
   bool rms;
+  bool keep;                 // add_norm forward: s is for the backward alone (kept_normal)
   int64_t rows, cols;
   int64_t h_stride, r_stride, gate_stride, gy_stride, gs_stride, sum_stride;
   int64_t gate_groups;       // rows of the gate
@@ -36,7 +37,7 @@ struct Args {
   void* y;                   // add_norm forward, contiguous
   void* s;                   // forward, contiguous; add_norm: may be null
   float* mean;               // [rows]; forward: written where not null; backward: read (null with rms);
-                             // add_norm: of s as it is stored
+                             // add_norm: of s as it is stored; rstd below 0: s is normalised (kept_normal)
   float* rstd;
   const void* gy;            // backward, add_norm: may be null
   const void* gs;            // backward; add_norm: may be null

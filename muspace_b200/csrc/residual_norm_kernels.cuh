@@ -18,7 +18,8 @@
 // as it was stored, and with it the statistics of what was stored, which the forward
 // takes in the same reductions: the gradients are those at the stored sum. (With the
 // statistics of the unrounded one, k's sum over a row is not 0, nor that of its squares
-// n; where a row's mean is large beside its spread nothing of the gradient is left.)
+// n; where a row's mean is large beside its spread nothing of the gradient is left.) Where
+// the sum is not an output, rows that their type cannot hold so are kept normalised (kept_normal).
 //
 // Times, forward and backward: 40000 x 256 bfloat16 with dropout 21.7 and 20.6 us (82 MB
 // each, 3.9 TB/s; bound by issue, 58 to 63 % of the slots), 184950 x 256 float16 norm_add
@@ -140,6 +141,16 @@ __device__ __forceinline__ void prefetch_row(const void* row, uint32_t bytes) {
 struct Moments {
   float mean, rstd;
 };
+
+// Rows of 16 bits whose sum is not an output (Args::keep): the backward pass takes the sum as it
+// was stored, so a normalised value k = (s - mean) rstd is off by half a step of |mean| rstd + |k|.
+// Where the mean is more than four times the spread, or the type's range does not hold the sum,
+// the row is kept normalised instead: k in the place of s, mean 0, and rstd with its sign turned.
+template <typename T>
+__device__ __forceinline__ bool kept_normal(const Args& a, Moments sum, Moments stored) {
+  return sizeof(T) == 2 && a.keep && sum.rstd > 0.f && sum.rstd < 3.402823466e38f &&
+         !(fabsf(sum.mean) * sum.rstd <= 4.f && stored.rstd > 0.f);
+}
 
 // Whether the warp has columns in its i-th chunk: what has none is skipped.
 template <int G, bool kVec>
@@ -314,15 +325,20 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, forward_blocks<T>(G, Shape
       Moments none;
       kept = m = moments<G, NV, kVec, false, T>(v, a, cols, lane, buf, turn, none);
     }
+    const bool normal = !kBranch && kept_normal<T>(a, m, kept);
     if (a.rstd && lane == 0 && r < rows) {
-      if (a.mean) a.mean[r] = kept.mean;
-      a.rstd[r] = kept.rstd;
+      if (a.mean) a.mean[r] = normal ? 0.f : kept.mean;
+      a.rstd[r] = normal ? -m.rstd : kept.rstd;
     }
     const float2 scale = both(m.rstd), minus = both(-m.mean);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[i][j] = mul2(add2(v[i][j], minus), scale);
+    if (normal) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) store_chunk<G, kVec>(static_cast<T*>(a.s) + at, there, lane, i, &v[i][0].x);
+    }
     if (kHold) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[0][j] = fma2(v[0][j], held_w.v[j], held_b.v[j]);
@@ -438,8 +454,10 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
       Chunk<T, kVec> x[NV], g[NV];
 #pragma unroll
       for (int i = 0; i < NV; ++i) x[i] = next_x[i], g[i] = next_g[i];
-      const float rstd = next_rstd;
-      const float2 scale = both(rstd), minus = both(-next_mean);
+      // a row that is kept normalised: rstd below 0, and x is k
+      const bool normal = !kBranch && sizeof(T) == 2 && next_rstd < 0.f;
+      const float rstd = normal ? -next_rstd : next_rstd, to_k = normal ? 1.f : rstd;
+      const float2 scale = both(to_k), minus = both(-next_mean);
       // what else the row needs, on its way while the sums are taken
       Chunk<T, kVec> more[kBranch ? 1 : NV], branch[kGate && !kBranch ? NV : 1];
       if (!kBranch) {
@@ -511,13 +529,13 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
       // the gradient of the norm's input in the place of d
       const auto through_norm = [&] {
         const Sums t = row_sums<G>(Sums{sum.x + sum.y, dot.x + dot.y}, buf, turn);
-        const float2 c1 = both(a.rms ? 0.f : -rstd * (t.a * a.share)), c2 = both(-rstd * rstd * (t.b * a.share));
+        const float2 c1 = both(a.rms ? 0.f : -rstd * (t.a * a.share)), c2 = both(-rstd * to_k * (t.b * a.share));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
           float2 k[4];
           centred(i, k);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[i][j] = fma2(k[j], c2, fma2(d[i][j], scale, c1));
+          for (int j = 0; j < 4; ++j) d[i][j] = fma2(k[j], c2, fma2(d[i][j], both(rstd), c1));
         }
       };
       const auto put_rows = [&](void* p, float2 v[NV][4]) {
@@ -728,17 +746,20 @@ __global__ void __launch_bounds__(kLong) forward_long_kernel(const Args a) {
       }
     });
     t = row_sums<kLong>(t, buf, turn);
-    const float rstd = rsqrtf(t.a / n + a.eps);
+    const float rstd = rsqrtf(t.a / n + a.eps), stored = rsqrtf(t.b / n + a.eps);
+    const bool normal = !kBranch && kept_normal<T>(a, Moments{mean.a, rstd}, Moments{mean.b, stored});
     if (a.rstd && threadIdx.x == 0) {
-      if (a.mean) a.mean[r] = mean.b;
-      a.rstd[r] = rsqrtf(t.b / n + a.eps);
+      if (a.mean) a.mean[r] = normal ? 0.f : mean.b;
+      a.rstd[r] = normal ? -rstd : stored;
     }
     over([&](const LongRow<T>& at, float* v) {
       float w[8], b[8];
-      if (!kBranch && a.s) at.put(a.s, v);
+      if (!kBranch && a.s && !normal) at.put(a.s, v);
       at.param(a.w, a.weight_f32, 1.f, w);
       at.param(a.b, a.weight_f32, 0.f, b);
-      for (int j = 0; j < 8; ++j) v[j] = fmaf((v[j] - mean.a) * rstd, w[j], b[j]);
+      for (int j = 0; j < 8; ++j) v[j] = (v[j] - mean.a) * rstd;
+      if (normal) at.put(a.s, v);
+      for (int j = 0; j < 8; ++j) v[j] = fmaf(v[j], w[j], b[j]);
       if (kBranch) {
         if (a.rule.threshold) drop::apply8(key, at.mask(key), v);
         at.param(gate_at(a, r, a.gate_f32 ? 4 : sizeof(T)), a.gate_f32, 1.f, w);
@@ -765,12 +786,14 @@ __global__ void __launch_bounds__(kLong) backward_long_kernel(const Args a, cons
     const Unit unit = unit_of(grid, u);
     float* gate_part = a.parts + static_cast<int64_t>(gridDim.x) * 2 * a.cols + u * a.cols;
     for (int64_t r = unit.begin; r < unit.end; ++r, first = false) {
-      const float mean = normed && a.mean ? a.mean[r] : 0.f, rstd = normed ? a.rstd[r] : 0.f;
+      const float mean = normed && a.mean ? a.mean[r] : 0.f, kept = normed ? a.rstd[r] : 0.f;
+      const bool normal = !kBranch && sizeof(T) == 2 && kept < 0.f;  // the row is kept normalised
+      const float rstd = normal ? -kept : kept, to_k = normal ? 1.f : rstd;
       const void* gate = gate_at(a, r, a.gate_f32 ? 4 : sizeof(T));
       // eight normalised values k and what reaches the norm's output, d
       const auto inputs = [&](const LongRow<T>& at, float k[8], float d[8]) {
         at.rows_of(kBranch ? a.h : a.sum, kBranch ? a.h_stride : a.sum_stride, k);
-        for (int j = 0; j < 8; ++j) k[j] = (k[j] - mean) * rstd;
+        for (int j = 0; j < 8; ++j) k[j] = (k[j] - mean) * to_k;
         at.rows_of(kBranch ? a.gs : a.gy, kBranch ? a.gs_stride : a.gy_stride, d);
         if (kBranch) {
           float p[8];

@@ -10,7 +10,11 @@ a root-mean-square norm; ``D`` is ``dropout``, with the same mask for the same s
 sequence, rows and columns.
 
 The backward pass of ``add_norm`` takes the sum as it was stored, and gives the
-gradients there; that of ``norm_add`` takes the input. Masks are made again. Gradients
+gradients there: with ``return_sum`` at the sum returned (in float16 they are not finite
+where it is not). Without it, rows that 16 bits would not hold as a sum, whose mean is
+more than four times their spread or which go beyond float16's range, are kept
+normalised, and their gradients are those of the sum before any rounding. That of
+``norm_add`` takes the input. Masks are made again. Gradients
 of weight, bias and gate are added up in an order that does not depend on scheduling.
 """
 
@@ -27,6 +31,7 @@ from ._layer_common import WIDE_DTYPE_CODES, autograd_sees, check_tensor, decide
 from .dropout import check_rule
 
 KINDS = {"layer": 0, "rms": 1}
+KEEP = 16  # MSDA_NORM_KEEP
 
 
 # What a call has beside its tensors, as a tuple: branch, kind, residual scale, eps,
@@ -61,6 +66,8 @@ def _forward(module: NativeModule, rule, x, residual, weight, bias, gate, seed_t
         statistics = torch.empty((2, count), dtype=torch.float32, device=x.device)
         mean = statistics.data_ptr()
         rstd = mean + 4 * count
+        if not branch and not want_sum:  # nobody but the backward pass sees the sum
+            kind |= KEEP
     module.plain_call("msda_norm_add_forward" if branch else "msda_add_norm_forward")(x.device, ResidualNormArgs(
         code, code if param is None else WIDE_DTYPE_CODES[param.dtype], gate_code, kind, count, width, groups,
         x_stride, r_stride, gate_stride, 0, 0, 0, scale, eps, threshold, seed, sequence, pointer(seed_tensor),
@@ -246,7 +253,8 @@ def add_norm(input: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor |
     ``(batch, 1, ..., n)`` those of each sample, and no copy is made of either; kind
     ``"layer"`` (``(s - mean) / sqrt(var + eps) * weight + bias``) or ``"rms"`` (``s /
     sqrt(mean(s^2) + eps) * weight + bias``). ``dropout``, ``seed`` and ``sequence`` as
-    in ``dropout``. The norm is taken of the sum before it is rounded to its dtype.
+    in ``dropout``. The norm is taken of the sum before it is rounded to its dtype; with
+    ``return_sum`` the gradients are those at the sum as it is returned.
     """
     return _call("add_norm", input, residual, weight, bias, gate, residual_scale, kind, eps, dropout, seed, sequence,
                  bool(return_sum), backend)

@@ -688,3 +688,82 @@ def test_c_entry_refusals():
     fails("msda_add_norm_backward", "mean is null", **{**back, "mean": None})
     fails("msda_norm_add_backward", "grad_sum is null", **{**back, "grad_sum": None})
     fails("msda_add_norm_backward", "workspace has 0 bytes", **{**back, "grad_weight": p})
+
+
+# ---- rows that their storage type cannot hold ------------------------------------------------------
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("n", [64, 100, 256, 520, 1500, 5001, 8192, 9000])
+def test_add_norm_gradients_are_those_of_its_output(cuda_device, n, kind, dtype):
+    """Of the norm alone, where the sum is not returned: rows whose offset is large beside their spread, and
+    float16 rows whose sum is beyond 65504, have the derivative of what the forward computed.
+
+    A row is kept for the backward pass as its sum or normalised, rounded to its type: the sum only where
+    its mean is at most four times its spread. So a normalised value k is off by HALF (4 + |k|) at most,
+    besides the float32 errors of the sum; call that e. Its mean and rstd follow: rstd is off by
+    mean(|k| e) + mean(e^2), relatively, and k by e + mean(e) + |k| times that."""
+    offsets = [0, 0, 0.5, -1, 3, -3, 5, 10, 100, -1000, 1000, 4096]
+    data = inputs((len(offsets) + 2, n), dtype, cuda_device, gate=(n,), seed=n)
+    for i, offset in enumerate(offsets):
+        if offset:
+            data["r"][i] = offset
+    if dtype == F16:
+        data["r"][-2:] = 60000
+        data["h"][-2:] = 40000 + 2000 * data["h"][-2:]
+    for p, gated in ((0.0, False), (0.25, True)):
+        x = {m: v.double() for m, v in data.items()}
+        f = factors(len(x["h"]), n, p, SEED, SEQUENCE).to(cuda_device) if p else torch.ones_like(x["h"])
+        gate = x["gate"] if gated else torch.ones_like(x["gate"])
+        s = x["r"] + gate * x["h"] * f
+        size = x["r"].abs() + (gate * x["h"] * f).abs()
+        k, rstd = normed64(kind, s)
+        e = HALF[dtype] * (4 + k.abs()) + SUM * rstd * (size + size.amax(-1, keepdim=True)) * (1 + k.abs())
+        rho = (k.abs() * e).mean(-1, keepdim=True) + e.square().mean(-1, keepdim=True)
+        off = e + e.mean(-1, keepdim=True) + k.abs() * rho
+        g = x["gy"]
+        ds, ds_size, m2 = norm_grad64(kind, g * x["w"], k, rstd)
+        loose = (rho + 2 * SUM) * ds_size + rstd * (off * m2.abs() + k.abs() * ((g * x["w"]).abs() * off).mean(-1, keepdim=True))
+        branch = x["h"] * f
+        expected = [gate * f * ds, ds, (g * k).sum(0), g.sum(0), (ds * branch).sum(0)]
+        errors = [gate.abs() * f * loose, loose, (g.abs() * off).sum(0), 0 * g.sum(0), (loose * branch.abs()).sum(0)]
+        terms = [(gate * f * ds).abs(), ds.abs(), (g * k).abs().sum(0), g.abs().sum(0), (ds * branch).abs().sum(0)]
+        names = ["h", "r", "w", "b", "gate"][:4 + gated]
+        leaves = [data[m].clone().requires_grad_(True) for m in names]
+        y = add_norm(*leaves[:4], gate=leaves[4] if gated else None, kind=kind, dropout=p, seed=SEED, sequence=SEQUENCE)
+        assert bool(y.isfinite().all())
+        for i, got in enumerate(torch.autograd.grad(y, leaves, data["gy"])):
+            near(got, expected[i], terms[i] + errors[i] / SUM, dtype)
+
+
+@pytest.mark.gpu
+def test_kept_rows_by_offset_repeat_and_stay_apart(cuda_device):
+    """A row with a large offset changes nothing of the gradients of the rows beside it, and its own are those
+    of the row without the offset, which the norm takes off."""
+    for n in (64, 256, 1024, 9000):
+        data = inputs((40, n), BF16, cuda_device)
+        data["r"].zero_()
+        plain = data["r"].clone()
+        data["r"][7] = 2048
+        run = lambda r: torch.autograd.grad(  # noqa: E731
+            add_norm(h, r, data["w"], data["b"]), [h], data["gy"])[0]
+        h = data["h"].requires_grad_(True)
+        a, b = run(data["r"]), run(plain)
+        rest = [i for i in range(40) if i != 7]
+        assert torch.equal(a[rest], b[rest]) and torch.equal(a, run(data["r"]))
+        # the float32 sum beside 2048 is off by 2^-13 in units of h, k by that and its rounding to bfloat16 (as b's h by its own)
+        assert bool(((a[7] - b[7]).double().abs() <= 0.05 * b[7].double().abs() + 0.05 * float(b[7].double().square().mean().sqrt())).all())
+
+
+def test_c_entry_refuses_keeping_what_is_no_forward_of_add_norm():
+    module = native.load_native_module()
+    p = 4096  # aligned, never dereferenced
+    import ctypes
+    for name, more in (("msda_norm_add_forward", {}), ("msda_add_norm_backward", dict(rstd=p, mean=p, grad_output=p, grad_input=p)),
+                       ("msda_add_norm_forward", dict(sum=None, mean=p, rstd=p)), ("msda_add_norm_forward", dict(rstd=None))):
+        args = native.ResidualNormArgs(**{**dict(rows=4, cols=8, gate_groups=1, input=p, residual=p, output=p, sum=p, kind=16), **more})
+        entry = getattr(module.lib, name)
+        entry.restype, entry.argtypes = ctypes.c_int, [ctypes.POINTER(native.ResidualNormArgs), ctypes.c_void_p]
+        assert entry(args, None) == 1 and "MSDA_NORM_KEEP" in module.last_error()
