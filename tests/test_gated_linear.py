@@ -488,3 +488,17 @@ def test_gated_zero_factors_hide_no_gradient(cuda_device, rows, n, p, dtype):
         assert torch.equal(dw[~hit], clean[1][~hit])
         rest = [r for r in range(rows) if r not in lines]
         assert bool(dx[lines].isnan().all()) and torch.equal(dx[rest], clean[0][rest])
+
+
+def test_gated_float32_workspace_holds_planes_and_sums():
+    """The three bfloat16 planes of x and of the weight, and behind them the sums, rows padded to eight."""
+    lib = native.load_native_module().lib
+    query = lib.msda_gated_linear_forward_workspace
+    query.restype, query.argtypes = ctypes.c_int, [ctypes.POINTER(native.GatedLinearArgs), ctypes.POINTER(ctypes.c_size_t)]
+    size, p = ctypes.c_size_t(), 4096  # aligned, never dereferenced
+    for rows in (2000, 40000):
+        for n in (1, 3, 7, 9, 33, 257):
+            args = native.GatedLinearArgs(dtype=0, rows=rows, in_features=256, out_features=n, input_stride=256,
+                                          weight_stride=256, output_stride=n, input=p, weight=p, output=p)
+            assert query(args, size) == 0
+            assert size.value >= 3 * 2 * 256 * (rows + 2 * n) + rows * -(-2 * n // 8) * 8 * 4
