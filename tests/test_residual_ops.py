@@ -767,3 +767,19 @@ def test_c_entry_refuses_keeping_what_is_no_forward_of_add_norm():
         entry = getattr(module.lib, name)
         entry.restype, entry.argtypes = ctypes.c_int, [ctypes.POINTER(native.ResidualNormArgs), ctypes.c_void_p]
         assert entry(args, None) == 1 and "MSDA_NORM_KEEP" in module.last_error()
+
+
+@pytest.mark.parametrize("cols,rows,per_block", [(128, 2000, 16), (96, 2368, 16), (100, 2000, 8), (256, 2000, 8)])
+def test_backward_units_are_whole_passes_of_a_block(cols, rows, per_block):
+    """Two float32 rows of partial sums (weight and bias) to each block, and a block's rows are a multiple of those
+    that it has under way: 16 where two rows of up to 128 columns share a warp."""
+    import ctypes
+    module = native.load_native_module()
+    query = module.lib.msda_add_norm_backward_workspace
+    query.restype, query.argtypes = ctypes.c_int, [ctypes.POINTER(native.ResidualNormArgs), ctypes.POINTER(ctypes.c_size_t)]
+    size, p = ctypes.c_size_t(), 4096  # aligned, never dereferenced
+    args = native.ResidualNormArgs(dtype=1, weight_dtype=1, gate_dtype=1, rows=rows, cols=cols, gate_groups=1, sum=p, rstd=p,
+                                   mean=p, grad_output=p, grad_input=p, grad_weight=p, grad_bias=p)
+    assert query(args, size) == 0
+    blocks = size.value // (2 * cols * 4)
+    assert size.value == blocks * 2 * cols * 4 and blocks == -(-rows // per_block)
