@@ -502,3 +502,33 @@ def test_gated_float32_workspace_holds_planes_and_sums():
                                           weight_stride=256, output_stride=n, input=p, weight=p, output=p)
             assert query(args, size) == 0
             assert size.value >= 3 * 2 * 256 * (rows + 2 * n) + rows * -(-2 * n // 8) * 8 * 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,n", [(40, 64), (40, 67), (3000, 512)])
+@pytest.mark.parametrize("activation,bias", [("silu", -18.0), ("silu", -20.0), ("gelu", -5.5), ("gelu", -6.0)])
+def test_gated_closed_gates_keep_the_digits_of_up_gradients(cuda_device, rows, n, activation, bias):
+    """Gates of one column in eight far on the flat side: Q is 1e-7 of its neighbours' and less. An error of the
+    pre-activation counts relatively, by |act'(z) / act(z)| <= |z| + 1 there."""
+    x, w, b, g = inputs(rows, 64, n, BF16, cuda_device, seed=6)
+    w[3:n:8] /= 64
+    b[3:n:8] = bias
+    leaf = b.clone().requires_grad_(True)
+    (db,) = torch.autograd.grad(gated_linear(x, w, leaf, activation=activation), [leaf], g)
+    x6, w6, b6 = x.double(), w[3:n:8].double(), b[3:n:8].double()
+    z, size = x6 @ w6.T + b6, x6.abs() @ w6.abs().T + b6.abs()
+    terms = (g[:, 3::8].double() * act64(activation, z)).abs()
+    loose = terms * (SUM * size * (z.abs() + 1) + FACTOR[BF16] + 2 * FAST[BF16])
+    near(db[n + 3::8], (g[:, 3::8].double() * act64(activation, z)).sum(0), (terms + loose / SUM).sum(0), BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32, F16], ids=["bf16", "f32", "f16"])
+@pytest.mark.parametrize("rows,n", [(2, 64), (300, 64), (300, 67)])
+def test_gated_everything_dropped(cuda_device, rows, n, dtype):
+    x, w, b, g = inputs(rows, 32, n, dtype, cuda_device)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = gated_linear(*leaves, dropout=1.0, seed=1)
+    assert not bool(y.any())
+    for d in torch.autograd.grad(y, leaves, torch.full_like(g, math.inf)):
+        assert not bool(d.any())
