@@ -212,14 +212,20 @@ cudaError_t forward_few_rows(const Args& a, cudaStream_t stream) {
   return a.dtype == DType::kF32 ? launch_rows<float>(a, stream) : launch_rows<bf16>(a, stream);
 }
 
-// The same of the gated operator. bfloat16: 1 x 4096 x 2 x 4096 13.2 / 20.2, 4 rows 22.0
-// / 20.2, and 4 x 4096 x 2 x 1024 8.2 / 11.6; 8 rows of up to 2^21 weights 6.4 / 7.4, of
-// 2^23 16.5 / 11.7. float32 as the plain operator of twice the columns: 16 x 4096 x 2 x
-// 4096 103 / 149, 64 x 256 x 2 x 512 7.5 / 15.4, 64 x 1024 x 2 x 1024 35 / 21.
+// The same of the gated operator, whose weight has W = 2 x out x in numbers. bfloat16: one row
+// always (4096 x 2 x 4096 13.0 / 20.8, 8192 x 2 x 8192 42.9 / 55.3); two to four while rows x W is
+// below 2^27, as the row kernel multiplies on the scalar pipe: 2, 3 and 4 rows of 4096 x 2 x 4096
+// 18.0, 19.7 and 21.8 / 20.9, 4 of 4096 x 2 x 2048 13.5 / 14.4, 2 and 4 of 4096 x 2 x 11008 52 and
+// 66 / 40; eight of up to 2^21 weights 6.4 / 7.4, of 2^23 16.5 / 11.7. float32 as the plain operator
+// of twice the columns: 16 x 4096 x 2 x 4096 103 / 149, 64 x 256 x 2 x 512 7.5 / 15.4, 64 x 1024 x 2 x
+// 1024 35 / 21.
 // In training, bfloat16's factors share exponents with their neighbours, which other warps hold here.
 bool gated_few_rows(const GatedArgs& a) {
-  if (a.dtype == DType::kBF16 && a.factors) return false;
-  if (a.dtype == DType::kBF16) return a.rows <= 4 || (a.rows <= 8 && 2 * a.out * a.in <= 1ll << 21);
+  if (a.dtype == DType::kBF16) {
+    const int64_t weights = 2 * a.out * a.in;
+    return !a.factors && (a.rows == 1 || (a.rows <= 4 && a.rows * weights < 1ll << 27) ||
+                          (a.rows <= 8 && weights <= 1ll << 21));
+  }
   Args as{};
   as.dtype = a.dtype, as.rows = a.rows, as.in = a.in, as.out = 2 * a.out;
   return few_rows(as);

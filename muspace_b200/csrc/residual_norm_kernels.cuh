@@ -366,8 +366,8 @@ __device__ __forceinline__ Unit unit_of(const Grid& grid, int64_t u) {
 }
 
 // Blocks to an SM: 128 registers a thread, for the sums, the parameters and a row ahead.
-// In 80, 20000 x 1024 with a gate takes 53 us instead of 61, 40000 x 512 53 instead of
-// 51, 44446 x 256 float32 39 instead of 32.
+// In 80, 20000 x 1024 with a gate takes 54 us instead of 52, 40000 x 512 with one 52
+// instead of 46, 44446 x 256 float32 39 instead of 33; 10000 x 2048 the same 47.
 constexpr int backward_blocks(int threads) { return 512 / threads; }
 
 template <int G, int NV, bool kVec, bool kBranch, bool kGate, typename T>

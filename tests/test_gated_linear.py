@@ -532,3 +532,17 @@ def test_gated_everything_dropped(cuda_device, rows, n, dtype):
     assert not bool(y.any())
     for d in torch.autograd.grad(y, leaves, torch.full_like(g, math.inf)):
         assert not bool(d.any())
+
+
+def test_gated_few_rows_of_large_weights_run_in_tiles():
+    """One row, and few rows of a weight that is not large, need no workspace: a warp takes a column. More
+    work than that runs in tiles, whose ranges of k leave partial sums."""
+    lib = native.load_native_module().lib
+    query = lib.msda_gated_linear_forward_workspace
+    query.restype, query.argtypes = ctypes.c_int, [ctypes.POINTER(native.GatedLinearArgs), ctypes.POINTER(ctypes.c_size_t)]
+    size, p = ctypes.c_size_t(), 4096  # aligned, never dereferenced
+    for rows, k, n, tiles in ((1, 8192, 8192, False), (2, 4096, 4096, False), (3, 4096, 4096, False), (4, 4096, 2048, False),
+                              (4, 4096, 4096, True), (2, 4096, 11008, True), (4, 256, 512, False), (9, 4096, 1024, True)):
+        args = native.GatedLinearArgs(dtype=1, rows=rows, in_features=k, out_features=n, input_stride=k, weight_stride=k,
+                                      output_stride=n, input=p, weight=p, output=p)
+        assert query(args, size) == 0 and (size.value > 0) == tiles
