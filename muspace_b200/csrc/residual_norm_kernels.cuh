@@ -4,7 +4,7 @@
 // A row is read once into the registers of G threads, 8 NV values each; dropout, gate,
 // residual and norm happen there in float32, and each result is rounded once. A dropout
 // mask is made again from its counter wherever it is needed. Short rows in 16 bits are
-// bound by issue, long rows by memory and its latency.
+// bound by issue forward and by latencies backward, long rows by memory and its latency.
 //
 //   add_norm backward, from what reaches y (gy) and s (gs):
 //     ds = gs + rstd (gy w - mean(gy w) - k mean(gy w k)), k = (s - mean) rstd
@@ -21,10 +21,10 @@
 // n; where a row's mean is large beside its spread nothing of the gradient is left.) Where
 // the sum is not an output, rows that their type cannot hold so are kept normalised (kept_normal).
 //
-// Times, forward and backward: 40000 x 256 bfloat16 with dropout 21.7 and 20.6 us (82 MB
-// each, 3.9 TB/s; bound by issue, 58 to 63 % of the slots), 184950 x 256 float16 norm_add
-// with dropout and a gate 80 and 112 (the same, 67 and 48 %), 8192 x 8192 bfloat16 with a
-// gate and both outputs 95 and 166 (537 and 805 MB, 5.7 and 4.8 TB/s).
+// Times, forward and backward: 40000 x 256 bfloat16 with dropout 22.2 and 20.8 us (82 MB
+// each, 3.8 TB/s; 64 and 59 % of the issue slots), 184950 x 256 float16 norm_add with
+// dropout and a gate 80 and 112 (67 and 48 %), 8192 x 8192 bfloat16 with a gate and both
+// outputs 97 and 166 (537 and 805 MB, 5.5 and 4.8 TB/s).
 //
 // A backward block takes whole units of neighbouring rows, a unit's rows all under
 // one row of the gate: so a thread sums dw, db and dgate of its columns in
