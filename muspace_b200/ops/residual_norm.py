@@ -113,15 +113,16 @@ def _backward(ctx, *grads):
     if not branch and grad_y is None:
         need_w = need_b = False
     dx = dr = dw = db = dgate = None
+    passed = None  # the residual's gradient where nothing of the norm is in it; dr is the kernel's to write
     same = False
     if branch:
         if need_r and (scale == 1.0 or not (need_x or need_w or need_b or need_gate)):
-            dr, need_r = grad_s if scale == 1.0 else grad_s * scale, False  # nothing of the norm is in it
+            passed, need_r = grad_s if scale == 1.0 else grad_s * scale, False
     elif need_x and need_r:
         # without gate and dropout both parts of the sum have one gradient
         same = scale == 1.0 and gate is None and threshold == 0
     if not (need_x or need_r or need_w or need_b or need_gate):
-        return None, dr, None, None, None, None, None
+        return None, passed, None, None, None, None, None
     param, gate_kind = ctx.kinds
     device, dtype = first.device, first.dtype
     code = WIDE_DTYPE_CODES[dtype]
@@ -163,7 +164,7 @@ def _backward(ctx, *grads):
             total_stride, y_stride, s_stride, scale, eps, threshold, seed, sequence, pointer(seed_tensor), pointer(x),
             None, pointer(gate), pointer(weight), pointer(bias), None, total_at, mean, rstd, y_at, s_at, pointer(dx),
             pointer(dr), pointer(dw), pointer(db), pointer(dgate)))
-    return dx, dx if same else dr, dw, db, dgate, None, None
+    return dx, dx if same else passed if dr is None else dr, dw, db, dgate, None, None
 
 
 _backward_once = once_differentiable(_backward)

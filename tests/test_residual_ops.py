@@ -783,3 +783,39 @@ def test_backward_units_are_whole_passes_of_a_block(cols, rows, per_block):
     assert query(args, size) == 0
     blocks = size.value // (2 * cols * 4)
     assert size.value == blocks * 2 * cols * 4 and blocks == -(-rows // per_block)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(30, 64), (6, 5, 67), (3, 700), (2, 3, 9000)], ids=lambda s: "x".join(map(str, s)))
+def test_a_gradient_that_comes_in_is_left_as_it_was(cuda_device, shape, dtype):
+    """Slices and expanded gradients, which the residual's gradient is where the scale is 1: what lies beside and
+    behind them stays."""
+    n = shape[-1]
+    data = inputs(shape, dtype, cuda_device, gate=(n,))
+    guard = torch.randn(4, *shape[:-1], n + 5, device=cuda_device).to(dtype)
+    slice_of, before = guard[2][..., 2:n + 2], guard.clone()
+    single = torch.randn(100 * n, device=cuda_device).to(dtype)
+    expanded, kept = single[50 * n:51 * n].expand(shape), single.clone()
+    for op in (add_norm, norm_add):
+        for need in ("hrwb", "rwb", "r", "hr"):
+            for gated in (False, True):
+                for grad in (slice_of, expanded):
+                    names = [{"h": "h", "r": "r", "w": "w", "b": "b"}[c] for c in need] + ["gate"] * gated
+                    leaves = {m: data[m].clone().requires_grad_(m in names) for m in ("h", "r", "w", "b", "gate")}
+                    call = lambda: op(leaves["h"], leaves["r"], leaves["w"], leaves["b"],  # noqa: E731
+                                      gate=leaves["gate"] if gated else None, dropout=0.1, seed=4)
+                    got = torch.autograd.grad(call(), [leaves[m] for m in names], grad)
+                    clean = torch.autograd.grad(call(), [leaves[m] for m in names], grad.clone(memory_format=torch.contiguous_format))
+                    for a, b in zip(got, clean):  # one rounding each, of float32 sums in two orders
+                        a, b = a.double(), b.double()
+                        assert bool(((a - b).abs() <= 2 * HALF[dtype] * b.abs() + 2 * LEAST[dtype] + 2.0 ** -14 * b.abs().max()).all())
+                    assert torch.equal(guard, before) and torch.equal(single, kept)
+                    if op is norm_add:
+                        assert torch.equal(got[names.index("r")], grad)
+    # the whole way through autograd: a sum's gradient is one number, expanded
+    for op in (add_norm, norm_add):
+        leaves = [data[m].clone().requires_grad_(True) for m in ("h", "r", "w", "b")]
+        op(*leaves).sum().backward()
+        if op is norm_add:
+            assert torch.equal(leaves[1].grad, torch.ones_like(leaves[1]))
