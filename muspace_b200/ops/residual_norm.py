@@ -196,7 +196,7 @@ def _groups_of(gate: torch.Tensor, shape) -> tuple[torch.Tensor, int]:
         while upto and own[upto - 1] == 1:
             upto -= 1
         if own[:upto] == tuple(lead[:upto]):
-            return gate, int(prod(lead[:upto]))  # tensors while tracing
+            return gate if gate.dim() else gate.reshape(1), int(prod(lead[:upto]))  # tensors while tracing
     return _expanded("gate", gate.float(), shape), int(prod(lead))
 
 

@@ -819,3 +819,13 @@ def test_a_gradient_that_comes_in_is_left_as_it_was(cuda_device, shape, dtype):
         op(*leaves).sum().backward()
         if op is norm_add:
             assert torch.equal(leaves[1].grad, torch.ones_like(leaves[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op", ["add_norm", "norm_add"])
+@pytest.mark.parametrize("shape", [(40, 1), (2, 6, 1), (1, 1), (1,), (0, 1)])
+def test_single_columns_with_every_gate(cuda_device, op, shape):
+    for gate in ((), (1,), (*([1] * len(shape)),), shape):
+        data = inputs(shape, F32, cuda_device, gate=gate)
+        _, grads = check(op, data)
+        assert grads["G"].shape == gate
