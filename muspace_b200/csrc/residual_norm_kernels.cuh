@@ -23,7 +23,7 @@
 //
 // Times, forward and backward: 40000 x 256 bfloat16 with dropout 22.2 and 20.8 us (82 MB
 // each, 3.8 TB/s; 64 and 59 % of the issue slots), 184950 x 256 float16 norm_add with
-// dropout and a gate 80 and 112 (67 and 48 %), 8192 x 8192 bfloat16 with a gate and both
+// dropout and a gate 80 and 108 (67 and 54 %), 8192 x 8192 bfloat16 with a gate and both
 // outputs 97 and 166 (537 and 805 MB, 5.5 and 4.8 TB/s).
 //
 // A backward block takes whole units of neighbouring rows, a unit's rows all under
@@ -470,8 +470,8 @@ __global__ void __launch_bounds__(Shape<G>::kThreads, backward_blocks(Shape<G>::
       if (kEarly && r - offset + kRows < end) load(r + kRows);
       // Short rows with the gate's gradient, whose kernels wait for loads more than the others:
       // the block's next rows, neighbours, by one request to a tensor (184950 x 256 float16
-      // norm_add 124 -> 112 us, 180000 x 256 add_norm with both outputs 111 -> 95; without a
-      // gate, 40000 x 256, 20.7 -> 23).
+      // norm_add, with dr written too, 124 -> 112 us, 180000 x 256 add_norm with both outputs
+      // 111 -> 95; without a gate, 40000 x 256, 20.7 -> 23).
       if (kVec && kGate && G <= 32 && threadIdx.x == 0 && r + kDistance * kRows < end) {
         const uint32_t row = r + kDistance * kRows, count = min(static_cast<uint32_t>(kRows), end - row);
         const auto ask = [&](const void* p, int64_t stride) {
