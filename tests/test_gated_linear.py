@@ -546,3 +546,15 @@ def test_gated_few_rows_of_large_weights_run_in_tiles():
         args = native.GatedLinearArgs(dtype=1, rows=rows, in_features=k, out_features=n, input_stride=k, weight_stride=k,
                                       output_stride=n, input=p, weight=p, output=p)
         assert query(args, size) == 0 and (size.value > 0) == tiles
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,k,n", [(2, 4096, 8200), (3, 4096, 5600), (4, 4096, 4096), (4, 4104, 4099)])
+def test_gated_few_rows_of_large_weights(cuda_device, rows, k, n):
+    x, w, b, _ = inputs(rows, k, n, BF16, cuda_device, seed=9)
+    y = gated_linear(x, w, b, dropout=0.2, seed=SEED, sequence=SEQUENCE)
+    f = factors(rows, n, 0.2, SEED, SEQUENCE).to(cuda_device)
+    z, size = x.double() @ w.double().T + b.double(), x.double().abs() @ w.double().abs().T + b.double().abs()
+    act, zu = act64("silu", z[:, :n]), z[:, n:]
+    off = 1.2 * size[:, :n] + FAST[BF16] / SUM * act.abs()
+    near(y, f * act * zu, f * (off * zu.abs() + act.abs() * size[:, n:] + (act * zu).abs()), BF16)
